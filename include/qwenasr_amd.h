@@ -205,6 +205,90 @@ int qa_qk_prep(float * qkv, int32_t n_tokens, int32_t n_heads, int32_t n_kv_head
                const float * q_norm_w, const float * k_norm_w, int32_t pos0, float rope_theta,
                float eps, void * stream);
 
+/* ---------------------------------------------------------------- a cache in pages
+ * For servers of many streams of unlike lengths: no counterpart in the reference, whose cache holds max_seq_len
+ * positions for its one stream.  A paged cache is a qa_kv_layout whose streams are pages: n_streams pages of max_seq
+ * positions (16, 32, 64, 128 or 256), so qa_kv_cache_alloc, qa_kv_cache_bytes and qa_kv_slot_index serve it as they are,
+ * and one page number means that page of every layer, K and V.  A sequence's table row lists its pages in order of
+ * position: position p lies in page table[p / max_seq], slot p % max_seq; -1 (any number outside [0, n_streams)) is no
+ * page: its positions are not stored and not attended.  table_stride * max_seq <= 2^30; head_dim 128; 1 to 16 query heads
+ * per KV head.  Every pointer is device memory of the current device, which the stream belongs to; calls allocate nothing,
+ * wait for nothing and can be captured into a graph.                                               */
+
+/* A ragged batch of sequences and their new tokens.  Rows row_start[s] .. row_start[s + 1] - 1 of the row buffers are
+ * sequence s's new tokens (none is allowed), the first of them at position n_past[s] >= 0; row_start does not fall.  Rows
+ * of no sequence are left as they were.  The three counts below are the host's bounds of what device memory says:
+ * max_tokens new tokens of any one sequence (0: n_rows), max_len positions of any sequence with its new tokens
+ * (0: what the table holds); max_len sets only how the work is split.                              */
+typedef struct qa_paged_batch {
+    const int32_t * tables;      /* device [n_seqs][table_stride] */
+    const int32_t * n_past;      /* device [n_seqs] */
+    const int32_t * row_start;   /* device [n_seqs + 1] */
+    int32_t n_seqs;
+    int32_t table_stride;
+    int32_t n_rows;              /* rows of the row buffers */
+    int32_t max_tokens;
+    int32_t max_len;
+} qa_paged_batch;
+
+/* qa_kv_append over pages, the same bits: q_out[r] <- RoPE(RMSNorm(q)), K and V rows into the page of the row's
+ * position (dropped where there is none).  qkv: [n_rows][q_dim + 2 kv_dim], q_out: [n_rows][q_dim].  A page that several
+ * tables hold is written as it is: qa_pages_extend makes it private first.                         */
+int qa_paged_append(const float * qkv, const float * q_norm_w, const float * k_norm_w, float * q_out, void * pages,
+                    const qa_kv_layout * layout, int32_t layer, const qa_paged_batch * batch, int32_t n_heads,
+                    float rope_theta, float eps, void * stream);
+
+/* Causal attention of every sequence's new tokens over its pages: the token at position p attends the positions
+ * 0 .. p that lie on a page (a chunk of a prompt, or one token per sequence: a decode step).  A token that sees no
+ * position gets zeros.  q: [n_rows][q_dim] f32 (post norm + RoPE), out: [n_rows][q_dim].  Products and sums have f32
+ * accuracy for either cache type (q and the probabilities are not rounded to f16 as qa_decode_attn does).  scale > 0.
+ * What masked positions hold never matters, NaN included.
+ * workspace: results of key ranges that are joined at the end.  Any size works, none included; with less than
+ * qa_paged_attn_workspace_bytes (of the same batch; its pointers are not read) the keys are cut into fewer ranges, which
+ * is slower and sums in another order.  Nothing in it outlives the call; calls that share one must be stream-ordered.
+ * q, pages, out and workspace aligned to 16 bytes.                                                 */
+size_t qa_paged_attn_workspace_bytes(const qa_kv_layout * layout, const qa_paged_batch * batch, int32_t n_heads);
+int qa_paged_attn(const float * q, const void * pages, const qa_kv_layout * layout, int32_t layer,
+                  const qa_paged_batch * batch, int32_t n_heads, float scale, float * out, void * workspace,
+                  size_t workspace_bytes, void * stream);
+
+/* Bookkeeping of pages on the device.  refs[p]: the number of table entries that hold page p; a page with none
+ * (refs[p] <= 0) is free.  tables: [n_rows][table_stride], one row per sequence the host keeps a place for; rows, src and
+ * dst are device int32[n] of row numbers, n <= 1024; a number outside [0, n_rows) is left out.  Results do not depend on
+ * the order in which the GPU works: pages are given lowest number first, to the rows in list order.
+ *
+ * qa_pages_extend   gives the sequences of rows[i] (NULL: row i) what they need to write n_new[i] tokens at n_past[i]:
+ *                   free pages for the entries of those positions that have none, and, where the first position written
+ *                   lies in a page that other entries hold too, a free page with that page's content (all layers) in its
+ *                   place; the last holder keeps the page itself.  Pages behind that one are taken as they are.  All or
+ *                   nothing: *missing = the pages that were lacking, and 0 means done.  Positions behind the table row
+ *                   are not provided for.  A row listed again is left out.
+ * qa_pages_fork     dst[i]'s row becomes src[i]'s entries of the first len[i] positions, which both hold from then on;
+ *                   the pages that dst[i] held are given back.  Nothing is copied: qa_pages_extend copies what is about
+ *                   to be written.  A pair whose dst is any pair's src, or is listed again later, is left out.
+ * qa_pages_free     gives back the pages of rows[i] behind its first keep[i] positions (NULL: all of them).
+ * qa_pages_copy     copies page src[i] to page dst[i], all layers, K and V; pairs outside the cache or with src = dst are
+ *                   left out.  A dst must be listed once and be no src.
+ * qa_pages_compact  moves the live pages to the numbers 0 .. *n_live - 1: those at or behind n_live take the free numbers
+ *                   before it, lowest to lowest, the others stay.  tables_out and refs_out get the new numbers and may be
+ *                   tables and refs themselves; entries of free pages and of none become -1.
+ * workspace: qa_pages_workspace_bytes(layout); nothing in it outlives a call; calls that share one must be
+ * stream-ordered.                                                                                   */
+size_t qa_pages_workspace_bytes(const qa_kv_layout * layout);
+int qa_pages_extend(void * pages, const qa_kv_layout * layout, int32_t * refs, int32_t * tables, int32_t n_rows,
+                    int32_t table_stride, const int32_t * rows, const int32_t * n_past, const int32_t * n_new, int32_t n,
+                    int32_t * missing, void * workspace, size_t workspace_bytes, void * stream);
+int qa_pages_fork(int32_t * refs, int32_t n_pages, int32_t * tables, int32_t n_rows, int32_t table_stride,
+                  int32_t page_size, const int32_t * src, const int32_t * dst, const int32_t * len, int32_t n,
+                  void * stream);
+int qa_pages_free(int32_t * refs, int32_t n_pages, int32_t * tables, int32_t n_rows, int32_t table_stride,
+                  int32_t page_size, const int32_t * rows, const int32_t * keep, int32_t n, void * stream);
+int qa_pages_copy(void * pages, const qa_kv_layout * layout, const int32_t * src, const int32_t * dst, int32_t n,
+                  void * stream);
+int qa_pages_compact(void * pages, const qa_kv_layout * layout, const int32_t * refs, const int32_t * tables,
+                     int32_t n_rows, int32_t table_stride, int32_t * refs_out, int32_t * tables_out, int32_t * n_live,
+                     void * workspace, size_t workspace_bytes, void * stream);
+
 /* ---------------------------------------------------------------- adjacent decoder ops (row f1)
  * f32 weights stored row-major [out][in] (GGML ne = [in, out], text-decoder.cpp:219-227).       */
 /* Skinny GEMM for the multi-stream decode step (one token per stream): y[rows][out] (+)= x[rows][in] *
@@ -263,6 +347,23 @@ int qa_gemv_fused(const float * W, const uint16_t * W_bf16, int32_t out_dim, int
  * gets bit 0 set when any low half is non-zero, i.e. when src is not bf16-exact.  A checkpoint      *
  * converted from bf16 weights (convert.py:386-387 widens them with tensor.float()) is bf16-exact.  */
 int qa_pack_bf16(const float * src, int64_t n, uint16_t * dst, uint32_t * inexact, void * stream);
+/* 4-bit weights, for servers that keep several models or long caches on one GPU (no counterpart in the reference):
+ * w = (q - 8) * d, q in 0..15, d an f16 scale per row and group of 32, 64 or 128 columns.  The packed form
+ * is 1 KB per block of 16 rows (tile t) x 128 columns (block kb, in_dim / 128 of them), blocks of a tile one after another:
+ * 64 lanes of four 32-bit words, lane 16 j + r = row 16 t + r, word w = columns 128 kb + 32 w + 8 j + e, e = 0..7, column e in
+ * bits 4 (e / 2) + 16 (e % 2).  scales: [tile][in_dim / group][16 rows].  Rows behind out_dim fill the last tile.
+ * qa_pack_q4 makes both from f32 rows src[out_dim][in_dim] (device): d = f16(max |w| / 7), q the nearest to w / d; weights
+ * must be finite and below 4.5e5.  in_dim % 128 == 0.                                              */
+size_t qa_q4_weight_bytes(int32_t out_dim, int32_t in_dim);
+size_t qa_q4_scale_count(int32_t out_dim, int32_t in_dim, int32_t group);
+int qa_pack_q4(const float * src, int32_t out_dim, int32_t in_dim, int32_t group, uint8_t * W_q4, uint16_t * scales,
+               void * stream);
+/* qa_gemv_fused on 4-bit weights and 1 to 32 rows: y[r] = W x[r] (epilogue 0), y[r] += W x[r] (1), or y[r] = silu(g) * u
+ * with W = the packed rows [gate; up], 2 out_dim of them, out_dim % 16 == 0 (2); norm_w != NULL first replaces x[r] by
+ * RMSNorm(x[r]) * norm_w (eps).  Products and sums have f32 accuracy.  x: [rows][in_dim], y: [rows][out_dim], which must
+ * not overlap.  W_q4, x and norm_w aligned to 16 bytes, scales to 8.                               */
+int qa_gemv_q4(const uint8_t * W_q4, const uint16_t * scales, int32_t group, int32_t out_dim, int32_t in_dim,
+               const float * x, int32_t rows, float * y, int32_t epilogue, const float * norm_w, float eps, void * stream);
 /* RMSNorm of each row (text-decoder.cpp:92-98): y = x * (1/sqrtf(mean(x^2) + eps)) * w.          */
 int qa_rmsnorm_rows(const float * x, const float * w, int32_t rows, int32_t dim, float eps, float * y,
                     void * stream);

@@ -51,6 +51,11 @@ class KvLayout(C.Structure):
                 ("cache_type", i32)]
 
 
+class PagedBatch(C.Structure):
+    _fields_ = [("tables", vp), ("n_past", vp), ("row_start", vp), ("n_seqs", i32), ("table_stride", i32),
+                ("n_rows", i32), ("max_tokens", i32), ("max_len", i32)]
+
+
 class LayerWeights(C.Structure):
     _fields_ = [(n, fp) for n in ("attn_norm", "ffn_norm", "q", "k", "v", "o", "q_norm", "k_norm", "gate", "up",
                                   "down")]
@@ -105,6 +110,19 @@ SIGNATURES = {
     "qa_prefill_attn": (C.c_int, vp, vp, C.POINTER(KvLayout), i32, i32, i32, i32, i32, f32, vp, vp, sz, vp),
     "qa_causal_attn_f32": (C.c_int, vp, vp, vp, i32, i32, i32, f32, vp, vp),
     "qa_qk_prep": (C.c_int, vp, i32, i32, i32, vp, vp, i32, f32, f32, vp),
+    "qa_paged_append": (C.c_int, vp, vp, vp, vp, vp, C.POINTER(KvLayout), i32, C.POINTER(PagedBatch), i32, f32, f32, vp),
+    "qa_paged_attn_workspace_bytes": (sz, C.POINTER(KvLayout), C.POINTER(PagedBatch), i32),
+    "qa_paged_attn": (C.c_int, vp, vp, C.POINTER(KvLayout), i32, C.POINTER(PagedBatch), i32, f32, vp, vp, sz, vp),
+    "qa_pages_workspace_bytes": (sz, C.POINTER(KvLayout)),
+    "qa_pages_extend": (C.c_int, vp, C.POINTER(KvLayout), vp, vp, i32, i32, vp, vp, vp, i32, vp, vp, sz, vp),
+    "qa_pages_fork": (C.c_int, vp, i32, vp, i32, i32, i32, vp, vp, vp, i32, vp),
+    "qa_pages_free": (C.c_int, vp, i32, vp, i32, i32, i32, vp, vp, i32, vp),
+    "qa_pages_copy": (C.c_int, vp, C.POINTER(KvLayout), vp, vp, i32, vp),
+    "qa_pages_compact": (C.c_int, vp, C.POINTER(KvLayout), vp, vp, i32, i32, vp, vp, vp, vp, sz, vp),
+    "qa_q4_weight_bytes": (sz, i32, i32),
+    "qa_q4_scale_count": (sz, i32, i32, i32),
+    "qa_pack_q4": (C.c_int, vp, i32, i32, i32, vp, vp, vp),
+    "qa_gemv_q4": (C.c_int, vp, vp, i32, i32, i32, vp, i32, vp, i32, vp, f32, vp),
     "qa_gemv": (C.c_int, vp, i32, i32, vp, i32, vp, i32, vp),
     "qa_gemv_fused": (C.c_int, vp, vp, i32, i32, vp, vp, i32, vp, f32, vp),
     "qa_pack_bf16": (C.c_int, vp, i64, vp, vp, vp),
