@@ -2,15 +2,18 @@
 // row and group of 32, 64 or 128 columns, with the RMSNorm before and the SwiGLU behind that the decoder's GEMVs fuse.
 //
 // What bounds it is the stream of W: half a byte per weight, 1/8 of the f32 GEMV's.  A block of 16 rows x 128 columns is
-// 1 KB, one 16-byte load per lane, and lies in the order in which v_mfma_f32_16x16x32_f16 takes it as its A operand: lane
-// 16 j + r holds row r, and its word w the columns 32 w + 8 j .. + 7, so no weight moves between lanes.  Nibbles become
-// f16 by bit operations: 0x6400 | q is 1024 + q, and a packed add takes 1032 off.  q - 8 is exact in f16.
+// 1 KB, one 16-byte load per lane, and lies in the order in which v_mfma_f32_16x16x32_f16 takes it as its B operand: lane
+// 16 j + r holds row r, and its word w the columns 32 w + 8 j .. + 7, so no weight moves between lanes.  Next to the loads
+// the instructions that turn nibbles into f16 set the pace: nine per eight weights.  0x6400 | q is the f16 1024 + q, with
+// the nibble in bits 4..7 it is 1024 + 16 q; one packed add or multiply-add makes q - 8 of either, exactly.  (Taking q as
+// the f16 subnormal q 2^-24 saves four of the nine, but the matrix unit aligns subnormal products by their exponent field
+// and loses seven bits of them: 2e-6 instead of 1e-7 relative error.)
 //
 // x is f32.  It is split into two f16 parts (a power of two per row brings the largest finite |x| to 2^14..2^15), which
-// stand side by side in the 16 columns of the B operand: 8 rows in one product, so that a single row costs no more
-// matrix instructions than eight.  Products are exact in f32, what the split leaves out is 2^-22 of a value (or 2^-39 of the
-// row's largest, where that is more), a group's sum
-// is multiplied by its scale in f32 and added up in f32.
+// stand in the 16 rows of the A operand: 8 rows of x in one product, so that a single one costs no more matrix instructions
+// than eight.  A lane's results then belong to one row of W, whose scale it needs alone: the block's 64 scales (of groups of
+// 32) are one 2-byte load per lane, which row swaps hand round.  Products are exact in f32, what the split leaves out is 2^-22 of a value (or 2^-39 of the
+// row's largest, where that is more), a group's sum is multiplied by its scale in f32 and added up in f32.
 #include "ops.hpp"
 #include "paged.hpp"
 #include "wave.hpp"
@@ -31,6 +34,7 @@ constexpr int kQ4MaxRows = 32;
 constexpr int kQ4Waves = 8;                        // per workgroup
 constexpr int kQ4Threads = kQ4Waves * kWave;
 constexpr int kXBytes = 64 * 1024;                 // of x in LDS at a time: two workgroups per CU
+constexpr size_t kQ4Lds = 158 * 1024;              // of the CU's 160 KB, the rest is the kernel's own
 constexpr int kQ4Exp = 15;                        // a row's largest finite |x| goes to [2^14, 2^15)
 
 struct Q4Params {
@@ -39,186 +43,366 @@ struct Q4Params {
     const float * x;
     float * y;
     const float * norm_w;
-    int32_t out_dim, in_dim, rows, group_shift;   // group = 32 << group_shift
-    int32_t n_tiles, tile_up;                     // tiles of y, and the distance to a tile's up rows
-    int32_t wt, wk;                               // waves over tiles and over columns: wt * wk = kQ4Waves
+    int32_t out_dim, in_dim, rows;
+    int32_t n_tiles, n_units;                     // tiles of y, and how many units of work they make
+    int32_t wt, wk;                               // waves over units and over columns: wt * wk = kQ4Waves
     int32_t chunk;                                // columns of x in LDS at a time
     int32_t epilogue;
     float eps;
 };
 
-// 8 nibbles of a word as q - 8 in f16, in column order: column e lies in bits 4 (e / 2) + 16 (e % 2).
-__device__ inline h8 unpack(uint32_t w) {
-    const h2 off = h2{static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
-    h8 r;
+// 8 nibbles of a word as q - 8 in column order (column e lies in bits 4 (e / 2) + 16 (e % 2)).
+struct Unpack {
+    uint32_t low, high, magic;
+    h2 off, off16, sixteenth;
+    __device__ inline Unpack() {
+        low = 0x000f000fu;
+        high = 0x00f000f0u;
+        magic = 0x64006400u;
+        // masks in registers: an instruction takes one constant that is none, and there are two
+        asm("" : "+v"(low), "+v"(high));
+        asm("" : "+s"(magic));
+        off = h2{static_cast<_Float16>(-1032.0f), static_cast<_Float16>(-1032.0f)};
+        off16 = h2{static_cast<_Float16>(-72.0f), static_cast<_Float16>(-72.0f)};
+        sixteenth = h2{static_cast<_Float16>(0.0625f), static_cast<_Float16>(0.0625f)};
+    }
+    __device__ inline h8 operator()(uint32_t w) const {
+        const uint32_t v = w >> 8;
+        const h2 a = __builtin_bit_cast(h2, (w & low) | magic) + off;
+        const h2 b = __builtin_elementwise_fma(__builtin_bit_cast(h2, (w & high) | magic), sixteenth, off16);
+        const h2 c = __builtin_bit_cast(h2, (v & low) | magic) + off;
+        const h2 d = __builtin_elementwise_fma(__builtin_bit_cast(h2, (v & high) | magic), sixteenth, off16);
+        return h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    }
+};
+
+// 4 neighbouring values of an x row, times the row's factor, as the two f16 parts.
+// inf: the row holds an infinity, whose second part is 0 instead of inf - inf.
+// The product is rounded to f32 once, in a register that both parts come from: contracted into one of the conversions it would
+// round differently there, and the parts would not add up where it lies half way between two f16.
+__device__ inline void split_x(f4 v, float factor, bool inf, _Float16 * to) {
+#pragma clang fp contract(off)
+    h4 hi, lo;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const h2 v = __builtin_bit_cast(h2, ((w >> (4 * e)) & 0x000f000fu) | 0x64006400u) + off;
-        r[2 * e] = v[0];
-        r[2 * e + 1] = v[1];
+        float s = v[e] * factor;
+        asm volatile("" : "+v"(s));
+        hi[e] = static_cast<_Float16>(s);
+        lo[e] = static_cast<_Float16>(s - static_cast<float>(hi[e]));
+        if (inf && fabsf(s) == INFINITY) lo[e] = static_cast<_Float16>(0.0f);
     }
-    return r;
+    *reinterpret_cast<h4 *>(to) = hi;
+    *reinterpret_cast<h4 *>(to + 32) = lo;
 }
 
-// NB: blocks of 8 x rows.  TW: tiles per wave whose blocks are in flight together (2 with SwiGLU: gate and up).
-template <int NB, int TW, bool SWIGLU>
+// The scales of a block's groups in every lane, from one value per lane: groups of 32 lie in the four rows of 16 lanes, groups
+// of 64 in the first two (and again in the others).
+template <int GS>
+__device__ inline void spread_scales(float v, float (&d)[4 >> GS]) {
+    const uint32_t x = __float_as_uint(v);
+    if constexpr (GS == 2) {
+        d[0] = v;
+    } else {
+        const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);   // rows 0 0 2 2 and 1 1 3 3
+        if constexpr (GS == 1) {
+            d[0] = __uint_as_float(a[0]);
+            d[1] = __uint_as_float(a[1]);
+        } else {
+            const auto even = __builtin_amdgcn_permlane32_swap(a[0], a[0], false, false);
+            const auto odd = __builtin_amdgcn_permlane32_swap(a[1], a[1], false, false);
+            d[0] = __uint_as_float(even[0]);
+            d[1] = __uint_as_float(odd[0]);
+            d[2] = __uint_as_float(even[1]);
+            d[3] = __uint_as_float(odd[1]);
+        }
+    }
+}
+
+// x row r of a block of 8 stands in rows (r % 2) 4 + r / 2 of the A operand, its second part 8 rows on: a lane's result i
+// belongs to x row 2 i + (lane / 16) % 2, so that up to 2 rows need the first result alone.
+// NB: blocks of 8 x rows.  NI: results of a lane that count (1 or 4).  TW: tiles of a wave's unit, whose blocks are in flight
+// together (2 with SwiGLU: gate and up).  GS: groups of 32 << GS columns.  WHOLE: x fits in LDS, and a wave's share of it in
+// its registers.
+template <int NB, int NI, int TW, bool SWIGLU, int GS, bool WHOLE>
 __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    _Float16 * sx = reinterpret_cast<_Float16 *>(lds);            // [chunk / 32][2 rows][32]
-    __shared__ float s_scale[kQ4MaxRows];                         // RMSNorm factor of each row
-    __shared__ int s_exp[kQ4MaxRows];
+    _Float16 * sx = reinterpret_cast<_Float16 *>(lds);            // [chunk / 32][row][part][32]
+    __shared__ float s_factor[kQ4MaxRows];                        // RMSNorm factor of each row, times its power of two
+    __shared__ int s_exp[kQ4MaxRows];                             // that power
+    __shared__ bool s_inf[kQ4MaxRows];
+    __shared__ float s_sum[kQ4Waves], s_max[kQ4Waves];            // of a row's parts; a sign: an infinity among them
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g4 = lane >> 4;
     const int wk = wave % p.wk, wt = wave / p.wk;
-    const int tile0 = (static_cast<int>(blockIdx.x) * p.wt + wt) * (SWIGLU ? 1 : TW);
     const int n_kb = p.in_dim / kTileCols;
+    // units go to the waves of all workgroups in turn, so that every CU gets as many
+    const int unit_step = static_cast<int>(gridDim.x) * p.wt;
+    const int unit0 = wt * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
 
-    // the factor of each x row: RMSNorm and the power of two of the split
-    for (int r = wave; r < p.rows; r += kQ4Waves) {
-        const float * x = p.x + static_cast<int64_t>(r) * p.in_dim;
-        double ss = 0.0;
-        float mx = 0.0f;
-        for (int k = lane; k < p.in_dim; k += kWave) {
-            const float v = x[k];
-            ss += static_cast<double>(v) * v;
-            const float a = fabsf(p.norm_w ? v * p.norm_w[k] : v);
-            if (a < INFINITY) mx = fmaxf(mx, a);                  // what is not finite passes through hi as it is
+    // weights and scales of the next kAhead blocks are in flight, the first ones while x is prepared; behind its last block a
+    // wave loads that one again, so that no branch makes it wait for all
+    constexpr int kAhead = WHOLE ? 2 : 1;
+    constexpr int kGroups = 4 >> GS;                              // of a block
+    u4 w[kAhead][TW];
+    _Float16 d[kAhead][TW];
+    const int n_it = (n_kb + p.wk * kAhead - 1) / (p.wk * kAhead) * kAhead;   // a wave's blocks of a unit, the last ones perhaps idle
+    const uint32_t w_lane = lane * 16, d_lane = (lane & (kGroups * kTileRows - 1)) * 2;
+    int f_unit = unit0, f_it = 0;
+    auto fetch = [&](int slot) {
+        const int kb = min(wk + f_it * p.wk, n_kb - 1), unit = f_unit < p.n_units ? f_unit : min(unit0, p.n_units - 1);
+#pragma unroll
+        for (int t = 0; t < TW; ++t) {
+            const int tile = SWIGLU ? unit + t * p.n_tiles : min(unit * TW + t, p.n_tiles - 1);
+            const int64_t at = static_cast<int64_t>(tile) * n_kb + kb;
+            const char * wb = reinterpret_cast<const char *>(p.W) + at * (kWave * 16);
+            const char * db = reinterpret_cast<const char *>(p.scales) + at * (kGroups * kTileRows * 2);
+            w[slot][t] = *reinterpret_cast<const u4 *>(wb + w_lane);
+            d[slot][t] = *reinterpret_cast<const _Float16 *>(db + d_lane);
         }
-        const float f = p.norm_w ? 1.0f / sqrtf(static_cast<float>(wave_sum_d_all(ss) / p.in_dim) + p.eps) : 1.0f;
-        mx = wave_max_all(mx) * f;
-        if (lane == 0) {
-            s_scale[r] = f;
-            s_exp[r] = mx > 0.0f && mx < INFINITY ? kQ4Exp - __builtin_amdgcn_frexp_expf(mx) : 0;
+        if (++f_it == n_it) {
+            f_it = 0;
+            f_unit += unit_step;
         }
-    }
+    };
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) fetch(u);
 
-    const u4 * wp[TW];
-    const _Float16 * dp[TW];
-    const int n_groups = p.in_dim >> (5 + p.group_shift);
-#pragma unroll
-    for (int t = 0; t < TW; ++t) {
-        // tiles behind the last one read it again and store nothing
-        const int tile = SWIGLU ? min(tile0, p.n_tiles - 1) + t * p.tile_up : min(tile0 + t, p.n_tiles - 1);
-        wp[t] = reinterpret_cast<const u4 *>(p.W) + static_cast<int64_t>(tile) * n_kb * kWave + lane;
-        dp[t] = p.scales + static_cast<int64_t>(tile) * n_groups * kTileRows + g4 * 4;
-    }
-    f4 acc[TW][NB];
-#pragma unroll
-    for (int t = 0; t < TW; ++t) {
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) acc[t][nb] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    // Sum of squares and largest |x| of each row: the 8 waves share up to 8 rows, each taking a part of a row whose loads are
+    // in flight together.  A workgroup that holds all of x writes its parts from those registers.
+    const f4 * nw = reinterpret_cast<const f4 *>(p.norm_w);
+    const int parts = p.rows <= 1 ? 8 : p.rows <= 2 ? 4 : p.rows <= 4 ? 2 : 1;
+    const int part = wave % parts, n4 = p.in_dim >> 2, step = parts * kWave;
     const int cols = 2 * p.rows;
-    int bcol[NB];
+    constexpr int kPer = 8;
+    f4 v[kPer];
+    float ss, mx;
+    bool inf;
+    auto read_part = [&](int r) {
+        const f4 * x = reinterpret_cast<const f4 *>(p.x + static_cast<int64_t>(r) * p.in_dim);
+        ss = mx = 0.0f;
+        // rounds that lie behind the row for the whole wave load nothing
+        for (int k0 = part * kWave; k0 < n4; k0 += kPer * step) {
+            f4 g[kPer];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) bcol[nb] = 2 * min(nb * 8 + (c16 & 7), p.rows - 1) + (c16 >> 3);
-
-    u4 w[TW], w_next[TW];
-    int kb = wk;
-#pragma unroll
-    for (int t = 0; t < TW; ++t) w_next[t] = wp[t][static_cast<int64_t>(min(kb, n_kb - 1)) * kWave];
-    for (int k0 = 0; k0 < p.in_dim; k0 += p.chunk) {
-        const int k1 = min(k0 + p.chunk, p.in_dim);
-        __syncthreads();
-        for (int idx = threadIdx.x; idx < p.rows * ((k1 - k0) >> 2); idx += kQ4Threads) {
-            const int r = idx / ((k1 - k0) >> 2), k = k0 + (idx - r * ((k1 - k0) >> 2)) * 4;
-            f4 v = *reinterpret_cast<const f4 *>(p.x + static_cast<int64_t>(r) * p.in_dim + k);
-            if (p.norm_w) v = v * s_scale[r] * *reinterpret_cast<const f4 *>(p.norm_w + k);
-            h4 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float s = ldexpf(v[e], s_exp[r]);
-                hi[e] = static_cast<_Float16>(s);
-                lo[e] = static_cast<_Float16>(fabsf(s) < INFINITY ? s - static_cast<float>(hi[e]) : 0.0f);
+            for (int u = 0; u < kPer; ++u) {
+                if (k0 + u * step >= n4) break;
+                const int at = min(k0 + lane + u * step, n4 - 1);
+                v[u] = x[at];
+                if (nw) g[u] = nw[at];
             }
-            _Float16 * d = sx + (static_cast<int64_t>((k - k0) >> 5) * cols + 2 * r) * 32 + (k & 31);
-            *reinterpret_cast<h4 *>(d) = hi;
-            *reinterpret_cast<h4 *>(d + 32) = lo;
+#pragma unroll
+            for (int u = 0; u < kPer; ++u) {
+                if (k0 + u * step >= n4) break;
+                if (k0 + lane + u * step >= n4) continue;
+                if (nw) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        ss = fmaf(v[u][e], v[u][e], ss);
+                        v[u][e] *= g[u][e];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(v[u][e]));
+            }
+        }
+        ss = wave_sum_all(ss);
+        mx = wave_max_all(mx);
+        inf = mx == INFINITY;
+        if (__builtin_expect(inf, 0)) {                           // rare: the largest of what is finite
+            mx = 0.0f;
+            for (int k = part * kWave + lane; k < n4; k += step) {
+                const f4 a = nw ? x[k] * nw[k] : x[k];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (fabsf(a[e]) < INFINITY) mx = fmaxf(mx, fabsf(a[e]));
+                }
+            }
+            mx = wave_max_all(mx);
+        }
+    };
+    auto finish_row = [&](int r) {
+        const float f = p.norm_w ? 1.0f / sqrtf(ss / static_cast<float>(p.in_dim) + p.eps) : 1.0f;
+        mx *= f;
+        // 2^127 at most, so that it is a float: x below 2^-112 keeps fewer bits of its own headroom, none of its value
+        const int ex = mx > 0.0f && mx < INFINITY ? min(kQ4Exp - __builtin_amdgcn_frexp_expf(mx), 127) : 0;
+        const float factor = f * ldexpf(1.0f, ex);
+        if (lane == 0 && part == 0) {
+            s_factor[r] = factor;
+            s_exp[r] = ex;
+            s_inf[r] = inf;
+        }
+        if constexpr (WHOLE) {
+#pragma unroll
+            for (int u = 0; u < kPer; ++u) {
+                const int k = part * kWave + lane + u * step;
+                if (k < n4) split_x(v[u], factor, inf, sx + ((k >> 3) * cols + 2 * r) * 32 + (k & 7) * 4);
+            }
+        }
+    };
+    if (parts > 1) {                                              // one row per wave at most, parts of it in several
+        const int r = wave / parts;
+        if (r < p.rows) read_part(r);
+        if (r < p.rows && lane == 0) {
+            s_sum[wave] = ss;
+            s_max[wave] = inf ? -mx : mx;
         }
         __syncthreads();
-        for (; kb * kTileCols < k1; kb += p.wk) {
+        if (r < p.rows) {
+            ss = mx = 0.0f;
+            inf = false;
+            for (int i = r * parts; i < (r + 1) * parts; ++i) {
+                ss += s_sum[i];
+                mx = fmaxf(mx, fabsf(s_max[i]));
+                inf = inf || __float_as_uint(s_max[i]) >> 31;
+            }
+            finish_row(r);
+        }
+    } else {
+        for (int r = wave; r < p.rows; r += kQ4Waves) {
+            read_part(r);
+            finish_row(r);
+        }
+    }
+    __syncthreads();
+
+    int arow[NB];
+    const int a8 = c16 & 7, xr = (a8 & 3) * 2 + (a8 >> 2);        // the x row of the A row c16
 #pragma unroll
-            for (int t = 0; t < TW; ++t) w[t] = w_next[t];
-            const int next = min(kb + p.wk, n_kb - 1);
+    for (int nb = 0; nb < NB; ++nb) arow[nb] = (2 * min(nb * 8 + xr, p.rows - 1) + (c16 >> 3)) * 32 + g4 * 8;
+    float acc[TW][NB][NI];
+    auto clear = [&]() {
 #pragma unroll
-            for (int t = 0; t < TW; ++t) w_next[t] = wp[t][static_cast<int64_t>(next) * kWave];
-            const _Float16 * xb = sx + static_cast<int64_t>((kb * kTileCols - k0) >> 5) * cols * 32 + g4 * 8;
-            f4 part[TW][NB];
+        for (int t = 0; t < TW; ++t) {
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const bool first = (s & ((1 << p.group_shift) - 1)) == 0;
-                const bool last = ((s + 1) & ((1 << p.group_shift) - 1)) == 0;
-                h8 b[NB];
+            for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) b[nb] = *reinterpret_cast<const h8 *>(xb + (s * cols + bcol[nb]) * 32);
+                for (int i = 0; i < NI; ++i) acc[t][nb][i] = 0.0f;
+            }
+        }
+    };
+    const Unpack unpack;
+    auto block = [&](int slot, int kb_in_lds, bool counts) {
+        const _Float16 * xb = sx + static_cast<int64_t>(kb_in_lds) * 4 * cols * 32;
+        f4 group[TW][NB];
+        float dg[TW][kGroups];
 #pragma unroll
-                for (int t = 0; t < TW; ++t) {
-                    const h8 a = unpack(w[t][s]);
+        for (int t = 0; t < TW; ++t) spread_scales<GS>(static_cast<float>(d[slot][t]), dg[t]);
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        if (first) part[t][nb] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-                        part[t][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b[nb], part[t][nb], 0, 0, 0);
-                    }
-                    if (last) {
-                        const h4 d = *reinterpret_cast<const h4 *>(dp[t] + static_cast<int64_t>((kb * 4 + s) >> p.group_shift) * kTileRows);
+        for (int s = 0; s < 4; ++s) {
+            const bool first = (s & ((1 << GS) - 1)) == 0, last = ((s + 1) & ((1 << GS) - 1)) == 0;
+            h8 a[NB];
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
+            for (int nb = 0; nb < NB; ++nb) a[nb] = *reinterpret_cast<const h8 *>(xb + s * cols * 32 + arow[nb]);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) acc[t][nb][i] = fmaf(part[t][nb][i], static_cast<float>(d[i]), acc[t][nb][i]);
-                        }
+            for (int t = 0; t < TW; ++t) {
+                const h8 b = unpack(w[slot][t][s]);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const f4 c = first ? f4{0.0f, 0.0f, 0.0f, 0.0f} : group[t][nb];
+                    group[t][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[nb], b, c, 0, 0, 0);
+                    if (last && counts) {
+#pragma unroll
+                        for (int i = 0; i < NI; ++i) acc[t][nb][i] = fmaf(group[t][nb][i], dg[t][s >> GS], acc[t][nb][i]);
                     }
                 }
             }
         }
-    }
-
-    // the columns' waves add up in LDS, in order; the parts of x in the lanes c16 and c16 + 8
-    if (p.wk > 1) {
-        __syncthreads();
-        f4 * sa = reinterpret_cast<f4 *>(lds);
+        fetch(slot);
+    };
+    // results of a unit: lane c16 + 16 g4 holds row c16 of the tile, the two parts of x lie 32 lanes apart
+    auto store = [&](int unit) {
 #pragma unroll
-        for (int t = 0; t < TW; ++t) {
+        for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) sa[(wave * TW * NB + t * NB + nb) * kWave + lane] = acc[t][nb];
+            for (int i = 0; i < NI; ++i) {
+                const int r = nb * 8 + 2 * i + (g4 & 1);
+                float v[TW];
+#pragma unroll
+                for (int t = 0; t < TW; ++t) v[t] = acc[t][nb][i] + __shfl_xor(acc[t][nb][i], 32, kWave);
+                if (g4 >= 2 || r >= p.rows) continue;
+#pragma unroll
+                for (int t = 0; t < (SWIGLU ? 1 : TW); ++t) {
+                    const int o = (SWIGLU ? unit : unit * TW + t) * kTileRows + c16;
+                    if (o >= p.out_dim) continue;                 // rows and tiles behind the last
+                    float * y = p.y + static_cast<int64_t>(r) * p.out_dim + o;
+                    float out = ldexpf(v[t], -s_exp[r]);
+                    if constexpr (SWIGLU) out = out / (1.0f + expf(-out)) * ldexpf(v[1], -s_exp[r]);
+                    *y = p.epilogue == kEpiAccumOp ? *y + out : out;
+                }
+            }
         }
-        __syncthreads();
-        if (wk != 0) return;
-        for (int k = 1; k < p.wk; ++k) {
+    };
+    // the waves of a unit's columns add up in LDS, in order (behind an x that the next unit takes again)
+    float * sa = reinterpret_cast<float *>(WHOLE ? lds + static_cast<size_t>(p.chunk) * p.rows * 4 : lds);
+    auto join = [&]() {
+        constexpr int kVals = TW * NB * NI;
+        __syncthreads();                                          // what lay there has been read
+        if (wk > 0) {
 #pragma unroll
             for (int t = 0; t < TW; ++t) {
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) acc[t][nb] += sa[((wave + k) * TW * NB + t * NB + nb) * kWave + lane];
-            }
-        }
-    }
+                for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        const int r = nb * 8 + c16;
-        f4 v[TW];
-#pragma unroll
-        for (int t = 0; t < TW; ++t) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[t][i] = acc[t][nb][i] + dpp_f<0x128>(acc[t][nb][i]);
-        }
-        if (c16 >= 8 || r >= p.rows) continue;
-#pragma unroll
-        for (int t = 0; t < (SWIGLU ? 1 : TW); ++t) {
-            const int tile = tile0 + t;
-            if (tile >= p.n_tiles) continue;
-            const int o = tile * kTileRows + g4 * 4;
-            float * y = p.y + static_cast<int64_t>(r) * p.out_dim + o;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (o + i >= p.out_dim) continue;
-                float out = ldexpf(v[t][i], -s_exp[r]);
-                if constexpr (SWIGLU) {
-                    const float up = ldexpf(v[1][i], -s_exp[r]);
-                    out = out / (1.0f + expf(-out)) * up;
+                    for (int i = 0; i < NI; ++i) sa[((wt * (p.wk - 1) + wk - 1) * kVals + (t * NB + nb) * NI + i) * kWave + lane] = acc[t][nb][i];
                 }
-                y[i] = p.epilogue == kEpiAccumOp ? y[i] + out : out;
             }
         }
+        __syncthreads();
+        for (int k = 0; k < p.wk - 1 && wk == 0; ++k) {
+#pragma unroll
+            for (int t = 0; t < TW; ++t) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) acc[t][nb][i] += sa[((wt * (p.wk - 1) + k) * kVals + (t * NB + nb) * NI + i) * kWave + lane];
+                }
+            }
+        }
+    };
+    if constexpr (WHOLE) {
+        // all waves of the workgroup go as many rounds: the join has barriers
+        const int rounds = (p.n_units + unit_step - 1) / unit_step;
+        for (int round = 0; round < rounds; ++round) {
+            const int unit = unit0 + round * unit_step;
+            clear();
+            for (int it = 0; it < n_it; it += kAhead) {
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int kb = wk + (it + u) * p.wk;
+                    block(u, min(kb, n_kb - 1), kb < n_kb);
+                }
+            }
+            if (p.wk > 1) join();
+            if (wk == 0 && unit < p.n_units) store(unit);
+        }
+    } else {
+        clear();
+        int kb = wk;
+        for (int k0 = 0; k0 < p.in_dim; k0 += p.chunk) {
+            const int k1 = min(k0 + p.chunk, p.in_dim), per = (k1 - k0) >> 2, n = p.rows * per;
+            __syncthreads();
+            for (int idx = threadIdx.x; idx < n; idx += kPer * kQ4Threads) {
+                f4 g[kPer];
+#pragma unroll
+                for (int u = 0; u < kPer; ++u) {
+                    const int at = min(idx + u * kQ4Threads, n - 1), r = at / per;
+                    v[u] = *reinterpret_cast<const f4 *>(p.x + static_cast<int64_t>(r) * p.in_dim + k0 + (at - r * per) * 4);
+                    if (nw) g[u] = nw[(k0 >> 2) + at - r * per];
+                }
+#pragma unroll
+                for (int u = 0; u < kPer; ++u) {
+                    const int at = idx + u * kQ4Threads, r = at / per, k = at - r * per;
+                    if (at >= n) continue;
+                    if (nw) v[u] *= g[u];
+                    split_x(v[u], s_factor[r], s_inf[r], sx + ((k >> 3) * cols + 2 * r) * 32 + (k & 7) * 4);
+                }
+            }
+            __syncthreads();
+            for (; kb * kTileCols < k1; kb += p.wk) block(0, kb - k0 / kTileCols, true);
+        }
+        if (p.wk > 1) join();
+        if (wk == 0 && unit0 < p.n_units) store(unit0);
     }
 }
 
@@ -269,30 +453,56 @@ int check_q4(int32_t out_dim, int32_t in_dim, int32_t group, const char * who) {
     return QA_OK;
 }
 
-template <int NB, int TW, bool SWIGLU>
+template <int NB, int NI, int TW, bool SWIGLU, int GS, bool WHOLE>
 int launch_q4(Q4Params p, hipStream_t stream) {
-    const int tiles = SWIGLU ? p.n_tiles : (p.n_tiles + TW - 1) / TW;      // units of a wave
+    p.n_units = SWIGLU ? p.n_tiles : (p.n_tiles + TW - 1) / TW;
     const int n_kb = p.in_dim / kTileCols;
-    // waves of a workgroup: over the columns of a tile while the tiles alone do not fill the GPU
+    // waves of a workgroup: over the columns of a unit while the units alone do not fill the GPU
+    const size_t join = static_cast<size_t>(TW) * NB * NI * kWave * 4, x_whole = static_cast<size_t>(p.in_dim) * p.rows * 4;
     p.wk = 1;
-    while (p.wk < kQ4Waves && p.wk * 2 <= n_kb && static_cast<int64_t>(tiles) * p.wk < 4096) p.wk *= 2;
+    while (p.wk < kQ4Waves && p.wk * 2 <= n_kb && static_cast<int64_t>(p.n_units) * p.wk < (NB == 1 ? 16384 : NB == 2 ? 8192 : 4096) &&
+           (!WHOLE || x_whole + (kQ4Waves - kQ4Waves / (p.wk * 2)) * join <= kQ4Lds)) {
+        p.wk *= 2;
+    }
     p.wt = kQ4Waves / p.wk;
     // x in LDS: all of it, or whole rounds of the waves' blocks
     const int round = p.wk * kTileCols;
-    p.chunk = std::min(p.in_dim, std::max(round, kXBytes / (4 * p.rows) / round * round));
-    const size_t lds = std::max<size_t>(static_cast<size_t>(p.chunk) * p.rows * 4, p.wk > 1 ? static_cast<size_t>(kQ4Threads) * TW * NB * 16 : 0);
-    const void * fn = reinterpret_cast<const void *>(gemv_q4_kernel<NB, TW, SWIGLU>);
-    QA_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-    hipLaunchKernelGGL((gemv_q4_kernel<NB, TW, SWIGLU>), dim3(static_cast<unsigned>((tiles + p.wt - 1) / p.wt)), dim3(kQ4Threads), lds, stream, p);
+    p.chunk = WHOLE ? p.in_dim : std::min(p.in_dim, std::max(round, kXBytes / (4 * p.rows) / round * round));
+    const size_t x_bytes = static_cast<size_t>(p.chunk) * p.rows * 4, joins = p.wt * (p.wk - 1) * join;
+    const size_t lds = WHOLE ? x_bytes + joins : std::max(x_bytes, joins);
+    if (lds > kXBytes / 2) {
+        const void * fn = reinterpret_cast<const void *>(gemv_q4_kernel<NB, NI, TW, SWIGLU, GS, WHOLE>);
+        QA_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+    }
+    // a unit per wave (or group of them); where x is whole, no more workgroups than are resident, which then take several
+    int blocks = (p.n_units + p.wt - 1) / p.wt;
+    if (WHOLE) blocks = std::min(blocks, lds <= 80 * 1024 - 1024 ? 512 : 256);
+    hipLaunchKernelGGL((gemv_q4_kernel<NB, NI, TW, SWIGLU, GS, WHOLE>), dim3(static_cast<unsigned>(blocks)), dim3(kQ4Threads), lds, stream, p);
     QA_LAUNCH_CHECK("gemv_q4_kernel");
     return QA_OK;
 }
 
-template <int TW, bool SWIGLU>
+template <int NB, int NI, int TW, bool SWIGLU, int GS>
+int launch_q4_x(const Q4Params & p, hipStream_t stream) {
+    const int parts = p.rows <= 1 ? 8 : p.rows <= 2 ? 4 : p.rows <= 4 ? 2 : 1;
+    const bool whole = p.in_dim <= 2048 * parts && static_cast<int64_t>(p.rows) * p.in_dim * 4 <= 2 * kXBytes;
+    return whole ? launch_q4<NB, NI, TW, SWIGLU, GS, true>(p, stream) : launch_q4<NB, NI, TW, SWIGLU, GS, false>(p, stream);
+}
+
+template <int TW, bool SWIGLU, int GS>
 int launch_q4_rows(const Q4Params & p, hipStream_t stream) {
-    if (p.rows <= 8) return launch_q4<1, TW, SWIGLU>(p, stream);
-    if (p.rows <= 16) return launch_q4<2, TW, SWIGLU>(p, stream);
-    return launch_q4<4, TW, SWIGLU>(p, stream);
+    if (p.rows <= 2) return launch_q4_x<1, 1, TW, SWIGLU, GS>(p, stream);
+    if (p.rows <= 8) return launch_q4_x<1, 4, TW, SWIGLU, GS>(p, stream);
+    if (p.rows <= 16) return launch_q4_x<2, 4, TW, SWIGLU, GS>(p, stream);
+    return launch_q4_x<4, 4, TW, SWIGLU, GS>(p, stream);
+}
+
+template <int GS>
+int launch_q4_tiles(const Q4Params & p, hipStream_t stream) {
+    if (p.epilogue == kEpiSwigluOp) return launch_q4_rows<2, true, GS>(p, stream);
+    // two tiles per wave where that still leaves every CU a workgroup
+    if (p.n_tiles >= 1024) return launch_q4_rows<2, false, GS>(p, stream);
+    return launch_q4_rows<1, false, GS>(p, stream);
 }
 
 }  // namespace
@@ -348,11 +558,12 @@ extern "C" int qa_gemv_q4(const uint8_t * W_q4, const uint16_t * scales, int32_t
     p.out_dim = out_dim;
     p.in_dim = in_dim;
     p.rows = rows;
-    p.group_shift = group_shift_of(group);
     p.n_tiles = (out_dim + kTileRows - 1) / kTileRows;
-    p.tile_up = p.n_tiles;
     p.epilogue = epilogue;
     p.eps = eps;
-    if (epilogue == kEpiSwigluOp) return launch_q4_rows<2, true>(p, as_stream(stream));
-    return launch_q4_rows<2, false>(p, as_stream(stream));
+    switch (group) {
+        case 32: return launch_q4_tiles<0>(p, as_stream(stream));
+        case 64: return launch_q4_tiles<1>(p, as_stream(stream));
+        default: return launch_q4_tiles<2>(p, as_stream(stream));
+    }
 }
