@@ -63,7 +63,20 @@ struct AttnParams {
 __device__ inline uint32_t lo_pair(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ inline uint32_t hi_pair(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 __device__ inline float row_ror8(float v) { return dpp_f<0x128>(v); }   // lane c of a row of 16 gets lane c ^ 8's
-__device__ inline bool finite(float v) { return fabsf(v) < INFINITY; }
+
+// Over the lanes c, c + 16, c + 32, c + 48, in each of them: row swaps, no LDS.
+__device__ inline float column_max(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ inline float column_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
 
 // A tile: a sequence and its columns [col0, col0 + R).
 struct Tile {
@@ -76,9 +89,10 @@ template <int R, bool FEW>
 __device__ inline Tile find_tile(const AttnParams & p, int tile, int lane) {
     for (int s0 = 0; s0 < p.seqs.n_seqs; s0 += kWave) {
         const int s = s0 + lane;
-        int n = 0, rows = 0, start = 0;
+        int n = 0, rows = 0, start = 0, past = 0;
         if (s < p.seqs.n_seqs) {
             start = p.seqs.row_start[s];
+            past = p.seqs.n_past[s];
             rows = rows_between(start, p.seqs.row_start[s + 1], p.seqs.n_rows);
             const bool few = static_cast<int64_t>(rows) * p.group <= p.few_max;
             if (rows > 0 && few == FEW) n = FEW ? 1 : static_cast<int>((static_cast<int64_t>(rows) * p.group + R - 1) / R);
@@ -98,7 +112,7 @@ __device__ inline Tile find_tile(const AttnParams & p, int tile, int lane) {
             t.tile = tile - (__builtin_amdgcn_readlane(sum, l) - t.n_tiles);
             t.rows = __builtin_amdgcn_readlane(rows, l);
             t.row0 = __builtin_amdgcn_readlane(start, l);
-            t.past = bounded_past(p.seqs.n_past[t.seq]);
+            t.past = bounded_past(__builtin_amdgcn_readlane(past, l));
             return t;
         }
         tile -= __builtin_amdgcn_readlane(sum, kWave - 1);
@@ -168,6 +182,154 @@ struct StepRegs<float> {
     f4 v[4][2];   // key 4 (l / 16) + i, dims 8 (l % 16) ..
 };
 
+// A column's q as the two f16 parts in MFMA order, c = the score unit in log2 (scale log2 e over the column's power of two).
+// Columns that do not exist are zeros.
+__device__ inline void split_q(const float * qp, bool ok, int g4, float scale, float & c, h8 (&qh)[4], h8 (&ql)[4]) {
+    f4 x[8];
+    float mx = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        x[i] = *reinterpret_cast<const f4 *>(qp + (i >> 1) * 32 + g4 * 8 + (i & 1) * 4);
+        if (!ok) x[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[i][e]));
+    }
+    mx = column_max(mx);
+    const int ex = mx > 0.0f && mx < INFINITY ? kQExp - __builtin_amdgcn_frexp_expf(mx) : 0;
+    c = ldexpf(scale * kLog2e, -ex);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float v = ldexpf(x[2 * ks + (e >> 2)][e & 3], ex);   // exact: the parts add up
+            qh[ks][e] = static_cast<_Float16>(v);
+            ql[ks][e] = static_cast<_Float16>(v - static_cast<float>(qh[ks][e]));
+        }
+    }
+}
+
+// One step's scores into the running maximum, sum and probabilities; the accumulators follow a maximum that has grown.
+// A masked score is -inf.
+template <int NB, int KB>
+__device__ inline void softmax_step(const f4 (&S)[NB][KB], const float (&c)[NB], float (&m)[NB], float (&l)[NB], f4 (&O)[NB][8],
+                                    float (&pr)[NB][KB][4]) {
+    float mn[NB];
+    bool up[NB], any = false;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        float t = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t = fmaxf(t, S[nb][kb][i]);
+        }
+        mn[nb] = fmaxf(m[nb], column_max(t));
+        up[nb] = (mn[nb] - m[nb]) * c[nb] > kLazyLog2;   // -inf to finite: yes; -inf to -inf: NaN, no
+        any = any || up[nb];
+    }
+    if (__any(any)) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const float f = up[nb] ? __builtin_amdgcn_exp2f((m[nb] - mn[nb]) * c[nb]) : 1.0f;
+#pragma unroll
+            for (int db = 0; db < 8; ++db) O[nb][db] *= f;
+            l[nb] *= f;
+            if (up[nb]) m[nb] = mn[nb];
+        }
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const float mc = m[nb] == -INFINITY ? INFINITY : fmaf(m[nb], c[nb], -kShiftLog2);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                pr[nb][kb][i] = __builtin_amdgcn_exp2f(fmaf(S[nb][kb][i], c[nb], -mc));
+                l[nb] += pr[nb][kb][i];
+            }
+        }
+    }
+}
+
+// Probabilities as two f16 parts in the order of the PV product.
+__device__ inline void split_p(const float (&pr)[2][4], h8 & hi, h8 & lo) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float v = pr[e >> 2][e & 3];
+        hi[e] = static_cast<_Float16>(v);
+        lo[e] = static_cast<_Float16>(v - static_cast<float>(hi[e]));
+    }
+}
+
+// 4 values of a column from dim on: the output, or the part of this split (lead: this lane also stores the part's weights).
+__device__ inline void store_column(const AttnParams & p, const int32_t * table, int split, int row, int lim, int dim, f4 v, float mc,
+                                    float l, bool lead) {
+    if (p.n_splits == 1) {
+        *reinterpret_cast<f4 *>(p.out + static_cast<int64_t>(row) * kHeadDim + dim) = v * inverse_sum(p, table, lim, l);
+    } else {
+        const int64_t at = static_cast<int64_t>(row) * p.n_splits + split;
+        *reinterpret_cast<f4 *>(p.part_o + at * kHeadDim + dim) = v;
+        if (lead) p.part_ml[at] = f2{mc, l};
+    }
+}
+
+// The end of a wave's steps: the column's sum over its 4 lanes, its reference in log2 units, and the columns of each block
+// whose values are not all finite.
+template <int NB, bool PACK>
+__device__ inline void close_columns(const int (&orow)[NB], const float (&c)[NB], const float (&m)[NB], float (&l)[NB], f4 (&O)[NB][8],
+                                     float (&mc)[NB], uint32_t (&redo)[NB]) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        l[nb] = column_sum(l[nb]);
+        mc[nb] = m[nb] == -INFINITY ? -INFINITY : fmaf(m[nb], c[nb], -kShiftLog2);
+        // 0 x is 0 unless x is not finite, and a sum of such products is then NaN
+        float zero = 0.0f * l[nb];
+#pragma unroll
+        for (int db = 0; db < 8; ++db) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (PACK) O[nb][db][i] += row_ror8(O[nb][db][i]);
+                zero = fmaf(0.0f, O[nb][db][i], zero);
+            }
+        }
+        const uint64_t bad = __ballot((!(zero == 0.0f) || m[nb] == INFINITY) && orow[nb] >= 0);
+        redo[nb] = static_cast<uint32_t>(bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & (PACK ? 0xffu : 0xffffu);
+    }
+}
+
+// Stores the columns of a wave that holds all of a split's steps.
+template <typename CT, int NB, int KS>
+__device__ inline void store_columns(const AttnParams & p, const int32_t * table, int head, int split, int lane, const int (&lim)[NB],
+                                     const int (&orow)[NB], const float (&mc)[NB], const float (&l)[NB], const f4 (&O)[NB][8],
+                                     const uint32_t (&redo)[NB], int step_lo, int step_hi) {
+    const int c16 = lane & 15, g4 = lane >> 4;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        if (orow[nb] >= 0 && !((redo[nb] >> c16) & 1)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f4 a, b;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    a[e] = O[nb][e][i];
+                    b[e] = O[nb][4 + e][i];
+                }
+                store_column(p, table, split, orow[nb], lim[nb], (g4 * 4 + i) * 8, a, mc[nb], l[nb], i == 0 && g4 == 0);
+                store_column(p, table, split, orow[nb], lim[nb], (g4 * 4 + i) * 8 + 4, b, mc[nb], l[nb], false);
+            }
+        }
+        for (uint32_t left = redo[nb]; left != 0; left &= left - 1) {
+            const int col = __ffs(left) - 1;
+            const int row = __builtin_amdgcn_readlane(orow[nb], col), lm = __builtin_amdgcn_readlane(lim[nb], col);
+            float cm, cl;
+            f2 co;
+            column_by_keys<CT, KS>(p, table, head, p.q + static_cast<int64_t>(row) * kHeadDim, lm, step_lo, step_hi, 1, lane, cm, cl, co);
+            const f2 nx = f2{__shfl_down(co[0], 1, kWave), __shfl_down(co[1], 1, kWave)};
+            if ((lane & 1) == 0) store_column(p, table, split, row, lm, 2 * lane, f4{co[0], co[1], nx[0], nx[1]}, cm, cl, lane == 0);
+        }
+    }
+}
+
 // The kernel.  NB blocks of 16 columns per wave, WC waves side by side over columns, WK waves over the steps of the keys
 // (merged in LDS).  A step is 32 keys of f16 or 16 keys of f32: 8 KB of K and 8 KB of V either way.
 template <typename CT, int NB, int WC, int WK, bool FEW>
@@ -216,33 +378,10 @@ __global__ __launch_bounds__(kWave * WC * WK, NB == 1 ? 3 : 2) void paged_attn_k
         orow[nb] = ok ? (tl.row0 + t) * p.n_heads + head * p.group + h : -1;
         const float * qp = p.q + (static_cast<int64_t>(tl.row0 + t) * p.n_heads + head * p.group + h) * kHeadDim;
         if constexpr (F16) {
-            f4 x[8];
-            float mx = 0.0f;
+            split_q(qp, ok, g4, p.scale, c[nb], qh[nb], ql[nb]);
+            if constexpr (PACK) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = *reinterpret_cast<const f4 *>(qp + (i >> 1) * 32 + g4 * 8 + (i & 1) * 4);
-                if (!ok) x[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[i][e]));
-            }
-            mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-            const int ex = mx > 0.0f && mx < INFINITY ? kQExp - __builtin_amdgcn_frexp_expf(mx) : 0;
-            c[nb] = ldexpf(p.scale * kLog2e, -ex);
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float v = ldexpf(x[2 * ks + (e >> 2)][e & 3], ex);
-                    const _Float16 hi = static_cast<_Float16>(v);
-                    const _Float16 lo = static_cast<_Float16>(v - static_cast<float>(hi));
-                    if constexpr (PACK) {
-                        qh[nb][ks][e] = c16 < 8 ? hi : lo;
-                    } else {
-                        qh[nb][ks][e] = hi;
-                        ql[nb][ks][e] = lo;
-                    }
-                }
+                for (int ks = 0; ks < 4; ++ks) qh[nb][ks] = c16 < 8 ? qh[nb][ks] : ql[nb][ks];
             }
         } else {
             c[nb] = p.scale * kLog2e;
@@ -371,46 +510,8 @@ __global__ __launch_bounds__(kWave * WC * WK, NB == 1 ? 3 : 2) void paged_attn_k
             }
         }
 
-        // running maximum of each column (its keys lie in lanes c16 + 16 g4)
-        float mn[NB];
-        bool up[NB], any = false;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            float t = -INFINITY;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) t = fmaxf(t, S[nb][kb][i]);
-            }
-            t = fmaxf(t, __shfl_xor(t, 16, kWave));
-            t = fmaxf(t, __shfl_xor(t, 32, kWave));
-            mn[nb] = fmaxf(m[nb], t);
-            up[nb] = (mn[nb] - m[nb]) * c[nb] > kLazyLog2;   // -inf to finite: yes; -inf to -inf: NaN, no
-            any = any || up[nb];
-        }
-        if (__any(any)) {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                const float f = up[nb] ? __builtin_amdgcn_exp2f((m[nb] - mn[nb]) * c[nb]) : 1.0f;
-#pragma unroll
-                for (int db = 0; db < 8; ++db) O[nb][db] *= f;
-                l[nb] *= f;
-                if (up[nb]) m[nb] = mn[nb];
-            }
-        }
         float pr[NB][KB][4];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            const float mc = m[nb] == -INFINITY ? INFINITY : fmaf(m[nb], c[nb], -kShiftLog2);
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    pr[nb][kb][i] = __builtin_amdgcn_exp2f(fmaf(S[nb][kb][i], c[nb], -mc));
-                    l[nb] += pr[nb][kb][i];
-                }
-            }
-        }
+        softmax_step<NB, KB>(S, c, m, l, O, pr);
 
         // rows of keys that no column sees, and of no page, are whatever memory holds: not even 0 times that
         if (st * KS + KS > kend || hole) {
@@ -430,18 +531,8 @@ __global__ __launch_bounds__(kWave * WC * WK, NB == 1 ? 3 : 2) void paged_attn_k
             h8 ph[NB], pl[NB];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float v = pr[nb][e >> 2][e & 3];
-                    const _Float16 hi = static_cast<_Float16>(v);
-                    const _Float16 lo = static_cast<_Float16>(v - static_cast<float>(hi));
-                    if constexpr (PACK) {
-                        ph[nb][e] = c16 < 8 ? hi : lo;
-                    } else {
-                        ph[nb][e] = hi;
-                        pl[nb][e] = lo;
-                    }
-                }
+                split_p(pr[nb], ph[nb], pl[nb]);
+                if constexpr (PACK) ph[nb] = c16 < 8 ? ph[nb] : pl[nb];
             }
 #pragma unroll
             for (int db = 0; db < 8; ++db) {
@@ -477,64 +568,11 @@ __global__ __launch_bounds__(kWave * WC * WK, NB == 1 ? 3 : 2) void paged_attn_k
         }
     }
 
-    // results of the wave's steps: the column's sum over its 4 lanes, its reference in log2 units
     float mc[NB];
     uint32_t redo[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        l[nb] += __shfl_xor(l[nb], 16, kWave);
-        l[nb] += __shfl_xor(l[nb], 32, kWave);
-        mc[nb] = m[nb] == -INFINITY ? -INFINITY : fmaf(m[nb], c[nb], -kShiftLog2);
-        bool fine = finite(l[nb]) && m[nb] < INFINITY;
-#pragma unroll
-        for (int db = 0; db < 8; ++db) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (PACK) O[nb][db][i] += row_ror8(O[nb][db][i]);
-                fine = fine && finite(O[nb][db][i]);
-            }
-        }
-        const uint64_t bad = __ballot(!fine && orow[nb] >= 0);
-        redo[nb] = static_cast<uint32_t>(bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & (PACK ? 0xffu : 0xffffu);
-    }
-
-    // destination of a column's values: the output, or its part of this split
-    auto store = [&](int row, int lim_col, int dim, f4 v, float mcol, float lcol, bool lead) {
-        if (p.n_splits == 1) {
-            const float inv = inverse_sum(p, table, lim_col, lcol);
-            *reinterpret_cast<f4 *>(p.out + static_cast<int64_t>(row) * kHeadDim + dim) = v * inv;
-        } else {
-            const int64_t at = static_cast<int64_t>(row) * p.n_splits + split;
-            *reinterpret_cast<f4 *>(p.part_o + at * kHeadDim + dim) = v;
-            if (lead) p.part_ml[at] = f2{mcol, lcol};
-        }
-    };
+    close_columns<NB, PACK>(orow, c, m, l, O, mc, redo);
     if constexpr (WK == 1) {
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            if (orow[nb] >= 0 && !((redo[nb] >> c16) & 1) && (!PACK || c16 < 8)) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    f4 a, b;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        a[e] = O[nb][e][i];
-                        b[e] = O[nb][4 + e][i];
-                    }
-                    store(orow[nb], lim[nb], (g4 * 4 + i) * 8, a, mc[nb], l[nb], i == 0 && g4 == 0);
-                    store(orow[nb], lim[nb], (g4 * 4 + i) * 8 + 4, b, mc[nb], l[nb], false);
-                }
-            }
-            for (uint32_t left = redo[nb]; left != 0; left &= left - 1) {
-                const int col = __ffs(left) - 1;
-                const int row = __builtin_amdgcn_readlane(orow[nb], col), lm = __builtin_amdgcn_readlane(lim[nb], col);
-                float cm, cl;
-                f2 co;
-                column_by_keys<CT, KS>(p, table, head, p.q + static_cast<int64_t>(row) * kHeadDim, lm, step_lo, step_hi, 1, lane, cm, cl, co);
-                const f2 nx = f2{__shfl_down(co[0], 1, kWave), __shfl_down(co[1], 1, kWave)};
-                if ((lane & 1) == 0) store(row, lm, 2 * lane, f4{co[0], co[1], nx[0], nx[1]}, cm, cl, lane == 0);
-            }
-        }
+        store_columns<CT, NB, KS>(p, table, head, split, lane, lim, orow, mc, l, O, redo, step_lo, step_hi);
     } else {
         // merge over the WK waves of a column in LDS
         constexpr int kStride = kHeadDim + 4;
@@ -600,66 +638,293 @@ __global__ __launch_bounds__(kWave * WC * WK, NB == 1 ? 3 : 2) void paged_attn_k
                 ls += sl[w * R + col] * f;
                 o += *reinterpret_cast<const f4 *>(so + (w * R + col) * kStride + dim) * f;
             }
-            store(row, slim[col], dim, o, M, ls, dim == 0);
+            store_column(p, table, split, row, slim[col], dim, o, M, ls, dim == 0);
         }
     }
 }
 
-// Joins the splits of each (row, head): one wave each, lane = split for the weights, then lane = 2 dims.
+// The kernel of long chunks on f16 pages: 8 waves of 32 columns each share the K and V of a tile through LDS, which cuts
+// what the CUs pull from L2 to an eighth (without it that traffic sets the pace).  A tile is 128 keys, four steps of 32; a
+// step lies in LDS as the MFMA operands themselves, 8 of K and 8 of V^T, 64 lanes x 16 bytes each: every read and write is
+// one unbroken kilobyte and no wave rearranges anything.  Wave w < 4 fetches and transposes V of step w, wave 4 + w fetches
+// K.  Two tiles in LDS, the next one's rows in registers: one barrier per tile.
+constexpr int kTileSteps = 4;
+constexpr int kTileWaves = 8, kTileColumns = kTileWaves * 32;
+constexpr int kStepHalfs = 16 * kWave * 8;   // a step's 16 operands
+constexpr size_t kTileLds = 2 * kTileSteps * kStepHalfs * sizeof(_Float16);
+
+__global__ __launch_bounds__(kTileWaves * kWave, 2) void paged_attn_tile_kernel(AttnParams p) {
+    constexpr int NB = 2;
+    extern __shared__ __attribute__((aligned(16))) _Float16 lds_kv[];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c16 = lane & 15, g4 = lane >> 4;
+    const int head = static_cast<int>(blockIdx.x) % p.n_kv;
+    const int rest = static_cast<int>(blockIdx.x) / p.n_kv;
+    const int split = rest / p.n_tiles;
+    const Tile tl = find_tile<kTileColumns, false>(p, rest - split * p.n_tiles, lane);
+    if (tl.seq < 0) return;
+    const int col0 = (tl.n_tiles - 1 - tl.tile) * kTileColumns;
+    const int n_cols = tl.rows * p.group;
+    const int cap = p.seqs.table_stride << p.page_shift;
+    const int32_t * table = p.seqs.tables + static_cast<int64_t>(tl.seq) * p.seqs.table_stride;
+    const int t_last = (min(col0 + kTileColumns, n_cols) - 1) / p.group;
+    const int kend = max(0, min(tl.past + t_last, cap - 1) + 1);
+    const int n_steps = (kend + 31) / 32;
+    const int step_lo = split * p.split_steps;
+    const int step_hi = split == p.n_splits - 1 ? n_steps : min(n_steps, step_lo + p.split_steps);
+    if (split > 0 && step_lo >= n_steps) return;                      // uniform for the workgroup
+    const int in_page = (1 << p.page_shift) - 1;
+
+    // this wave's share of a tile: step `wave % 4`, V (waves 0..3) or K
+    const bool fetch_v = wave < kTileSteps;
+    u4 r[8];
+    int pg[2];
+    __shared__ int s_holes[2][kTileSteps];                            // bit kb: 16-key block kb of the step lies on no page
+    auto pages_of = [&](int st, int (&out)[2]) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const int j = st * 32 + kb * 16;
+            out[kb] = j < kend ? page_of(table, p.seqs.table_stride, p.page_shift, p.n_pages, j) : -1;
+        }
+    };
+    int st_held = 0;
+    auto fetch = [&](int st, const int (&from)[2]) {
+        st_held = st;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            pg[kb] = from[kb];
+            const _Float16 * base = page_rows<_Float16>(p, fetch_v ? 1 : 0, max(from[kb], 0), head) +
+                                    static_cast<int64_t>((st * 32 + kb * 16) & in_page) * kHeadDim;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // V: row 4 g4 + i, dims 8 c16 ..; K: row c16, dims 32 i + 8 g4 ..
+                const int off = fetch_v ? (g4 * 4 + i) * kHeadDim + c16 * 8 : c16 * kHeadDim + i * 32 + g4 * 8;
+                r[kb * 4 + i] = *reinterpret_cast<const u4 *>(base + off);
+            }
+        }
+    };
+    auto put = [&](int buf) {
+        _Float16 * to = lds_kv + (buf * kTileSteps + (wave & (kTileSteps - 1))) * kStepHalfs + lane * 8;
+        if (fetch_v) {
+            if (st_held * 32 + 32 > kend || pg[0] < 0 || pg[1] < 0) {   // rows that no column sees, and of no page: not even 0 times them
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (st_held * 32 + (e >> 2) * 16 + g4 * 4 + (e & 3) >= kend || pg[e >> 2] < 0) r[e] = u4{0, 0, 0, 0};
+                }
+            }
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+                u4 a;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    a[w] = db & 1 ? hi_pair(r[2 * w][db >> 1], r[2 * w + 1][db >> 1]) : lo_pair(r[2 * w][db >> 1], r[2 * w + 1][db >> 1]);
+                }
+                *reinterpret_cast<u4 *>(to + (8 + db) * kWave * 8) = a;
+            }
+        } else {
+#pragma unroll
+            for (int f = 0; f < 8; ++f) *reinterpret_cast<u4 *>(to + f * kWave * 8) = r[f];
+            if (lane == 0) s_holes[buf][wave & (kTileSteps - 1)] = (pg[0] < 0 ? 1 : 0) | (pg[1] < 0 ? 2 : 0);
+        }
+    };
+
+    const int mine = wave & (kTileSteps - 1);
+    const int n_tiles = (step_hi - step_lo + kTileSteps - 1) / kTileSteps;
+    int pg_next[2];
+    if (n_tiles > 0) {
+        pages_of(step_lo + mine, pg_next);
+        fetch(step_lo + mine, pg_next);
+        pages_of(step_lo + kTileSteps + mine, pg_next);
+    }
+
+    // columns
+    int lim[NB], orow[NB];
+    float c[NB];
+    h8 qh[NB][4], ql[NB][4];
+    int wave_lim = -1, wave_first = 1 << 30;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const int col = col0 + wave * 32 + nb * 16 + c16;
+        const bool ok = col < n_cols;
+        const int t = ok ? col / p.group : t_last;
+        const int h = ok ? col - t * p.group : 0;
+        lim[nb] = ok ? min(tl.past + t, cap - 1) : -1;
+        orow[nb] = ok ? (tl.row0 + t) * p.n_heads + head * p.group + h : -1;
+        const float * qp = p.q + (static_cast<int64_t>(tl.row0 + t) * p.n_heads + head * p.group + h) * kHeadDim;
+        split_q(qp, ok, g4, p.scale, c[nb], qh[nb], ql[nb]);
+    }
+    {
+        // keys that the wave's last and first token see (its columns are in order of token)
+        const int first_col = col0 + wave * 32, last_col = min(first_col + 32, n_cols) - 1;
+        if (first_col < n_cols) {
+            wave_first = min(tl.past + first_col / p.group, cap - 1);
+            wave_lim = min(tl.past + last_col / p.group, cap - 1);
+        }
+    }
+    const int wave_steps = min(step_hi, (wave_lim + 32) / 32);        // steps behind it hold nothing that the wave sees
+    const int full = max(0, wave_first + 1) / 32;
+
+    float m[NB], l[NB];
+    f4 O[NB][8];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        m[nb] = -INFINITY;
+        l[nb] = 0.0f;
+#pragma unroll
+        for (int db = 0; db < 8; ++db) O[nb][db] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    if (n_tiles > 0) {
+        put(0);
+        fetch(step_lo + kTileSteps + mine, pg_next);
+        pages_of(step_lo + 2 * kTileSteps + mine, pg_next);
+    }
+    __syncthreads();
+    for (int tile = 0; tile < n_tiles; ++tile) {
+        const _Float16 * buf = lds_kv + (tile & 1) * kTileSteps * kStepHalfs + lane * 8;
+        const int st0 = step_lo + tile * kTileSteps;
+#pragma unroll 1
+        for (int s = 0; s < kTileSteps; ++s) {
+            const int st = st0 + s;
+            if (st >= wave_steps) break;                              // uniform for the wave
+            const _Float16 * op = buf + s * kStepHalfs;
+            f4 S[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) S[nb][0] = S[nb][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            h8 a[8];
+#pragma unroll
+            for (int f = 0; f < 8; ++f) a[f] = *reinterpret_cast<const h8 *>(op + f * kWave * 8);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) S[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[kb * 4 + ks], qh[nb][ks], S[nb][kb], 0, 0, 0);
+                }
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) S[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[kb * 4 + ks], ql[nb][ks], S[nb][kb], 0, 0, 0);
+                }
+            }
+            h8 v[8];
+#pragma unroll
+            for (int db = 0; db < 8; ++db) v[db] = *reinterpret_cast<const h8 *>(op + (8 + db) * kWave * 8);
+            const int holes = __builtin_amdgcn_readfirstlane(s_holes[tile & 1][s]);
+            if (st >= full || holes != 0) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (st * 32 + kb * 16 + g4 * 4 + i > lim[nb] || ((holes >> kb) & 1)) S[nb][kb][i] = -INFINITY;
+                        }
+                    }
+                }
+            }
+            float pr[NB][2][4];
+            softmax_step<NB, 2>(S, c, m, l, O, pr);
+            h8 ph[NB], pl[NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) split_p(pr[nb], ph[nb], pl[nb]);
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) O[nb][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[db], ph[nb], O[nb][db], 0, 0, 0);
+            }
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) O[nb][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[db], pl[nb], O[nb][db], 0, 0, 0);
+            }
+        }
+        if (tile + 1 < n_tiles) {
+            put((tile + 1) & 1);
+            if (tile + 2 < n_tiles) {
+                fetch(st0 + 2 * kTileSteps + mine, pg_next);
+                pages_of(st0 + 3 * kTileSteps + mine, pg_next);
+            }
+        }
+        __syncthreads();
+    }
+    float mc[NB];
+    uint32_t redo[NB];
+    close_columns<NB, false>(orow, c, m, l, O, mc, redo);
+    store_columns<_Float16, NB, 32>(p, table, head, split, lane, lim, orow, mc, l, O, redo, step_lo, step_hi);
+}
+
+// Joins the splits of each (row, head): one wave each, lane = split for the weights, then lane = 2 dims.  Its time is
+// dependent loads, so the sequences, the weights and the first results are read together; a split that the row does not
+// reach holds whatever the workspace held, and is selected away.
 __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int ks) {
+    constexpr int kFirst = 8;
     const int lane = threadIdx.x & (kWave - 1);
     const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (item >= static_cast<int64_t>(p.seqs.n_rows) * p.n_heads) return;
     const int row = static_cast<int>(item / p.n_heads);
+    const float * po = p.part_o + item * p.n_splits * kHeadDim + 2 * lane;
+    f2 ml = p.part_ml[item * p.n_splits + min(lane, p.n_splits - 1)];
+    f2 part[kFirst];
+#pragma unroll
+    for (int s = 0; s < kFirst; ++s) part[s] = *reinterpret_cast<const f2 *>(po + min(s, p.n_splits - 1) * kHeadDim);
     const RowPlace at = row_place(p.seqs, row, lane);
     if (at.seq < 0) return;
     const int cap = p.seqs.table_stride << p.page_shift;
     const int lim = min(at.pos, cap - 1);
     // splits that hold a key which this row sees (the first is always computed)
     const int active = lim < 0 ? 1 : min(p.n_splits, lim / ks / p.split_steps + 1);
-    const float * po = p.part_o + item * p.n_splits * kHeadDim + 2 * lane;
-    f2 ml = f2{-INFINITY, 0.0f};
-    if (lane < active) ml = p.part_ml[item * p.n_splits + lane];
+    if (lane >= active) ml = f2{-INFINITY, 0.0f};
     const float M = wave_max_all(ml[0]);
     const float f = ml[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[0] - M);
     const float L = wave_sum_all(ml[1] * f);
     f2 o = f2{0.0f, 0.0f};
-#pragma unroll 8
-    for (int s = 0; s < active; ++s) {
+#pragma unroll
+    for (int s = 0; s < kFirst; ++s) {
         const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s));
-        o += *reinterpret_cast<const f2 *>(po + static_cast<int64_t>(s) * kHeadDim) * w;
+        if (s < active) o += part[s] * w;
+    }
+    for (int s0 = kFirst; s0 < active; s0 += kFirst) {
+#pragma unroll
+        for (int s = 0; s < kFirst; ++s) part[s] = *reinterpret_cast<const f2 *>(po + min(s0 + s, active - 1) * kHeadDim);
+#pragma unroll
+        for (int s = 0; s < kFirst; ++s) {
+            if (s0 + s < active) o += part[s] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s0 + s));
+        }
     }
     const float inv = inverse_sum(p, p.seqs.tables + static_cast<int64_t>(at.seq) * p.seqs.table_stride, lim, L);
     *reinterpret_cast<f2 *>(p.out + item * kHeadDim + 2 * lane) = o * inv;
 }
 
-// How one launch cuts its work.
+constexpr int kMidCols = 64;   // columns of a sequence up to which waves share no LDS tile
+
+// How a call cuts its work: which kernels run, their upper bounds of tiles, and the key ranges.
 struct AttnPlan {
-    bool few, many;          // which kernels run
+    bool few;                // sequences of few columns, when the host's bounds allow any
+    int many_cols;           // columns of a tile of the other kernel, 0: all sequences are of few
     int tiles_few, tiles_many;
     int splits, split_steps; // of both, in steps of the cache type
 };
-
-constexpr int kManyCols = 128;   // columns of a tile of the kernel for longer chunks
 
 AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_heads, size_t workspace_bytes) {
     const bool f16 = l.cache_type == QA_CACHE_F16;
     const int ks = f16 ? 32 : 16;
     const int group = n_heads / l.n_kv_heads;
+    const int seqs = std::min(b.n_seqs, b.n_rows);
     const int64_t most = std::min<int64_t>(b.n_rows, b.max_tokens > 0 ? b.max_tokens : b.n_rows);
+    const int64_t cols = static_cast<int64_t>(b.n_rows) * group;
     AttnPlan pl{};
     // one sequence is either; the host's bounds say whether all are of few columns
-    pl.many = most * group > few_cols(f16);
-    pl.few = !pl.many || b.n_seqs > 1;
-    pl.tiles_few = std::min(b.n_seqs, b.n_rows);
-    pl.tiles_many = static_cast<int>(static_cast<int64_t>(b.n_rows) * group / kManyCols + std::min(b.n_seqs, b.n_rows));
+    if (most * group > few_cols(f16)) pl.many_cols = f16 ? (most * group > kMidCols ? kTileColumns : 64) : 64;
+    pl.few = pl.many_cols == 0 || b.n_seqs > 1;
+    pl.tiles_few = seqs;
+    pl.tiles_many = pl.many_cols ? static_cast<int>(cols / pl.many_cols + seqs) : 0;
     const int64_t cap = static_cast<int64_t>(b.table_stride) * l.max_seq;
     const int64_t len = std::min<int64_t>(cap, b.max_len > 0 ? b.max_len : cap);
     const int steps = static_cast<int>((len + ks - 1) / ks);
-    const int64_t tiles = pl.many ? std::max<int64_t>(1, static_cast<int64_t>(b.n_rows) * group / kManyCols) : pl.tiles_few;
-    const int64_t blocks = tiles * l.n_kv_heads;
-    const int64_t target = 1024;
-    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({target / std::max<int64_t>(blocks, 1), (steps + 3) / 4, kMaxSplits}));
+    const int64_t tiles = pl.many_cols ? std::max<int64_t>(1, (cols + pl.many_cols - 1) / pl.many_cols) : pl.tiles_few;
+    const int64_t target = pl.many_cols == kTileColumns ? 256 : pl.many_cols ? 1024 : 1024, least = pl.many_cols == kTileColumns ? 4 : 8;
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({target / std::max<int64_t>(tiles * l.n_kv_heads, 1), (steps + least - 1) / least, kMaxSplits}));
     const size_t per_split = static_cast<size_t>(b.n_rows) * n_heads * (kHeadDim + 2) * sizeof(float);
     if (splits > 1 && per_split * splits > workspace_bytes) splits = std::max<int64_t>(1, static_cast<int64_t>(workspace_bytes / per_split));
     pl.split_steps = std::max<int>(1, static_cast<int>((steps + splits - 1) / splits));
@@ -668,13 +933,21 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
 }
 
 template <typename CT>
-void launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
+int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
     constexpr bool F16 = std::is_same<CT, _Float16>::value;
     const unsigned per = static_cast<unsigned>(p.n_kv) * pl.splits;
     p.few_max = pl.few ? few_cols(F16) : 0;
-    if (pl.many) {
+    if (pl.many_cols) {
         p.n_tiles = pl.tiles_many;
-        hipLaunchKernelGGL((paged_attn_kernel<CT, 2, 4, 1, false>), dim3(per * p.n_tiles), dim3(256), 0, stream, p);
+        if constexpr (!F16) {
+            hipLaunchKernelGGL((paged_attn_kernel<CT, 1, 4, 1, false>), dim3(per * p.n_tiles), dim3(256), 0, stream, p);
+        } else if (pl.many_cols == kTileColumns) {
+            QA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(paged_attn_tile_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(kTileLds)));
+            hipLaunchKernelGGL(paged_attn_tile_kernel, dim3(per * p.n_tiles), dim3(kTileWaves * kWave), kTileLds, stream, p);
+        } else {
+            hipLaunchKernelGGL((paged_attn_kernel<CT, 2, 2, 2, false>), dim3(per * p.n_tiles), dim3(256), 0, stream, p);
+        }
     }
     if (pl.few) {
         p.n_tiles = pl.tiles_few;
@@ -684,6 +957,8 @@ void launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
         const int64_t items = static_cast<int64_t>(p.seqs.n_rows) * p.n_heads;
         hipLaunchKernelGGL(paged_join_kernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, p, F16 ? 32 : 16);
     }
+    QA_LAUNCH_CHECK("paged_attn_kernel");
+    return QA_OK;
 }
 
 }  // namespace
@@ -731,8 +1006,5 @@ extern "C" int qa_paged_attn(const float * q, const void * pages, const qa_kv_la
     p.n_splits = pl.splits;
     p.split_steps = pl.split_steps;
     p.scale = scale;
-    if (layout->cache_type == QA_CACHE_F16) launch_attn<_Float16>(pl, p, as_stream(stream));
-    else launch_attn<float>(pl, p, as_stream(stream));
-    QA_LAUNCH_CHECK("paged_attn_kernel");
-    return QA_OK;
+    return layout->cache_type == QA_CACHE_F16 ? launch_attn<_Float16>(pl, p, as_stream(stream)) : launch_attn<float>(pl, p, as_stream(stream));
 }

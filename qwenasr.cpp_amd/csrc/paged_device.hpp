@@ -22,21 +22,19 @@ struct RowPlace {
 };
 
 // The sequence whose rows hold `row`: row_start does not fall, so it is the number of sequences that end at or before
-// it.  64 sequences per load, every lane of the wave takes part.
+// it.  64 sequences per load, every lane of the wave takes part; what the place needs is read along with the search.
 __device__ inline RowPlace row_place(const PagedSeqs & b, int row, int lane) {
-    int seq = 0;
     for (int s0 = 0; s0 < b.n_seqs; s0 += kWave) {
-        const int s = s0 + lane;
-        const int end = s < b.n_seqs ? b.row_start[s + 1] : row + 1;
-        const int n = __popcll(__ballot(end <= row));
-        seq += n;
-        if (n < kWave) break;
+        const int s = min(s0 + lane, b.n_seqs - 1);
+        const int start = b.row_start[s], end = b.row_start[s + 1], past = b.n_past[s];
+        const uint64_t over = __ballot(s0 + lane >= b.n_seqs || end > row);
+        const int l = over != 0 ? __ffsll(static_cast<unsigned long long>(over)) - 1 : kWave;
+        if (l == kWave) continue;
+        const int first = __builtin_amdgcn_readlane(start, l);
+        if (s0 + l >= b.n_seqs || first < 0 || first > row) break;
+        return RowPlace{s0 + l, bounded_past(__builtin_amdgcn_readlane(past, l)) + row - first};
     }
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    if (seq >= b.n_seqs) return RowPlace{-1, 0};
-    const int start = b.row_start[seq];
-    if (start < 0 || start > row) return RowPlace{-1, 0};
-    return RowPlace{seq, bounded_past(b.n_past[seq]) + row - start};
+    return RowPlace{-1, 0};
 }
 
 }  // namespace qa
