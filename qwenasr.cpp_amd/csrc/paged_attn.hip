@@ -182,26 +182,33 @@ struct StepRegs<float> {
     f4 v[4][2];   // key 4 (l / 16) + i, dims 8 (l % 16) ..
 };
 
-// A column's q as the two f16 parts in MFMA order, c = the score unit in log2 (scale log2 e over the column's power of two).
-// Columns that do not exist are zeros.
-__device__ inline void split_q(const float * qp, bool ok, int g4, float scale, float & c, h8 (&qh)[4], h8 (&ql)[4]) {
-    f4 x[8];
-    float mx = 0.0f;
+// A column's q in MFMA order (dims 32 ks + 8 (l / 16) .. at [2 ks]); columns that do not exist are zeros.
+__device__ inline void load_q(const float * qp, bool ok, int g4, f4 (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         x[i] = *reinterpret_cast<const f4 *>(qp + (i >> 1) * 32 + g4 * 8 + (i & 1) * 4);
         if (!ok) x[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+}
+
+// Its two f16 parts, c = the score unit in log2 (scale log2 e over the column's power of two).
+__device__ inline void split_q(const f4 (&x)[8], float scale, float & c, h8 (&qh)[4], h8 (&ql)[4]) {
+    float mx = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[i][e]));
     }
     mx = column_max(mx);
-    const int ex = mx > 0.0f && mx < INFINITY ? kQExp - __builtin_amdgcn_frexp_expf(mx) : 0;
+    // 2^127 at most, so that it is a float; the parts of smaller q need no more
+    const int ex = mx > 0.0f && mx < INFINITY ? min(kQExp - __builtin_amdgcn_frexp_expf(mx), 127) : 0;
+    const float unit = ldexpf(1.0f, ex);
     c = ldexpf(scale * kLog2e, -ex);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float v = ldexpf(x[2 * ks + (e >> 2)][e & 3], ex);   // exact: the parts add up
+            const float v = x[2 * ks + (e >> 2)][e & 3] * unit;        // exact: the parts add up
             qh[ks][e] = static_cast<_Float16>(v);
             ql[ks][e] = static_cast<_Float16>(v - static_cast<float>(qh[ks][e]));
         }
@@ -297,6 +304,21 @@ __device__ inline void close_columns(const int (&orow)[NB], const float (&c)[NB]
     }
 }
 
+// The flagged columns of a block, key by key; their values are stored at once.
+template <typename CT, int KS>
+__device__ inline void redo_columns(const AttnParams & p, const int32_t * table, int head, int split, int lane, int lim, int orow,
+                                    uint32_t redo, int step_lo, int step_hi) {
+    for (uint32_t left = redo; left != 0; left &= left - 1) {
+        const int col = __ffs(left) - 1;
+        const int row = __builtin_amdgcn_readlane(orow, col), lm = __builtin_amdgcn_readlane(lim, col);
+        float cm, cl;
+        f2 co;
+        column_by_keys<CT, KS>(p, table, head, p.q + static_cast<int64_t>(row) * kHeadDim, lm, step_lo, step_hi, 1, lane, cm, cl, co);
+        const f2 nx = f2{__shfl_down(co[0], 1, kWave), __shfl_down(co[1], 1, kWave)};
+        if ((lane & 1) == 0) store_column(p, table, split, row, lm, 2 * lane, f4{co[0], co[1], nx[0], nx[1]}, cm, cl, lane == 0);
+    }
+}
+
 // Stores the columns of a wave that holds all of a split's steps.
 template <typename CT, int NB, int KS>
 __device__ inline void store_columns(const AttnParams & p, const int32_t * table, int head, int split, int lane, const int (&lim)[NB],
@@ -318,15 +340,7 @@ __device__ inline void store_columns(const AttnParams & p, const int32_t * table
                 store_column(p, table, split, orow[nb], lim[nb], (g4 * 4 + i) * 8 + 4, b, mc[nb], l[nb], false);
             }
         }
-        for (uint32_t left = redo[nb]; left != 0; left &= left - 1) {
-            const int col = __ffs(left) - 1;
-            const int row = __builtin_amdgcn_readlane(orow[nb], col), lm = __builtin_amdgcn_readlane(lim[nb], col);
-            float cm, cl;
-            f2 co;
-            column_by_keys<CT, KS>(p, table, head, p.q + static_cast<int64_t>(row) * kHeadDim, lm, step_lo, step_hi, 1, lane, cm, cl, co);
-            const f2 nx = f2{__shfl_down(co[0], 1, kWave), __shfl_down(co[1], 1, kWave)};
-            if ((lane & 1) == 0) store_column(p, table, split, row, lm, 2 * lane, f4{co[0], co[1], nx[0], nx[1]}, cm, cl, lane == 0);
-        }
+        redo_columns<CT, KS>(p, table, head, split, lane, lim[nb], orow[nb], redo[nb], step_lo, step_hi);
     }
 }
 
@@ -378,7 +392,9 @@ __global__ __launch_bounds__(kWave * WC * WK, NB == 1 ? 3 : 2) void paged_attn_k
         orow[nb] = ok ? (tl.row0 + t) * p.n_heads + head * p.group + h : -1;
         const float * qp = p.q + (static_cast<int64_t>(tl.row0 + t) * p.n_heads + head * p.group + h) * kHeadDim;
         if constexpr (F16) {
-            split_q(qp, ok, g4, p.scale, c[nb], qh[nb], ql[nb]);
+            f4 x[8];
+            load_q(qp, ok, g4, x);
+            split_q(x, p.scale, c[nb], qh[nb], ql[nb]);
             if constexpr (PACK) {
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) qh[nb][ks] = c16 < 8 ? qh[nb][ks] : ql[nb][ks];
@@ -643,15 +659,18 @@ __global__ __launch_bounds__(kWave * WC * WK, NB == 1 ? 3 : 2) void paged_attn_k
     }
 }
 
-// The kernel of long chunks on f16 pages: 8 waves of 32 columns each share the K and V of a tile through LDS, which cuts
-// what the CUs pull from L2 to an eighth (without it that traffic sets the pace).  A tile is 128 keys, four steps of 32; a
+// The kernel of long chunks on f16 pages: 4 waves of 32 columns each share the K and V of a tile through LDS, which cuts
+// what the CUs pull from L2 to a quarter (without it that traffic sets the pace).  A tile is 64 keys, two steps of 32; a
 // step lies in LDS as the MFMA operands themselves, 8 of K and 8 of V^T, 64 lanes x 16 bytes each: every read and write is
-// one unbroken kilobyte and no wave rearranges anything.  Wave w < 4 fetches and transposes V of step w, wave 4 + w fetches
-// K.  Two tiles in LDS, the next one's rows in registers: one barrier per tile.
-constexpr int kTileSteps = 4;
-constexpr int kTileWaves = 8, kTileColumns = kTileWaves * 32;
+// one unbroken kilobyte and no wave rearranges anything.  Waves 0 and 1 fetch and transpose V of the two steps, waves 2 and
+// 3 fetch K.  Two tiles in LDS, the next one's rows in registers: one barrier per tile, and two workgroups per CU, each
+// multiplying while the other waits at its barrier.
+constexpr int kTileSteps = 2;
+constexpr int kTileWaves = 2 * kTileSteps, kTileColumns = kTileWaves * 32;
 constexpr int kStepHalfs = 16 * kWave * 8;   // a step's 16 operands
 constexpr size_t kTileLds = 2 * kTileSteps * kStepHalfs * sizeof(_Float16);
+constexpr int kOutStride = kHeadDim + 4, kOutFloats = 16 * kOutStride;   // a wave's 16 columns on their way out
+static_assert(kTileWaves * kOutFloats * sizeof(float) <= kTileLds, "the outputs go through the operands' LDS");
 
 __global__ __launch_bounds__(kTileWaves * kWave, 2) void paged_attn_tile_kernel(AttnParams p) {
     constexpr int NB = 2;
@@ -676,25 +695,48 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void paged_attn_tile_kernel(
     if (split > 0 && step_lo >= n_steps) return;                      // uniform for the workgroup
     const int in_page = (1 << p.page_shift) - 1;
 
+    // columns: their q is on its way while the first tile is fetched
+    int lim[NB], orow[NB];
+    f4 x[NB][8];
+    int wave_lim = -1, wave_first = 1 << 30;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const int col = col0 + wave * 32 + nb * 16 + c16;
+        const bool ok = col < n_cols;
+        const int t = ok ? col / p.group : t_last;
+        const int h = ok ? col - t * p.group : 0;
+        lim[nb] = ok ? min(tl.past + t, cap - 1) : -1;
+        orow[nb] = ok ? (tl.row0 + t) * p.n_heads + head * p.group + h : -1;
+        load_q(p.q + (static_cast<int64_t>(tl.row0 + t) * p.n_heads + head * p.group + h) * kHeadDim, ok, g4, x[nb]);
+    }
+    {
+        // keys that the wave's last and first token see (its columns are in order of token)
+        const int first_col = col0 + wave * 32, last_col = min(first_col + 32, n_cols) - 1;
+        if (first_col < n_cols) {
+            wave_first = min(tl.past + first_col / p.group, cap - 1);
+            wave_lim = min(tl.past + last_col / p.group, cap - 1);
+        }
+    }
+    const int wave_steps = min(step_hi, (wave_lim + 32) / 32);        // steps behind it hold nothing that the wave sees
+    const int full = max(0, wave_first + 1) / 32;
+
     // this wave's share of a tile: step `wave % 4`, V (waves 0..3) or K
     const bool fetch_v = wave < kTileSteps;
     u4 r[8];
     int pg[2];
     __shared__ int s_holes[2][kTileSteps];                            // bit kb: 16-key block kb of the step lies on no page
-    auto pages_of = [&](int st, int (&out)[2]) {
+    // table entries of a step's two 16-key blocks as they are, looked at when they have arrived
+    auto entries_of = [&](int st, int (&out)[2]) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const int j = st * 32 + kb * 16;
-            out[kb] = j < kend ? page_of(table, p.seqs.table_stride, p.page_shift, p.n_pages, j) : -1;
-        }
+        for (int kb = 0; kb < 2; ++kb) out[kb] = table[min((st * 32 + kb * 16) >> p.page_shift, p.seqs.table_stride - 1)];
     };
     int st_held = 0;
     auto fetch = [&](int st, const int (&from)[2]) {
         st_held = st;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-            pg[kb] = from[kb];
-            const _Float16 * base = page_rows<_Float16>(p, fetch_v ? 1 : 0, max(from[kb], 0), head) +
+            pg[kb] = st * 32 + kb * 16 < kend && from[kb] >= 0 && from[kb] < p.n_pages ? from[kb] : -1;
+            const _Float16 * base = page_rows<_Float16>(p, fetch_v ? 1 : 0, max(pg[kb], 0), head) +
                                     static_cast<int64_t>((st * 32 + kb * 16) & in_page) * kHeadDim;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -733,38 +775,15 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void paged_attn_tile_kernel(
     const int n_tiles = (step_hi - step_lo + kTileSteps - 1) / kTileSteps;
     int pg_next[2];
     if (n_tiles > 0) {
-        pages_of(step_lo + mine, pg_next);
+        entries_of(step_lo + mine, pg_next);
         fetch(step_lo + mine, pg_next);
-        pages_of(step_lo + kTileSteps + mine, pg_next);
+        entries_of(step_lo + kTileSteps + mine, pg_next);
     }
 
-    // columns
-    int lim[NB], orow[NB];
     float c[NB];
     h8 qh[NB][4], ql[NB][4];
-    int wave_lim = -1, wave_first = 1 << 30;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        const int col = col0 + wave * 32 + nb * 16 + c16;
-        const bool ok = col < n_cols;
-        const int t = ok ? col / p.group : t_last;
-        const int h = ok ? col - t * p.group : 0;
-        lim[nb] = ok ? min(tl.past + t, cap - 1) : -1;
-        orow[nb] = ok ? (tl.row0 + t) * p.n_heads + head * p.group + h : -1;
-        const float * qp = p.q + (static_cast<int64_t>(tl.row0 + t) * p.n_heads + head * p.group + h) * kHeadDim;
-        split_q(qp, ok, g4, p.scale, c[nb], qh[nb], ql[nb]);
-    }
-    {
-        // keys that the wave's last and first token see (its columns are in order of token)
-        const int first_col = col0 + wave * 32, last_col = min(first_col + 32, n_cols) - 1;
-        if (first_col < n_cols) {
-            wave_first = min(tl.past + first_col / p.group, cap - 1);
-            wave_lim = min(tl.past + last_col / p.group, cap - 1);
-        }
-    }
-    const int wave_steps = min(step_hi, (wave_lim + 32) / 32);        // steps behind it hold nothing that the wave sees
-    const int full = max(0, wave_first + 1) / 32;
-
+    for (int nb = 0; nb < NB; ++nb) split_q(x[nb], p.scale, c[nb], qh[nb], ql[nb]);
     float m[NB], l[NB];
     f4 O[NB][8];
 #pragma unroll
@@ -777,7 +796,7 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void paged_attn_tile_kernel(
     if (n_tiles > 0) {
         put(0);
         fetch(step_lo + kTileSteps + mine, pg_next);
-        pages_of(step_lo + 2 * kTileSteps + mine, pg_next);
+        entries_of(step_lo + 2 * kTileSteps + mine, pg_next);
     }
     __syncthreads();
     for (int tile = 0; tile < n_tiles; ++tile) {
@@ -843,7 +862,7 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void paged_attn_tile_kernel(
             put((tile + 1) & 1);
             if (tile + 2 < n_tiles) {
                 fetch(st0 + 2 * kTileSteps + mine, pg_next);
-                pages_of(st0 + 3 * kTileSteps + mine, pg_next);
+                entries_of(st0 + 3 * kTileSteps + mine, pg_next);
             }
         }
         __syncthreads();
@@ -851,7 +870,30 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void paged_attn_tile_kernel(
     float mc[NB];
     uint32_t redo[NB];
     close_columns<NB, false>(orow, c, m, l, O, mc, redo);
-    store_columns<_Float16, NB, 32>(p, table, head, split, lane, lim, orow, mc, l, O, redo, step_lo, step_hi);
+    // through the wave's own part of LDS, so that a store instruction writes two whole rows; a lane's values would lie 16 bytes
+    // in each of 64 lines
+    float * so = reinterpret_cast<float *>(lds_kv) + wave * kOutFloats;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        float * to = so + c16 * kOutStride + g4 * 32;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                *reinterpret_cast<f4 *>(to + i * 8 + h * 4) = f4{O[nb][4 * h][i], O[nb][4 * h + 1][i], O[nb][4 * h + 2][i], O[nb][4 * h + 3][i]};
+            }
+        }
+        // lane -> column 2 i + lane / 32, dims 4 (lane % 32) ..; what belongs to a column comes from its lane
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int col = 2 * i + (lane >> 5), dim = (lane & 31) * 4;
+            const int row = __shfl(orow[nb], col, kWave), lm = __shfl(lim[nb], col, kWave);
+            const float cm = __shfl(mc[nb], col, kWave), cl = __shfl(l[nb], col, kWave);
+            const f4 v = *reinterpret_cast<const f4 *>(so + col * kOutStride + dim);
+            if (row >= 0 && !((redo[nb] >> col) & 1)) store_column(p, table, split, row, lm, dim, v, cm, cl, dim == 0);
+        }
+        redo_columns<_Float16, 32>(p, table, head, split, lane, lim[nb], orow[nb], redo[nb], step_lo, step_hi);
+    }
 }
 
 // Joins the splits of each (row, head): one wave each, lane = split for the weights, then lane = 2 dims.  Its time is
@@ -923,7 +965,7 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     const int64_t len = std::min<int64_t>(cap, b.max_len > 0 ? b.max_len : cap);
     const int steps = static_cast<int>((len + ks - 1) / ks);
     const int64_t tiles = pl.many_cols ? std::max<int64_t>(1, (cols + pl.many_cols - 1) / pl.many_cols) : pl.tiles_few;
-    const int64_t target = pl.many_cols == kTileColumns ? 256 : pl.many_cols ? 1024 : 1024, least = pl.many_cols == kTileColumns ? 4 : 8;
+    const int64_t target = pl.many_cols == kTileColumns ? 512 : 1024, least = pl.many_cols == kTileColumns ? 4 : 8;
     int64_t splits = std::max<int64_t>(1, std::min<int64_t>({target / std::max<int64_t>(tiles * l.n_kv_heads, 1), (steps + least - 1) / least, kMaxSplits}));
     const size_t per_split = static_cast<size_t>(b.n_rows) * n_heads * (kHeadDim + 2) * sizeof(float);
     if (splits > 1 && per_split * splits > workspace_bytes) splits = std::max<int64_t>(1, static_cast<int64_t>(workspace_bytes / per_split));
