@@ -4,7 +4,9 @@
 //
 // in one pass over the keys with a running maximum m and sum (the accumulators are rescaled when m grows).  The query
 // heads of a KV head and the tokens of a sequence are columns of the same products: column c of a tile is token c / group
-// and head c % group, so one token of 2 heads and a chunk of a thousand run the same code.
+// and head c % group, so one token of 2 heads and a chunk of a thousand run the same code, in two shapes: up to 64 columns
+// a workgroup takes 16 of them (8 in the packed form) and its 4 waves share the keys (attn_rows); of longer chunks it
+// takes 128, 32 per wave, and the waves share K and V (attn_tile).  A batch of both kinds is one launch.
 //
 // f16 pages on v_mfma_f32_16x16x32_f16: q and p are f32, split into two f16 parts each (a power of two per column brings
 // the largest |q| to 2^14..2^15, p is scaled by 2^6, so the second part keeps its bits); K and V are exact f16.  What the
@@ -42,9 +44,11 @@ constexpr float kLazyLog2 = 8.0f;    // the reference maximum follows when it is
 constexpr float kShiftLog2 = 6.0f;   // p is scaled by 2^6: at most 2^14 in f16, and its second part stays normal
 constexpr int kQExp = 15;            // a column's largest |q| goes to [2^14, 2^15)
 constexpr int kMaxSplits = 64;       // key ranges whose results the joining kernel adds, one lane each
-// (token, head) columns of a sequence up to which the kernel of few columns takes it: one 16-column product, which on
-// f16 pages carries 8 columns in two parts
+constexpr int kWaves = 4, kThreads = kWaves * kWave;
+constexpr int kMidCols = 64;         // columns of a sequence up to which attn_rows takes it
+// Sequences of few columns: a workgroup holds all of them.  On f16 pages 8 columns lie in both parts in one product.
 constexpr int few_cols(bool f16) { return f16 ? 8 : 16; }
+constexpr int step_keys(bool f16) { return f16 ? 32 : 16; }   // 8 KB of K and 8 KB of V
 
 struct AttnParams {
     const float * q;
@@ -54,9 +58,9 @@ struct AttnParams {
     f2 * part_ml;         // [rows * heads][n_splits]: reference maximum (log2 units) and sum
     PagedSeqs seqs;
     int32_t n_heads, n_kv, group, n_pages, page_shift, layer;
-    int32_t n_tiles;      // upper bound of the tiles of the sequences this launch takes
+    int32_t few_max;      // sequences of at most so many columns are of few columns
+    int32_t tiles_many, tiles_few;   // upper bounds of both kinds of tiles
     int32_t n_splits, split_steps;
-    int32_t few_max;      // sequences of at most so many columns are the few-column kernel's
     float scale;
 };
 
@@ -78,15 +82,25 @@ __device__ inline float column_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// A tile: a sequence and its columns [col0, col0 + R).
+// A tile of the batch: a sequence, its first column, and what its keys are.
 struct Tile {
-    int seq, rows, row0, past, tile, n_tiles;
+    const int32_t * table;
+    int rows, row0, past;     // the sequence's new tokens, the first one's row and position
+    int col0, n_cols;         // the tile's first column, the sequence's columns
+    int cap, kend;            // positions of the table row; keys that the tile's last token sees
+    int n_steps, step_lo, step_hi;   // steps of kend, and those of this split
 };
 
-// Tile number -> sequence: every lane counts one sequence's tiles, a prefix sum over the wave finds the one that holds
-// the tile.  few: the sequences of 1..few_max columns, otherwise the longer ones.
-template <int R, bool FEW>
-__device__ inline Tile find_tile(const AttnParams & p, int tile, int lane) {
+// Block -> (KV head, split, tile); false: nothing to do.  Neighbouring blocks, which go to different XCDs, take different heads.
+// Every lane counts one sequence's tiles, a prefix sum over the wave finds the sequence that holds the tile; what the tile
+// needs is read along.  FEW: the sequences of 1 .. few_max columns, otherwise the longer ones.
+template <int R, int KS, bool FEW>
+__device__ inline bool find_tile(const AttnParams & p, int block, int lane, Tile & t, int & head, int & split) {
+    const int n_tiles = FEW ? p.tiles_few : p.tiles_many;
+    head = block % p.n_kv;
+    const int rest = block / p.n_kv;
+    split = rest / n_tiles;
+    int tile = rest - split * n_tiles;
     for (int s0 = 0; s0 < p.seqs.n_seqs; s0 += kWave) {
         const int s = s0 + lane;
         int n = 0, rows = 0, start = 0, past = 0;
@@ -94,8 +108,8 @@ __device__ inline Tile find_tile(const AttnParams & p, int tile, int lane) {
             start = p.seqs.row_start[s];
             past = p.seqs.n_past[s];
             rows = rows_between(start, p.seqs.row_start[s + 1], p.seqs.n_rows);
-            const bool few = static_cast<int64_t>(rows) * p.group <= p.few_max;
-            if (rows > 0 && few == FEW) n = FEW ? 1 : static_cast<int>((static_cast<int64_t>(rows) * p.group + R - 1) / R);
+            const bool few = rows * p.group <= p.few_max;
+            if (rows > 0 && few == FEW) n = FEW ? 1 : (rows * p.group + R - 1) / R;
         }
         int sum = n;
 #pragma unroll
@@ -103,21 +117,58 @@ __device__ inline Tile find_tile(const AttnParams & p, int tile, int lane) {
             const int o = __shfl_up(sum, d, kWave);
             if (lane >= d) sum += o;
         }
-        const uint64_t past_it = __ballot(sum > tile);
-        if (past_it != 0) {
-            const int l = __ffsll(static_cast<unsigned long long>(past_it)) - 1;
-            Tile t;
-            t.seq = __builtin_amdgcn_readfirstlane(s0 + l);
-            t.n_tiles = __builtin_amdgcn_readlane(n, l);
-            t.tile = tile - (__builtin_amdgcn_readlane(sum, l) - t.n_tiles);
+        const uint64_t holds = __ballot(sum > tile);
+        if (holds != 0) {
+            const int l = __ffsll(static_cast<unsigned long long>(holds)) - 1;
+            const int count = __builtin_amdgcn_readlane(n, l), before = __builtin_amdgcn_readlane(sum, l) - count;
+            t.table = p.seqs.tables + static_cast<int64_t>(s0 + l) * p.seqs.table_stride;
             t.rows = __builtin_amdgcn_readlane(rows, l);
             t.row0 = __builtin_amdgcn_readlane(start, l);
             t.past = bounded_past(__builtin_amdgcn_readlane(past, l));
-            return t;
+            t.col0 = (count - 1 - (tile - before)) * R;               // the last tile has the most keys: first
+            t.n_cols = t.rows * p.group;
+            t.cap = p.seqs.table_stride << p.page_shift;
+            t.kend = max(0, min(t.past + (min(t.col0 + R, t.n_cols) - 1) / p.group, t.cap - 1) + 1);
+            t.n_steps = (t.kend + KS - 1) / KS;
+            t.step_lo = split * p.split_steps;
+            t.step_hi = split == p.n_splits - 1 ? t.n_steps : min(t.n_steps, t.step_lo + p.split_steps);
+            return split == 0 || t.step_lo < t.n_steps;               // the first split answers for rows without keys
         }
         tile -= __builtin_amdgcn_readlane(sum, kWave - 1);
     }
-    return Tile{-1, 0, 0, 0, 0, 0};
+    return false;
+}
+
+// A column: its output row (token and head; -1: none), the last position it sees and its q.
+struct Column {
+    int row, lim;
+    const float * q;
+};
+
+__device__ inline Column column_of(const AttnParams & p, const Tile & t, int head, int col) {
+    const bool ok = col < t.n_cols;
+    const int token = (ok ? col : t.n_cols - 1) / p.group;
+    const int row = (t.row0 + token) * p.n_heads + head * p.group + (ok ? col - token * p.group : 0);
+    return Column{ok ? row : -1, ok ? min(t.past + token, t.cap - 1) : -1, p.q + static_cast<int64_t>(row) * kHeadDim};
+}
+
+// The K and V rows of one KV head: page + page_elems per page, V v_elems behind K.
+template <typename CT>
+struct HeadRows {
+    const CT * k;
+    int64_t page_elems, v_elems;
+    __device__ inline HeadRows(const AttnParams & p, int head) {
+        const int64_t rows = static_cast<int64_t>(1) << p.page_shift;
+        page_elems = p.n_kv * rows * kHeadDim;
+        v_elems = p.n_pages * page_elems;
+        k = static_cast<const CT *>(p.pages) + 2 * p.layer * v_elems + head * rows * kHeadDim;
+    }
+    __device__ inline const CT * page(int page) const { return k + page * page_elems; }
+};
+
+// A table entry as the page of the 16 keys from j on, -1 for none.
+__device__ inline int entry_page(const AttnParams & p, const Tile & t, int entry, int j) {
+    return j < t.kend && entry >= 0 && entry < p.n_pages ? entry : -1;
 }
 
 // Whether any position up to lim lies on a page.
@@ -134,11 +185,6 @@ __device__ inline float inverse_sum(const AttnParams & p, const int32_t * table,
     return 1.0f / l;
 }
 
-template <typename CT>
-__device__ inline const CT * page_rows(const AttnParams & p, int kv, int page, int head) {
-    return static_cast<const CT *>(p.pages) + cache_row_offset(p.layer, kv, page, head, 0, p.n_pages, p.n_kv, 1 << p.page_shift);
-}
-
 // One column over the visible keys of steps step0, step0 + step_inc, .. < step1, in f32, key by key: lane holds dims
 // 2 lane and 2 lane + 1.  m in log2 units.
 template <typename CT, int KS>
@@ -146,6 +192,7 @@ __device__ inline void column_by_keys(const AttnParams & p, const int32_t * tabl
                                       int step1, int step_inc, int lane, float & m, float & l, f2 & o) {
     const f2 qv = *reinterpret_cast<const f2 *>(q + 2 * lane);
     const float c = p.scale * kLog2e;
+    const HeadRows<CT> rows(p, head);
     m = -INFINITY;
     l = 0.0f;
     o = f2{0.0f, 0.0f};
@@ -154,8 +201,8 @@ __device__ inline void column_by_keys(const AttnParams & p, const int32_t * tabl
             const int page = page_of(table, p.seqs.table_stride, p.page_shift, p.n_pages, j);
             if (page < 0) continue;
             const int64_t at = static_cast<int64_t>(j & ((1 << p.page_shift) - 1)) * kHeadDim + 2 * lane;
-            const CT * k = page_rows<CT>(p, 0, page, head) + at;
-            const CT * v = page_rows<CT>(p, 1, page, head) + at;
+            const CT * k = rows.page(page) + at;
+            const CT * v = k + rows.v_elems;
             const float s = wave_sum_all(fmaf(qv[0], static_cast<float>(k[0]), qv[1] * static_cast<float>(k[1]))) * c;
             const float mn = fmaxf(m, s);
             const float ref = mn == -INFINITY ? 0.0f : mn;
@@ -168,28 +215,91 @@ __device__ inline void column_by_keys(const AttnParams & p, const int32_t * tabl
     }
 }
 
-// A step's K and V in registers, and whether each 16-key block of it lies on a page.
-template <typename CT>
-struct StepRegs;
-template <>
-struct StepRegs<_Float16> {
-    u4 k[2][4];   // [key block][32 dims]: key l % 16, dims 32 ks + 8 (l / 16) ..
-    u4 v[8];      // key 16 kb + 4 (l / 16) + i at [4 kb + i], dims 8 (l % 16) ..
-};
-template <>
-struct StepRegs<float> {
-    f4 k[8];      // key l % 16, dims 16 t + 4 (l / 16) ..
-    f4 v[4][2];   // key 4 (l / 16) + i, dims 8 (l % 16) ..
-};
-
-// A column's q in MFMA order (dims 32 ks + 8 (l / 16) .. at [2 ks]); columns that do not exist are zeros.
-__device__ inline void load_q(const float * qp, bool ok, int g4, f4 (&x)[8]) {
+// A column's q in MFMA order: f16 pages dims 32 ks + 8 (l / 16) .. at [2 ks], f32 pages dims 16 i + 4 (l / 16) .. at [i].
+// Columns that do not exist are zeros.
+template <bool F16>
+__device__ inline void load_q(const Column & col, int g4, f4 (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        x[i] = *reinterpret_cast<const f4 *>(qp + (i >> 1) * 32 + g4 * 8 + (i & 1) * 4);
-        if (!ok) x[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        x[i] = *reinterpret_cast<const f4 *>(col.q + (F16 ? (i >> 1) * 32 + g4 * 8 + (i & 1) * 4 : i * 16 + g4 * 4));
+        if (col.row < 0) x[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 }
+
+// A step of scores S^T = K Q^T from its 8 K operands.  Q: the two parts on f16 pages (the packed form has both in the first),
+// the values themselves on f32 pages.
+template <bool F16, bool PACK, int NB>
+__device__ inline void scores_step(const u4 (&a)[8], const h8 (&qh)[NB][4], const h8 (&ql)[NB][4], const f4 (&x)[NB][8],
+                                   f4 (&S)[NB][F16 ? 2 : 1]) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int kb = 0; kb < (F16 ? 2 : 1); ++kb) S[nb][kb] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    if constexpr (F16) {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+#pragma unroll
+            for (int part = 0; part < (PACK ? 1 : 2); ++part) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        S[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a[kb * 4 + ks]), part ? ql[nb][ks] : qh[nb][ks],
+                                                                           S[nb][kb], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    S[nb][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, a[i])[e], x[nb][i][e], S[nb][0], 0, 0, 0);
+                }
+            }
+        }
+    }
+}
+
+// -inf where a key lies behind the column's last position or on no page (bit kb of holes: the 16-key block kb).
+template <int NB, int KB>
+__device__ inline void mask_step(f4 (&S)[NB][KB], const int (&lim)[NB], int key0, int g4, int holes) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (key0 + kb * 16 + g4 * 4 + i > lim[nb] || ((holes >> kb) & 1)) S[nb][kb][i] = -INFINITY;
+            }
+        }
+    }
+}
+
+// V^T operand db of a step's f16 rows: dims 8 r + db, two keys per register.
+__device__ inline u4 transposed(const u4 (&v)[8], int db) {
+    u4 a;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        a[w] = db & 1 ? hi_pair(v[2 * w][db >> 1], v[2 * w + 1][db >> 1]) : lo_pair(v[2 * w][db >> 1], v[2 * w + 1][db >> 1]);
+    }
+    return a;
+}
+
+// Element offset of operand f of a step inside its 16-key block, and that block.  K: key l % 16, dims as q's.  V on f16 pages:
+// key 16 (f / 4) + 4 (l / 16) + f % 4, dims 8 (l % 16) ..; on f32 pages key 4 (l / 16) + f / 2, dims 8 (l % 16) + 4 (f % 2) ...
+template <bool F16>
+__device__ inline int k_offset(int f, int c16, int g4) { return c16 * kHeadDim + (F16 ? (f & 3) * 32 + g4 * 8 : f * 16 + g4 * 4); }
+template <bool F16>
+__device__ inline int v_offset(int f, int c16, int g4) {
+    return F16 ? (g4 * 4 + (f & 3)) * kHeadDim + c16 * 8 : (g4 * 4 + (f >> 1)) * kHeadDim + c16 * 8 + (f & 1) * 4;
+}
+template <bool F16>
+__device__ inline int v_key(int f, int g4) { return F16 ? (f >> 2) * 16 + g4 * 4 + (f & 3) : g4 * 4 + (f >> 1); }
 
 // Its two f16 parts, c = the score unit in log2 (scale log2 e over the column's power of two).
 __device__ inline void split_q(const f4 (&x)[8], float scale, float & c, h8 (&qh)[4], h8 (&ql)[4]) {
@@ -319,193 +429,93 @@ __device__ inline void redo_columns(const AttnParams & p, const int32_t * table,
     }
 }
 
-// Stores the columns of a wave that holds all of a split's steps.
-template <typename CT, int NB, int KS>
-__device__ inline void store_columns(const AttnParams & p, const int32_t * table, int head, int split, int lane, const int (&lim)[NB],
-                                     const int (&orow)[NB], const float (&mc)[NB], const float (&l)[NB], const f4 (&O)[NB][8],
-                                     const uint32_t (&redo)[NB], int step_lo, int step_hi) {
-    const int c16 = lane & 15, g4 = lane >> 4;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        if (orow[nb] >= 0 && !((redo[nb] >> c16) & 1)) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                f4 a, b;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    a[e] = O[nb][e][i];
-                    b[e] = O[nb][4 + e][i];
-                }
-                store_column(p, table, split, orow[nb], lim[nb], (g4 * 4 + i) * 8, a, mc[nb], l[nb], i == 0 && g4 == 0);
-                store_column(p, table, split, orow[nb], lim[nb], (g4 * 4 + i) * 8 + 4, b, mc[nb], l[nb], false);
-            }
-        }
-        redo_columns<CT, KS>(p, table, head, split, lane, lim[nb], orow[nb], redo[nb], step_lo, step_hi);
-    }
-}
+// Up to 16 columns (FEW on f16 pages: 8, in both parts), whose keys the 4 waves take in turn, step by step, straight from
+// memory into the operands: a decode step is the stream of K and V, and nothing stands between the loads and the products.
+// The waves' results are merged in LDS.
+constexpr int kRowsStride = kHeadDim + 4;
+constexpr int rows_cols(bool f16, bool few) { return f16 && few ? 8 : 16; }
+constexpr size_t rows_lds(bool f16, bool few) { return kWaves * rows_cols(f16, few) * (kRowsStride + 2) * 4 + 2 * rows_cols(f16, few) * 4; }
 
-// The kernel.  NB blocks of 16 columns per wave, WC waves side by side over columns, WK waves over the steps of the keys
-// (merged in LDS).  A step is 32 keys of f16 or 16 keys of f32: 8 KB of K and 8 KB of V either way.
-template <typename CT, int NB, int WC, int WK, bool FEW>
-__global__ __launch_bounds__(kWave * WC * WK, NB == 1 ? 3 : 2) void paged_attn_kernel(AttnParams p) {
-    constexpr bool F16 = std::is_same<CT, _Float16>::value;
-    constexpr bool PACK = FEW && F16;                // one block of 8 columns in two parts
-    static_assert(!FEW || (NB == 1 && WC == 1), "the kernel of few columns has one block of them");
-    constexpr int KS = F16 ? 32 : 16, KB = F16 ? 2 : 1;
-    constexpr int kCols = PACK ? 8 : NB * 16;        // a wave's columns
-    constexpr int R = WC * kCols;                    // the tile's
+template <typename CT, bool FEW>
+__device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
+    constexpr bool F16 = std::is_same<CT, _Float16>::value, PACK = FEW && F16;
+    constexpr int KS = step_keys(F16), KB = KS / 16, R = rows_cols(F16, FEW), NB = 1;
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wc = wave % WC, wk = wave / WC;
     const int c16 = lane & 15, g4 = lane >> 4;
+    Tile t;
+    int head, split;
+    if (!find_tile<R, KS, FEW>(p, block, lane, t, head, split)) return;          // uniform for the workgroup
+    const Column col = column_of(p, t, head, t.col0 + (PACK ? c16 & 7 : c16));
+    f4 x[NB][8];
+    load_q<F16>(col, g4, x[0]);
 
-    // block -> (split, tile, KV head): neighbouring blocks, which go to different XCDs, take different heads
-    const int head = static_cast<int>(blockIdx.x) % p.n_kv;
-    const int rest = static_cast<int>(blockIdx.x) / p.n_kv;
-    const int split = rest / p.n_tiles;
-    const Tile tl = find_tile<R, FEW>(p, rest - split * p.n_tiles, lane);
-    if (tl.seq < 0) return;
-    const int col0 = (tl.n_tiles - 1 - tl.tile) * R;                  // the last tile has the most keys: first
-    const int n_cols = tl.rows * p.group;
-    const int cap = p.seqs.table_stride << p.page_shift;
-    const int32_t * table = p.seqs.tables + static_cast<int64_t>(tl.seq) * p.seqs.table_stride;
-    const int t_first = col0 / p.group, t_last = (min(col0 + R, n_cols) - 1) / p.group;
-    const int kend = max(0, min(tl.past + t_last, cap - 1) + 1);      // keys that the tile's last token sees
-    const int n_steps = (kend + KS - 1) / KS;
-    const int step_lo = split * p.split_steps;
-    const int step_hi = split == p.n_splits - 1 ? n_steps : min(n_steps, step_lo + p.split_steps);
-    if (split > 0 && step_lo >= n_steps) return;                      // uniform for the workgroup
-    const int full = max(0, min(tl.past + t_first, cap - 1) + 1) / KS;   // steps that every column sees whole
-
-    // columns: q in MFMA order, visible keys, output row
-    int lim[NB], orow[NB];
-    float c[NB];
-    h8 qh[F16 ? NB : 1][4], ql[F16 ? NB : 1][4];
-    f4 qf[F16 ? 1 : NB][8];
+    const HeadRows<CT> rows(p, head);
+    const int in_page = (1 << p.page_shift) - 1, last_entry = p.seqs.table_stride - 1;
+    auto entries_of = [&](int st, int (&out)[KB]) {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        const int col = col0 + wc * kCols + nb * 16 + (PACK ? c16 & 7 : c16);
-        const bool ok = col < n_cols;
-        const int t = ok ? col / p.group : t_last;
-        const int h = ok ? col - t * p.group : 0;
-        lim[nb] = ok ? min(tl.past + t, cap - 1) : kend - 1;
-        orow[nb] = ok ? (tl.row0 + t) * p.n_heads + head * p.group + h : -1;
-        const float * qp = p.q + (static_cast<int64_t>(tl.row0 + t) * p.n_heads + head * p.group + h) * kHeadDim;
-        if constexpr (F16) {
-            f4 x[8];
-            load_q(qp, ok, g4, x);
-            split_q(x, p.scale, c[nb], qh[nb], ql[nb]);
-            if constexpr (PACK) {
+        for (int kb = 0; kb < KB; ++kb) out[kb] = t.table[min((st * KS + kb * 16) >> p.page_shift, last_entry)];
+    };
+    u4 rk[8], rv[8];
+    int pg[KB], pg_next[KB], entry[KB];
+    const CT * at[KB];
+    // a block on no page reads page 0, which there always is, and is masked
+    auto place = [&](int st) {
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) qh[nb][ks] = c16 < 8 ? qh[nb][ks] : ql[nb][ks];
-            }
-        } else {
-            c[nb] = p.scale * kLog2e;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                qf[nb][i] = *reinterpret_cast<const f4 *>(qp + i * 16 + g4 * 4);
-                if (!ok) qf[nb][i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
+        for (int kb = 0; kb < KB; ++kb) {
+            pg_next[kb] = entry_page(p, t, entry[kb], st * KS + kb * 16);
+            at[kb] = rows.page(max(pg_next[kb], 0)) + ((st * KS + kb * 16) & in_page) * kHeadDim;
         }
+    };
+    auto load_k = [&]() {
+#pragma unroll
+        for (int f = 0; f < 8; ++f) rk[f] = *reinterpret_cast<const u4 *>(at[F16 ? f >> 2 : 0] + k_offset<F16>(f, c16, g4));
+    };
+    auto load_v = [&]() {
+#pragma unroll
+        for (int f = 0; f < 8; ++f) rv[f] = *reinterpret_cast<const u4 *>(at[F16 ? f >> 2 : 0] + rows.v_elems + v_offset<F16>(f, c16, g4));
+    };
+    int st = t.step_lo + wave;
+    if (st < t.step_hi) {
+        entries_of(st, entry);
+        place(st);
+        load_k();
+        load_v();
+        entries_of(st + kWaves, entry);
     }
 
-    float m[NB], l[NB];
+    float c[NB];
+    h8 qh[NB][4], ql[NB][4];
+    if constexpr (F16) {
+        split_q(x[0], p.scale, c[0], qh[0], ql[0]);
+        if constexpr (PACK) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) qh[0][ks] = c16 < 8 ? qh[0][ks] : ql[0][ks];
+        }
+    } else {
+        c[0] = p.scale * kLog2e;
+    }
+    const int lim[NB] = {col.lim}, orow[NB] = {col.row};
+    const int full = max(0, min(t.past + t.col0 / p.group, t.cap - 1) + 1) / KS;   // steps that every column sees whole
+    float m[NB] = {-INFINITY}, l[NB] = {0.0f};
     f4 O[NB][8];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        m[nb] = -INFINITY;
-        l[nb] = 0.0f;
-#pragma unroll
-        for (int db = 0; db < 8; ++db) O[nb][db] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int db = 0; db < 8; ++db) O[0][db] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    // the page of each 16-key block of a step, -1 for none (uniform)
-    auto pages_of = [&](int st, int (&pg)[KB]) {
+    for (; st < t.step_hi; st += kWaves) {
+        int holes = 0;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-            const int j = st * KS + kb * 16;
-            pg[kb] = j < kend ? page_of(table, p.seqs.table_stride, p.page_shift, p.n_pages, j) : -1;
+            pg[kb] = pg_next[kb];
+            holes |= pg[kb] < 0 ? 1 << kb : 0;
         }
-    };
-    const int in_page = (1 << p.page_shift) - 1;
-    StepRegs<CT> r;
-    auto load_k = [&](int st, const int (&pg)[KB]) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            // a block on no page reads page 0, which there always is, and is masked
-            const CT * base = page_rows<CT>(p, 0, max(pg[kb], 0), head) + static_cast<int64_t>((st * KS + kb * 16) & in_page) * kHeadDim;
-            if constexpr (F16) {
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) r.k[kb][ks] = *reinterpret_cast<const u4 *>(base + c16 * kHeadDim + ks * 32 + g4 * 8);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) r.k[i] = *reinterpret_cast<const f4 *>(base + c16 * kHeadDim + i * 16 + g4 * 4);
-            }
-        }
-    };
-    auto load_v = [&](int st, const int (&pg)[KB]) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            const CT * base = page_rows<CT>(p, 1, max(pg[kb], 0), head) + static_cast<int64_t>((st * KS + kb * 16) & in_page) * kHeadDim;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const CT * v = base + (g4 * 4 + i) * kHeadDim + c16 * 8;
-                if constexpr (F16) {
-                    r.v[kb * 4 + i] = *reinterpret_cast<const u4 *>(v);
-                } else {
-                    r.v[i][0] = *reinterpret_cast<const f4 *>(v);
-                    r.v[i][1] = *reinterpret_cast<const f4 *>(v + 4);
-                }
-            }
-        }
-    };
-
-    int st = step_lo + wk;
-    int pg[KB], pg_next[KB];
-    if (st < step_hi) {
-        pages_of(st, pg);
-        load_k(st, pg);
-        load_v(st, pg);
-        pages_of(min(st + WK, n_steps - 1), pg_next);
-    }
-    for (; st < step_hi; st += WK) {
-        const bool more = st + WK < step_hi;
-        bool hole = false;
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) hole = hole || pg[kb] < 0;
-
+        const bool more = st + kWaves < t.step_hi;
         f4 S[NB][KB];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                S[nb][kb] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
+        scores_step<F16, PACK, NB>(rk, qh, ql, x, S);
+        if (more) {
+            place(st + kWaves);
+            load_k();
         }
-        if constexpr (F16) {
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    const h8 a = __builtin_bit_cast(h8, r.k[kb][ks]);
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        S[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[nb][ks], S[nb][kb], 0, 0, 0);
-                        if constexpr (!PACK) S[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[nb][ks], S[nb][kb], 0, 0, 0);
-                    }
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) S[nb][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(r.k[i][e], qf[nb][i][e], S[nb][0], 0, 0, 0);
-                }
-            }
-        }
-        if (more) load_k(st + WK, pg_next);
         if constexpr (PACK) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
@@ -513,277 +523,209 @@ __global__ __launch_bounds__(kWave * WC * WK, NB == 1 ? 3 : 2) void paged_attn_k
                 for (int i = 0; i < 4; ++i) S[0][kb][i] += row_ror8(S[0][kb][i]);
             }
         }
-        if (st >= full || hole) {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (st * KS + kb * 16 + g4 * 4 + i > lim[nb] || pg[kb] < 0) S[nb][kb][i] = -INFINITY;
-                    }
-                }
-            }
-        }
-
+        if (st >= full || holes != 0) mask_step<NB, KB>(S, lim, st * KS, g4, holes);
         float pr[NB][KB][4];
         softmax_step<NB, KB>(S, c, m, l, O, pr);
 
         // rows of keys that no column sees, and of no page, are whatever memory holds: not even 0 times that
-        if (st * KS + KS > kend || hole) {
-            if constexpr (F16) {
+        if (st * KS + KS > t.kend || holes != 0) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (st * KS + (e >> 2) * 16 + g4 * 4 + (e & 3) >= kend || pg[e >> 2] < 0) r.v[e] = u4{0, 0, 0, 0};
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (st * KS + g4 * 4 + i >= kend || pg[0] < 0) r.v[i][0] = r.v[i][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-                }
+            for (int f = 0; f < 8; ++f) {
+                if (st * KS + v_key<F16>(f, g4) >= t.kend || pg[F16 ? f >> 2 : 0] < 0) rv[f] = u4{0, 0, 0, 0};
             }
         }
         if constexpr (F16) {
-            h8 ph[NB], pl[NB];
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                split_p(pr[nb], ph[nb], pl[nb]);
-                if constexpr (PACK) ph[nb] = c16 < 8 ? ph[nb] : pl[nb];
-            }
+            h8 ph, pl;
+            split_p(pr[0], ph, pl);
+            if constexpr (PACK) ph = c16 < 8 ? ph : pl;
 #pragma unroll
             for (int db = 0; db < 8; ++db) {
-                u4 a;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t x = r.v[2 * w][db >> 1], y = r.v[2 * w + 1][db >> 1];
-                    a[w] = db & 1 ? hi_pair(x, y) : lo_pair(x, y);
-                }
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    O[nb][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), ph[nb], O[nb][db], 0, 0, 0);
-                    if constexpr (!PACK) O[nb][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), pl[nb], O[nb][db], 0, 0, 0);
-                }
+                const h8 a = __builtin_bit_cast(h8, transposed(rv, db));
+                O[0][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, O[0][db], 0, 0, 0);
+                if constexpr (!PACK) O[0][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, O[0][db], 0, 0, 0);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int f = 0; f < 8; ++f) {
 #pragma unroll
-                for (int db = 0; db < 8; ++db) {
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        O[nb][db] = __builtin_amdgcn_mfma_f32_16x16x4f32(r.v[i][db >> 2][db & 3], pr[nb][0][i], O[nb][db], 0, 0, 0);
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    O[0][(f & 1) * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, rv[f])[e], pr[0][0][f >> 1],
+                                                                                 O[0][(f & 1) * 4 + e], 0, 0, 0);
                 }
             }
         }
         if (more) {
-            load_v(st + WK, pg_next);
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) pg[kb] = pg_next[kb];
-            pages_of(min(st + 2 * WK, n_steps - 1), pg_next);
+            load_v();
+            entries_of(st + 2 * kWaves, entry);
         }
     }
 
     float mc[NB];
     uint32_t redo[NB];
     close_columns<NB, PACK>(orow, c, m, l, O, mc, redo);
-    if constexpr (WK == 1) {
-        store_columns<CT, NB, KS>(p, table, head, split, lane, lim, orow, mc, l, O, redo, step_lo, step_hi);
-    } else {
-        // merge over the WK waves of a column in LDS
-        constexpr int kStride = kHeadDim + 4;
-        __shared__ __attribute__((aligned(16))) float so[WK * R * kStride];
-        __shared__ float sm[WK * R], sl[WK * R];
-        __shared__ int srow[R], slim[R];
-        const int base = wk * R + wc * kCols;
+    // merge over the waves
+    float * so = reinterpret_cast<float *>(lds);
+    float * sm = so + kWaves * R * kRowsStride;
+    float * sl = sm + kWaves * R;
+    int * srow = reinterpret_cast<int *>(sl + kWaves * R);
+    int * slim = srow + R;
+    const int base = wave * R;
+    if (!PACK || c16 < 8) {
+        float * to = so + (base + c16) * kRowsStride + g4 * 32;
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            if (!PACK || c16 < 8) {
-                const int at = base + nb * 16 + c16;
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    f4 a, b;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        a[e] = O[nb][e][i];
-                        b[e] = O[nb][4 + e][i];
-                    }
-                    *reinterpret_cast<f4 *>(so + at * kStride + (g4 * 4 + i) * 8) = a;
-                    *reinterpret_cast<f4 *>(so + at * kStride + (g4 * 4 + i) * 8 + 4) = b;
-                }
-                if (g4 == 0) {
-                    sm[at] = mc[nb];
-                    sl[at] = l[nb];
-                    if (wk == 0) {
-                        srow[wc * kCols + nb * 16 + c16] = orow[nb];
-                        slim[wc * kCols + nb * 16 + c16] = lim[nb];
-                    }
-                }
-            }
-            for (uint32_t left = redo[nb]; left != 0; left &= left - 1) {
-                const int col = __ffs(left) - 1;
-                const int row = __builtin_amdgcn_readlane(orow[nb], col), lm = __builtin_amdgcn_readlane(lim[nb], col);
-                float cm, cl;
-                f2 co;
-                column_by_keys<CT, KS>(p, table, head, p.q + static_cast<int64_t>(row) * kHeadDim, lm, step_lo + wk, step_hi, WK, lane,
-                                       cm, cl, co);
-                // after this wave's own stores above: one wave's LDS accesses stay in order
-                __builtin_amdgcn_wave_barrier();
-                const int at = base + nb * 16 + col;
-                *reinterpret_cast<f2 *>(so + at * kStride + 2 * lane) = co;
-                if (lane == 0) {
-                    sm[at] = cm;
-                    sl[at] = cl;
-                }
+            for (int h = 0; h < 2; ++h) {
+                *reinterpret_cast<f4 *>(to + i * 8 + h * 4) = f4{O[0][4 * h][i], O[0][4 * h + 1][i], O[0][4 * h + 2][i], O[0][4 * h + 3][i]};
             }
         }
-        __syncthreads();
-        for (int idx = threadIdx.x; idx < R * (kHeadDim / 4); idx += kWave * WC * WK) {
-            const int col = idx / (kHeadDim / 4), dim = (idx % (kHeadDim / 4)) * 4;
-            const int row = srow[col];
-            if (row < 0) continue;
-            float M = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < WK; ++w) M = fmaxf(M, sm[w * R + col]);
-            float ls = 0.0f;
-            f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < WK; ++w) {
-                const float mw = sm[w * R + col];
-                const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
-                ls += sl[w * R + col] * f;
-                o += *reinterpret_cast<const f4 *>(so + (w * R + col) * kStride + dim) * f;
+        if (g4 == 0) {
+            sm[base + c16] = mc[0];
+            sl[base + c16] = l[0];
+            if (wave == 0) {
+                srow[c16] = col.row;
+                slim[c16] = col.lim;
             }
-            store_column(p, table, split, row, slim[col], dim, o, M, ls, dim == 0);
         }
+    }
+    for (uint32_t left = redo[0]; left != 0; left &= left - 1) {
+        const int cc = __ffs(left) - 1;
+        const int row = __builtin_amdgcn_readlane(col.row, cc), lm = __builtin_amdgcn_readlane(col.lim, cc);
+        float cm, cl;
+        f2 co;
+        column_by_keys<CT, KS>(p, t.table, head, p.q + static_cast<int64_t>(row) * kHeadDim, lm, t.step_lo + wave, t.step_hi, kWaves, lane, cm, cl, co);
+        // after this wave's own stores above: one wave's LDS accesses stay in order
+        __builtin_amdgcn_wave_barrier();
+        *reinterpret_cast<f2 *>(so + (base + cc) * kRowsStride + 2 * lane) = co;
+        if (lane == 0) {
+            sm[base + cc] = cm;
+            sl[base + cc] = cl;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int idx = threadIdx.x; idx < R * (kHeadDim / 4); idx += kThreads) {
+        const int cc = idx / (kHeadDim / 4), dim = (idx % (kHeadDim / 4)) * 4;
+        const int row = srow[cc];
+        if (row < 0) continue;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, sm[w * R + cc]);
+        float ls = 0.0f;
+        f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float mw = sm[w * R + cc];
+            const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
+            ls += sl[w * R + cc] * f;
+            o += *reinterpret_cast<const f4 *>(so + (w * R + cc) * kRowsStride + dim) * f;
+        }
+        store_column(p, t.table, split, row, slim[cc], dim, o, M, ls, dim == 0);
     }
 }
 
-// The kernel of long chunks on f16 pages: 4 waves of 32 columns each share the K and V of a tile through LDS, which cuts
-// what the CUs pull from L2 to a quarter (without it that traffic sets the pace).  A tile is 64 keys, two steps of 32; a
-// step lies in LDS as the MFMA operands themselves, 8 of K and 8 of V^T, 64 lanes x 16 bytes each: every read and write is
-// one unbroken kilobyte and no wave rearranges anything.  Waves 0 and 1 fetch and transpose V of the two steps, waves 2 and
-// 3 fetch K.  Two tiles in LDS, the next one's rows in registers: one barrier per tile, and two workgroups per CU, each
+// 128 columns of a long chunk: 4 waves of 32 columns each share the K and V of a tile of keys through LDS, which cuts what the
+// CUs pull from L2 to a quarter (without it that traffic sets the pace).  A tile of keys is two steps; a step lies in LDS as
+// the MFMA operands themselves, 8 of K and 8 of V^T, 64 lanes x 16 bytes each: every read and write is one unbroken
+// kilobyte and no wave rearranges anything.  Waves 0 and 1 fetch (and on f16 pages transpose) V of the two steps, waves 2
+// and 3 fetch K.  Two tiles in LDS, the next one's rows in registers: one barrier per tile, and two workgroups per CU, each
 // multiplying while the other waits at its barrier.
 constexpr int kTileSteps = 2;
-constexpr int kTileWaves = 2 * kTileSteps, kTileColumns = kTileWaves * 32;
-constexpr int kStepHalfs = 16 * kWave * 8;   // a step's 16 operands
-constexpr size_t kTileLds = 2 * kTileSteps * kStepHalfs * sizeof(_Float16);
+static_assert(kWaves == 2 * kTileSteps, "a wave fetches K or V of one step");
+constexpr int kTileColumns = kWaves * 32;
+constexpr int kStepBytes = 16 * kWave * 16;   // a step's 16 operands
+constexpr size_t kTileLds = 2 * kTileSteps * kStepBytes;
 constexpr int kOutStride = kHeadDim + 4, kOutFloats = 16 * kOutStride;   // a wave's 16 columns on their way out
-static_assert(kTileWaves * kOutFloats * sizeof(float) <= kTileLds, "the outputs go through the operands' LDS");
+static_assert(kWaves * kOutFloats * sizeof(float) <= kTileLds, "the outputs go through the operands' LDS");
 
-__global__ __launch_bounds__(kTileWaves * kWave, 2) void paged_attn_tile_kernel(AttnParams p) {
-    constexpr int NB = 2;
-    extern __shared__ __attribute__((aligned(16))) _Float16 lds_kv[];
+template <typename CT>
+__device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
+    constexpr bool F16 = std::is_same<CT, _Float16>::value;
+    constexpr int KS = step_keys(F16), KB = KS / 16, NB = 2;
+    __shared__ int s_holes[2][kTileSteps];                            // bit kb: 16-key block kb of the step lies on no page
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g4 = lane >> 4;
-    const int head = static_cast<int>(blockIdx.x) % p.n_kv;
-    const int rest = static_cast<int>(blockIdx.x) / p.n_kv;
-    const int split = rest / p.n_tiles;
-    const Tile tl = find_tile<kTileColumns, false>(p, rest - split * p.n_tiles, lane);
-    if (tl.seq < 0) return;
-    const int col0 = (tl.n_tiles - 1 - tl.tile) * kTileColumns;
-    const int n_cols = tl.rows * p.group;
-    const int cap = p.seqs.table_stride << p.page_shift;
-    const int32_t * table = p.seqs.tables + static_cast<int64_t>(tl.seq) * p.seqs.table_stride;
-    const int t_last = (min(col0 + kTileColumns, n_cols) - 1) / p.group;
-    const int kend = max(0, min(tl.past + t_last, cap - 1) + 1);
-    const int n_steps = (kend + 31) / 32;
-    const int step_lo = split * p.split_steps;
-    const int step_hi = split == p.n_splits - 1 ? n_steps : min(n_steps, step_lo + p.split_steps);
-    if (split > 0 && step_lo >= n_steps) return;                      // uniform for the workgroup
-    const int in_page = (1 << p.page_shift) - 1;
+    Tile t;
+    int head, split;
+    if (!find_tile<kTileColumns, KS, false>(p, block, lane, t, head, split)) return;   // uniform for the workgroup
 
     // columns: their q is on its way while the first tile is fetched
     int lim[NB], orow[NB];
     f4 x[NB][8];
-    int wave_lim = -1, wave_first = 1 << 30;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-        const int col = col0 + wave * 32 + nb * 16 + c16;
-        const bool ok = col < n_cols;
-        const int t = ok ? col / p.group : t_last;
-        const int h = ok ? col - t * p.group : 0;
-        lim[nb] = ok ? min(tl.past + t, cap - 1) : -1;
-        orow[nb] = ok ? (tl.row0 + t) * p.n_heads + head * p.group + h : -1;
-        load_q(p.q + (static_cast<int64_t>(tl.row0 + t) * p.n_heads + head * p.group + h) * kHeadDim, ok, g4, x[nb]);
+        const Column col = column_of(p, t, head, t.col0 + wave * 32 + nb * 16 + c16);
+        lim[nb] = col.lim;
+        orow[nb] = col.row;
+        load_q<F16>(col, g4, x[nb]);
     }
-    {
-        // keys that the wave's last and first token see (its columns are in order of token)
-        const int first_col = col0 + wave * 32, last_col = min(first_col + 32, n_cols) - 1;
-        if (first_col < n_cols) {
-            wave_first = min(tl.past + first_col / p.group, cap - 1);
-            wave_lim = min(tl.past + last_col / p.group, cap - 1);
-        }
+    // keys that the wave's last and first token see (its columns are in order of token)
+    const int first_col = t.col0 + wave * 32;
+    int wave_steps = 0, full = 0;                                     // steps behind the first hold nothing that the wave sees
+    if (first_col < t.n_cols) {
+        wave_steps = min(t.step_hi, (min(t.past + (min(first_col + 32, t.n_cols) - 1) / p.group, t.cap - 1) + KS) / KS);
+        full = max(0, min(t.past + first_col / p.group, t.cap - 1) + 1) / KS;
     }
-    const int wave_steps = min(step_hi, (wave_lim + 32) / 32);        // steps behind it hold nothing that the wave sees
-    const int full = max(0, wave_first + 1) / 32;
 
-    // this wave's share of a tile: step `wave % 4`, V (waves 0..3) or K
+    // this wave's share of a tile: K or V of step `mine`
     const bool fetch_v = wave < kTileSteps;
+    const int mine = wave & (kTileSteps - 1);
+    const HeadRows<CT> rows(p, head);
+    const int in_page = (1 << p.page_shift) - 1, last_entry = p.seqs.table_stride - 1;
     u4 r[8];
-    int pg[2];
-    __shared__ int s_holes[2][kTileSteps];                            // bit kb: 16-key block kb of the step lies on no page
-    // table entries of a step's two 16-key blocks as they are, looked at when they have arrived
-    auto entries_of = [&](int st, int (&out)[2]) {
+    int pg[KB], entry[KB], st_held = 0;
+    auto entries_of = [&](int st) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) out[kb] = table[min((st * 32 + kb * 16) >> p.page_shift, p.seqs.table_stride - 1)];
+        for (int kb = 0; kb < KB; ++kb) entry[kb] = t.table[min((st * KS + kb * 16) >> p.page_shift, last_entry)];
     };
-    int st_held = 0;
-    auto fetch = [&](int st, const int (&from)[2]) {
+    auto fetch = [&](int st) {
         st_held = st;
+        const CT * at[KB];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            pg[kb] = st * 32 + kb * 16 < kend && from[kb] >= 0 && from[kb] < p.n_pages ? from[kb] : -1;
-            const _Float16 * base = page_rows<_Float16>(p, fetch_v ? 1 : 0, max(pg[kb], 0), head) +
-                                    static_cast<int64_t>((st * 32 + kb * 16) & in_page) * kHeadDim;
+        for (int kb = 0; kb < KB; ++kb) {
+            pg[kb] = entry_page(p, t, entry[kb], st * KS + kb * 16);
+            at[kb] = rows.page(max(pg[kb], 0)) + ((st * KS + kb * 16) & in_page) * kHeadDim + (fetch_v ? rows.v_elems : 0);
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // V: row 4 g4 + i, dims 8 c16 ..; K: row c16, dims 32 i + 8 g4 ..
-                const int off = fetch_v ? (g4 * 4 + i) * kHeadDim + c16 * 8 : c16 * kHeadDim + i * 32 + g4 * 8;
-                r[kb * 4 + i] = *reinterpret_cast<const u4 *>(base + off);
-            }
+        for (int f = 0; f < 8; ++f) {
+            r[f] = *reinterpret_cast<const u4 *>(at[F16 ? f >> 2 : 0] + (fetch_v ? v_offset<F16>(f, c16, g4) : k_offset<F16>(f, c16, g4)));
         }
     };
     auto put = [&](int buf) {
-        _Float16 * to = lds_kv + (buf * kTileSteps + (wave & (kTileSteps - 1))) * kStepHalfs + lane * 8;
+        char * to = lds + (buf * kTileSteps + mine) * kStepBytes + lane * 16;
         if (fetch_v) {
-            if (st_held * 32 + 32 > kend || pg[0] < 0 || pg[1] < 0) {   // rows that no column sees, and of no page: not even 0 times them
+            bool hole = st_held * KS + KS > t.kend;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (st_held * 32 + (e >> 2) * 16 + g4 * 4 + (e & 3) >= kend || pg[e >> 2] < 0) r[e] = u4{0, 0, 0, 0};
+            for (int kb = 0; kb < KB; ++kb) hole = hole || pg[kb] < 0;
+            if (hole) {   // rows that no column sees, and of no page: not even 0 times what memory holds
+#pragma unroll
+                for (int f = 0; f < 8; ++f) {
+                    if (st_held * KS + v_key<F16>(f, g4) >= t.kend || pg[F16 ? f >> 2 : 0] < 0) r[f] = u4{0, 0, 0, 0};
                 }
             }
 #pragma unroll
-            for (int db = 0; db < 8; ++db) {
-                u4 a;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    a[w] = db & 1 ? hi_pair(r[2 * w][db >> 1], r[2 * w + 1][db >> 1]) : lo_pair(r[2 * w][db >> 1], r[2 * w + 1][db >> 1]);
-                }
-                *reinterpret_cast<u4 *>(to + (8 + db) * kWave * 8) = a;
-            }
+            for (int f = 0; f < 8; ++f) *reinterpret_cast<u4 *>(to + (8 + f) * kWave * 16) = F16 ? transposed(r, f) : r[f];
         } else {
 #pragma unroll
-            for (int f = 0; f < 8; ++f) *reinterpret_cast<u4 *>(to + f * kWave * 8) = r[f];
-            if (lane == 0) s_holes[buf][wave & (kTileSteps - 1)] = (pg[0] < 0 ? 1 : 0) | (pg[1] < 0 ? 2 : 0);
+            for (int f = 0; f < 8; ++f) *reinterpret_cast<u4 *>(to + f * kWave * 16) = r[f];
+            if (lane == 0) s_holes[buf][mine] = (pg[0] < 0 ? 1 : 0) | (pg[KB - 1] < 0 ? 1 << (KB - 1) : 0);
         }
     };
 
-    const int mine = wave & (kTileSteps - 1);
-    const int n_tiles = (step_hi - step_lo + kTileSteps - 1) / kTileSteps;
-    int pg_next[2];
+    const int n_tiles = (t.step_hi - t.step_lo + kTileSteps - 1) / kTileSteps;
     if (n_tiles > 0) {
-        entries_of(step_lo + mine, pg_next);
-        fetch(step_lo + mine, pg_next);
-        entries_of(step_lo + kTileSteps + mine, pg_next);
+        entries_of(t.step_lo + mine);
+        fetch(t.step_lo + mine);
+        entries_of(t.step_lo + kTileSteps + mine);
     }
-
     float c[NB];
     h8 qh[NB][4], ql[NB][4];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) split_q(x[nb], p.scale, c[nb], qh[nb], ql[nb]);
+    for (int nb = 0; nb < NB; ++nb) {
+        if constexpr (F16) split_q(x[nb], p.scale, c[nb], qh[nb], ql[nb]);
+        else c[nb] = p.scale * kLog2e;
+    }
     float m[NB], l[NB];
     f4 O[NB][8];
 #pragma unroll
@@ -795,74 +737,62 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void paged_attn_tile_kernel(
     }
     if (n_tiles > 0) {
         put(0);
-        fetch(step_lo + kTileSteps + mine, pg_next);
-        entries_of(step_lo + 2 * kTileSteps + mine, pg_next);
+        fetch(t.step_lo + kTileSteps + mine);
+        entries_of(t.step_lo + 2 * kTileSteps + mine);
     }
     __syncthreads();
     for (int tile = 0; tile < n_tiles; ++tile) {
-        const _Float16 * buf = lds_kv + (tile & 1) * kTileSteps * kStepHalfs + lane * 8;
-        const int st0 = step_lo + tile * kTileSteps;
+        const char * buf = lds + (tile & 1) * kTileSteps * kStepBytes + lane * 16;
+        const int st0 = t.step_lo + tile * kTileSteps;
 #pragma unroll 1
         for (int s = 0; s < kTileSteps; ++s) {
             const int st = st0 + s;
             if (st >= wave_steps) break;                              // uniform for the wave
-            const _Float16 * op = buf + s * kStepHalfs;
-            f4 S[NB][2];
+            const char * op = buf + s * kStepBytes;
+            u4 a[8], v[8];
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) S[nb][0] = S[nb][1] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-            h8 a[8];
+            for (int f = 0; f < 8; ++f) a[f] = *reinterpret_cast<const u4 *>(op + f * kWave * 16);
+            f4 S[NB][KB];
+            scores_step<F16, false, NB>(a, qh, ql, x, S);
 #pragma unroll
-            for (int f = 0; f < 8; ++f) a[f] = *reinterpret_cast<const h8 *>(op + f * kWave * 8);
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) S[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[kb * 4 + ks], qh[nb][ks], S[nb][kb], 0, 0, 0);
-                }
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) S[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[kb * 4 + ks], ql[nb][ks], S[nb][kb], 0, 0, 0);
-                }
-            }
-            h8 v[8];
-#pragma unroll
-            for (int db = 0; db < 8; ++db) v[db] = *reinterpret_cast<const h8 *>(op + (8 + db) * kWave * 8);
+            for (int f = 0; f < 8; ++f) v[f] = *reinterpret_cast<const u4 *>(op + (8 + f) * kWave * 16);
             const int holes = __builtin_amdgcn_readfirstlane(s_holes[tile & 1][s]);
-            if (st >= full || holes != 0) {
+            if (st >= full || holes != 0) mask_step<NB, KB>(S, lim, st * KS, g4, holes);
+            float pr[NB][KB][4];
+            softmax_step<NB, KB>(S, c, m, l, O, pr);
+            if constexpr (F16) {
+                h8 ph[NB], pl[NB];
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
+                for (int nb = 0; nb < NB; ++nb) split_p(pr[nb], ph[nb], pl[nb]);
 #pragma unroll
-                    for (int kb = 0; kb < 2; ++kb) {
+                for (int part = 0; part < 2; ++part) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (st * 32 + kb * 16 + g4 * 4 + i > lim[nb] || ((holes >> kb) & 1)) S[nb][kb][i] = -INFINITY;
+                    for (int db = 0; db < 8; ++db) {
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            O[nb][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, v[db]), part ? pl[nb] : ph[nb], O[nb][db], 0, 0, 0);
                         }
                     }
                 }
-            }
-            float pr[NB][2][4];
-            softmax_step<NB, 2>(S, c, m, l, O, pr);
-            h8 ph[NB], pl[NB];
+            } else {
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) split_p(pr[nb], ph[nb], pl[nb]);
+                for (int f = 0; f < 8; ++f) {
 #pragma unroll
-            for (int db = 0; db < 8; ++db) {
+                    for (int e = 0; e < 4; ++e) {
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) O[nb][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[db], ph[nb], O[nb][db], 0, 0, 0);
-            }
-#pragma unroll
-            for (int db = 0; db < 8; ++db) {
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) O[nb][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[db], pl[nb], O[nb][db], 0, 0, 0);
+                        for (int nb = 0; nb < NB; ++nb) {
+                            O[nb][(f & 1) * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, v[f])[e], pr[nb][0][f >> 1],
+                                                                                          O[nb][(f & 1) * 4 + e], 0, 0, 0);
+                        }
+                    }
+                }
             }
         }
         if (tile + 1 < n_tiles) {
             put((tile + 1) & 1);
             if (tile + 2 < n_tiles) {
-                fetch(st0 + 2 * kTileSteps + mine, pg_next);
-                entries_of(st0 + 3 * kTileSteps + mine, pg_next);
+                fetch(st0 + 2 * kTileSteps + mine);
+                entries_of(st0 + 3 * kTileSteps + mine);
             }
         }
         __syncthreads();
@@ -872,7 +802,7 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void paged_attn_tile_kernel(
     close_columns<NB, false>(orow, c, m, l, O, mc, redo);
     // through the wave's own part of LDS, so that a store instruction writes two whole rows; a lane's values would lie 16 bytes
     // in each of 64 lines
-    float * so = reinterpret_cast<float *>(lds_kv) + wave * kOutFloats;
+    float * so = reinterpret_cast<float *>(lds) + wave * kOutFloats;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         float * to = so + c16 * kOutStride + g4 * 32;
@@ -890,10 +820,33 @@ __global__ __launch_bounds__(kTileWaves * kWave, 2) void paged_attn_tile_kernel(
             const int row = __shfl(orow[nb], col, kWave), lm = __shfl(lim[nb], col, kWave);
             const float cm = __shfl(mc[nb], col, kWave), cl = __shfl(l[nb], col, kWave);
             const f4 v = *reinterpret_cast<const f4 *>(so + col * kOutStride + dim);
-            if (row >= 0 && !((redo[nb] >> col) & 1)) store_column(p, table, split, row, lm, dim, v, cm, cl, dim == 0);
+            if (row >= 0 && !((redo[nb] >> col) & 1)) store_column(p, t.table, split, row, lm, dim, v, cm, cl, dim == 0);
         }
-        redo_columns<_Float16, 32>(p, table, head, split, lane, lim[nb], orow[nb], redo[nb], step_lo, step_hi);
+        redo_columns<CT, KS>(p, t.table, head, split, lane, lim[nb], orow[nb], redo[nb], t.step_lo, t.step_hi);
     }
+}
+
+// The launches.  One kind of tile, or longer chunks first and the sequences of few columns behind them.
+template <typename CT, bool FEW>
+__global__ __launch_bounds__(kThreads, 3) void paged_rows_kernel(AttnParams p) {
+    extern __shared__ __attribute__((aligned(16))) char lds_rows[];
+    attn_rows<CT, FEW>(p, blockIdx.x, lds_rows);
+}
+
+template <typename CT>
+__global__ __launch_bounds__(kThreads, 3) void paged_rows_both_kernel(AttnParams p) {
+    extern __shared__ __attribute__((aligned(16))) char lds_rows[];
+    const int many = p.tiles_many * p.n_kv * p.n_splits, block = blockIdx.x;
+    if (block < many) attn_rows<CT, false>(p, block, lds_rows);
+    else attn_rows<CT, true>(p, block - many, lds_rows);
+}
+
+template <typename CT, bool BOTH>
+__global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(AttnParams p) {
+    extern __shared__ __attribute__((aligned(16))) char lds_tile[];
+    const int many = p.tiles_many * p.n_kv * p.n_splits, block = blockIdx.x;
+    if (!BOTH || block < many) attn_tile<CT>(p, block, lds_tile);
+    else attn_rows<CT, true>(p, block - many, lds_tile);
 }
 
 // Joins the splits of each (row, head): one wave each, lane = split for the weights, then lane = 2 dims.  Its time is
@@ -938,35 +891,39 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int ks) {
     *reinterpret_cast<f2 *>(p.out + item * kHeadDim + 2 * lane) = o * inv;
 }
 
-constexpr int kMidCols = 64;   // columns of a sequence up to which waves share no LDS tile
-
-// How a call cuts its work: which kernels run, their upper bounds of tiles, and the key ranges.
+// How a call cuts its work: which kinds of tiles there are, their upper bounds, and the key ranges.
 struct AttnPlan {
-    bool few;                // sequences of few columns, when the host's bounds allow any
-    int many_cols;           // columns of a tile of the other kernel, 0: all sequences are of few
-    int tiles_few, tiles_many;
-    int splits, split_steps; // of both, in steps of the cache type
+    bool tile;               // the longer sequences' tiles are attn_tile's
+    int tiles_many, tiles_few;
+    int few_max;             // 0: sequences of few columns are the longer ones' tiles, too
+    int splits, split_steps; // in steps of the cache type
 };
 
 AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_heads, size_t workspace_bytes) {
     const bool f16 = l.cache_type == QA_CACHE_F16;
-    const int ks = f16 ? 32 : 16;
+    const int ks = step_keys(f16);
     const int group = n_heads / l.n_kv_heads;
     const int seqs = std::min(b.n_seqs, b.n_rows);
-    const int64_t most = std::min<int64_t>(b.n_rows, b.max_tokens > 0 ? b.max_tokens : b.n_rows);
+    const int64_t most = std::min<int64_t>(b.n_rows, b.max_tokens > 0 ? b.max_tokens : b.n_rows) * group;   // columns of a sequence
     const int64_t cols = static_cast<int64_t>(b.n_rows) * group;
     AttnPlan pl{};
-    // one sequence is either; the host's bounds say whether all are of few columns
-    if (most * group > few_cols(f16)) pl.many_cols = f16 ? (most * group > kMidCols ? kTileColumns : 64) : 64;
-    pl.few = pl.many_cols == 0 || b.n_seqs > 1;
-    pl.tiles_few = seqs;
-    pl.tiles_many = pl.many_cols ? static_cast<int>(cols / pl.many_cols + seqs) : 0;
+    // Up to 64 columns four waves that share the keys beat four that share K and V (one sequence behind 3900 positions, 8 / 16
+    // / 32 tokens: 14.1 / 16.6 / 20.6 against 22.3 / 23.4 / 24.1 us; eight of 32 tokens 30.3 against 49.3); at 128 they are even.
+    pl.tile = most > kMidCols;
+    const bool many = most > few_cols(f16);
+    const int width = pl.tile ? kTileColumns : 16;
+    pl.tiles_many = many ? static_cast<int>(cols / width + seqs) : 0;
+    // f32 pages have no packed form: short sequences are tiles of attn_rows like the others.  One sequence is of one kind.
+    const bool few = !many || ((f16 || pl.tile) && b.n_seqs > 1);
+    pl.few_max = few ? few_cols(f16) : 0;
+    pl.tiles_few = few ? seqs : 0;
     const int64_t cap = static_cast<int64_t>(b.table_stride) * l.max_seq;
     const int64_t len = std::min<int64_t>(cap, b.max_len > 0 ? b.max_len : cap);
     const int steps = static_cast<int>((len + ks - 1) / ks);
-    const int64_t tiles = pl.many_cols ? std::max<int64_t>(1, (cols + pl.many_cols - 1) / pl.many_cols) : pl.tiles_few;
-    const int64_t target = pl.many_cols == kTileColumns ? 512 : 1024, least = pl.many_cols == kTileColumns ? 4 : 8;
-    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({target / std::max<int64_t>(tiles * l.n_kv_heads, 1), (steps + least - 1) / least, kMaxSplits}));
+    // workgroups that fill the GPU, each of two steps per wave or four of a tile at least
+    const int64_t tiles = std::max<int64_t>(1, many ? (cols + width - 1) / width : seqs);
+    const int64_t target = pl.tile ? 512 : 1024, least = pl.tile ? 4 : 8;
+    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({target / (tiles * l.n_kv_heads), (steps + least - 1) / least, kMaxSplits}));
     const size_t per_split = static_cast<size_t>(b.n_rows) * n_heads * (kHeadDim + 2) * sizeof(float);
     if (splits > 1 && per_split * splits > workspace_bytes) splits = std::max<int64_t>(1, static_cast<int64_t>(workspace_bytes / per_split));
     pl.split_steps = std::max<int>(1, static_cast<int>((steps + splits - 1) / splits));
@@ -977,29 +934,26 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
 template <typename CT>
 int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
     constexpr bool F16 = std::is_same<CT, _Float16>::value;
-    const unsigned per = static_cast<unsigned>(p.n_kv) * pl.splits;
-    p.few_max = pl.few ? few_cols(F16) : 0;
-    if (pl.many_cols) {
-        p.n_tiles = pl.tiles_many;
-        if constexpr (!F16) {
-            hipLaunchKernelGGL((paged_attn_kernel<CT, 1, 4, 1, false>), dim3(per * p.n_tiles), dim3(256), 0, stream, p);
-        } else if (pl.many_cols == kTileColumns) {
-            QA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(paged_attn_tile_kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(kTileLds)));
-            hipLaunchKernelGGL(paged_attn_tile_kernel, dim3(per * p.n_tiles), dim3(kTileWaves * kWave), kTileLds, stream, p);
-        } else {
-            hipLaunchKernelGGL((paged_attn_kernel<CT, 2, 2, 2, false>), dim3(per * p.n_tiles), dim3(256), 0, stream, p);
-        }
+    const dim3 grid(static_cast<unsigned>(p.n_kv) * pl.splits * (pl.tiles_many + pl.tiles_few));
+    constexpr size_t lds_few = rows_lds(F16, true), lds_many = rows_lds(F16, false);
+    static_assert(lds_few <= kTileLds && lds_few <= lds_many, "a launch of both kinds has the longer ones' LDS");
+    if (pl.tile) {
+        const auto kernel = pl.few_max ? &paged_tile_kernel<CT, true> : &paged_tile_kernel<CT, false>;
+        QA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kTileLds)));
+        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), kTileLds, stream, p);
+    } else if (!pl.tiles_many) {
+        hipLaunchKernelGGL((paged_rows_kernel<CT, true>), grid, dim3(kThreads), lds_few, stream, p);
+    } else if (F16 && pl.few_max) {
+        hipLaunchKernelGGL((paged_rows_both_kernel<_Float16>), grid, dim3(kThreads), lds_many, stream, p);
+    } else {
+        hipLaunchKernelGGL((paged_rows_kernel<CT, false>), grid, dim3(kThreads), lds_many, stream, p);
     }
-    if (pl.few) {
-        p.n_tiles = pl.tiles_few;
-        hipLaunchKernelGGL((paged_attn_kernel<CT, 1, 1, 4, true>), dim3(per * p.n_tiles), dim3(256), 0, stream, p);
-    }
+    QA_LAUNCH_CHECK("paged attention kernel");
     if (pl.splits > 1) {
         const int64_t items = static_cast<int64_t>(p.seqs.n_rows) * p.n_heads;
-        hipLaunchKernelGGL(paged_join_kernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, p, F16 ? 32 : 16);
+        hipLaunchKernelGGL(paged_join_kernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, p, step_keys(F16));
+        QA_LAUNCH_CHECK("paged_join_kernel");
     }
-    QA_LAUNCH_CHECK("paged_attn_kernel");
     return QA_OK;
 }
 
@@ -1029,7 +983,7 @@ extern "C" int qa_paged_attn(const float * q, const void * pages, const qa_kv_la
     if (static_cast<int64_t>(batch->n_rows) * n_heads > INT32_MAX) return fail(QA_ERR_INVALID, "qa_paged_attn: too many rows");
     if (const int rc = check_stream(stream, "qa_paged_attn"); rc != QA_OK) return rc;
     const AttnPlan pl = attn_plan(*layout, *batch, n_heads, workspace_bytes);
-    if (static_cast<int64_t>(std::max(pl.tiles_many, pl.tiles_few)) * layout->n_kv_heads * pl.splits > INT32_MAX / 256) {
+    if ((static_cast<int64_t>(pl.tiles_many) + pl.tiles_few) * layout->n_kv_heads * pl.splits > INT32_MAX / kThreads) {
         return fail(QA_ERR_INVALID, "qa_paged_attn: too many rows");
     }
     AttnParams p{};
@@ -1045,6 +999,9 @@ extern "C" int qa_paged_attn(const float * q, const void * pages, const qa_kv_la
     p.n_pages = layout->n_streams;
     p.page_shift = page_shift_of(layout->max_seq);
     p.layer = layer;
+    p.few_max = pl.few_max;
+    p.tiles_many = pl.tiles_many;
+    p.tiles_few = pl.tiles_few;
     p.n_splits = pl.splits;
     p.split_steps = pl.split_steps;
     p.scale = scale;
