@@ -6,7 +6,7 @@
 // heads of a KV head and the tokens of a sequence are columns of the same products: column c of a tile is token c / group
 // and head c % group, so one token of 2 heads and a chunk of a thousand run the same code, in two shapes: up to 64 columns
 // a workgroup takes 16 of them (8 in the packed form) and its 4 waves share the keys (attn_rows); of longer chunks it
-// takes 128, 32 per wave, and the waves share K and V (attn_tile).  A batch of both kinds is one launch.
+// takes 128 (f32 pages: 64), a quarter per wave, and the waves share K and V (attn_tile).  A batch of both kinds is one launch.
 //
 // f16 pages on v_mfma_f32_16x16x32_f16: q and p are f32, split into two f16 parts each (a power of two per column brings
 // the largest |q| to 2^14..2^15, p is scaled by 2^6, so the second part keeps its bits); K and V are exact f16.  What the
@@ -252,16 +252,23 @@ __device__ inline void scores_step(const u4 (&a)[8], const h8 (&qh)[NB][4], cons
             }
         }
     } else {
+        // two sums, so that a product does not wait for the one before it
+        f4 T[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) T[nb] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    S[nb][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, a[i])[e], x[nb][i][e], S[nb][0], 0, 0, 0);
+                    f4 & to = e & 1 ? T[nb] : S[nb][0];
+                    to = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, a[i])[e], x[nb][i][e], to, 0, 0, 0);
                 }
             }
         }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) S[nb][0] += T[nb];
     }
 }
 
@@ -624,15 +631,18 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
     }
 }
 
-// 128 columns of a long chunk: 4 waves of 32 columns each share the K and V of a tile of keys through LDS, which cuts what the
-// CUs pull from L2 to a quarter (without it that traffic sets the pace).  A tile of keys is two steps; a step lies in LDS as
+// 128 columns of a long chunk (f32 pages: 64): 4 waves of 32 (16) each share the K and V of a tile of keys through LDS, which
+// cuts what the CUs pull from L2 to a quarter (without it that traffic sets the pace).  On f32 pages, whose products take
+// eight times as long, narrower tiles leave fewer columns empty: two sequences of 157 and 144 tokens behind 1037 and 701
+// positions 45.7 instead of 50.3 us.  A tile of keys is two steps; a step lies in LDS as
 // the MFMA operands themselves, 8 of K and 8 of V^T, 64 lanes x 16 bytes each: every read and write is one unbroken
 // kilobyte and no wave rearranges anything.  Waves 0 and 1 fetch (and on f16 pages transpose) V of the two steps, waves 2
 // and 3 fetch K.  Two tiles in LDS, the next one's rows in registers: one barrier per tile, and two workgroups per CU, each
 // multiplying while the other waits at its barrier.
 constexpr int kTileSteps = 2;
 static_assert(kWaves == 2 * kTileSteps, "a wave fetches K or V of one step");
-constexpr int kTileColumns = kWaves * 32;
+constexpr int tile_blocks(bool f16) { return f16 ? 2 : 1; }       // of 16 columns per wave
+constexpr int tile_cols(bool f16) { return kWaves * 16 * tile_blocks(f16); }
 constexpr int kStepBytes = 16 * kWave * 16;   // a step's 16 operands
 constexpr size_t kTileLds = 2 * kTileSteps * kStepBytes;
 constexpr int kOutStride = kHeadDim + 4, kOutFloats = 16 * kOutStride;   // a wave's 16 columns on their way out
@@ -641,30 +651,30 @@ static_assert(kWaves * kOutFloats * sizeof(float) <= kTileLds, "the outputs go t
 template <typename CT>
 __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
     constexpr bool F16 = std::is_same<CT, _Float16>::value;
-    constexpr int KS = step_keys(F16), KB = KS / 16, NB = 2;
+    constexpr int KS = step_keys(F16), KB = KS / 16, NB = tile_blocks(F16);
     __shared__ int s_holes[2][kTileSteps];                            // bit kb: 16-key block kb of the step lies on no page
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g4 = lane >> 4;
     Tile t;
     int head, split;
-    if (!find_tile<kTileColumns, KS, false>(p, block, lane, t, head, split)) return;   // uniform for the workgroup
+    if (!find_tile<tile_cols(F16), KS, false>(p, block, lane, t, head, split)) return;   // uniform for the workgroup
 
     // columns: their q is on its way while the first tile is fetched
     int lim[NB], orow[NB];
     f4 x[NB][8];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-        const Column col = column_of(p, t, head, t.col0 + wave * 32 + nb * 16 + c16);
+        const Column col = column_of(p, t, head, t.col0 + wave * 16 * NB + nb * 16 + c16);
         lim[nb] = col.lim;
         orow[nb] = col.row;
         load_q<F16>(col, g4, x[nb]);
     }
     // keys that the wave's last and first token see (its columns are in order of token)
-    const int first_col = t.col0 + wave * 32;
+    const int first_col = t.col0 + wave * 16 * NB;
     int wave_steps = 0, full = 0;                                     // steps behind the first hold nothing that the wave sees
     if (first_col < t.n_cols) {
-        wave_steps = min(t.step_hi, (min(t.past + (min(first_col + 32, t.n_cols) - 1) / p.group, t.cap - 1) + KS) / KS);
+        wave_steps = min(t.step_hi, (min(t.past + (min(first_col + 16 * NB, t.n_cols) - 1) / p.group, t.cap - 1) + KS) / KS);
         full = max(0, min(t.past + first_col / p.group, t.cap - 1) + 1) / KS;
     }
 
@@ -911,7 +921,7 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     // / 32 tokens: 14.1 / 16.6 / 20.6 against 22.3 / 23.4 / 24.1 us; eight of 32 tokens 30.3 against 49.3); at 128 they are even.
     pl.tile = most > kMidCols;
     const bool many = most > few_cols(f16);
-    const int width = pl.tile ? kTileColumns : 16;
+    const int width = pl.tile ? tile_cols(f16) : 16;
     pl.tiles_many = many ? static_cast<int>(cols / width + seqs) : 0;
     // f32 pages have no packed form: short sequences are tiles of attn_rows like the others.  One sequence is of one kind.
     const bool few = !many || ((f16 || pl.tile) && b.n_seqs > 1);
