@@ -62,7 +62,11 @@ struct ExtendParams {
     int32_t n_pages, n_rows, stride, shift, n;
 };
 
-// Thread i < n plans list entry i, then a wave per entry counts and fills its table entries.
+// Thread i < n plans list entry i.  The kernel's time is its dependent loads, so each is made for all entries at once: up to
+// kSpan table entries per list entry (a decode step's one or two) by the entry's thread, longer spans by a wave each; the
+// counts of the first pages are read before anything is known.
+constexpr int kSpan = 4;
+
 __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams p) {
     __shared__ int s_row[kMaxList], s_claim[kMaxList], s_j0[kMaxList], s_j1[kMaxList];
     __shared__ int s_need[kMaxList];
@@ -71,6 +75,16 @@ __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams
     int32_t * src = p.ws + kWsHead;
     int32_t * dst = src + kMaxList;
     int32_t * list = dst + kMaxList;          // the free pages that are given, lowest first
+    // free pages among kScan counts, as a mask
+    auto free_mask = [&](int64_t at) {
+        unsigned mask = 0;
+#pragma unroll
+        for (int u = 0; u < kScan; ++u) {
+            if (at + u < p.n_pages && p.refs[at + u] <= 0) mask |= 1u << u;
+        }
+        return mask;
+    };
+    unsigned mask = free_mask(static_cast<int64_t>(i) * kScan);
     int row = -1, j0 = 0, j1 = 0, claim = -1;
     if (i < p.n) {
         row = p.rows ? p.rows[i] : i;
@@ -82,82 +96,100 @@ __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams
             j0 = min(past >> p.shift, j1);
         }
     }
+    const bool wide = __syncthreads_or(j1 - j0 > kSpan);
     s_row[i] = row;
+    int32_t * table = p.tables + static_cast<int64_t>(max(row, 0)) * p.stride;
+    int entry[kSpan];
+#pragma unroll
+    for (int k = 0; k < kSpan; ++k) entry[k] = j0 + k < j1 ? table[j0 + k] : 0;
     __syncthreads();
-    for (int k = 0; k < min(i, p.n) && row >= 0; ++k) {
-        if (s_row[k] == row) row = -1, j0 = j1 = 0;       // listed before
-    }
-    if (row >= 0 && j0 < j1) {
-        const int e = p.tables[static_cast<int64_t>(row) * p.stride + j0];
-        if (is_page(e, p.n_pages) && p.refs[e] > 1) claim = e;
+    bool again = false;
+    for (int k = 0; k < min(i, p.n); ++k) again = again || s_row[k] == row;
+    if (again) row = -1, j0 = j1 = 0;                     // listed before
+    int holders = 0;
+    if (row >= 0 && j0 < j1 && is_page(entry[0], p.n_pages)) {
+        holders = p.refs[entry[0]];
+        if (holders > 1) claim = entry[0];
     }
     s_claim[i] = claim;
-    s_j0[i] = j0;
-    s_j1[i] = j1;
     __syncthreads();
     if (claim >= 0) {
         int before = 0;                                   // holders ahead in the list that take a copy
         for (int k = 0; k < i; ++k) before += s_claim[k] == claim;
-        if (p.refs[claim] - before <= 1) claim = -1;      // the last holder keeps the page
+        if (holders - before <= 1) claim = -1;            // the last holder keeps the page
+    }
+    int need = claim >= 0 ? 1 : 0;
+    if (!wide) {
+#pragma unroll
+        for (int k = 0; k < kSpan; ++k) need += j0 + k < j1 && !is_page(entry[k], p.n_pages);
     }
     __syncthreads();
     s_claim[i] = claim;
     s_row[i] = row;
-    s_need[i] = claim >= 0 ? 1 : 0;
-    __syncthreads();
-    for (int s = wave; s < p.n; s += kPlanThreads / kWave) {
-        const int32_t * table = p.tables + static_cast<int64_t>(max(s_row[s], 0)) * p.stride;
-        int need = 0;
-        for (int b = s_j0[s]; b < s_j1[s]; b += kWave) {
-            const int j = b + lane;
-            need += __popcll(__ballot(j < s_j1[s] && !is_page(table[min(j, s_j1[s] - 1)], p.n_pages)));
+    s_j0[i] = j0;
+    s_j1[i] = j1;
+    s_need[i] = need;
+    if (wide) {
+        __syncthreads();
+        for (int s = wave; s < p.n; s += kPlanThreads / kWave) {
+            const int32_t * of = p.tables + static_cast<int64_t>(max(s_row[s], 0)) * p.stride;
+            int count = 0;
+            for (int b = s_j0[s]; b < s_j1[s]; b += kWave) {
+                const int j = b + lane;
+                count += __popcll(__ballot(j < s_j1[s] && !is_page(of[min(j, s_j1[s] - 1)], p.n_pages)));
+            }
+            if (lane == 0) s_need[s] += count;
         }
-        if (lane == 0) s_need[s] += need;
+        __syncthreads();
     }
-    __syncthreads();
     long long total = 0;
-    s_base[i] = block_scan<long long>(i < p.n ? s_need[i] : 0, s_part, &total);
+    const long long base = block_scan<long long>(i < p.n ? s_need[i] : 0, s_part, &total);
+    s_base[i] = base;
     // free pages, lowest first, until there are enough (or none left: then the count tells what is lacking)
     long long found = 0;
     for (int64_t b = 0; b < p.n_pages && found < total; b += kPlanThreads * kScan) {
         const int64_t at = b + static_cast<int64_t>(i) * kScan;
-        unsigned mask = 0;
-#pragma unroll
-        for (int u = 0; u < kScan; ++u) {
-            if (at + u < p.n_pages && p.refs[at + u] <= 0) mask |= 1u << u;
-        }
+        if (b > 0) mask = free_mask(at);
         long long here = 0;
         long long r = found + block_scan<long long>(__popc(mask), s_part, &here);
         for (; mask != 0 && r < total; mask &= mask - 1, ++r) list[r] = static_cast<int32_t>(at + __ffs(mask) - 1);
         found += here;
     }
     if (i == 0) *p.missing = total <= found ? 0 : static_cast<int32_t>(min(total - found, static_cast<long long>(INT32_MAX)));
-    if (i < p.n && (total > found || s_claim[i] < 0)) dst[i] = -1;   // nothing to copy for this entry
+    if (i < p.n && (total > found || claim < 0)) dst[i] = -1;   // nothing to copy for this entry
     if (total > found) return;                            // nothing is changed
     __syncthreads();
+    if (i < p.n && need > 0 && claim >= 0) {
+        const int page = list[base];
+        src[i] = claim;
+        dst[i] = page;
+        table[j0] = page;
+        p.refs[page] = 1;
+        atomicSub(&p.refs[claim], 1);
+    }
+    if (!wide) {
+        long long at = base + (claim >= 0 ? 1 : 0);
+#pragma unroll
+        for (int k = 0; k < kSpan; ++k) {
+            if (j0 + k >= j1 || is_page(entry[k], p.n_pages)) continue;
+            const int page = list[at++];
+            table[j0 + k] = page;
+            p.refs[page] = 1;
+        }
+        return;
+    }
     for (int s = wave; s < p.n; s += kPlanThreads / kWave) {
         if (s_need[s] == 0) continue;
-        int32_t * table = p.tables + static_cast<int64_t>(s_row[s]) * p.stride;
-        long long at = s_base[s];
-        if (s_claim[s] >= 0) {
-            if (lane == 0) {
-                const int page = list[at];
-                src[s] = s_claim[s];
-                dst[s] = page;
-                table[s_j0[s]] = page;
-                p.refs[page] = 1;
-                atomicSub(&p.refs[s_claim[s]], 1);
-            }
-            ++at;
-        }
-        // entry j0 of a claim holds a page and is passed over here, whether its new number is visible yet or not
+        int32_t * of = p.tables + static_cast<int64_t>(s_row[s]) * p.stride;
+        long long at = s_base[s] + (s_claim[s] >= 0 ? 1 : 0);
+        // the first entry of a claim holds a page and is passed over here, whether its new number is visible yet or not
         for (int b = s_j0[s]; b < s_j1[s]; b += kWave) {
             const int j = b + lane;
-            const bool want = j < s_j1[s] && !is_page(table[min(j, s_j1[s] - 1)], p.n_pages);
+            const bool want = j < s_j1[s] && !is_page(of[min(j, s_j1[s] - 1)], p.n_pages);
             const uint64_t all = __ballot(want);
             if (want) {
                 const int page = list[at + __popcll(all & ((1ull << lane) - 1))];
-                table[j] = page;
+                of[j] = page;
                 p.refs[page] = 1;
             }
             at += __popcll(all);
