@@ -124,10 +124,11 @@ __device__ inline void spread_scales(float v, float (&d)[4 >> GS]) {
 // x row r of a block of 8 stands in rows (r % 2) 4 + r / 2 of the A operand, its second part 8 rows on: a lane's result i
 // belongs to x row 2 i + (lane / 16) % 2, so that up to 2 rows need the first result alone.
 // NB: blocks of 8 x rows.  NI: results of a lane that count (1 or 4).  TW: tiles of a wave's unit, whose blocks are in flight
-// together (2 with SwiGLU: gate and up).  GS: groups of 32 << GS columns.  WHOLE: x fits in LDS, and a wave's share of it in
-// its registers.
-template <int NB, int NI, int TW, bool SWIGLU, int GS, bool WHOLE>
+// together (2 with SwiGLU: gate and up).  GS: groups of 32 << GS columns.  AHEAD: blocks whose weights are in flight while one
+// is multiplied, 0 where x does not fit in LDS (or a wave's share of it in its registers) and comes in pieces.
+template <int NB, int NI, int TW, bool SWIGLU, int GS, int AHEAD>
 __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
+    constexpr bool WHOLE = AHEAD > 0;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     _Float16 * sx = reinterpret_cast<_Float16 *>(lds);            // [chunk / 32][row][part][32]
     __shared__ float s_factor[kQ4MaxRows];                        // RMSNorm factor of each row, times its power of two
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
 
     // weights and scales of the next kAhead blocks are in flight, the first ones while x is prepared; behind its last block a
     // wave loads that one again, so that no branch makes it wait for all
-    constexpr int kAhead = WHOLE ? 2 : 1;
+    constexpr int kAhead = WHOLE ? AHEAD : 1;
     constexpr int kGroups = 4 >> GS;                              // of a block
     u4 w[kAhead][TW];
     _Float16 d[kAhead][TW];
@@ -461,33 +462,46 @@ int check_q4(int32_t out_dim, int32_t in_dim, int32_t group, const char * who) {
     return QA_OK;
 }
 
-template <int NB, int NI, int TW, bool SWIGLU, int GS, bool WHOLE>
-int launch_q4(Q4Params p, hipStream_t stream) {
+template <int NB, int NI, int TW, bool SWIGLU, int GS, int AHEAD>
+int launch_q4_kernel(const Q4Params & p, int blocks, size_t lds, hipStream_t stream) {
+    if (lds > kXBytes / 2) {
+        const void * fn = reinterpret_cast<const void *>(gemv_q4_kernel<NB, NI, TW, SWIGLU, GS, AHEAD>);
+        QA_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+    }
+    hipLaunchKernelGGL((gemv_q4_kernel<NB, NI, TW, SWIGLU, GS, AHEAD>), dim3(static_cast<unsigned>(blocks)), dim3(kQ4Threads), lds, stream, p);
+    QA_LAUNCH_CHECK("gemv_q4_kernel");
+    return QA_OK;
+}
+
+// How the waves divide the work.  Units alone rarely fill the GPU evenly (9496 tiles over 4096 waves are two rounds and a
+// bit), so a unit's columns are shared by up to 8 waves, the more of them the fewer rows x has to be read for: a tile's
+// partial sums then meet in LDS.  x is whole in LDS where it can be, and then no more workgroups run than are resident.
+// Measured with 1 / 2 / 4 / 8 waves per unit, 151936 x 2048: one row 54 / 40 / 34 / 35 us, 8 rows 53 / 45 / 41 / 41, 16 rows
+// 55 / 54 / 59 / 73.
+template <int NB, int NI, int TW, bool SWIGLU, int GS>
+int launch_q4(Q4Params p, bool whole, hipStream_t stream) {
     p.n_units = SWIGLU ? p.n_tiles : (p.n_tiles + TW - 1) / TW;
     const int n_kb = p.in_dim / kTileCols;
-    // waves of a workgroup: over the columns of a unit while the units alone do not fill the GPU
+    const int64_t waves = NB == 1 ? 16384 : NB == 2 ? 8192 : 4096;
     const size_t join = static_cast<size_t>(TW) * NB * NI * kWave * 4, x_whole = static_cast<size_t>(p.in_dim) * p.rows * 4;
     p.wk = 1;
-    while (p.wk < kQ4Waves && p.wk * 2 <= n_kb && static_cast<int64_t>(p.n_units) * p.wk < (NB == 1 ? 16384 : NB == 2 ? 8192 : 4096) &&
-           (!WHOLE || x_whole + (kQ4Waves - kQ4Waves / (p.wk * 2)) * join <= kQ4Lds)) {
+    while (p.wk < kQ4Waves && p.wk * 2 <= n_kb && static_cast<int64_t>(p.n_units) * p.wk < waves &&
+           (!whole || x_whole + (kQ4Waves - kQ4Waves / (p.wk * 2)) * join <= kQ4Lds)) {
         p.wk *= 2;
     }
     p.wt = kQ4Waves / p.wk;
     // x in LDS: all of it, or whole rounds of the waves' blocks
     const int round = p.wk * kTileCols;
-    p.chunk = WHOLE ? p.in_dim : std::min(p.in_dim, std::max(round, kXBytes / (4 * p.rows) / round * round));
+    p.chunk = whole ? p.in_dim : std::min(p.in_dim, std::max(round, kXBytes / (4 * p.rows) / round * round));
     const size_t x_bytes = static_cast<size_t>(p.chunk) * p.rows * 4, joins = p.wt * (p.wk - 1) * join;
-    const size_t lds = WHOLE ? x_bytes + joins : std::max(x_bytes, joins);
-    if (lds > kXBytes / 2) {
-        const void * fn = reinterpret_cast<const void *>(gemv_q4_kernel<NB, NI, TW, SWIGLU, GS, WHOLE>);
-        QA_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-    }
-    // a unit per wave (or group of them); where x is whole, no more workgroups than are resident, which then take several
-    int blocks = (p.n_units + p.wt - 1) / p.wt;
-    if (WHOLE) blocks = std::min(blocks, lds <= 80 * 1024 - 1024 ? 512 : 256);
-    hipLaunchKernelGGL((gemv_q4_kernel<NB, NI, TW, SWIGLU, GS, WHOLE>), dim3(static_cast<unsigned>(blocks)), dim3(kQ4Threads), lds, stream, p);
-    QA_LAUNCH_CHECK("gemv_q4_kernel");
-    return QA_OK;
+    const int units = (p.n_units + p.wt - 1) / p.wt;
+    if (!whole) return launch_q4_kernel<NB, NI, TW, SWIGLU, GS, 0>(p, units, std::max(x_bytes, joins), stream);
+    const size_t lds = x_bytes + joins;
+    const int blocks = std::min(units, lds <= 80 * 1024 - 1024 ? 512 : 256);
+    // a wave that has one unit fetches nothing behind it; with several, two blocks in flight carry over from one to the next
+    // (12288 gate|up rows, one row of x: 7.6 instead of 8.7 us; 151936 rows, 8 rows of x: 41 instead of 42)
+    if (blocks == units) return launch_q4_kernel<NB, NI, TW, SWIGLU, GS, 1>(p, blocks, lds, stream);
+    return launch_q4_kernel<NB, NI, TW, SWIGLU, GS, 2>(p, blocks, lds, stream);
 }
 
 // Whether x fits in LDS and a wave's share of a row in its registers.
@@ -495,30 +509,24 @@ bool whole_x(int rows, int in_dim) {
     return in_dim <= 2048 * row_parts(rows) && static_cast<int64_t>(rows) * in_dim * 4 <= 2 * kXBytes;
 }
 
-template <int NB, int NI, int TW, bool SWIGLU, int GS>
-int launch_q4_x(const Q4Params & p, hipStream_t stream) {
-    const bool whole = whole_x(p.rows, p.in_dim);
-    return whole ? launch_q4<NB, NI, TW, SWIGLU, GS, true>(p, stream) : launch_q4<NB, NI, TW, SWIGLU, GS, false>(p, stream);
-}
-
 template <int TW, bool SWIGLU, int GS>
 int launch_q4_rows(const Q4Params & p, hipStream_t stream) {
-    if (p.rows <= 2) return launch_q4_x<1, 1, TW, SWIGLU, GS>(p, stream);
-    if (p.rows <= 8) return launch_q4_x<1, 4, TW, SWIGLU, GS>(p, stream);
-    if (p.rows <= 16) return launch_q4_x<2, 4, TW, SWIGLU, GS>(p, stream);
+    if (p.rows <= 2) return launch_q4<1, 1, TW, SWIGLU, GS>(p, whole_x(p.rows, p.in_dim), stream);
+    if (p.rows <= 8) return launch_q4<1, 4, TW, SWIGLU, GS>(p, whole_x(p.rows, p.in_dim), stream);
+    if (p.rows <= 16) return launch_q4<2, 4, TW, SWIGLU, GS>(p, whole_x(p.rows, p.in_dim), stream);
     // more than 16 rows whose x does not fit in LDS at once, but half of which does: W is read twice (32 rows of 2048
     // columns: 12288 gate|up rows 33 instead of 57 us, 151936 rows 108 instead of 139)
     if (!whole_x(p.rows, p.in_dim) && whole_x(16, p.in_dim)) {
         Q4Params half = p;
         half.rows = 16;
-        if (const int rc = launch_q4_x<2, 4, TW, SWIGLU, GS>(half, stream); rc != QA_OK) return rc;
+        if (const int rc = launch_q4<2, 4, TW, SWIGLU, GS>(half, whole_x(half.rows, half.in_dim), stream); rc != QA_OK) return rc;
         half.x += static_cast<int64_t>(16) * p.in_dim;
         half.y += static_cast<int64_t>(16) * p.out_dim;
         half.rows = p.rows - 16;
-        if (half.rows <= 8) return launch_q4_x<1, 4, TW, SWIGLU, GS>(half, stream);
-        return launch_q4_x<2, 4, TW, SWIGLU, GS>(half, stream);
+        if (half.rows <= 8) return launch_q4<1, 4, TW, SWIGLU, GS>(half, whole_x(half.rows, half.in_dim), stream);
+        return launch_q4<2, 4, TW, SWIGLU, GS>(half, whole_x(half.rows, half.in_dim), stream);
     }
-    return launch_q4_x<4, 4, TW, SWIGLU, GS>(p, stream);
+    return launch_q4<4, 4, TW, SWIGLU, GS>(p, whole_x(p.rows, p.in_dim), stream);
 }
 
 template <int GS>
