@@ -990,7 +990,7 @@ extern "C" int qa_paged_attn(const float * q, const void * pages, const qa_kv_la
           reinterpret_cast<uintptr_t>(workspace)) & 15) != 0) {
         return fail(QA_ERR_INVALID, "qa_paged_attn: pointers must be aligned to 16 bytes");
     }
-    if (static_cast<int64_t>(batch->n_rows) * n_heads > INT32_MAX) return fail(QA_ERR_INVALID, "qa_paged_attn: too many rows");
+    if (static_cast<int64_t>(batch->n_rows) * n_heads > INT32_MAX / 2) return fail(QA_ERR_INVALID, "qa_paged_attn: too many rows");
     if (const int rc = check_stream(stream, "qa_paged_attn"); rc != QA_OK) return rc;
     const AttnPlan pl = attn_plan(*layout, *batch, n_heads, workspace_bytes);
     if ((static_cast<int64_t>(pl.tiles_many) + pl.tiles_few) * layout->n_kv_heads * pl.splits > INT32_MAX / kThreads) {

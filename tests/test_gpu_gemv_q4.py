@@ -132,12 +132,21 @@ def test_epilogues_and_norm(qa, rows, epi, norm):
     close(gemv(qa, q, d, x, group, epi, w, y0), *plain(q, d, x, epi, w, y0), rel=8e-6 if epi == 2 else 2e-6)
 
 
-def test_vocabulary(qa):
-    """As many rows as the LM head has, several workgroups per CU."""
-    rng = np.random.default_rng(3)
-    q, d = weights(rng, 151936, 256, 32)
-    x = rng.standard_normal((3, 256)).astype(np.float32)
-    close(gemv(qa, q, d, x, 32), *plain(q, d, x))
+@pytest.mark.parametrize("rows,k,group", [(1, 256, 64), (3, 256, 32), (9, 384, 128), (20, 256, 64), (32, 128, 32)])
+def test_vocabulary(qa, rows, k, group):
+    """As many rows as the LM head has: workgroups that take several units each, with and without a join."""
+    rng = np.random.default_rng(rows)
+    q, d = weights(rng, 151936, k, group)
+    x = rng.standard_normal((rows, k)).astype(np.float32)
+    close(gemv(qa, q, d, x, group), *plain(q, d, x))
+
+
+@pytest.mark.parametrize("rows,k", [(2, 128), (8, 384)])
+def test_many_gated_rows(qa, rows, k):
+    rng = np.random.default_rng(k)
+    q, d = weights(rng, 2 * 70016, k, 32)
+    x = rng.standard_normal((rows, k)).astype(np.float32)
+    close(gemv(qa, q, d, x, 32, 2), *plain(q, d, x, 2), rel=8e-6)
 
 
 @pytest.mark.parametrize("scale", [1e-38, 1e-30, 1e-6, 1e5, 1e30])
