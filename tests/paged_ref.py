@@ -50,7 +50,7 @@ def attention(q, pool, layer, tables, page, past, start, n_heads, scale=SCALE, o
     for s in range(len(past)):
         places = None
         for r in range(start[s], min(start[s + 1], len(q))):
-            pos = past[s] + r - start[s]
+            pos = int(past[s]) + r - int(start[s])
             places = visible(tables[s], pool.shape[2], page, pos)
             if not places:
                 out[r] = 0.0

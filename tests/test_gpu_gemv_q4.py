@@ -132,6 +132,28 @@ def test_epilogues_and_norm(qa, rows, epi, norm):
     close(gemv(qa, q, d, x, group, epi, w, y0), *plain(q, d, x, epi, w, y0), rel=8e-6 if epi == 2 else 2e-6)
 
 
+@pytest.mark.parametrize("rows,k", [(1, 16384), (1, 16512), (2, 24576), (9, 8192), (32, 8320)])
+def test_wide_rows(qa, rows, k):
+    """More columns than x has room for in LDS: it comes in pieces (sqrt(k / 32 + 128) 2^-24 + 2^-22: 2.1e-6 at 24576)."""
+    rng = np.random.default_rng(k)
+    q, d = weights(rng, 40, k, 32)
+    x = rng.standard_normal((rows, k)).astype(np.float32)
+    norm = (1 + 0.1 * rng.standard_normal(k)).astype(np.float32)
+    close(gemv(qa, q, d, x, 32, 0, norm), *plain(q, d, x, 0, norm), rel=3e-6)
+
+
+@pytest.mark.parametrize("rows,epi", [(17, 1), (24, 2), (25, 1), (32, 2)])
+def test_two_halves_of_the_rows(qa, rows, epi):
+    """More than 16 rows of 2048 columns run as two halves, each with its own x and y."""
+    rng = np.random.default_rng(rows)
+    out, k, group = 48, 2048, 64
+    q, d = weights(rng, out * (2 if epi == 2 else 1), k, group)
+    x = rng.standard_normal((rows, k)).astype(np.float32)
+    norm = (1 + 0.1 * rng.standard_normal(k)).astype(np.float32)
+    y0 = rng.standard_normal((rows, out)).astype(np.float32) if epi == 1 else None
+    close(gemv(qa, q, d, x, group, epi, norm, y0), *plain(q, d, x, epi, norm, y0), rel=8e-6 if epi == 2 else 2e-6)
+
+
 @pytest.mark.parametrize("rows,k,group", [(1, 256, 64), (3, 256, 32), (9, 384, 128), (20, 256, 64), (32, 128, 32)])
 def test_vocabulary(qa, rows, k, group):
     """As many rows as the LM head has: workgroups that take several units each, with and without a join."""

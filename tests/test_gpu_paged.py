@@ -222,6 +222,103 @@ def test_growing_maximum_and_long_tail(qa):
         assert np.abs(got - want).max() <= 4e-4 * 2 * 6
 
 
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("news", [[1, 1], [3, 20], [70, 1]])
+def test_not_finite_q_stays_in_its_row(qa, f16, news):
+    rng = np.random.default_rng(12)
+    tables, pages = ref.tables_of(rng, [200 + news[0], 9 + news[1]], 16)
+    pool = ref.pool_of(rng, 1, pages, 8, 16, f16)
+    b = ref.Batch(qa, tables, [200, 9], news)
+    q = rng.standard_normal((b.rows, 16, 128)).astype(np.float32)
+    q[0, 3, 7], q[0, 4, 0], q[-1, 9, 100] = np.nan, np.inf, -np.inf
+    got = ref.run_attention(qa, q.reshape(b.rows, -1), pool, 0, b, 16, 16)
+    want = ref.attention(q, pool, 0, tables, 16, b.past, b.start, 16)
+    bad = np.isnan(want)
+    assert bad[0, 3].all() and bad.sum() >= 2 * 128
+    assert np.array_equal(np.isnan(got), bad)
+    close(got[~bad], want[~bad], np.abs(pool.astype(np.float64)).max())
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("max_len", [1, 300, 100000])
+@pytest.mark.parametrize("news", [[1, 1], [90, 1]])
+def test_max_len_is_a_hint(qa, f16, max_len, news):
+    """The last key range takes whatever lies behind the host's bound."""
+    rng = np.random.default_rng(max_len)
+    past = [900, 20]
+    tables, pages = ref.tables_of(rng, [p + n for p, n in zip(past, news)], 32)
+    pool = ref.pool_of(rng, 1, pages, 8, 32, f16)
+    b = ref.Batch(qa, tables, past, news, max_len=max_len)
+    q = rng.standard_normal((b.rows, 2048)).astype(np.float32)
+    got = ref.run_attention(qa, q, pool, 0, b, 32, 16)
+    close(got, ref.attention(q, pool, 0, tables, 32, b.past, b.start, 16), np.abs(pool.astype(np.float64)).max())
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("past", [-3, -(2 ** 31), 2 ** 31 - 1, 2 ** 30])
+@pytest.mark.parametrize("new", [2, 50])
+def test_positions_outside_every_table(qa, f16, past, new):
+    """Tokens before position 0 see nothing; tokens behind the table row see all of it."""
+    rng = np.random.default_rng(1)
+    tables, pages = ref.tables_of(rng, [48, 20], 16, extra=0)
+    pool = ref.pool_of(rng, 1, pages, 8, 16, f16)
+    b = ref.Batch(qa, tables, [past, 19], [new, 1], max_len=64)
+    q = rng.standard_normal((b.rows, 2048)).astype(np.float32)
+    got = ref.run_attention(qa, q, pool, 0, b, 16, 16, fill=2.0)
+    want = ref.attention(q, pool, 0, tables, 16, [int(past), 19], b.start, 16)
+    if past > 0:
+        assert (want[:new] != 0).all()
+    close(got, want, np.abs(pool.astype(np.float64)).max())
+
+
+def test_cache_beyond_32_bit_offsets(qa):
+    """Pages whose K rows lie 3 GB and whose V rows lie 6 GB into the cache: append, attention and copies reach them."""
+    page, pages = 16, 100000
+    lay = ref.layout(qa, 1, pages, 8, page, True)
+    total = qa.lib.qa_kv_cache_bytes(C.byref(lay))
+    assert total > 6 << 30
+    block = 8 * page * 128 * 2
+    base = C.c_void_p()
+    qa.check(qa.lib.qa_device_malloc(C.byref(base), total))
+    try:
+        def at(kv, p):
+            return C.c_void_p(base.value + (kv * pages + int(p)) * block)
+
+        rng = np.random.default_rng(2)
+        past, new = [50, 30], [1, 40]
+        small, count = ref.tables_of(rng, [51, 70], page, spare=0)
+        place = pages - 1 - rng.permutation(400)[:count]              # the last pages of the cache
+        place[0] = pages - 1
+        tables = np.where(small >= 0, place[np.maximum(small, 0)], -1).astype(np.int32)
+        pool = ref.pool_of(rng, 1, count, 8, page, True)
+        for i, p in enumerate(place):
+            for kv in (0, 1):
+                rows = np.ascontiguousarray(pool[0, kv, i])
+                qa.check(qa.lib.qa_copy_to_device(at(kv, p), rows.ctypes.data, block))
+        b = ref.Batch(qa, tables, past, new)
+        qkv = rng.standard_normal((41, 4096)).astype(np.float32)
+        w = np.ones(128, np.float32)
+        d = [qa.DeviceArray.from_numpy(a) for a in (qkv, w, w)]
+        q, out = qa.DeviceArray((41, 2048)), qa.DeviceArray((41, 2048))
+        qa.check(qa.lib.qa_paged_append(*(x.ptr for x in d), q.ptr, base, C.byref(lay), 0, b.ref, 16, 1e6, 1e-6, None))
+        qa.check(qa.lib.qa_paged_attn(q.ptr, base, C.byref(lay), 0, b.ref, 16, ref.SCALE, out.ptr, None, 0, None))
+        src, dst = int(tables[1, 3]), 7                               # and back into the first pages
+        pair = [qa.DeviceArray.from_numpy(np.array([v], np.int32)) for v in (src, dst)]
+        qa.check(qa.lib.qa_pages_copy(base, C.byref(lay), pair[0].ptr, pair[1].ptr, 1, None))
+        qa.synchronize()
+        for i, p in enumerate(place):
+            for kv in (0, 1):
+                qa.check(qa.lib.qa_copy_to_host(pool[0, kv, i].ctypes.data, at(kv, p), block))
+        np.testing.assert_array_equal(pool[0, 1, small[1, 4], :, 5], qkv[40, 3 * 1024:].reshape(8, 128).astype(np.float16))
+        copied = np.empty((8, page, 128), np.float16)
+        qa.check(qa.lib.qa_copy_to_host(copied.ctypes.data, at(1, dst), block))
+        np.testing.assert_array_equal(copied, pool[0, 1, small[1, 3]])
+        want = ref.attention(q.numpy(), pool, 0, small, page, b.past, b.start, 16)
+        close(out.numpy().reshape(want.shape), want, np.abs(pool.astype(np.float64)).max())
+    finally:
+        qa.lib.qa_device_free(base)
+
+
 # ------------------------------------------------------------------------------------------ append
 @pytest.mark.parametrize("f16", [True, False])
 @pytest.mark.parametrize("past,news,page", [([0], [1], 16), ([15, 16, 200], [1, 1, 1], 16), ([3, 0, 60], [40, 0, 5], 32),
