@@ -134,7 +134,8 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     __shared__ float s_factor[kQ4MaxRows];                        // RMSNorm factor of each row, times its power of two
     __shared__ int s_exp[kQ4MaxRows];                             // that power
     __shared__ bool s_inf[kQ4MaxRows];
-    __shared__ float s_sum[kQ4Waves], s_max[kQ4Waves];            // of a row's parts; a sign: an infinity among them
+    __shared__ double s_sum[kQ4Waves];                            // of a row's parts
+    __shared__ float s_max[kQ4Waves];                             // a sign: an infinity among them
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g4 = lane >> 4;
@@ -180,11 +181,13 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     const int cols = 2 * p.rows;
     constexpr int kPer = 8;
     f4 v[kPer];
-    float ss, mx;
+    double ss;
+    float mx;
     bool inf;
     auto read_part = [&](int r) {
         const f4 * x = reinterpret_cast<const f4 *>(p.x + static_cast<int64_t>(r) * p.in_dim);
-        ss = mx = 0.0f;
+        ss = 0.0;
+        mx = 0.0f;
         // rounds that lie behind the row for the whole wave load nothing
         for (int k0 = part * kWave; k0 < n4; k0 += kPer * step) {
             f4 g[kPer];
@@ -202,7 +205,7 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
                 if (nw) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        ss = fmaf(v[u][e], v[u][e], ss);
+                        ss += static_cast<double>(v[u][e]) * v[u][e];
                         v[u][e] *= g[u][e];
                     }
                 }
@@ -210,7 +213,7 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
                 for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(v[u][e]));
             }
         }
-        ss = wave_sum_all(ss);
+        ss = nw ? wave_sum_d_all(ss) : 0.0;
         mx = wave_max_all(mx);
         inf = mx == INFINITY;
         if (__builtin_expect(inf, 0)) {                           // rare: the largest of what is finite
@@ -226,7 +229,7 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
         }
     };
     auto finish_row = [&](int r) {
-        const float f = p.norm_w ? 1.0f / sqrtf(ss / static_cast<float>(p.in_dim) + p.eps) : 1.0f;
+        const float f = p.norm_w ? 1.0f / sqrtf(static_cast<float>(ss / p.in_dim) + p.eps) : 1.0f;
         mx *= f;
         // 2^127 at most, so that it is a float: x below 2^-112 keeps fewer bits of its own headroom, none of its value
         const int ex = mx > 0.0f && mx < INFINITY ? min(kQ4Exp - __builtin_amdgcn_frexp_expf(mx), 127) : 0;
@@ -253,7 +256,8 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
         }
         __syncthreads();
         if (r < p.rows) {
-            ss = mx = 0.0f;
+            ss = 0.0;
+            mx = 0.0f;
             inf = false;
             for (int i = r * parts; i < (r + 1) * parts; ++i) {
                 ss += s_sum[i];

@@ -188,6 +188,15 @@ def test_magnitudes_of_x(qa, scale):
         assert np.linalg.norm(got[r] - want[r]) <= 2e-6 * np.linalg.norm(want[r]) + tiny, (r, scale)
 
 
+def test_norm_of_large_x(qa):
+    """Squares are summed in 64 bits: x whose sum of squares passes f32's range, but not its mean."""
+    rng = np.random.default_rng(8)
+    q, d = weights(rng, 32, 2048, 32)
+    x = (rng.standard_normal((3, 2048)) * 3e18).astype(np.float32)
+    norm = np.ones(2048, np.float32)
+    close(gemv(qa, q, d, x, 32, 0, norm), *plain(q, d, x, 0, norm))
+
+
 @pytest.mark.parametrize("norm", [False, True])
 def test_outliers_in_x(qa, norm):
     """One value 2^20 times the others: the rest keeps its bits."""
