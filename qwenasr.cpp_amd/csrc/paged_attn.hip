@@ -4,9 +4,9 @@
 //
 // in one pass over the keys with a running maximum m and sum (the accumulators are rescaled when m grows).  The query
 // heads of a KV head and the tokens of a sequence are columns of the same products: column c of a tile is token c / group
-// and head c % group, so one token of 2 heads and a chunk of a thousand run the same code, in two shapes: up to 64 columns
-// a workgroup takes 16 of them (8 in the packed form) and its 4 waves share the keys (attn_rows); of longer chunks it
-// takes 128 (f32 pages: 64), a quarter per wave, and the waves share K and V (attn_tile).  A batch of both kinds is one launch.
+// and head c % group, so one token of 2 heads and a chunk of a thousand run the same code, in two shapes: a workgroup
+// takes 16 columns (8 in the packed form) and its 4 waves share the keys (attn_rows), or 128, a quarter per wave, and the
+// waves share K and V (attn_tile, long chunks on f16 pages).  A batch with short and long sequences is one launch.
 //
 // f16 pages on v_mfma_f32_16x16x32_f16: q and p are f32, split into two f16 parts each (a power of two per column brings
 // the largest |q| to 2^14..2^15, p is scaled by 2^6, so the second part keeps its bits); K and V are exact f16.  What the
@@ -45,7 +45,6 @@ constexpr float kShiftLog2 = 6.0f;   // p is scaled by 2^6: at most 2^14 in f16,
 constexpr int kQExp = 15;            // a column's largest |q| goes to [2^14, 2^15)
 constexpr int kMaxSplits = 64;       // key ranges whose results the joining kernel adds, one lane each
 constexpr int kWaves = 4, kThreads = kWaves * kWave;
-constexpr int kMidCols = 64;         // columns of a sequence up to which attn_rows takes it
 // Sequences of few columns: a workgroup holds all of them.  On f16 pages 8 columns lie in both parts in one product.
 constexpr int few_cols(bool f16) { return f16 ? 8 : 16; }
 constexpr int step_keys(bool f16) { return f16 ? 32 : 16; }   // 8 KB of K and 8 KB of V
@@ -54,13 +53,14 @@ struct AttnParams {
     const float * q;
     const void * pages;
     float * out;
-    float * part_o;       // [rows * heads][n_splits][128]
-    f2 * part_ml;         // [rows * heads][n_splits]: reference maximum (log2 units) and sum
+    float * part_o;       // [rows * heads][n_parts][128]
+    f2 * part_ml;         // [rows * heads][n_parts]: reference maximum (log2 units) and sum
     PagedSeqs seqs;
     int32_t n_heads, n_kv, group, n_pages, page_shift, layer;
     int32_t few_max;      // sequences of at most so many columns are of few columns
     int32_t tiles_many, tiles_few;   // upper bounds of both kinds of tiles
-    int32_t n_splits, split_steps;
+    int32_t splits_many, splits_few, steps_many, steps_few;   // key ranges of each kind, and their steps
+    int32_t n_parts;      // ranges that the workspace holds of a (row, head): the more of the two
     float scale;
 };
 
@@ -89,18 +89,20 @@ struct Tile {
     int col0, n_cols;         // the tile's first column, the sequence's columns
     int cap, kend;            // positions of the table row; keys that the tile's last token sees
     int n_steps, step_lo, step_hi;   // steps of kend, and those of this split
+    int split, n_splits;
 };
 
 // Block -> (KV head, split, tile); false: nothing to do.  Neighbouring blocks, which go to different XCDs, take different heads.
 // Every lane counts one sequence's tiles, a prefix sum over the wave finds the sequence that holds the tile; what the tile
 // needs is read along.  FEW: the sequences of 1 .. few_max columns, otherwise the longer ones.
 template <int R, int KS, bool FEW>
-__device__ inline bool find_tile(const AttnParams & p, int block, int lane, Tile & t, int & head, int & split) {
-    const int n_tiles = FEW ? p.tiles_few : p.tiles_many;
+__device__ inline bool find_tile(const AttnParams & p, int block, int lane, Tile & t, int & head) {
+    const int n_tiles = FEW ? p.tiles_few : p.tiles_many, split_steps = FEW ? p.steps_few : p.steps_many;
     head = block % p.n_kv;
     const int rest = block / p.n_kv;
-    split = rest / n_tiles;
-    int tile = rest - split * n_tiles;
+    t.split = rest / n_tiles;
+    t.n_splits = FEW ? p.splits_few : p.splits_many;
+    int tile = rest - t.split * n_tiles;
     for (int s0 = 0; s0 < p.seqs.n_seqs; s0 += kWave) {
         const int s = s0 + lane;
         int n = 0, rows = 0, start = 0, past = 0;
@@ -130,9 +132,9 @@ __device__ inline bool find_tile(const AttnParams & p, int block, int lane, Tile
             t.cap = p.seqs.table_stride << p.page_shift;
             t.kend = max(0, min(t.past + (min(t.col0 + R, t.n_cols) - 1) / p.group, t.cap - 1) + 1);
             t.n_steps = (t.kend + KS - 1) / KS;
-            t.step_lo = split * p.split_steps;
-            t.step_hi = split == p.n_splits - 1 ? t.n_steps : min(t.n_steps, t.step_lo + p.split_steps);
-            return split == 0 || t.step_lo < t.n_steps;               // the first split answers for rows without keys
+            t.step_lo = t.split * split_steps;
+            t.step_hi = t.split == t.n_splits - 1 ? t.n_steps : min(t.n_steps, t.step_lo + split_steps);
+            return t.split == 0 || t.step_lo < t.n_steps;               // the first split answers for rows without keys
         }
         tile -= __builtin_amdgcn_readlane(sum, kWave - 1);
     }
@@ -386,12 +388,11 @@ __device__ inline void split_p(const float (&pr)[2][4], h8 & hi, h8 & lo) {
 }
 
 // 4 values of a column from dim on: the output, or the part of this split (lead: this lane also stores the part's weights).
-__device__ inline void store_column(const AttnParams & p, const int32_t * table, int split, int row, int lim, int dim, f4 v, float mc,
-                                    float l, bool lead) {
-    if (p.n_splits == 1) {
-        *reinterpret_cast<f4 *>(p.out + static_cast<int64_t>(row) * kHeadDim + dim) = v * inverse_sum(p, table, lim, l);
+__device__ inline void store_column(const AttnParams & p, const Tile & t, int row, int lim, int dim, f4 v, float mc, float l, bool lead) {
+    if (t.n_splits == 1) {
+        *reinterpret_cast<f4 *>(p.out + static_cast<int64_t>(row) * kHeadDim + dim) = v * inverse_sum(p, t.table, lim, l);
     } else {
-        const int64_t at = static_cast<int64_t>(row) * p.n_splits + split;
+        const int64_t at = static_cast<int64_t>(row) * p.n_parts + t.split;
         *reinterpret_cast<f4 *>(p.part_o + at * kHeadDim + dim) = v;
         if (lead) p.part_ml[at] = f2{mc, l};
     }
@@ -423,16 +424,15 @@ __device__ inline void close_columns(const int (&orow)[NB], const float (&c)[NB]
 
 // The flagged columns of a block, key by key; their values are stored at once.
 template <typename CT, int KS>
-__device__ inline void redo_columns(const AttnParams & p, const int32_t * table, int head, int split, int lane, int lim, int orow,
-                                    uint32_t redo, int step_lo, int step_hi) {
+__device__ inline void redo_columns(const AttnParams & p, const Tile & t, int head, int lane, int lim, int orow, uint32_t redo) {
     for (uint32_t left = redo; left != 0; left &= left - 1) {
         const int col = __ffs(left) - 1;
         const int row = __builtin_amdgcn_readlane(orow, col), lm = __builtin_amdgcn_readlane(lim, col);
         float cm, cl;
         f2 co;
-        column_by_keys<CT, KS>(p, table, head, p.q + static_cast<int64_t>(row) * kHeadDim, lm, step_lo, step_hi, 1, lane, cm, cl, co);
+        column_by_keys<CT, KS>(p, t.table, head, p.q + static_cast<int64_t>(row) * kHeadDim, lm, t.step_lo, t.step_hi, 1, lane, cm, cl, co);
         const f2 nx = f2{__shfl_down(co[0], 1, kWave), __shfl_down(co[1], 1, kWave)};
-        if ((lane & 1) == 0) store_column(p, table, split, row, lm, 2 * lane, f4{co[0], co[1], nx[0], nx[1]}, cm, cl, lane == 0);
+        if ((lane & 1) == 0) store_column(p, t, row, lm, 2 * lane, f4{co[0], co[1], nx[0], nx[1]}, cm, cl, lane == 0);
     }
 }
 
@@ -451,8 +451,8 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g4 = lane >> 4;
     Tile t;
-    int head, split;
-    if (!find_tile<R, KS, FEW>(p, block, lane, t, head, split)) return;          // uniform for the workgroup
+    int head;
+    if (!find_tile<R, KS, FEW>(p, block, lane, t, head)) return;          // uniform for the workgroup
     const Column col = column_of(p, t, head, t.col0 + (PACK ? c16 & 7 : c16));
     f4 x[NB][8];
     load_q<F16>(col, g4, x[0]);
@@ -627,38 +627,37 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
             ls += sl[w * R + cc] * f;
             o += *reinterpret_cast<const f4 *>(so + (w * R + cc) * kRowsStride + dim) * f;
         }
-        store_column(p, t.table, split, row, slim[cc], dim, o, M, ls, dim == 0);
+        store_column(p, t, row, slim[cc], dim, o, M, ls, dim == 0);
     }
 }
 
-// 128 columns of a long chunk (f32 pages: 64): 4 waves of 32 (16) each share the K and V of a tile of keys through LDS, which
-// cuts what the CUs pull from L2 to a quarter (without it that traffic sets the pace).  On f32 pages, whose products take
-// eight times as long, narrower tiles leave fewer columns empty: two sequences of 157 and 144 tokens behind 1037 and 701
-// positions 45.7 instead of 50.3 us.  A tile of keys is two steps; a step lies in LDS as
-// the MFMA operands themselves, 8 of K and 8 of V^T, 64 lanes x 16 bytes each: every read and write is one unbroken
-// kilobyte and no wave rearranges anything.  Waves 0 and 1 fetch (and on f16 pages transpose) V of the two steps, waves 2
-// and 3 fetch K.  Two tiles in LDS, the next one's rows in registers: one barrier per tile, and two workgroups per CU, each
-// multiplying while the other waits at its barrier.
+// 128 columns of a long chunk on f16 pages: 4 waves of 32 each share the K and V of a tile of keys through LDS, which cuts what
+// the CUs pull from L2 to an eighth of what attn_rows' tiles do; for long chunks far behind that traffic sets the pace.  A tile of
+// keys is two steps; a step lies in LDS as the MFMA operands themselves, 8 of K and 8 of V^T, 64 lanes x 16 bytes each:
+// every read and write is one unbroken kilobyte and no wave rearranges anything.  Waves 0 and 1 fetch and transpose V of
+// the two steps, waves 2 and 3 fetch K.  Two tiles in LDS, the next one's rows in registers: one barrier per tile, and two
+// workgroups per CU, each multiplying while the other waits at its barrier.  (On f32 pages, whose products take four times
+// as long, the same scheme took 101 us against 112 of attn_rows at 300 tokens behind 3500 positions, 281 / 302 at 1024 behind
+// 2889, but 88 / 58 at 1024 behind none and 136 / 111 at four of 256 behind 500 to 1500: attn_rows takes them all.)
 constexpr int kTileSteps = 2;
 static_assert(kWaves == 2 * kTileSteps, "a wave fetches K or V of one step");
-constexpr int tile_blocks(bool f16) { return f16 ? 2 : 1; }       // of 16 columns per wave
-constexpr int tile_cols(bool f16) { return kWaves * 16 * tile_blocks(f16); }
+constexpr int kTileCols = kWaves * 32;
 constexpr int kStepBytes = 16 * kWave * 16;   // a step's 16 operands
 constexpr size_t kTileLds = 2 * kTileSteps * kStepBytes;
 constexpr int kOutStride = kHeadDim + 4, kOutFloats = 16 * kOutStride;   // a wave's 16 columns on their way out
 static_assert(kWaves * kOutFloats * sizeof(float) <= kTileLds, "the outputs go through the operands' LDS");
 
-template <typename CT>
 __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
-    constexpr bool F16 = std::is_same<CT, _Float16>::value;
-    constexpr int KS = step_keys(F16), KB = KS / 16, NB = tile_blocks(F16);
+    typedef _Float16 CT;
+    constexpr bool F16 = true;
+    constexpr int KS = step_keys(F16), KB = KS / 16, NB = 2;
     __shared__ int s_holes[2][kTileSteps];                            // bit kb: 16-key block kb of the step lies on no page
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g4 = lane >> 4;
     Tile t;
-    int head, split;
-    if (!find_tile<tile_cols(F16), KS, false>(p, block, lane, t, head, split)) return;   // uniform for the workgroup
+    int head;
+    if (!find_tile<kTileCols, KS, false>(p, block, lane, t, head)) return;   // uniform for the workgroup
 
     // columns: their q is on its way while the first tile is fetched
     int lim[NB], orow[NB];
@@ -699,7 +698,7 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
         }
 #pragma unroll
         for (int f = 0; f < 8; ++f) {
-            r[f] = *reinterpret_cast<const u4 *>(at[F16 ? f >> 2 : 0] + (fetch_v ? v_offset<F16>(f, c16, g4) : k_offset<F16>(f, c16, g4)));
+            r[f] = *reinterpret_cast<const u4 *>(at[f >> 2] + (fetch_v ? v_offset<F16>(f, c16, g4) : k_offset<F16>(f, c16, g4)));
         }
     };
     auto put = [&](int buf) {
@@ -711,15 +710,15 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
             if (hole) {   // rows that no column sees, and of no page: not even 0 times what memory holds
 #pragma unroll
                 for (int f = 0; f < 8; ++f) {
-                    if (st_held * KS + v_key<F16>(f, g4) >= t.kend || pg[F16 ? f >> 2 : 0] < 0) r[f] = u4{0, 0, 0, 0};
+                    if (st_held * KS + v_key<F16>(f, g4) >= t.kend || pg[f >> 2] < 0) r[f] = u4{0, 0, 0, 0};
                 }
             }
 #pragma unroll
-            for (int f = 0; f < 8; ++f) *reinterpret_cast<u4 *>(to + (8 + f) * kWave * 16) = F16 ? transposed(r, f) : r[f];
+            for (int f = 0; f < 8; ++f) *reinterpret_cast<u4 *>(to + (8 + f) * kWave * 16) = transposed(r, f);
         } else {
 #pragma unroll
             for (int f = 0; f < 8; ++f) *reinterpret_cast<u4 *>(to + f * kWave * 16) = r[f];
-            if (lane == 0) s_holes[buf][mine] = (pg[0] < 0 ? 1 : 0) | (pg[KB - 1] < 0 ? 1 << (KB - 1) : 0);
+            if (lane == 0) s_holes[buf][mine] = (pg[0] < 0 ? 1 : 0) | (pg[1] < 0 ? 2 : 0);
         }
     };
 
@@ -733,8 +732,7 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
     h8 qh[NB][4], ql[NB][4];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-        if constexpr (F16) split_q(x[nb], p.scale, c[nb], qh[nb], ql[nb]);
-        else c[nb] = p.scale * kLog2e;
+        split_q(x[nb], p.scale, c[nb], qh[nb], ql[nb]);
     }
     float m[NB], l[NB];
     f4 O[NB][8];
@@ -770,30 +768,16 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
             if (st >= full || holes != 0) mask_step<NB, KB>(S, lim, st * KS, g4, holes);
             float pr[NB][KB][4];
             softmax_step<NB, KB>(S, c, m, l, O, pr);
-            if constexpr (F16) {
-                h8 ph[NB], pl[NB];
+            h8 ph[NB], pl[NB];
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) split_p(pr[nb], ph[nb], pl[nb]);
+            for (int nb = 0; nb < NB; ++nb) split_p(pr[nb], ph[nb], pl[nb]);
 #pragma unroll
-                for (int part = 0; part < 2; ++part) {
+            for (int part = 0; part < 2; ++part) {
 #pragma unroll
-                    for (int db = 0; db < 8; ++db) {
+                for (int db = 0; db < 8; ++db) {
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
-                            O[nb][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, v[db]), part ? pl[nb] : ph[nb], O[nb][db], 0, 0, 0);
-                        }
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int f = 0; f < 8; ++f) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
-                            O[nb][(f & 1) * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f4, v[f])[e], pr[nb][0][f >> 1],
-                                                                                          O[nb][(f & 1) * 4 + e], 0, 0, 0);
-                        }
+                    for (int nb = 0; nb < NB; ++nb) {
+                        O[nb][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, v[db]), part ? pl[nb] : ph[nb], O[nb][db], 0, 0, 0);
                     }
                 }
             }
@@ -830,9 +814,9 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
             const int row = __shfl(orow[nb], col, kWave), lm = __shfl(lim[nb], col, kWave);
             const float cm = __shfl(mc[nb], col, kWave), cl = __shfl(l[nb], col, kWave);
             const f4 v = *reinterpret_cast<const f4 *>(so + col * kOutStride + dim);
-            if (row >= 0 && !((redo[nb] >> col) & 1)) store_column(p, t.table, split, row, lm, dim, v, cm, cl, dim == 0);
+            if (row >= 0 && !((redo[nb] >> col) & 1)) store_column(p, t, row, lm, dim, v, cm, cl, dim == 0);
         }
-        redo_columns<CT, KS>(p, t.table, head, split, lane, lim[nb], orow[nb], redo[nb], t.step_lo, t.step_hi);
+        redo_columns<CT, KS>(p, t, head, lane, lim[nb], orow[nb], redo[nb]);
     }
 }
 
@@ -846,17 +830,17 @@ __global__ __launch_bounds__(kThreads, 3) void paged_rows_kernel(AttnParams p) {
 template <typename CT>
 __global__ __launch_bounds__(kThreads, 3) void paged_rows_both_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_rows[];
-    const int many = p.tiles_many * p.n_kv * p.n_splits, block = blockIdx.x;
+    const int many = p.tiles_many * p.n_kv * p.splits_many, block = blockIdx.x;
     if (block < many) attn_rows<CT, false>(p, block, lds_rows);
     else attn_rows<CT, true>(p, block - many, lds_rows);
 }
 
-template <typename CT, bool BOTH>
+template <bool BOTH>
 __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_tile[];
-    const int many = p.tiles_many * p.n_kv * p.n_splits, block = blockIdx.x;
-    if (!BOTH || block < many) attn_tile<CT>(p, block, lds_tile);
-    else attn_rows<CT, true>(p, block - many, lds_tile);
+    const int many = p.tiles_many * p.n_kv * p.splits_many, block = blockIdx.x;
+    if (!BOTH || block < many) attn_tile(p, block, lds_tile);
+    else attn_rows<_Float16, true>(p, block - many, lds_tile);
 }
 
 // Joins the splits of each (row, head): one wave each, lane = split for the weights, then lane = 2 dims.  Its time is
@@ -868,17 +852,20 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int ks) {
     const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (item >= static_cast<int64_t>(p.seqs.n_rows) * p.n_heads) return;
     const int row = static_cast<int>(item / p.n_heads);
-    const float * po = p.part_o + item * p.n_splits * kHeadDim + 2 * lane;
-    f2 ml = p.part_ml[item * p.n_splits + min(lane, p.n_splits - 1)];
+    const float * po = p.part_o + item * p.n_parts * kHeadDim + 2 * lane;
+    f2 ml = p.part_ml[item * p.n_parts + min(lane, p.n_parts - 1)];
     f2 part[kFirst];
 #pragma unroll
-    for (int s = 0; s < kFirst; ++s) part[s] = *reinterpret_cast<const f2 *>(po + min(s, p.n_splits - 1) * kHeadDim);
+    for (int s = 0; s < kFirst; ++s) part[s] = *reinterpret_cast<const f2 *>(po + min(s, p.n_parts - 1) * kHeadDim);
     const RowPlace at = row_place(p.seqs, row, lane);
     if (at.seq < 0) return;
+    const bool few = at.rows * p.group <= p.few_max;
+    const int n_splits = few ? p.splits_few : p.splits_many, split_steps = few ? p.steps_few : p.steps_many;
+    if (n_splits == 1) return;                                        // stored by its tile
     const int cap = p.seqs.table_stride << p.page_shift;
     const int lim = min(at.pos, cap - 1);
     // splits that hold a key which this row sees (the first is always computed)
-    const int active = lim < 0 ? 1 : min(p.n_splits, lim / ks / p.split_steps + 1);
+    const int active = lim < 0 ? 1 : min(n_splits, lim / ks / split_steps + 1);
     if (lane >= active) ml = f2{-INFINITY, 0.0f};
     const float M = wave_max_all(ml[0]);
     const float f = ml[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[0] - M);
@@ -901,65 +888,84 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int ks) {
     *reinterpret_cast<f2 *>(p.out + item * kHeadDim + 2 * lane) = o * inv;
 }
 
-// How a call cuts its work: which kinds of tiles there are, their upper bounds, and the key ranges.
+// How a call cuts its work: which kinds of tiles there are, their upper bounds, and the key ranges of each kind.
 struct AttnPlan {
     bool tile;               // the longer sequences' tiles are attn_tile's
     int tiles_many, tiles_few;
     int few_max;             // 0: sequences of few columns are the longer ones' tiles, too
-    int splits, split_steps; // in steps of the cache type
+    int splits_many, splits_few, steps_many, steps_few;
+    int parts() const { return std::max(splits_many, splits_few); }
 };
+
+// Key ranges of `steps` steps for workgroups of which one range has `blocks`: enough to make `target` of them, none shorter
+// than `least` steps.
+void cut_keys(int steps, int64_t blocks, int64_t target, int64_t least, int64_t most, int & splits, int & split_steps) {
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>({target / std::max<int64_t>(blocks, 1), (steps + least - 1) / least, most}));
+    split_steps = std::max<int>(1, static_cast<int>((steps + n - 1) / n));
+    splits = std::max(1, (steps + split_steps - 1) / split_steps);
+}
 
 AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_heads, size_t workspace_bytes) {
     const bool f16 = l.cache_type == QA_CACHE_F16;
     const int ks = step_keys(f16);
     const int group = n_heads / l.n_kv_heads;
     const int seqs = std::min(b.n_seqs, b.n_rows);
-    const int64_t most = std::min<int64_t>(b.n_rows, b.max_tokens > 0 ? b.max_tokens : b.n_rows) * group;   // columns of a sequence
-    const int64_t cols = static_cast<int64_t>(b.n_rows) * group;
-    AttnPlan pl{};
-    // Up to 64 columns four waves that share the keys beat four that share K and V (one sequence behind 3900 positions, 8 / 16
-    // / 32 tokens: 14.1 / 16.6 / 20.6 against 22.3 / 23.4 / 24.1 us; eight of 32 tokens 30.3 against 49.3); at 128 they are even.
-    pl.tile = most > kMidCols;
-    const bool many = most > few_cols(f16);
-    const int width = pl.tile ? tile_cols(f16) : 16;
-    pl.tiles_many = many ? static_cast<int>(cols / width + seqs) : 0;
-    // f32 pages have no packed form: short sequences are tiles of attn_rows like the others.  One sequence is of one kind.
-    const bool few = !many || ((f16 || pl.tile) && b.n_seqs > 1);
-    pl.few_max = few ? few_cols(f16) : 0;
-    pl.tiles_few = few ? seqs : 0;
+    const int64_t tokens = std::min<int64_t>(b.n_rows, b.max_tokens > 0 ? b.max_tokens : b.n_rows);
+    const int64_t most = tokens * group, cols = static_cast<int64_t>(b.n_rows) * group;   // columns of a sequence, of all
     const int64_t cap = static_cast<int64_t>(b.table_stride) * l.max_seq;
     const int64_t len = std::min<int64_t>(cap, b.max_len > 0 ? b.max_len : cap);
     const int steps = static_cast<int>((len + ks - 1) / ks);
-    // workgroups that fill the GPU, each of two steps per wave or four of a tile at least
-    const int64_t tiles = std::max<int64_t>(1, many ? (cols + width - 1) / width : seqs);
-    const int64_t target = pl.tile ? 512 : 1024, least = pl.tile ? 4 : 8;
-    int64_t splits = std::max<int64_t>(1, std::min<int64_t>({target / (tiles * l.n_kv_heads), (steps + least - 1) / least, kMaxSplits}));
-    const size_t per_split = static_cast<size_t>(b.n_rows) * n_heads * (kHeadDim + 2) * sizeof(float);
-    if (splits > 1 && per_split * splits > workspace_bytes) splits = std::max<int64_t>(1, static_cast<int64_t>(workspace_bytes / per_split));
-    pl.split_steps = std::max<int>(1, static_cast<int>((steps + splits - 1) / splits));
-    pl.splits = std::max(1, (steps + pl.split_steps - 1) / pl.split_steps);
+    const size_t per_part = static_cast<size_t>(b.n_rows) * n_heads * (kHeadDim + 2) * sizeof(float);
+    const int64_t parts = std::min<int64_t>(kMaxSplits, std::max<size_t>(1, workspace_bytes / per_part));
+    AttnPlan pl{};
+    const bool many = most > few_cols(f16);
+    // attn_tile (f16 pages) against attn_rows, us.  256 tokens behind 3000 positions 37 / 39, 400 behind 2000 38 / 46, 700 behind
+    // 1500 46 / 58, 1024 behind 500 45.5 / 47, behind 2889 80 / 129; but 512 behind 1000 34 / 31, 1024 behind none 38 / 31,
+    // eight of 100 tokens behind 2000 (columns left empty) 65 / 53: by the products, where a sequence fills three tiles.
+    pl.tile = f16 && most > 2 * kTileCols && cols * (len - std::min(len, tokens / 2)) > 1600000;
+    const int width = pl.tile ? kTileCols : 16;
+    pl.tiles_many = many ? static_cast<int>(cols / width + seqs) : 0;
+    const bool few = !many || b.n_seqs > 1;                           // one sequence is of one kind
+    pl.few_max = few ? few_cols(f16) : 0;
+    pl.tiles_few = few ? seqs : 0;
+    // Workgroups to make of the keys, us.  Decode steps, and sequences of one tile: K and V are what they read, and more, shorter
+    // ranges keep more of them in flight.  Longer ones read K and V once per tile, from L2, and every range writes and reads
+    // its columns' partial results: 256 tokens behind 1000 positions (256 tiles) in 1 / 2 / 3 ranges 17.5 / 23 / 24, 64 behind
+    // 3000 (64 tiles) in 4 / 6 / 8 38 / 30 / 34 (f32 pages).  With few CUs left over by the tiles of a long context their
+    // partial results cost less than the wait for the CUs that have one more: 300 behind 3500 (304 tiles), f32 pages, 112 in
+    // three, 140 in one.  Sequences differ in length, and the ranges are cut for the longest: 16 of 70 behind 300 to 2000 at
+    // 384 / 640 workgroups 38 / 33 (f32: 76 / 59).  attn_tile has 512 at a time: one sequence of 400 behind 3500 at 512 / 768
+    // 47 / 56, but two of 600 and ten of one token behind 24 to 3500 98 / 73, four of 256 behind 500 to 1500 53 / 57.
+    const int64_t tiles = std::max<int64_t>(1, (cols + width - 1) / width) * l.n_kv_heads, heads = static_cast<int64_t>(seqs) * l.n_kv_heads;
+    const bool one = b.n_seqs == 1;
+    if (pl.tile) cut_keys(steps, tiles, one ? 512 : 768, 4, parts, pl.splits_many, pl.steps_many);
+    else if (most <= 16) cut_keys(steps, heads, 1024, 8, parts, pl.splits_many, pl.steps_many);
+    else cut_keys(steps, tiles, !one ? 640 : steps >= 128 && tiles > 192 ? 1024 : 384, 16, parts, pl.splits_many, pl.steps_many);
+    cut_keys(steps, heads, 1024, 8, parts, pl.splits_few, pl.steps_few);
+    if (!many) pl.splits_many = 1;
+    if (!few) pl.splits_few = 1;
     return pl;
 }
 
 template <typename CT>
 int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
     constexpr bool F16 = std::is_same<CT, _Float16>::value;
-    const dim3 grid(static_cast<unsigned>(p.n_kv) * pl.splits * (pl.tiles_many + pl.tiles_few));
+    const dim3 grid(static_cast<unsigned>(p.n_kv) * (pl.tiles_many * pl.splits_many + pl.tiles_few * pl.splits_few));
     constexpr size_t lds_few = rows_lds(F16, true), lds_many = rows_lds(F16, false);
     static_assert(lds_few <= kTileLds && lds_few <= lds_many, "a launch of both kinds has the longer ones' LDS");
-    if (pl.tile) {
-        const auto kernel = pl.few_max ? &paged_tile_kernel<CT, true> : &paged_tile_kernel<CT, false>;
+    if (F16 && pl.tile) {
+        const auto kernel = pl.few_max ? &paged_tile_kernel<true> : &paged_tile_kernel<false>;
         QA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kTileLds)));
         hipLaunchKernelGGL(kernel, grid, dim3(kThreads), kTileLds, stream, p);
     } else if (!pl.tiles_many) {
         hipLaunchKernelGGL((paged_rows_kernel<CT, true>), grid, dim3(kThreads), lds_few, stream, p);
-    } else if (F16 && pl.few_max) {
-        hipLaunchKernelGGL((paged_rows_both_kernel<_Float16>), grid, dim3(kThreads), lds_many, stream, p);
+    } else if (pl.few_max) {
+        hipLaunchKernelGGL((paged_rows_both_kernel<CT>), grid, dim3(kThreads), lds_many, stream, p);
     } else {
         hipLaunchKernelGGL((paged_rows_kernel<CT, false>), grid, dim3(kThreads), lds_many, stream, p);
     }
     QA_LAUNCH_CHECK("paged attention kernel");
-    if (pl.splits > 1) {
+    if (pl.parts() > 1) {
         const int64_t items = static_cast<int64_t>(p.seqs.n_rows) * p.n_heads;
         hipLaunchKernelGGL(paged_join_kernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, p, step_keys(F16));
         QA_LAUNCH_CHECK("paged_join_kernel");
@@ -974,8 +980,8 @@ extern "C" size_t qa_paged_attn_workspace_bytes(const qa_kv_layout * layout, con
     using namespace qa;
     if (check_batch(layout, 0, batch, n_heads, "qa_paged_attn_workspace_bytes") != QA_OK || batch->n_rows == 0) return 0;
     const AttnPlan pl = attn_plan(*layout, *batch, n_heads, SIZE_MAX);
-    if (pl.splits <= 1) return 0;
-    return static_cast<size_t>(batch->n_rows) * n_heads * pl.splits * (kHeadDim + 2) * sizeof(float);
+    if (pl.parts() <= 1) return 0;
+    return static_cast<size_t>(batch->n_rows) * n_heads * pl.parts() * (kHeadDim + 2) * sizeof(float);
 }
 
 extern "C" int qa_paged_attn(const float * q, const void * pages, const qa_kv_layout * layout, int32_t layer,
@@ -993,7 +999,7 @@ extern "C" int qa_paged_attn(const float * q, const void * pages, const qa_kv_la
     if (static_cast<int64_t>(batch->n_rows) * n_heads > INT32_MAX / 2) return fail(QA_ERR_INVALID, "qa_paged_attn: too many rows");
     if (const int rc = check_stream(stream, "qa_paged_attn"); rc != QA_OK) return rc;
     const AttnPlan pl = attn_plan(*layout, *batch, n_heads, workspace_bytes);
-    if ((static_cast<int64_t>(pl.tiles_many) + pl.tiles_few) * layout->n_kv_heads * pl.splits > INT32_MAX / kThreads) {
+    if ((static_cast<int64_t>(pl.tiles_many) * pl.splits_many + static_cast<int64_t>(pl.tiles_few) * pl.splits_few) * layout->n_kv_heads > INT32_MAX / kThreads) {
         return fail(QA_ERR_INVALID, "qa_paged_attn: too many rows");
     }
     AttnParams p{};
@@ -1001,7 +1007,7 @@ extern "C" int qa_paged_attn(const float * q, const void * pages, const qa_kv_la
     p.pages = pages;
     p.out = out;
     p.part_o = static_cast<float *>(workspace);
-    p.part_ml = reinterpret_cast<f2 *>(p.part_o + static_cast<int64_t>(batch->n_rows) * n_heads * pl.splits * kHeadDim);
+    p.part_ml = reinterpret_cast<f2 *>(p.part_o + static_cast<int64_t>(batch->n_rows) * n_heads * pl.parts() * kHeadDim);
     p.seqs = paged_seqs(*batch);
     p.n_heads = n_heads;
     p.n_kv = layout->n_kv_heads;
@@ -1012,8 +1018,11 @@ extern "C" int qa_paged_attn(const float * q, const void * pages, const qa_kv_la
     p.few_max = pl.few_max;
     p.tiles_many = pl.tiles_many;
     p.tiles_few = pl.tiles_few;
-    p.n_splits = pl.splits;
-    p.split_steps = pl.split_steps;
+    p.splits_many = pl.splits_many;
+    p.splits_few = pl.splits_few;
+    p.steps_many = pl.steps_many;
+    p.steps_few = pl.steps_few;
+    p.n_parts = pl.parts();
     p.scale = scale;
     return layout->cache_type == QA_CACHE_F16 ? launch_attn<_Float16>(pl, p, as_stream(stream)) : launch_attn<float>(pl, p, as_stream(stream));
 }

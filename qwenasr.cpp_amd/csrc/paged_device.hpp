@@ -17,8 +17,9 @@ inline PagedSeqs paged_seqs(const qa_paged_batch & b) {
 }
 
 struct RowPlace {
-    int seq;   // -1: the row belongs to no sequence
+    int seq;    // -1: the row belongs to no sequence
     int pos;
+    int rows;   // the sequence's
 };
 
 // The sequence whose rows hold `row`: row_start does not fall, so it is the number of sequences that end at or before
@@ -32,9 +33,10 @@ __device__ inline RowPlace row_place(const PagedSeqs & b, int row, int lane) {
         if (l == kWave) continue;
         const int first = __builtin_amdgcn_readlane(start, l);
         if (s0 + l >= b.n_seqs || first < 0 || first > row) break;
-        return RowPlace{s0 + l, bounded_past(__builtin_amdgcn_readlane(past, l)) + row - first};
+        return RowPlace{s0 + l, bounded_past(__builtin_amdgcn_readlane(past, l)) + row - first,
+                        rows_between(first, __builtin_amdgcn_readlane(end, l), b.n_rows)};
     }
-    return RowPlace{-1, 0};
+    return RowPlace{-1, 0, 0};
 }
 
 }  // namespace qa
