@@ -35,6 +35,7 @@ constexpr int kQ4Waves = 8;                        // per workgroup
 constexpr int kQ4Threads = kQ4Waves * kWave;
 constexpr int kXBytes = 64 * 1024;                 // of x in LDS at a time: two workgroups per CU
 constexpr size_t kQ4Lds = 158 * 1024;              // of the CU's 160 KB, the rest is the kernel's own
+constexpr int kMaxExp = 127;                       // a power of two that is a float: x below 2^-112 keeps fewer bits
 constexpr int kQ4Exp = 15;                        // a row's largest finite |x| goes to [2^14, 2^15)
 
 struct Q4Params {
@@ -46,7 +47,6 @@ struct Q4Params {
     int32_t out_dim, in_dim, rows;
     int32_t n_tiles, n_units;                     // tiles of y, and how many units of work they make
     int32_t wt, wk;                               // waves over units and over columns: wt * wk = kQ4Waves
-    int32_t chunk;                                // columns of x in LDS at a time
     int32_t epilogue;
     float eps;
 };
@@ -98,6 +98,28 @@ __device__ inline void split_x(f4 v, float factor, bool inf, _Float16 * to) {
     *reinterpret_cast<h4 *>(to + 32) = lo;
 }
 
+// The A operand of lanes c16 and c16 + 8 of a row from four scaled values each: the first parts of the eight in one, the second
+// parts in the other.  Scaling was by a power of two, so that no product is rounded here.
+__device__ inline h8 split_pair(f4 v, bool inf, bool second) {
+    h4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        hi[e] = static_cast<_Float16>(v[e]);
+        lo[e] = static_cast<_Float16>(v[e] - static_cast<float>(hi[e]));
+    }
+    if (__builtin_expect(inf, 0)) {
+        asm volatile("");                                         // a branch, not a selection per value
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lo[e] = fabsf(v[e]) == INFINITY ? static_cast<_Float16>(0.0f) : lo[e];
+    }
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    const u2 h = __builtin_bit_cast(u2, hi), l = __builtin_bit_cast(u2, lo);
+    const u2 send = second ? h : l;                               // to the other lane
+    const u2 got = {__float_as_uint(row_ror8(__uint_as_float(send[0]))), __float_as_uint(row_ror8(__uint_as_float(send[1])))};
+    const u4 a = second ? u4{got[0], got[1], l[0], l[1]} : u4{h[0], h[1], got[0], got[1]};
+    return __builtin_bit_cast(h8, a);
+}
+
 // The scales of a block's groups in every lane, from one value per lane: groups of 32 lie in the four rows of 16 lanes, groups
 // of 64 in the first two (and again in the others).
 template <int GS>
@@ -125,12 +147,11 @@ __device__ inline void spread_scales(float v, float (&d)[4 >> GS]) {
 // belongs to x row 2 i + (lane / 16) % 2, so that up to 2 rows need the first result alone.
 // NB: blocks of 8 x rows.  NI: results of a lane that count (1 or 4).  TW: tiles of a wave's unit, whose blocks are in flight
 // together (2 with SwiGLU: gate and up).  GS: groups of 32 << GS columns.  AHEAD: blocks whose weights are in flight while one
-// is multiplied, 0 where x does not fit in LDS (or a wave's share of it in its registers) and comes in pieces.
+// is multiplied.  All of x lies in LDS.
 template <int NB, int NI, int TW, bool SWIGLU, int GS, int AHEAD>
 __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
-    constexpr bool WHOLE = AHEAD > 0;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    _Float16 * sx = reinterpret_cast<_Float16 *>(lds);            // [chunk / 32][row][part][32]
+    _Float16 * sx = reinterpret_cast<_Float16 *>(lds);            // [in_dim / 32][row][part][32]
     __shared__ float s_factor[kQ4MaxRows];                        // RMSNorm factor of each row, times its power of two
     __shared__ int s_exp[kQ4MaxRows];                             // that power
     __shared__ bool s_inf[kQ4MaxRows];
@@ -145,13 +166,12 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     const int unit_step = static_cast<int>(gridDim.x) * p.wt;
     const int unit0 = wt * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
 
-    // weights and scales of the next kAhead blocks are in flight, the first ones while x is prepared; behind its last block a
+    // weights and scales of the next AHEAD blocks are in flight, the first ones while x is prepared; behind its last block a
     // wave loads that one again, so that no branch makes it wait for all
-    constexpr int kAhead = WHOLE ? AHEAD : 1;
     constexpr int kGroups = 4 >> GS;                              // of a block
-    u4 w[kAhead][TW];
-    _Float16 d[kAhead][TW];
-    const int n_it = (n_kb + p.wk * kAhead - 1) / (p.wk * kAhead) * kAhead;   // a wave's blocks of a unit, the last ones perhaps idle
+    u4 w[AHEAD][TW];
+    _Float16 d[AHEAD][TW];
+    const int n_it = (n_kb + p.wk * AHEAD - 1) / (p.wk * AHEAD) * AHEAD;   // a wave's blocks of a unit, the last ones perhaps idle
     const uint32_t w_lane = lane * 16, d_lane = (lane & (kGroups * kTileRows - 1)) * 2;
     int f_unit = unit0, f_it = 0;
     auto fetch = [&](int slot) {
@@ -171,7 +191,7 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
         }
     };
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) fetch(u);
+    for (int u = 0; u < AHEAD; ++u) fetch(u);
 
     // Sum of squares and largest |x| of each row: the 8 waves share up to 8 rows, each taking a part of a row whose loads are
     // in flight together.  A workgroup that holds all of x writes its parts from those registers.
@@ -239,12 +259,10 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
             s_exp[r] = ex;
             s_inf[r] = inf;
         }
-        if constexpr (WHOLE) {
 #pragma unroll
-            for (int u = 0; u < kPer; ++u) {
-                const int k = part * kWave + lane + u * step;
-                if (k < n4) split_x(v[u], factor, inf, sx + ((k >> 3) * cols + 2 * r) * 32 + (k & 7) * 4);
-            }
+        for (int u = 0; u < kPer; ++u) {
+            const int k = part * kWave + lane + u * step;
+            if (k < n4) split_x(v[u], factor, inf, sx + ((k >> 3) * cols + 2 * r) * 32 + (k & 7) * 4);
         }
     };
     if (parts > 1) {                                              // one row per wave at most, parts of it in several
@@ -341,8 +359,8 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
             }
         }
     };
-    // the waves of a unit's columns add up in LDS, in order (behind an x that the next unit takes again)
-    float * sa = reinterpret_cast<float *>(WHOLE ? lds + static_cast<size_t>(p.chunk) * p.rows * 4 : lds);
+    // the waves of a unit's columns add up in LDS, in order, behind the x that the next unit takes again
+    float * sa = reinterpret_cast<float *>(lds + static_cast<size_t>(p.in_dim) * p.rows * 4);
     auto join = [&]() {
         constexpr int kVals = TW * NB * NI;
         __syncthreads();                                          // what lay there has been read
@@ -368,54 +386,198 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
             }
         }
     };
-    if constexpr (WHOLE) {
-        // all waves of the workgroup go as many rounds: the join has barriers
-        const int rounds = (p.n_units + unit_step - 1) / unit_step;
-        for (int round = 0; round < rounds; ++round) {
-            const int unit = unit0 + round * unit_step;
-            clear();
-            for (int it = 0; it < n_it; it += kAhead) {
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    const int kb = wk + (it + u) * p.wk;
-                    block(u, min(kb, n_kb - 1), kb < n_kb);
-                }
-            }
-            if (p.wk > 1) join();
-            if (wk == 0 && unit < p.n_units) store(unit);
-        }
-    } else {
+    // all waves of the workgroup go as many rounds: the join has barriers
+    const int rounds = (p.n_units + unit_step - 1) / unit_step;
+    for (int round = 0; round < rounds; ++round) {
+        const int unit = unit0 + round * unit_step;
         clear();
-        int kb = wk;
-        for (int k0 = 0; k0 < p.in_dim; k0 += p.chunk) {
-            const int k1 = min(k0 + p.chunk, p.in_dim), q0 = k0 >> 2, q1 = k1 >> 2;
-            __syncthreads();
-            for (int r = wave; r < p.rows; r += kQ4Waves) {
-                const f4 * x = reinterpret_cast<const f4 *>(p.x + static_cast<int64_t>(r) * p.in_dim);
-                const float factor = s_factor[r];
-                const bool has_inf = s_inf[r];
-                for (int k = q0 + lane; k < q1; k += kPer * kWave) {
-                    f4 g[kPer];
+        for (int it = 0; it < n_it; it += AHEAD) {
 #pragma unroll
-                    for (int u = 0; u < kPer; ++u) {
-                        const int at = min(k + u * kWave, q1 - 1);
-                        v[u] = x[at];
-                        if (nw) g[u] = nw[at];
-                    }
-#pragma unroll
-                    for (int u = 0; u < kPer; ++u) {
-                        const int at = k + u * kWave - q0;
-                        if (at >= q1 - q0) continue;
-                        if (nw) v[u] *= g[u];
-                        split_x(v[u], factor, has_inf, sx + ((at >> 3) * cols + 2 * r) * 32 + (at & 7) * 4);
-                    }
-                }
+            for (int u = 0; u < AHEAD; ++u) {
+                const int kb = wk + (it + u) * p.wk;
+                block(u, min(kb, n_kb - 1), kb < n_kb);
             }
-            __syncthreads();
-            for (; kb * kTileCols < k1; kb += p.wk) block(0, kb - k0 / kTileCols, true);
         }
         if (p.wk > 1) join();
-        if (wk == 0 && unit0 < p.n_units) store(unit0);
+        if (wk == 0 && unit < p.n_units) store(unit);
+    }
+}
+
+// The form for an x that does not fit in LDS, or that only a unit or two of a workgroup would share: a workgroup is one tile (with
+// SwiGLU: gate and up), its 8 waves share the columns, and a wave reads the x of its own blocks as the A operand, with no
+// barrier before the end.  Its lane c16 holds x row r's columns 8 g4 .. + 3 of a step and lane c16 + 8 those .. + 7; each splits its four
+// and the two exchange the parts, so that one has the first parts of all eight and the other the second.  One pass over x:
+// a wave keeps a power of two per row that fits what it has seen and rescales its sums when that falls; the sum of squares
+// comes along, and its factor is one of the result.  What bounds it is the arithmetic on x, 9 (with the norm 12)
+// instructions a value: 2048 x 6144, 8 / 16 / 32 rows 9.8 / 16.0 / 29.6 us (with x in LDS piece by piece 16 / 33 / 60).
+template <int NB, bool SWIGLU, int GS>
+__global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_rows_kernel(Q4Params p) {
+    constexpr int TW = SWIGLU ? 2 : 1, kRows = NB * 8, kGroups = 4 >> GS;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float * sa = reinterpret_cast<float *>(lds);                  // [wave][result][lane]
+    __shared__ double s_sum[kQ4Waves][kRows];
+    __shared__ int s_exp[kQ4Waves][kRows];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c16 = lane & 15, g4 = lane >> 4;
+    const bool second = c16 >= 8;
+    const int a8 = c16 & 7, xr = (a8 & 3) * 2 + (a8 >> 2);        // the x row of the A row c16, as in the form above
+    const int n_kb = p.in_dim / kTileCols, unit = blockIdx.x;
+    const float * xrow[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) xrow[nb] = p.x + static_cast<int64_t>(min(nb * 8 + xr, p.rows - 1)) * p.in_dim + g4 * 8 + (second ? 4 : 0);
+    const float * nrow = p.norm_w ? p.norm_w + g4 * 8 + (second ? 4 : 0) : nullptr;
+
+    u4 w[TW];
+    _Float16 d[TW];
+    f4 x[NB][4], g[4];
+    auto fetch = [&](int kb) {
+#pragma unroll
+        for (int t = 0; t < TW; ++t) {
+            const int64_t at = static_cast<int64_t>(unit + t * p.n_tiles) * n_kb + kb;
+            w[t] = reinterpret_cast<const u4 *>(p.W)[at * kWave + lane];
+            d[t] = p.scales[at * kGroups * kTileRows + (lane & (kGroups * kTileRows - 1))];
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) x[nb][s] = *reinterpret_cast<const f4 *>(xrow[nb] + kb * kTileCols + s * 32);
+            if (nrow) g[s] = *reinterpret_cast<const f4 *>(nrow + kb * kTileCols + s * 32);
+        }
+    };
+    float acc[TW][NB][4];
+    double ss[NB];
+    int ex[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        ss[nb] = 0.0;
+        ex[nb] = kMaxExp;
+#pragma unroll
+        for (int t = 0; t < TW; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t][nb][i] = 0.0f;
+        }
+    }
+    const Unpack unpack;
+    if (wave < n_kb) fetch(wave);
+    for (int kb = wave; kb < n_kb; kb += kQ4Waves) {
+        h8 a[NB][4];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            if (nrow) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        ss[nb] += static_cast<double>(x[nb][s][e]) * x[nb][s][e];
+                        x[nb][s][e] *= g[s][e];
+                    }
+                }
+            }
+            float mx = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[nb][s][e]));
+            }
+            mx = column_max(fmaxf(mx, row_ror8(mx)));
+            const bool inf = __ballot(mx == INFINITY) != 0;
+            if (__builtin_expect(inf, 0)) {                       // rare: the largest of what is finite
+                mx = 0.0f;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx = fabsf(x[nb][s][e]) < INFINITY ? fmaxf(mx, fabsf(x[nb][s][e])) : mx;
+                }
+                mx = column_max(fmaxf(mx, row_ror8(mx)));
+            }
+            const int to = mx > 0.0f ? min(ex[nb], kQ4Exp - __builtin_amdgcn_frexp_expf(mx)) : ex[nb];
+            if (__ballot(to < ex[nb]) != 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int by = __shfl(to - ex[nb], 4 * (g4 & 1) + i, kWave);
+#pragma unroll
+                    for (int t = 0; t < TW; ++t) acc[t][nb][i] = ldexpf(acc[t][nb][i], by);
+                }
+                ex[nb] = to;
+            }
+            const float factor = ldexpf(1.0f, ex[nb]);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) a[nb][s] = split_pair(x[nb][s] * factor, inf, second);
+        }
+        const u4 wb[2] = {w[0], w[TW - 1]};
+        float dg[TW][kGroups];
+#pragma unroll
+        for (int t = 0; t < TW; ++t) spread_scales<GS>(static_cast<float>(d[t]), dg[t]);
+        fetch(min(kb + kQ4Waves, n_kb - 1));                      // behind its last block a wave loads one that nobody uses
+        f4 group[TW][NB];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const bool first = (s & ((1 << GS) - 1)) == 0, last = ((s + 1) & ((1 << GS) - 1)) == 0;
+#pragma unroll
+            for (int t = 0; t < TW; ++t) {
+                const h8 b = unpack(wb[t][s]);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const f4 c = first ? f4{0.0f, 0.0f, 0.0f, 0.0f} : group[t][nb];
+                    group[t][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[nb][s], b, c, 0, 0, 0);
+                    if (last) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[t][nb][i] = fmaf(group[t][nb][i], dg[t][s >> GS], acc[t][nb][i]);
+                    }
+                }
+            }
+        }
+    }
+    // the waves' sums meet at the smallest of their powers of two, and add up in order
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int m = 8; m < kWave; m <<= 1) ss[nb] += __shfl_xor(ss[nb], m, kWave);
+        if (lane < 8) {
+            s_sum[wave][nb * 8 + xr] = ss[nb];
+            s_exp[wave][nb * 8 + xr] = ex[nb];
+        }
+    }
+    __syncthreads();
+    constexpr int kVals = TW * NB * 4;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = nb * 8 + 2 * i + (g4 & 1);
+            int least = s_exp[0][r];
+#pragma unroll
+            for (int k = 1; k < kQ4Waves; ++k) least = min(least, s_exp[k][r]);
+            const int by = least - s_exp[wave][r];
+#pragma unroll
+            for (int t = 0; t < TW; ++t) sa[(wave * kVals + (nb * 4 + i) * TW + t) * kWave + lane] = ldexpf(acc[t][nb][i], by);
+        }
+    }
+    __syncthreads();
+    for (int j = wave; j < NB * 4; j += kQ4Waves) {
+        float v[TW];
+#pragma unroll
+        for (int t = 0; t < TW; ++t) {
+            v[t] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kQ4Waves; ++k) v[t] += sa[(k * kVals + j * TW + t) * kWave + lane];
+            v[t] += __shfl_xor(v[t], 32, kWave);
+        }
+        const int r = (j >> 2) * 8 + 2 * (j & 3) + (g4 & 1), o = unit * kTileRows + c16;
+        if (g4 >= 2 || r >= p.rows || o >= p.out_dim) continue;
+        double sum = 0.0;
+        int least = kMaxExp;
+#pragma unroll
+        for (int k = 0; k < kQ4Waves; ++k) {
+            sum += s_sum[k][r];
+            least = min(least, s_exp[k][r]);
+        }
+        const float f = p.norm_w ? 1.0f / sqrtf(static_cast<float>(sum / p.in_dim) + p.eps) : 1.0f;
+        float * y = p.y + static_cast<int64_t>(r) * p.out_dim + o;
+        float out = ldexpf(v[0] * f, -least);
+        if constexpr (SWIGLU) out = out / (1.0f + expf(-out)) * ldexpf(v[1] * f, -least);
+        *y = p.epilogue == kEpiAccumOp ? *y + out : out;
     }
 }
 
@@ -466,46 +628,44 @@ int check_q4(int32_t out_dim, int32_t in_dim, int32_t group, const char * who) {
     return QA_OK;
 }
 
-template <int NB, int NI, int TW, bool SWIGLU, int GS, int AHEAD>
-int launch_q4_kernel(const Q4Params & p, int blocks, size_t lds, hipStream_t stream) {
+int launch_q4_kernel(void (*kernel)(Q4Params), const Q4Params & p, int blocks, size_t lds, hipStream_t stream) {
     if (lds > kXBytes / 2) {
-        const void * fn = reinterpret_cast<const void *>(gemv_q4_kernel<NB, NI, TW, SWIGLU, GS, AHEAD>);
-        QA_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+        QA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
     }
-    hipLaunchKernelGGL((gemv_q4_kernel<NB, NI, TW, SWIGLU, GS, AHEAD>), dim3(static_cast<unsigned>(blocks)), dim3(kQ4Threads), lds, stream, p);
-    QA_LAUNCH_CHECK("gemv_q4_kernel");
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kQ4Threads), lds, stream, p);
+    QA_LAUNCH_CHECK("4-bit matrix-vector kernel");
     return QA_OK;
 }
 
-// How the waves divide the work.  Units alone rarely fill the GPU evenly (9496 tiles over 4096 waves are two rounds and a
-// bit), so a unit's columns are shared by up to 8 waves, the more of them the fewer rows x has to be read for: a tile's
-// partial sums then meet in LDS.  x is whole in LDS where it can be, and then no more workgroups run than are resident.
+// How the waves divide the work where x is whole in LDS.  Units alone rarely fill the GPU evenly (9496 tiles over 4096 waves are
+// two rounds and a bit), so a unit's columns are shared by up to 8 waves, the more of them the fewer rows x has to be read
+// for: a tile's partial sums then meet in LDS.  No more workgroups run than are resident.
 // Measured with 1 / 2 / 4 / 8 waves per unit, 151936 x 2048: one row 54 / 40 / 34 / 35 us, 8 rows 53 / 45 / 41 / 41, 16 rows
 // 55 / 54 / 59 / 73.
 template <int NB, int NI, int TW, bool SWIGLU, int GS>
-int launch_q4(Q4Params p, bool whole, hipStream_t stream) {
+int launch_q4(Q4Params p, hipStream_t stream) {
     p.n_units = SWIGLU ? p.n_tiles : (p.n_tiles + TW - 1) / TW;
     const int n_kb = p.in_dim / kTileCols;
     const int64_t waves = NB == 1 ? 16384 : NB == 2 ? 8192 : 4096;
-    const size_t join = static_cast<size_t>(TW) * NB * NI * kWave * 4, x_whole = static_cast<size_t>(p.in_dim) * p.rows * 4;
+    const size_t join = static_cast<size_t>(TW) * NB * NI * kWave * 4, x_bytes = static_cast<size_t>(p.in_dim) * p.rows * 4;
     p.wk = 1;
     while (p.wk < kQ4Waves && p.wk * 2 <= n_kb && static_cast<int64_t>(p.n_units) * p.wk < waves &&
-           (!whole || x_whole + (kQ4Waves - kQ4Waves / (p.wk * 2)) * join <= kQ4Lds)) {
+           x_bytes + (kQ4Waves - kQ4Waves / (p.wk * 2)) * join <= kQ4Lds) {
         p.wk *= 2;
     }
     p.wt = kQ4Waves / p.wk;
-    // x in LDS: all of it, or whole rounds of the waves' blocks
-    const int round = p.wk * kTileCols;
-    p.chunk = whole ? p.in_dim : std::min(p.in_dim, std::max(round, kXBytes / (4 * p.rows) / round * round));
-    const size_t x_bytes = static_cast<size_t>(p.chunk) * p.rows * 4, joins = p.wt * (p.wk - 1) * join;
     const int units = (p.n_units + p.wt - 1) / p.wt;
-    if (!whole) return launch_q4_kernel<NB, NI, TW, SWIGLU, GS, 0>(p, units, std::max(x_bytes, joins), stream);
-    const size_t lds = x_bytes + joins;
+    const size_t lds = x_bytes + p.wt * (p.wk - 1) * join;
     const int blocks = std::min(units, lds <= 80 * 1024 - 1024 ? 512 : 256);
     // a wave that has one unit fetches nothing behind it; with several, two blocks in flight carry over from one to the next
     // (12288 gate|up rows, one row of x: 7.6 instead of 8.7 us; 151936 rows, 8 rows of x: 41 instead of 42)
-    if (blocks == units) return launch_q4_kernel<NB, NI, TW, SWIGLU, GS, 1>(p, blocks, lds, stream);
-    return launch_q4_kernel<NB, NI, TW, SWIGLU, GS, 2>(p, blocks, lds, stream);
+    const auto kernel = blocks == units ? &gemv_q4_kernel<NB, NI, TW, SWIGLU, GS, 1> : &gemv_q4_kernel<NB, NI, TW, SWIGLU, GS, 2>;
+    return launch_q4_kernel(kernel, p, blocks, lds, stream);
+}
+
+template <int NB, bool SWIGLU, int GS>
+int launch_q4_own(const Q4Params & p, hipStream_t stream) {
+    return launch_q4_kernel(&gemv_q4_rows_kernel<NB, SWIGLU, GS>, p, p.n_tiles, static_cast<size_t>(kQ4Waves) * (SWIGLU ? 2 : 1) * NB * 4 * kWave * 4, stream);
 }
 
 // Whether x fits in LDS and a wave's share of a row in its registers.
@@ -514,31 +674,41 @@ bool whole_x(int rows, int in_dim) {
 }
 
 template <int TW, bool SWIGLU, int GS>
+int launch_q4_shared(const Q4Params & p, hipStream_t stream) {
+    if (p.rows <= 2) return launch_q4<1, 1, TW, SWIGLU, GS>(p, stream);
+    if (p.rows <= 8) return launch_q4<1, 4, TW, SWIGLU, GS>(p, stream);
+    if (p.rows <= 16) return launch_q4<2, 4, TW, SWIGLU, GS>(p, stream);
+    return launch_q4<4, 4, TW, SWIGLU, GS>(p, stream);
+}
+
+template <bool SWIGLU, int GS>
 int launch_q4_rows(const Q4Params & p, hipStream_t stream) {
-    if (p.rows <= 2) return launch_q4<1, 1, TW, SWIGLU, GS>(p, whole_x(p.rows, p.in_dim), stream);
-    if (p.rows <= 8) return launch_q4<1, 4, TW, SWIGLU, GS>(p, whole_x(p.rows, p.in_dim), stream);
-    if (p.rows <= 16) return launch_q4<2, 4, TW, SWIGLU, GS>(p, whole_x(p.rows, p.in_dim), stream);
-    // more than 16 rows whose x does not fit in LDS at once, but half of which does: W is read twice (32 rows of 2048
-    // columns: 12288 gate|up rows 33 instead of 57 us, 151936 rows 108 instead of 139)
-    if (!whole_x(p.rows, p.in_dim) && whole_x(16, p.in_dim)) {
-        Q4Params half = p;
-        half.rows = 16;
-        if (const int rc = launch_q4<2, 4, TW, SWIGLU, GS>(half, whole_x(half.rows, half.in_dim), stream); rc != QA_OK) return rc;
-        half.x += static_cast<int64_t>(16) * p.in_dim;
-        half.y += static_cast<int64_t>(16) * p.out_dim;
-        half.rows = p.rows - 16;
-        if (half.rows <= 8) return launch_q4<1, 4, TW, SWIGLU, GS>(half, whole_x(half.rows, half.in_dim), stream);
-        return launch_q4<2, 4, TW, SWIGLU, GS>(half, whole_x(half.rows, half.in_dim), stream);
+    // its own x per wave where it does not fit in LDS, and where there are few tiles for the x in LDS to serve:
+    // (us) 128 tiles of 2048 columns: 8 rows 6.5 / 5.3, 16 rows 9.7 / 8.3, 32 rows 19.1 / 14.7; 384 pairs of tiles (12288 gate|up rows):
+    // 8 rows 12.4 / 10.9, 16 rows 17.5 / 19.7.  Up to 4 rows the x in LDS is as fast or faster.
+    const int at_once = whole_x(p.rows, p.in_dim) ? p.rows : std::min(p.rows, 16);   // of more, 16 rows at a time: W is read twice
+    if (!whole_x(at_once, p.in_dim) || (p.rows > 4 && p.n_tiles <= (p.rows <= 8 ? 512 : 256))) {
+        if (p.rows <= 8) return launch_q4_own<1, SWIGLU, GS>(p, stream);
+        if (p.rows <= 16) return launch_q4_own<2, SWIGLU, GS>(p, stream);
+        return launch_q4_own<4, SWIGLU, GS>(p, stream);
     }
-    return launch_q4<4, 4, TW, SWIGLU, GS>(p, whole_x(p.rows, p.in_dim), stream);
+    Q4Params part = p;
+    for (int r = 0; r < p.rows; r += at_once) {
+        part.rows = std::min(at_once, p.rows - r);
+        // two tiles per wave where that still leaves every CU a workgroup
+        int rc;
+        if constexpr (SWIGLU) rc = launch_q4_shared<2, true, GS>(part, stream);
+        else rc = p.n_tiles >= 1024 ? launch_q4_shared<2, false, GS>(part, stream) : launch_q4_shared<1, false, GS>(part, stream);
+        if (rc != QA_OK) return rc;
+        part.x += static_cast<int64_t>(16) * p.in_dim;
+        part.y += static_cast<int64_t>(16) * p.out_dim;
+    }
+    return QA_OK;
 }
 
 template <int GS>
 int launch_q4_tiles(const Q4Params & p, hipStream_t stream) {
-    if (p.epilogue == kEpiSwigluOp) return launch_q4_rows<2, true, GS>(p, stream);
-    // two tiles per wave where that still leaves every CU a workgroup
-    if (p.n_tiles >= 1024) return launch_q4_rows<2, false, GS>(p, stream);
-    return launch_q4_rows<1, false, GS>(p, stream);
+    return p.epilogue == kEpiSwigluOp ? launch_q4_rows<true, GS>(p, stream) : launch_q4_rows<false, GS>(p, stream);
 }
 
 }  // namespace

@@ -92,4 +92,14 @@ __device__ inline float wave_sum_all(float v) { return bcast63_f(wave_sum_lane63
 __device__ inline float wave_max_all(float v) { return bcast63_f(wave_max_lane63(v)); }
 __device__ inline double wave_sum_d_all(double v) { return bcast63_d(wave_sum_d_lane63(v)); }
 
+__device__ inline float row_ror8(float v) { return dpp_f<0x128>(v); }   // lane c of a row of 16 gets lane c ^ 8's
+
+// Over the lanes c, c + 16, c + 32, c + 48, in each of them: row swaps, no LDS.
+__device__ inline float column_max(float v) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 }  // namespace qa

@@ -244,3 +244,80 @@ def test_pack_then_multiply(qa):
     qa.synchronize()
     q, d = quantise(w, group)
     close(y.numpy(), *plain(q, d, x))
+
+
+@pytest.mark.parametrize("rows,k,epi", [(17, 2048, 1), (28, 2048, 2), (32, 512, 0), (13, 2048, 2), (32, 2176, 0)])
+def test_many_tiles_and_rows(qa, rows, k, epi):
+    """More tiles than workgroups run at a time, and up to 32 rows: x once in LDS, in two parts, or with every tile."""
+    rng = np.random.default_rng(rows)
+    out, group = 8208, 128
+    q, d = weights(rng, out * (2 if epi == 2 else 1), k, group)
+    x = rng.standard_normal((rows, k)).astype(np.float32)
+    norm = (1 + 0.1 * rng.standard_normal(k)).astype(np.float32)
+    y0 = rng.standard_normal((rows, out)).astype(np.float32) if epi == 1 else None
+    close(gemv(qa, q, d, x, group, epi, norm, y0), *plain(q, d, x, epi, norm, y0), rel=8e-6 if epi == 2 else 2e-6)
+
+
+@pytest.mark.parametrize("rows", [6, 14, 30])
+@pytest.mark.parametrize("scale", [1e-38, 1e-30, 1e-6, 1e5, 1e30])
+def test_magnitudes_of_x_in_more_rows(qa, rows, scale):
+    rng = np.random.default_rng(rows)
+    q, d = weights(rng, 64, 2304, 32)
+    x = rng.standard_normal((rows, 2304)).astype(np.float32)
+    x[1::3] *= np.float32(scale)
+    x[3] = 0.0
+    got = gemv(qa, q, d, x, 32).astype(np.float64)
+    want, size = plain(q, d, x)
+    assert (got[3] == 0).all()
+    for r in range(rows):
+        tiny = 2304 * 2.0 ** -149
+        assert np.linalg.norm(got[r] - want[r]) <= 2e-6 * np.linalg.norm(want[r]) + tiny, (r, scale)
+
+
+@pytest.mark.parametrize("rows", [5, 12, 32])
+@pytest.mark.parametrize("norm", [False, True])
+def test_columns_of_unlike_size(qa, rows, norm):
+    """Columns that grow and shrink by 2^40 along a row: whatever is split first, the large ones keep their bits."""
+    rng = np.random.default_rng(rows)
+    k = 128 * 41
+    q, d = weights(rng, 48, k, 64)
+    x = rng.standard_normal((rows, k)).astype(np.float32)
+    up = np.exp2(np.arange(k) // 128 - 20).astype(np.float32)
+    x[0] *= up
+    x[1] *= up[::-1]
+    x[2] *= rng.permutation(up)
+    x[3, :128 * 40] = 0.0
+    w = np.ones(k, np.float32) if norm else None
+    close(gemv(qa, q, d, x, 64, 0, w), *plain(q, d, x, 0, w))
+
+
+@pytest.mark.parametrize("rows", [7, 15, 32])
+@pytest.mark.parametrize("norm", [False, True])
+def test_not_finite_x_in_more_rows(qa, rows, norm):
+    rng = np.random.default_rng(6)
+    q, d = weights(rng, 32, 2304, 64)
+    q[:16, 2009], q[16:31, 2009], q[31, 2009] = 12, 3, 8
+    x = rng.standard_normal((rows, 2304)).astype(np.float32)
+    x[0, 2009], x[1, 2009], x[2, 2009], x[4, 2009] = np.inf, -np.inf, np.nan, 3e38
+    w = np.ones(2304, np.float32) if norm else None
+    got = gemv(qa, q, d, x, 64, 0, w)
+    if norm:
+        assert np.isnan(got[:3]).all()                            # inf times its row's factor 0
+    else:
+        assert (got[0, :16] == np.inf).all() and (got[0, 16:31] == -np.inf).all() and np.isnan(got[0, 31])
+        assert (got[1, :16] == -np.inf).all() and (got[1, 16:31] == np.inf).all() and np.isnan(got[1, 31])
+        assert np.isnan(got[2]).all()
+    rest = [3] + list(range(5, rows))
+    want, size = plain(q, d, x[rest], 0, w)
+    close(got[rest], want, size)
+    assert np.isfinite(got[4]).all()
+
+
+@pytest.mark.parametrize("rows", [3, 7, 20])
+def test_norm_of_large_x_in_more_rows(qa, rows):
+    """The sum of squares, and x times its weights, pass f32's range before the factor brings them back."""
+    rng = np.random.default_rng(8)
+    q, d = weights(rng, 32, 2304, 32)
+    x = (rng.standard_normal((rows, 2304)) * 3e18).astype(np.float32)
+    norm = np.full(2304, 1e18, np.float32)
+    close(gemv(qa, q, d, x, 32, 0, norm), *plain(q, d, x, 0, norm))
