@@ -1,6 +1,8 @@
 """Attention over pages with long chunks: many tokens behind many positions, which the call cuts into larger tiles and key
 ranges of their own, alone and beside sequences of one token.  Statements and tolerances are those of the shorter calls
 (a relative 2-norm error of 5e-6, a value within 2^-16 of the largest |v|)."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -110,3 +112,37 @@ def test_max_len_is_a_hint(qa, f16):
         b = ref.Batch(qa, tables, past, news, max_len=max_len)
         got = ref.run_attention(qa, q, pool, 0, b, 32, 16)
         close(got, ref.attention(q, pool, 0, tables, 32, b.past, b.start, 16), np.abs(pool.astype(np.float64)).max())
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("rows", [1023, 1024, 1500])
+def test_long_append_gives_the_bits_of_the_contiguous_append(qa, f16, rows):
+    """Two sequences of many tokens and one of one, each against its own append; rows of no sequence stay."""
+    rng = np.random.default_rng(rows)
+    past, news, page = [37, 0, 900], [rows - 420, 417, 1], 64
+    qkv = rng.standard_normal((rows, 4096)).astype(np.float32)
+    qn, kn = ((1 + 0.1 * rng.standard_normal(128)).astype(np.float32) for _ in range(2))
+    tables, pages = ref.tables_of(rng, [p + n for p, n in zip(past, news)], page)
+    pool = ref.pool_of(rng, 1, pages, 8, page, f16)
+    b = ref.Batch(qa, tables, past, news, n_rows=rows)
+    d = [qa.DeviceArray.from_numpy(a) for a in (qkv, qn, kn, np.full((rows, 2048), 3.5, np.float32), pool)]
+    lay = ref.layout(qa, 1, pages, 8, page, f16)
+    print(f"append of {rows} rows f16={f16}", flush=True)
+    qa.check(qa.lib.qa_paged_append(*(x.ptr for x in d), C.byref(lay), 0, b.ref, 16, 1e6, 1e-6, None))
+    qa.synchronize()
+    q, got = d[3].numpy(), d[4].numpy()
+    assert (q[sum(news):] == 3.5).all()
+    expect = pool.copy()
+    flat_lay = ref.layout(qa, 1, 1, 8, 2048, f16)
+    for s, (p, n) in enumerate(zip(past, news)):
+        r0 = int(b.start[s])
+        x = qa.DeviceArray.from_numpy(np.ascontiguousarray(qkv[r0:r0 + n]))
+        flat, q0 = qa.DeviceArray((2, 8, 2048, 128), pool.dtype), qa.DeviceArray((n, 2048))
+        d_past = qa.DeviceArray.from_numpy(np.array([p], np.int32))
+        qa.check(qa.lib.qa_kv_append(x.ptr, d[1].ptr, d[2].ptr, q0.ptr, flat.ptr, C.byref(flat_lay), 0, d_past.ptr, 1, n, 16, 1e6, 1e-6, None))
+        qa.synchronize()
+        np.testing.assert_array_equal(q0.numpy().view(np.uint32), q[r0:r0 + n].view(np.uint32))
+        a = flat.numpy()
+        for pos in range(p, p + n):
+            expect[0, :, tables[s, pos // page], :, pos % page] = a[:, :, pos]
+    np.testing.assert_array_equal(got, expect)
