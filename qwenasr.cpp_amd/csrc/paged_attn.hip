@@ -897,10 +897,12 @@ struct AttnPlan {
     int parts() const { return std::max(splits_many, splits_few); }
 };
 
-// Key ranges of `steps` steps for workgroups of which one range has `blocks`: enough to make `target` of them, none shorter
-// than `least` steps.
+// Key ranges of `steps` steps for workgroups of which one range has `blocks`: enough to make `target` of them, of `least` steps or
+// so, and more than one only where there are twice as many: two of 5 or 7 steps lose more to the join than they gain (one
+// token behind 400 positions 9.7 us, in one range 8.4; 128 tokens behind 500, `least` 16, 15.3 and 11.6).
 void cut_keys(int steps, int64_t blocks, int64_t target, int64_t least, int64_t most, int & splits, int & split_steps) {
-    const int64_t n = std::max<int64_t>(1, std::min<int64_t>({target / std::max<int64_t>(blocks, 1), (steps + least - 1) / least, most}));
+    const int64_t by_length = steps < 2 * least ? 1 : (steps + least - 1) / least;
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>({target / std::max<int64_t>(blocks, 1), by_length, most}));
     split_steps = std::max<int>(1, static_cast<int>((steps + n - 1) / n));
     splits = std::max(1, (steps + split_steps - 1) / split_steps);
 }
@@ -938,10 +940,12 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     // 47 / 56, but two of 600 and ten of one token behind 24 to 3500 98 / 73, four of 256 behind 500 to 1500 53 / 57.
     const int64_t tiles = std::max<int64_t>(1, (cols + width - 1) / width) * l.n_kv_heads, heads = static_cast<int64_t>(seqs) * l.n_kv_heads;
     const bool one = b.n_seqs == 1;
+    // one round of workgroups where their ranges stay short: four sequences of 501 to 3001 in 8 / 12 ranges 13.3 / 16.2 us, f32 pages 18.3 / 23.6
+    const int64_t round = std::max<int64_t>(1, 256 / heads), decode = (steps + round - 1) / round <= 24 ? 256 : 1024;
     if (pl.tile) cut_keys(steps, tiles, one ? 512 : 768, 4, parts, pl.splits_many, pl.steps_many);
-    else if (most <= 16) cut_keys(steps, heads, 1024, 8, parts, pl.splits_many, pl.steps_many);
+    else if (most <= 16) cut_keys(steps, heads, decode, 8, parts, pl.splits_many, pl.steps_many);
     else cut_keys(steps, tiles, !one ? 640 : steps >= 128 && tiles > 192 ? 1024 : 384, 16, parts, pl.splits_many, pl.steps_many);
-    cut_keys(steps, heads, 1024, 8, parts, pl.splits_few, pl.steps_few);
+    cut_keys(steps, heads, decode, 8, parts, pl.splits_few, pl.steps_few);
     if (!many) pl.splits_many = 1;
     if (!few) pl.splits_few = 1;
     return pl;
