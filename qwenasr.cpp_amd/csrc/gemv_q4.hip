@@ -667,9 +667,12 @@ int launch_q4(Q4Params p, hipStream_t stream) {
     return launch_q4_kernel(kernel, p, blocks, lds, stream);
 }
 
-template <int NB, bool SWIGLU, int GS>
+template <bool SWIGLU, int GS>
 int launch_q4_own(const Q4Params & p, hipStream_t stream) {
-    return launch_q4_kernel(&gemv_q4_rows_kernel<NB, SWIGLU, GS>, p, p.n_tiles, static_cast<size_t>(kQ4Waves) * (SWIGLU ? 2 : 1) * NB * 4 * kWave * 4, stream);
+    const int nb = p.rows <= 8 ? 1 : p.rows <= 16 ? 2 : 4;
+    auto kernel = nb == 1 ? &gemv_q4_rows_kernel<1, SWIGLU, GS> : &gemv_q4_rows_kernel<2, SWIGLU, GS>;
+    if constexpr (!SWIGLU) kernel = nb == 4 ? &gemv_q4_rows_kernel<4, false, GS> : kernel;
+    return launch_q4_kernel(kernel, p, p.n_tiles, static_cast<size_t>(kQ4Waves) * (SWIGLU ? 2 : 1) * nb * 4 * kWave * 4, stream);
 }
 
 // Whether x fits in LDS and a wave's share of a row in its registers.
@@ -690,18 +693,17 @@ int launch_q4_rows(const Q4Params & p, hipStream_t stream) {
     // its own x per wave where it does not fit in LDS, and where there are few tiles for the x in LDS to serve:
     // (us) 128 tiles of 2048 columns: 8 rows 6.5 / 5.3, 16 rows 9.7 / 8.3, 32 rows 19.1 / 14.7; 384 pairs of tiles (12288 gate|up rows):
     // 8 rows 12.4 / 10.9, 16 rows 17.5 / 19.7.  Up to 4 rows the x in LDS is as fast or faster.
-    const int at_once = whole_x(p.rows, p.in_dim) ? p.rows : std::min(p.rows, 16);   // of more, 16 rows at a time: W is read twice
-    if (!whole_x(at_once, p.in_dim) || (p.rows > 4 && p.n_tiles <= (p.rows <= 8 ? 512 : 256))) {
-        if (p.rows <= 8) return launch_q4_own<1, SWIGLU, GS>(p, stream);
-        if (p.rows <= 16) return launch_q4_own<2, SWIGLU, GS>(p, stream);
-        return launch_q4_own<4, SWIGLU, GS>(p, stream);
-    }
+    const int shared = whole_x(p.rows, p.in_dim) ? p.rows : std::min(p.rows, 16);   // of more, 16 rows at a time: W is read twice
+    const bool own = !whole_x(shared, p.in_dim) || (p.rows > 4 && p.n_tiles <= (p.rows <= 8 ? 512 : 256));
+    // gate and up of 32 rows with their x pass the 256 registers of a lane: 16 rows at a time there, too
+    const int at_once = !own ? shared : SWIGLU ? std::min(p.rows, 16) : p.rows;
     Q4Params part = p;
     for (int r = 0; r < p.rows; r += at_once) {
         part.rows = std::min(at_once, p.rows - r);
         // two tiles per wave where that still leaves every CU a workgroup
         int rc;
-        if constexpr (SWIGLU) rc = launch_q4_shared<2, true, GS>(part, stream);
+        if (own) rc = launch_q4_own<SWIGLU, GS>(part, stream);
+        else if constexpr (SWIGLU) rc = launch_q4_shared<2, true, GS>(part, stream);
         else rc = p.n_tiles >= 1024 ? launch_q4_shared<2, false, GS>(part, stream) : launch_q4_shared<1, false, GS>(part, stream);
         if (rc != QA_OK) return rc;
         part.x += static_cast<int64_t>(16) * p.in_dim;
