@@ -35,6 +35,7 @@ constexpr int kQ4Waves = 8;                        // per workgroup
 constexpr int kQ4Threads = kQ4Waves * kWave;
 constexpr int kXBytes = 64 * 1024;                 // of x in LDS at a time: two workgroups per CU
 constexpr size_t kQ4Lds = 158 * 1024;              // of the CU's 160 KB, the rest is the kernel's own
+constexpr int kUnitTiles = 2;                     // tiles of a wave's unit where x is whole in LDS
 constexpr int kMaxExp = 127;                       // a power of two that is a float: x below 2^-112 keeps fewer bits
 constexpr int kQ4Exp = 15;                        // a row's largest finite |x| goes to [2^14, 2^15)
 
@@ -145,10 +146,9 @@ __device__ inline void spread_scales(float v, float (&d)[4 >> GS]) {
 
 // x row r of a block of 8 stands in rows (r % 2) 4 + r / 2 of the A operand, its second part 8 rows on: a lane's result i
 // belongs to x row 2 i + (lane / 16) % 2, so that up to 2 rows need the first result alone.
-// NB: blocks of 8 x rows.  NI: results of a lane that count (1 or 4).  TW: tiles of a wave's unit, whose blocks are in flight
-// together (2 with SwiGLU: gate and up).  GS: groups of 32 << GS columns.  AHEAD: blocks whose weights are in flight while one
+// NB: blocks of 8 x rows.  NI: results of a lane that count (1 or 4).  A wave's unit is two tiles, with SwiGLU gate and up.  GS: groups of 32 << GS columns.  AHEAD: blocks whose weights are in flight while one
 // is multiplied.  All of x lies in LDS.
-template <int NB, int NI, int TW, bool SWIGLU, int GS, int AHEAD>
+template <int NB, int NI, bool SWIGLU, int GS, int AHEAD>
 __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     _Float16 * sx = reinterpret_cast<_Float16 *>(lds);            // [in_dim / 32][row][part][32]
@@ -169,23 +169,23 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     // weights and scales of the next AHEAD blocks are in flight, the first ones while x is prepared; behind its last block a
     // wave loads that one again, so that no branch makes it wait for all
     constexpr int kGroups = 4 >> GS;                              // of a block
-    u4 w[AHEAD][TW];
-    _Float16 d[AHEAD][TW];
+    u4 w[AHEAD][kUnitTiles];
+    _Float16 d[AHEAD][kUnitTiles];
     const int n_it = (n_kb + p.wk * AHEAD - 1) / (p.wk * AHEAD) * AHEAD;   // a wave's blocks of a unit, the last ones perhaps idle
     const uint32_t w_lane = lane * 16, d_lane = (lane & (kGroups * kTileRows - 1)) * 2;
     int f_unit = unit0, f_it = 0;
     auto fetch = [&](int slot) {
         const int kb = min(wk + f_it * p.wk, n_kb - 1), unit = f_unit < p.n_units ? f_unit : min(unit0, p.n_units - 1);
 #pragma unroll
-        for (int t = 0; t < TW; ++t) {
-            const int tile = SWIGLU ? unit + t * p.n_tiles : min(unit * TW + t, p.n_tiles - 1);
+        for (int t = 0; t < kUnitTiles; ++t) {
+            const int tile = SWIGLU ? unit + t * p.n_tiles : min(unit * kUnitTiles + t, p.n_tiles - 1);
             const int64_t at = static_cast<int64_t>(tile) * n_kb + kb;
             const char * wb = reinterpret_cast<const char *>(p.W) + at * (kWave * 16);
             const char * db = reinterpret_cast<const char *>(p.scales) + at * (kGroups * kTileRows * 2);
             // a matrix of many tiles past the caches, which hold it no better (151936 x 2048: 34.5 instead of 35.5 us, 8 rows 44 / 45);
             // 12288 gate|up rows stay (8.2 instead of 8.5)
             const u4 * wl = reinterpret_cast<const u4 *>(wb + w_lane);
-            if constexpr (TW == 2 && !SWIGLU) w[slot][t] = __builtin_nontemporal_load(wl);
+            if constexpr (!SWIGLU) w[slot][t] = __builtin_nontemporal_load(wl);
             else w[slot][t] = *wl;
             d[slot][t] = *reinterpret_cast<const _Float16 *>(db + d_lane);
         }
@@ -300,10 +300,10 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     const int a8 = c16 & 7, xr = (a8 & 3) * 2 + (a8 >> 2);        // the x row of the A row c16
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) arow[nb] = (2 * min(nb * 8 + xr, p.rows - 1) + (c16 >> 3)) * 32 + g4 * 8;
-    float acc[TW][NB][NI];
+    float acc[kUnitTiles][NB][NI];
     auto clear = [&]() {
 #pragma unroll
-        for (int t = 0; t < TW; ++t) {
+        for (int t = 0; t < kUnitTiles; ++t) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -314,10 +314,10 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     const Unpack unpack;
     auto block = [&](int slot, int kb_in_lds, bool counts) {
         const _Float16 * xb = sx + static_cast<int64_t>(kb_in_lds) * 4 * cols * 32;
-        f4 group[TW][NB];
-        float dg[TW][kGroups];
+        f4 group[kUnitTiles][NB];
+        float dg[kUnitTiles][kGroups];
 #pragma unroll
-        for (int t = 0; t < TW; ++t) spread_scales<GS>(static_cast<float>(d[slot][t]), dg[t]);
+        for (int t = 0; t < kUnitTiles; ++t) spread_scales<GS>(static_cast<float>(d[slot][t]), dg[t]);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             const bool first = (s & ((1 << GS) - 1)) == 0, last = ((s + 1) & ((1 << GS) - 1)) == 0;
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) a[nb] = *reinterpret_cast<const h8 *>(xb + s * cols * 32 + arow[nb]);
 #pragma unroll
-            for (int t = 0; t < TW; ++t) {
+            for (int t = 0; t < kUnitTiles; ++t) {
                 const h8 b = unpack(w[slot][t][s]);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
@@ -347,13 +347,13 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 const int r = nb * 8 + 2 * i + (g4 & 1);
-                float v[TW];
+                float v[kUnitTiles];
 #pragma unroll
-                for (int t = 0; t < TW; ++t) v[t] = acc[t][nb][i] + __shfl_xor(acc[t][nb][i], 32, kWave);
+                for (int t = 0; t < kUnitTiles; ++t) v[t] = acc[t][nb][i] + __shfl_xor(acc[t][nb][i], 32, kWave);
                 if (g4 >= 2 || r >= p.rows) continue;
 #pragma unroll
-                for (int t = 0; t < (SWIGLU ? 1 : TW); ++t) {
-                    const int o = (SWIGLU ? unit : unit * TW + t) * kTileRows + c16;
+                for (int t = 0; t < (SWIGLU ? 1 : kUnitTiles); ++t) {
+                    const int o = (SWIGLU ? unit : unit * kUnitTiles + t) * kTileRows + c16;
                     if (o >= p.out_dim) continue;                 // rows and tiles behind the last
                     float * y = p.y + static_cast<int64_t>(r) * p.out_dim + o;
                     float out = ldexpf(v[t], -s_exp[r]);
@@ -366,11 +366,11 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     // the waves of a unit's columns add up in LDS, in order, behind the x that the next unit takes again
     float * sa = reinterpret_cast<float *>(lds + static_cast<size_t>(p.in_dim) * p.rows * 4);
     auto join = [&]() {
-        constexpr int kVals = TW * NB * NI;
+        constexpr int kVals = kUnitTiles * NB * NI;
         __syncthreads();                                          // what lay there has been read
         if (wk > 0) {
 #pragma unroll
-            for (int t = 0; t < TW; ++t) {
+            for (int t = 0; t < kUnitTiles; ++t) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -381,7 +381,7 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
         __syncthreads();
         for (int k = 0; k < p.wk - 1 && wk == 0; ++k) {
 #pragma unroll
-            for (int t = 0; t < TW; ++t) {
+            for (int t = 0; t < kUnitTiles; ++t) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -407,18 +407,18 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     }
 }
 
-// The form for an x that does not fit in LDS, or that only a unit or two of a workgroup would share: a workgroup is one tile (with
-// SwiGLU: gate and up), its 8 waves share the columns, and a wave reads the x of its own blocks as the A operand, with no
-// barrier before the end.  Its lane c16 holds x row r's columns 8 g4 .. + 3 of a step and lane c16 + 8 those .. + 7; each splits its four
-// and the two exchange the parts, so that one has the first parts of all eight and the other the second.  One pass over x:
-// a wave keeps a power of two per row that fits what it has seen and rescales its sums when that falls; the sum of squares
+// The form for an x that does not fit in LDS, or that only a few tiles would share: a workgroup is 8 rows of x and NU tiles (with
+// SwiGLU: of gate and as many of up), its 8 waves share the columns, and a wave reads the x of its own blocks as the A operand, with
+// no barrier before the end.  Its lane c16 holds x row r's columns 8 g4 .. + 3 of a step and lane c16 + 8 those .. + 7; each splits its
+// four and the two exchange the parts, so that one has the first parts of all eight and the other the second.  One pass over
+// x: a wave keeps a power of two per row that fits what it has seen and rescales its sums when that falls; the sum of squares
 // comes along, and its factor is one of the result.  What bounds it is the arithmetic on x, 9 (with the norm 12)
-// instructions a value: 2048 x 6144, 8 / 16 / 32 rows 9.8 / 16.0 / 29.6 us (with x in LDS piece by piece 16 / 33 / 60).
-template <int NB, bool SWIGLU, int GS>
+// instructions a value: the rows of more than 8 are workgroups of their own, which read W again, from L2 (2048 x 6144, 16
+// rows: 10.2 us, as one workgroup's 16.0), and tiles go together where there are workgroups enough without.
+template <int NU, bool SWIGLU, int GS>
 __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_rows_kernel(Q4Params p) {
-    constexpr int TW = SWIGLU ? 2 : 1, kRows = NB * 8, kGroups = 4 >> GS;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    float * sa = reinterpret_cast<float *>(lds);                  // [wave][result][lane]
+    constexpr int TW = SWIGLU ? 2 * NU : NU, kRows = 8, kGroups = 4 >> GS, kVals = TW * 4;   // tile t: with SwiGLU of the pair t / 2
+    __shared__ float sa[kQ4Waves][kVals][kWave];
     __shared__ double s_sum[kQ4Waves][kRows];
     __shared__ int s_exp[kQ4Waves][kRows];
     const int lane = threadIdx.x & (kWave - 1);
@@ -427,149 +427,134 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_rows_kernel(Q4Params p)
     const bool second = c16 >= 8;
     const int a8 = c16 & 7, xr = (a8 & 3) * 2 + (a8 >> 2);        // the x row of the A row c16, as in the form above
     const int n_kb = p.in_dim / kTileCols, unit = blockIdx.x;
-    const float * xrow[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) xrow[nb] = p.x + static_cast<int64_t>(min(nb * 8 + xr, p.rows - 1)) * p.in_dim + g4 * 8 + (second ? 4 : 0);
+    const int row0 = blockIdx.y * kRows, rows = min(kRows, p.rows - row0);
+    const float * xrow = p.x + static_cast<int64_t>(row0 + min(xr, rows - 1)) * p.in_dim + g4 * 8 + (second ? 4 : 0);
     const float * nrow = p.norm_w ? p.norm_w + g4 * 8 + (second ? 4 : 0) : nullptr;
 
     u4 w[TW];
     _Float16 d[TW];
-    f4 x[NB][4], g[4];
+    f4 x[4], g[4];
     auto fetch = [&](int kb) {
 #pragma unroll
         for (int t = 0; t < TW; ++t) {
-            const int64_t at = static_cast<int64_t>(unit + t * p.n_tiles) * n_kb + kb;
+            const int tile = SWIGLU ? min(unit * NU + t / 2, p.n_tiles - 1) + (t & 1) * p.n_tiles : min(unit * NU + t, p.n_tiles - 1);
+            const int64_t at = static_cast<int64_t>(tile) * n_kb + kb;
             w[t] = reinterpret_cast<const u4 *>(p.W)[at * kWave + lane];
             d[t] = p.scales[at * kGroups * kTileRows + (lane & (kGroups * kTileRows - 1))];
         }
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) x[nb][s] = *reinterpret_cast<const f4 *>(xrow[nb] + kb * kTileCols + s * 32);
+            x[s] = *reinterpret_cast<const f4 *>(xrow + kb * kTileCols + s * 32);
             if (nrow) g[s] = *reinterpret_cast<const f4 *>(nrow + kb * kTileCols + s * 32);
         }
     };
-    float acc[TW][NB][4];
-    double ss[NB];
-    int ex[NB];
+    float acc[TW][4];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        ss[nb] = 0.0;
-        ex[nb] = kMaxExp;
+    for (int t = 0; t < TW; ++t) {
 #pragma unroll
-        for (int t = 0; t < TW; ++t) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t][nb][i] = 0.0f;
-        }
+        for (int i = 0; i < 4; ++i) acc[t][i] = 0.0f;
     }
+    double ss = 0.0;
+    int ex = kMaxExp;
     const Unpack unpack;
     if (wave < n_kb) fetch(wave);
     for (int kb = wave; kb < n_kb; kb += kQ4Waves) {
-        h8 a[NB][4];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            if (nrow) {
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        ss[nb] += static_cast<double>(x[nb][s][e]) * x[nb][s][e];
-                        x[nb][s][e] *= g[s][e];
-                    }
-                }
-            }
-            float mx = 0.0f;
+        if (nrow) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[nb][s][e]));
+                for (int e = 0; e < 4; ++e) {
+                    ss += static_cast<double>(x[s][e]) * x[s][e];
+                    x[s][e] *= g[s][e];
+                }
+            }
+        }
+        float mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[s][e]));
+        }
+        mx = column_max(fmaxf(mx, row_ror8(mx)));
+        const bool inf = __ballot(mx == INFINITY) != 0;
+        if (__builtin_expect(inf, 0)) {                           // rare: the largest of what is finite
+            mx = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fabsf(x[s][e]) < INFINITY ? fmaxf(mx, fabsf(x[s][e])) : mx;
             }
             mx = column_max(fmaxf(mx, row_ror8(mx)));
-            const bool inf = __ballot(mx == INFINITY) != 0;
-            if (__builtin_expect(inf, 0)) {                       // rare: the largest of what is finite
-                mx = 0.0f;
-#pragma unroll
-                for (int s = 0; s < 4; ++s) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) mx = fabsf(x[nb][s][e]) < INFINITY ? fmaxf(mx, fabsf(x[nb][s][e])) : mx;
-                }
-                mx = column_max(fmaxf(mx, row_ror8(mx)));
-            }
-            const int to = mx > 0.0f ? min(ex[nb], kQ4Exp - __builtin_amdgcn_frexp_expf(mx)) : ex[nb];
-            if (__ballot(to < ex[nb]) != 0) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int by = __shfl(to - ex[nb], 4 * (g4 & 1) + i, kWave);
-#pragma unroll
-                    for (int t = 0; t < TW; ++t) acc[t][nb][i] = ldexpf(acc[t][nb][i], by);
-                }
-                ex[nb] = to;
-            }
-            const float factor = ldexpf(1.0f, ex[nb]);
-#pragma unroll
-            for (int s = 0; s < 4; ++s) a[nb][s] = split_pair(x[nb][s] * factor, inf, second);
         }
-        const u4 wb[2] = {w[0], w[TW - 1]};
+        const int to = mx > 0.0f ? min(ex, kQ4Exp - __builtin_amdgcn_frexp_expf(mx)) : ex;
+        if (__ballot(to < ex) != 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int by = __shfl(to - ex, 4 * (g4 & 1) + i, kWave);
+#pragma unroll
+                for (int t = 0; t < TW; ++t) acc[t][i] = ldexpf(acc[t][i], by);
+            }
+            ex = to;
+        }
+        const float factor = ldexpf(1.0f, ex);
+        h8 a[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) a[s] = split_pair(x[s] * factor, inf, second);
+        u4 wb[TW];
         float dg[TW][kGroups];
 #pragma unroll
-        for (int t = 0; t < TW; ++t) spread_scales<GS>(static_cast<float>(d[t]), dg[t]);
+        for (int t = 0; t < TW; ++t) {
+            wb[t] = w[t];
+            spread_scales<GS>(static_cast<float>(d[t]), dg[t]);
+        }
         fetch(min(kb + kQ4Waves, n_kb - 1));                      // behind its last block a wave loads one that nobody uses
-        f4 group[TW][NB];
+        f4 group[TW];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             const bool first = (s & ((1 << GS) - 1)) == 0, last = ((s + 1) & ((1 << GS) - 1)) == 0;
 #pragma unroll
             for (int t = 0; t < TW; ++t) {
-                const h8 b = unpack(wb[t][s]);
+                const f4 c = first ? f4{0.0f, 0.0f, 0.0f, 0.0f} : group[t];
+                group[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[s], unpack(wb[t][s]), c, 0, 0, 0);
+                if (last) {
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    const f4 c = first ? f4{0.0f, 0.0f, 0.0f, 0.0f} : group[t][nb];
-                    group[t][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[nb][s], b, c, 0, 0, 0);
-                    if (last) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[t][nb][i] = fmaf(group[t][nb][i], dg[t][s >> GS], acc[t][nb][i]);
-                    }
+                    for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(group[t][i], dg[t][s >> GS], acc[t][i]);
                 }
             }
         }
     }
     // the waves' sums meet at the smallest of their powers of two, and add up in order
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int m = 8; m < kWave; m <<= 1) ss[nb] += __shfl_xor(ss[nb], m, kWave);
-        if (lane < 8) {
-            s_sum[wave][nb * 8 + xr] = ss[nb];
-            s_exp[wave][nb * 8 + xr] = ex[nb];
-        }
+    for (int m = 8; m < kWave; m <<= 1) ss += __shfl_xor(ss, m, kWave);
+    if (lane < 8) {
+        s_sum[wave][xr] = ss;
+        s_exp[wave][xr] = ex;
     }
     __syncthreads();
-    constexpr int kVals = TW * NB * 4;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
+    for (int i = 0; i < 4; ++i) {
+        const int r = 2 * i + (g4 & 1);
+        int least = s_exp[0][r];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = nb * 8 + 2 * i + (g4 & 1);
-            int least = s_exp[0][r];
+        for (int k = 1; k < kQ4Waves; ++k) least = min(least, s_exp[k][r]);
+        const int by = least - s_exp[wave][r];
 #pragma unroll
-            for (int k = 1; k < kQ4Waves; ++k) least = min(least, s_exp[k][r]);
-            const int by = least - s_exp[wave][r];
-#pragma unroll
-            for (int t = 0; t < TW; ++t) sa[(wave * kVals + (nb * 4 + i) * TW + t) * kWave + lane] = ldexpf(acc[t][nb][i], by);
-        }
+        for (int t = 0; t < TW; ++t) sa[wave][t * 4 + i][lane] = ldexpf(acc[t][i], by);
     }
     __syncthreads();
-    for (int j = wave; j < NB * 4; j += kQ4Waves) {
-        float v[TW];
+    constexpr int kOf = SWIGLU ? 2 : 1;                           // sums of a result
+    for (int j = wave; j < NU * 4; j += kQ4Waves) {
+        const int n = j >> 2, i = j & 3;
+        float v[kOf];
 #pragma unroll
-        for (int t = 0; t < TW; ++t) {
+        for (int t = 0; t < kOf; ++t) {
             v[t] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < kQ4Waves; ++k) v[t] += sa[(k * kVals + j * TW + t) * kWave + lane];
+            for (int k = 0; k < kQ4Waves; ++k) v[t] += sa[k][(n * kOf + t) * 4 + i][lane];
             v[t] += __shfl_xor(v[t], 32, kWave);
         }
-        const int r = (j >> 2) * 8 + 2 * (j & 3) + (g4 & 1), o = unit * kTileRows + c16;
-        if (g4 >= 2 || r >= p.rows || o >= p.out_dim) continue;
+        const int r = 2 * i + (g4 & 1), o = (unit * NU + n) * kTileRows + c16;
+        if (g4 >= 2 || r >= rows || o >= p.out_dim) continue;     // rows and tiles behind the last
         double sum = 0.0;
         int least = kMaxExp;
 #pragma unroll
@@ -578,7 +563,7 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_rows_kernel(Q4Params p)
             least = min(least, s_exp[k][r]);
         }
         const float f = p.norm_w ? 1.0f / sqrtf(static_cast<float>(sum / p.in_dim) + p.eps) : 1.0f;
-        float * y = p.y + static_cast<int64_t>(r) * p.out_dim + o;
+        float * y = p.y + static_cast<int64_t>(row0 + r) * p.out_dim + o;
         float out = ldexpf(v[0] * f, -least);
         if constexpr (SWIGLU) out = out / (1.0f + expf(-out)) * ldexpf(v[1] * f, -least);
         *y = p.epilogue == kEpiAccumOp ? *y + out : out;
@@ -632,11 +617,11 @@ int check_q4(int32_t out_dim, int32_t in_dim, int32_t group, const char * who) {
     return QA_OK;
 }
 
-int launch_q4_kernel(void (*kernel)(Q4Params), const Q4Params & p, int blocks, size_t lds, hipStream_t stream) {
+int launch_q4_kernel(void (*kernel)(Q4Params), const Q4Params & p, dim3 blocks, size_t lds, hipStream_t stream) {
     if (lds > kXBytes / 2) {
         QA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
     }
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kQ4Threads), lds, stream, p);
+    hipLaunchKernelGGL(kernel, blocks, dim3(kQ4Threads), lds, stream, p);
     QA_LAUNCH_CHECK("4-bit matrix-vector kernel");
     return QA_OK;
 }
@@ -646,12 +631,12 @@ int launch_q4_kernel(void (*kernel)(Q4Params), const Q4Params & p, int blocks, s
 // for: a tile's partial sums then meet in LDS.  No more workgroups run than are resident.
 // Measured with 1 / 2 / 4 / 8 waves per unit, 151936 x 2048: one row 54 / 40 / 34 / 35 us, 8 rows 53 / 45 / 41 / 41, 16 rows
 // 55 / 54 / 59 / 73.
-template <int NB, int NI, int TW, bool SWIGLU, int GS>
+template <int NB, int NI, bool SWIGLU, int GS>
 int launch_q4(Q4Params p, hipStream_t stream) {
-    p.n_units = SWIGLU ? p.n_tiles : (p.n_tiles + TW - 1) / TW;
+    p.n_units = SWIGLU ? p.n_tiles : (p.n_tiles + kUnitTiles - 1) / kUnitTiles;
     const int n_kb = p.in_dim / kTileCols;
     const int64_t waves = NB == 1 ? 16384 : NB == 2 ? 8192 : 4096;
-    const size_t join = static_cast<size_t>(TW) * NB * NI * kWave * 4, x_bytes = static_cast<size_t>(p.in_dim) * p.rows * 4;
+    const size_t join = static_cast<size_t>(kUnitTiles) * NB * NI * kWave * 4, x_bytes = static_cast<size_t>(p.in_dim) * p.rows * 4;
     p.wk = 1;
     while (p.wk < kQ4Waves && p.wk * 2 <= n_kb && static_cast<int64_t>(p.n_units) * p.wk < waves &&
            x_bytes + (kQ4Waves - kQ4Waves / (p.wk * 2)) * join <= kQ4Lds) {
@@ -663,16 +648,24 @@ int launch_q4(Q4Params p, hipStream_t stream) {
     const int blocks = std::min(units, lds <= 80 * 1024 - 1024 ? 512 : 256);
     // a wave that has one unit fetches nothing behind it; with several, two blocks in flight carry over from one to the next
     // (12288 gate|up rows, one row of x: 7.6 instead of 8.7 us; 151936 rows, 8 rows of x: 41 instead of 42)
-    const auto kernel = blocks == units ? &gemv_q4_kernel<NB, NI, TW, SWIGLU, GS, 1> : &gemv_q4_kernel<NB, NI, TW, SWIGLU, GS, 2>;
-    return launch_q4_kernel(kernel, p, blocks, lds, stream);
+    const auto kernel = blocks == units ? &gemv_q4_kernel<NB, NI, SWIGLU, GS, 1> : &gemv_q4_kernel<NB, NI, SWIGLU, GS, 2>;
+    return launch_q4_kernel(kernel, p, dim3(blocks), lds, stream);
 }
+
+int row_groups(int rows) { return (rows + 7) / 8; }
 
 template <bool SWIGLU, int GS>
 int launch_q4_own(const Q4Params & p, hipStream_t stream) {
-    const int nb = p.rows <= 8 ? 1 : p.rows <= 16 ? 2 : 4;
-    auto kernel = nb == 1 ? &gemv_q4_rows_kernel<1, SWIGLU, GS> : &gemv_q4_rows_kernel<2, SWIGLU, GS>;
-    if constexpr (!SWIGLU) kernel = nb == 4 ? &gemv_q4_rows_kernel<4, false, GS> : kernel;
-    return launch_q4_kernel(kernel, p, p.n_tiles, static_cast<size_t>(kQ4Waves) * (SWIGLU ? 2 : 1) * nb * 4 * kWave * 4, stream);
+    const int parts = row_groups(p.rows);
+    // one workgroup per CU, and the fewest tiles that bring it to that: a workgroup splits its x once for all of them.  256 tiles, 32 rows
+    // in 1 / 2 / 4 16.4 / 10.4 / 8.8 us; 384 pairs, 8 rows 11.1 / 9.1 / 11.9.
+    int nu = 1;
+    while (nu < 4 && (p.n_tiles + nu - 1) / nu * parts > 256) ++nu;
+    const dim3 blocks((p.n_tiles + nu - 1) / nu, parts);
+    if (nu == 1) return launch_q4_kernel(&gemv_q4_rows_kernel<1, SWIGLU, GS>, p, blocks, 0, stream);
+    if (nu == 2) return launch_q4_kernel(&gemv_q4_rows_kernel<2, SWIGLU, GS>, p, blocks, 0, stream);
+    if (nu == 3) return launch_q4_kernel(&gemv_q4_rows_kernel<3, SWIGLU, GS>, p, blocks, 0, stream);
+    return launch_q4_kernel(&gemv_q4_rows_kernel<4, SWIGLU, GS>, p, blocks, 0, stream);
 }
 
 // Whether x fits in LDS and a wave's share of a row in its registers.
@@ -680,34 +673,29 @@ bool whole_x(int rows, int in_dim) {
     return in_dim <= 2048 * row_parts(rows) && static_cast<int64_t>(rows) * in_dim * 4 <= 2 * kXBytes;
 }
 
-template <int TW, bool SWIGLU, int GS>
+template <bool SWIGLU, int GS>
 int launch_q4_shared(const Q4Params & p, hipStream_t stream) {
-    if (p.rows <= 2) return launch_q4<1, 1, TW, SWIGLU, GS>(p, stream);
-    if (p.rows <= 8) return launch_q4<1, 4, TW, SWIGLU, GS>(p, stream);
-    if (p.rows <= 16) return launch_q4<2, 4, TW, SWIGLU, GS>(p, stream);
-    return launch_q4<4, 4, TW, SWIGLU, GS>(p, stream);
+    if (p.rows <= 2) return launch_q4<1, 1, SWIGLU, GS>(p, stream);
+    if (p.rows <= 8) return launch_q4<1, 4, SWIGLU, GS>(p, stream);
+    if (p.rows <= 16) return launch_q4<2, 4, SWIGLU, GS>(p, stream);
+    return launch_q4<4, 4, SWIGLU, GS>(p, stream);
 }
 
 template <bool SWIGLU, int GS>
 int launch_q4_rows(const Q4Params & p, hipStream_t stream) {
-    // its own x per wave where it does not fit in LDS, and where there are few tiles for the x in LDS to serve:
-    // (us) 128 tiles of 2048 columns: 8 rows 6.5 / 5.3, 16 rows 9.7 / 8.3, 32 rows 19.1 / 14.7; 384 pairs of tiles (12288 gate|up rows):
-    // 8 rows 12.4 / 10.9, 16 rows 17.5 / 19.7.  Up to 4 rows the x in LDS is as fast or faster.
-    const int shared = whole_x(p.rows, p.in_dim) ? p.rows : std::min(p.rows, 16);   // of more, 16 rows at a time: W is read twice
-    const bool own = !whole_x(shared, p.in_dim) || (p.rows > 4 && p.n_tiles <= (p.rows <= 8 ? 512 : 256));
-    // gate and up of 32 rows with their x pass the 256 registers of a lane: 16 rows at a time there, too
-    const int at_once = !own ? shared : SWIGLU ? std::min(p.rows, 16) : p.rows;
+    // Up to 1024 tiles every wave splits the x of its own columns, us against x in LDS: 128 tiles of 2048 columns 1 / 8 / 32 rows 4.4 / 5.4 /
+    // 5.9 against 5.0 / 6.6 / 19.2, 256 tiles 5.3 / 6.0 / 8.7 against 5.4 / 7.4 / 21.7, 1024 tiles 8.6 / 9.3 / 30.6 against 8.4 / 12.7 /
+    // 33.4, 384 pairs of tiles (12288 gate|up rows) 8.5 / 8.8 / 22.1 against 8.1 / 12.2 / 33.8; 2048 tiles 15.7 / 17.4 / 59.7
+    // against 12.1 / 16.6 / 48.3, and 1024 pairs of 1024 columns 24 rows 24.1 against 21.5.
+    const int at_once = whole_x(p.rows, p.in_dim) ? p.rows : std::min(p.rows, 16);   // of more, 16 rows at a time: W is read twice
+    const bool few = p.n_tiles <= 1024 && (!SWIGLU || (p.n_tiles * row_groups(p.rows) <= 2048 && (p.rows > 1 || p.n_tiles <= 256)));
+    if (few || !whole_x(at_once, p.in_dim)) return launch_q4_own<SWIGLU, GS>(p, stream);
     Q4Params part = p;
     for (int r = 0; r < p.rows; r += at_once) {
         part.rows = std::min(at_once, p.rows - r);
-        // two tiles per wave where that still leaves every CU a workgroup
-        int rc;
-        if (own) rc = launch_q4_own<SWIGLU, GS>(part, stream);
-        else if constexpr (SWIGLU) rc = launch_q4_shared<2, true, GS>(part, stream);
-        else rc = p.n_tiles >= 1024 ? launch_q4_shared<2, false, GS>(part, stream) : launch_q4_shared<1, false, GS>(part, stream);
-        if (rc != QA_OK) return rc;
-        part.x += static_cast<int64_t>(16) * p.in_dim;
-        part.y += static_cast<int64_t>(16) * p.out_dim;
+        if (const int rc = launch_q4_shared<SWIGLU, GS>(part, stream); rc != QA_OK) return rc;
+        part.x += static_cast<int64_t>(at_once) * p.in_dim;
+        part.y += static_cast<int64_t>(at_once) * p.out_dim;
     }
     return QA_OK;
 }
