@@ -36,6 +36,7 @@ constexpr int kQ4Threads = kQ4Waves * kWave;
 constexpr int kXBytes = 64 * 1024;                 // of x in LDS at a time: two workgroups per CU
 constexpr size_t kQ4Lds = 158 * 1024;              // of the CU's 160 KB, the rest is the kernel's own
 constexpr int kUnitTiles = 2;                     // tiles of a wave's unit where x is whole in LDS
+constexpr int kAhead = 2;                         // blocks whose weights are in flight while one is multiplied (1: 42 instead of 41 us)
 constexpr int kMaxExp = 127;                       // a power of two that is a float: x below 2^-112 keeps fewer bits
 constexpr int kQ4Exp = 15;                        // a row's largest finite |x| goes to [2^14, 2^15)
 
@@ -146,9 +147,8 @@ __device__ inline void spread_scales(float v, float (&d)[4 >> GS]) {
 
 // x row r of a block of 8 stands in rows (r % 2) 4 + r / 2 of the A operand, its second part 8 rows on: a lane's result i
 // belongs to x row 2 i + (lane / 16) % 2, so that up to 2 rows need the first result alone.
-// NB: blocks of 8 x rows.  NI: results of a lane that count (1 or 4).  A wave's unit is two tiles, with SwiGLU gate and up.  GS: groups of 32 << GS columns.  AHEAD: blocks whose weights are in flight while one
-// is multiplied.  All of x lies in LDS.
-template <int NB, int NI, bool SWIGLU, int GS, int AHEAD>
+// NB: blocks of 8 x rows.  NI: results of a lane that count (1 or 4).  A wave's unit is two tiles, with SwiGLU gate and up.  GS: groups of 32 << GS columns.  All of x lies in LDS.
+template <int NB, int NI, bool SWIGLU, int GS>
 __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     _Float16 * sx = reinterpret_cast<_Float16 *>(lds);            // [in_dim / 32][row][part][32]
@@ -166,12 +166,12 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     const int unit_step = static_cast<int>(gridDim.x) * p.wt;
     const int unit0 = wt * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
 
-    // weights and scales of the next AHEAD blocks are in flight, the first ones while x is prepared; behind its last block a
+    // weights and scales of the next kAhead blocks are in flight, the first ones while x is prepared; behind its last block a
     // wave loads that one again, so that no branch makes it wait for all
     constexpr int kGroups = 4 >> GS;                              // of a block
-    u4 w[AHEAD][kUnitTiles];
-    _Float16 d[AHEAD][kUnitTiles];
-    const int n_it = (n_kb + p.wk * AHEAD - 1) / (p.wk * AHEAD) * AHEAD;   // a wave's blocks of a unit, the last ones perhaps idle
+    u4 w[kAhead][kUnitTiles];
+    _Float16 d[kAhead][kUnitTiles];
+    const int n_it = (n_kb + p.wk * kAhead - 1) / (p.wk * kAhead) * kAhead;   // a wave's blocks of a unit, the last ones perhaps idle
     const uint32_t w_lane = lane * 16, d_lane = (lane & (kGroups * kTileRows - 1)) * 2;
     int f_unit = unit0, f_it = 0;
     auto fetch = [&](int slot) {
@@ -182,11 +182,8 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
             const int64_t at = static_cast<int64_t>(tile) * n_kb + kb;
             const char * wb = reinterpret_cast<const char *>(p.W) + at * (kWave * 16);
             const char * db = reinterpret_cast<const char *>(p.scales) + at * (kGroups * kTileRows * 2);
-            // a matrix of many tiles past the caches, which hold it no better (151936 x 2048: 34.5 instead of 35.5 us, 8 rows 44 / 45);
-            // 12288 gate|up rows stay (8.2 instead of 8.5)
-            const u4 * wl = reinterpret_cast<const u4 *>(wb + w_lane);
-            if constexpr (!SWIGLU) w[slot][t] = __builtin_nontemporal_load(wl);
-            else w[slot][t] = *wl;
+            // a matrix of more than 1024 tiles past the caches, which hold it no better (151936 x 2048: 34.5 instead of 35.5 us, 8 rows 44 / 45)
+            w[slot][t] = __builtin_nontemporal_load(reinterpret_cast<const u4 *>(wb + w_lane));
             d[slot][t] = *reinterpret_cast<const _Float16 *>(db + d_lane);
         }
         if (++f_it == n_it) {
@@ -195,7 +192,7 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
         }
     };
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) fetch(u);
+    for (int u = 0; u < kAhead; ++u) fetch(u);
 
     // Sum of squares and largest |x| of each row: the 8 waves share up to 8 rows, each taking a part of a row whose loads are
     // in flight together.  A workgroup that holds all of x writes its parts from those registers.
@@ -395,9 +392,9 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     for (int round = 0; round < rounds; ++round) {
         const int unit = unit0 + round * unit_step;
         clear();
-        for (int it = 0; it < n_it; it += AHEAD) {
+        for (int it = 0; it < n_it; it += kAhead) {
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) {
+            for (int u = 0; u < kAhead; ++u) {
                 const int kb = wk + (it + u) * p.wk;
                 block(u, min(kb, n_kb - 1), kb < n_kb);
             }
@@ -570,6 +567,144 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_rows_kernel(Q4Params p)
     }
 }
 
+// The same for a single x: its 8 rows of the A operand are 8 blocks of columns instead, split at once, so that the arithmetic on x is an
+// eighth; the product with W's block j gives its result in row j, and the others, of unlike blocks, are dropped.  All of a wave's
+// weights are in flight at once.  us with the form above: 2048 x 6144 6.1 / 7.9, 12288 gate|up rows 7.1 / 8.5, 4096 x 2048 4.9 / 5.3.
+template <int NU, bool SWIGLU, int GS>
+__global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_token_kernel(Q4Params p) {
+    constexpr int TW = SWIGLU ? 2 * NU : NU, kGroups = 4 >> GS, kBlocks = 8;
+    __shared__ float sa[kQ4Waves][TW][kWave];
+    __shared__ double s_sum[kQ4Waves];
+    __shared__ int s_exp[kQ4Waves];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c16 = lane & 15, g4 = lane >> 4, a8 = c16 & 7;
+    const bool second = c16 >= 8;
+    const int n_kb = p.in_dim / kTileCols, unit = blockIdx.x;
+    const int col = g4 * 8 + (second ? 4 : 0);
+    float acc[TW];
+#pragma unroll
+    for (int t = 0; t < TW; ++t) acc[t] = 0.0f;
+    double ss = 0.0;
+    int ex = kMaxExp;
+    const Unpack unpack;
+    for (int kb0 = wave; kb0 < n_kb; kb0 += kBlocks * kQ4Waves) {
+        // every load of the 8 blocks at once; behind the last block it is that one again
+        const int mine = kb0 + a8 * kQ4Waves;
+        const bool counts = mine < n_kb;
+        const int at = min(mine, n_kb - 1) * kTileCols + col;
+        f4 x[4], g[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            x[s] = *reinterpret_cast<const f4 *>(p.x + at + s * 32);
+            if (p.norm_w) g[s] = *reinterpret_cast<const f4 *>(p.norm_w + at + s * 32);
+        }
+        u4 w[kBlocks][TW];
+        _Float16 d[kBlocks][TW];
+#pragma unroll
+        for (int j = 0; j < kBlocks; ++j) {
+            if (kb0 + j * kQ4Waves >= n_kb) break;                // uniform for the wave
+#pragma unroll
+            for (int t = 0; t < TW; ++t) {
+                const int tile = SWIGLU ? min(unit * NU + t / 2, p.n_tiles - 1) + (t & 1) * p.n_tiles : min(unit * NU + t, p.n_tiles - 1);
+                const int64_t b = static_cast<int64_t>(tile) * n_kb + kb0 + j * kQ4Waves;
+                w[j][t] = reinterpret_cast<const u4 *>(p.W)[b * kWave + lane];
+                d[j][t] = p.scales[b * kGroups * kTileRows + (lane & (kGroups * kTileRows - 1))];
+            }
+        }
+        if (p.norm_w) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (counts) ss += static_cast<double>(x[s][e]) * x[s][e];
+                    x[s][e] *= g[s][e];
+                }
+            }
+        }
+        float mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(x[s][e]));
+        }
+        mx = wave_max_all(mx);
+        const bool inf = mx == INFINITY;
+        if (__builtin_expect(inf, 0)) {                           // rare: the largest of what is finite
+            mx = 0.0f;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fabsf(x[s][e]) < INFINITY ? fmaxf(mx, fabsf(x[s][e])) : mx;
+            }
+            mx = wave_max_all(mx);
+        }
+        const int to = mx > 0.0f ? min(ex, kQ4Exp - __builtin_amdgcn_frexp_expf(mx)) : ex;
+#pragma unroll
+        for (int t = 0; t < TW; ++t) acc[t] = ldexpf(acc[t], to - ex);
+        ex = to;
+        const float factor = ldexpf(1.0f, ex);
+        h8 a[4];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) a[s] = split_pair(x[s] * factor, inf, second);
+#pragma unroll
+        for (int j = 0; j < kBlocks; ++j) {
+            if (kb0 + j * kQ4Waves >= n_kb) break;
+            const bool row = (g4 & 1) == j / 4;                   // this lane's results are rows 4 (g4 % 2) .. + 3, in one part of x
+#pragma unroll
+            for (int t = 0; t < TW; ++t) {
+                float dg[kGroups];
+                spread_scales<GS>(static_cast<float>(d[j][t]), dg);
+                f4 group;
+                float sum = 0.0f;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const bool first = (s & ((1 << GS) - 1)) == 0, last = ((s + 1) & ((1 << GS) - 1)) == 0;
+                    const f4 c = first ? f4{0.0f, 0.0f, 0.0f, 0.0f} : group;
+                    group = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[s], unpack(w[j][t][s]), c, 0, 0, 0);
+                    if (last) sum = fmaf(group[j & 3], dg[s >> GS], sum);
+                }
+                acc[t] += row ? sum : 0.0f;
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) ss += __shfl_xor(ss, m, kWave);   // every x is in one lane
+    if (lane == 0) {
+        s_sum[wave] = ss;
+        s_exp[wave] = ex;
+    }
+    __syncthreads();
+    int least = s_exp[0];
+    double sum = s_sum[0];
+#pragma unroll
+    for (int k = 1; k < kQ4Waves; ++k) {
+        least = min(least, s_exp[k]);
+        sum += s_sum[k];
+    }
+#pragma unroll
+    for (int t = 0; t < TW; ++t) sa[wave][t][lane] = ldexpf(acc[t], least - ex);
+    __syncthreads();
+    constexpr int kOf = SWIGLU ? 2 : 1;                           // sums of a result
+    for (int n = wave; n < NU; n += kQ4Waves) {
+        float v[kOf];
+#pragma unroll
+        for (int t = 0; t < kOf; ++t) {
+            v[t] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kQ4Waves; ++k) v[t] += sa[k][n * kOf + t][lane];
+            v[t] += __shfl_xor(v[t], 16, kWave);
+            v[t] += __shfl_xor(v[t], 32, kWave);
+        }
+        const int o = (unit * NU + n) * kTileRows + c16;
+        if (g4 > 0 || o >= p.out_dim) continue;
+        const float f = p.norm_w ? 1.0f / sqrtf(static_cast<float>(sum / p.in_dim) + p.eps) : 1.0f;
+        float out = ldexpf(v[0] * f, -least);
+        if constexpr (SWIGLU) out = out / (1.0f + expf(-out)) * ldexpf(v[1] * f, -least);
+        p.y[o] = p.epilogue == kEpiAccumOp ? p.y[o] + out : out;
+    }
+}
+
 // Packing: a workgroup takes a block of 16 rows x 128 columns, thread 16 r + s the 8 columns 8 s .. of row r.
 __global__ __launch_bounds__(256) void pack_q4_kernel(const float * src, int out_dim, int in_dim, int group_shift, uint8_t * dst, _Float16 * scales) {
     const int n_kb = in_dim / kTileCols;
@@ -646,10 +781,7 @@ int launch_q4(Q4Params p, hipStream_t stream) {
     const int units = (p.n_units + p.wt - 1) / p.wt;
     const size_t lds = x_bytes + p.wt * (p.wk - 1) * join;
     const int blocks = std::min(units, lds <= 80 * 1024 - 1024 ? 512 : 256);
-    // a wave that has one unit fetches nothing behind it; with several, two blocks in flight carry over from one to the next
-    // (12288 gate|up rows, one row of x: 7.6 instead of 8.7 us; 151936 rows, 8 rows of x: 41 instead of 42)
-    const auto kernel = blocks == units ? &gemv_q4_kernel<NB, NI, SWIGLU, GS, 1> : &gemv_q4_kernel<NB, NI, SWIGLU, GS, 2>;
-    return launch_q4_kernel(kernel, p, dim3(blocks), lds, stream);
+    return launch_q4_kernel(&gemv_q4_kernel<NB, NI, SWIGLU, GS>, p, dim3(blocks), lds, stream);
 }
 
 int row_groups(int rows) { return (rows + 7) / 8; }
@@ -662,6 +794,11 @@ int launch_q4_own(const Q4Params & p, hipStream_t stream) {
     int nu = 1;
     while (nu < 4 && (p.n_tiles + nu - 1) / nu * parts > 256) ++nu;
     const dim3 blocks((p.n_tiles + nu - 1) / nu, parts);
+    if (p.rows == 1 && nu * (SWIGLU ? 2 : 1) <= 4) {              // more tiles' blocks than that pass a lane's registers
+        if (nu == 1) return launch_q4_kernel(&gemv_q4_token_kernel<1, SWIGLU, GS>, p, blocks, 0, stream);
+        if (nu == 2) return launch_q4_kernel(&gemv_q4_token_kernel<2, SWIGLU, GS>, p, blocks, 0, stream);
+        if constexpr (!SWIGLU) return launch_q4_kernel(&gemv_q4_token_kernel<4, SWIGLU, GS>, p, dim3((p.n_tiles + 3) / 4), 0, stream);
+    }
     if (nu == 1) return launch_q4_kernel(&gemv_q4_rows_kernel<1, SWIGLU, GS>, p, blocks, 0, stream);
     if (nu == 2) return launch_q4_kernel(&gemv_q4_rows_kernel<2, SWIGLU, GS>, p, blocks, 0, stream);
     if (nu == 3) return launch_q4_kernel(&gemv_q4_rows_kernel<3, SWIGLU, GS>, p, blocks, 0, stream);
@@ -684,11 +821,11 @@ int launch_q4_shared(const Q4Params & p, hipStream_t stream) {
 template <bool SWIGLU, int GS>
 int launch_q4_rows(const Q4Params & p, hipStream_t stream) {
     // Up to 1024 tiles every wave splits the x of its own columns, us against x in LDS: 128 tiles of 2048 columns 1 / 8 / 32 rows 4.4 / 5.4 /
-    // 5.9 against 5.0 / 6.6 / 19.2, 256 tiles 5.3 / 6.0 / 8.7 against 5.4 / 7.4 / 21.7, 1024 tiles 8.6 / 9.3 / 30.6 against 8.4 / 12.7 /
-    // 33.4, 384 pairs of tiles (12288 gate|up rows) 8.5 / 8.8 / 22.1 against 8.1 / 12.2 / 33.8; 2048 tiles 15.7 / 17.4 / 59.7
+    // 5.9 against 5.0 / 6.6 / 19.2, 256 tiles 4.9 / 6.0 / 8.7 against 5.4 / 7.4 / 21.7, 1024 tiles 7.3 / 9.3 / 30.6 against 8.4 / 12.7 /
+    // 33.4, 384 pairs of tiles (12288 gate|up rows) 7.1 / 8.8 / 22.1 against 8.1 / 12.2 / 33.8; 2048 tiles 15.7 / 17.4 / 59.7
     // against 12.1 / 16.6 / 48.3, and 1024 pairs of 1024 columns 24 rows 24.1 against 21.5.
     const int at_once = whole_x(p.rows, p.in_dim) ? p.rows : std::min(p.rows, 16);   // of more, 16 rows at a time: W is read twice
-    const bool few = p.n_tiles <= 1024 && (!SWIGLU || (p.n_tiles * row_groups(p.rows) <= 2048 && (p.rows > 1 || p.n_tiles <= 256)));
+    const bool few = p.n_tiles <= 1024 && (!SWIGLU || p.n_tiles * row_groups(p.rows) <= 2048);
     if (few || !whole_x(at_once, p.in_dim)) return launch_q4_own<SWIGLU, GS>(p, stream);
     Q4Params part = p;
     for (int r = 0; r < p.rows; r += at_once) {

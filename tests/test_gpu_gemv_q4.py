@@ -321,3 +321,64 @@ def test_norm_of_large_x_in_more_rows(qa, rows):
     x = (rng.standard_normal((rows, 2304)) * 3e18).astype(np.float32)
     norm = np.full(2304, 1e18, np.float32)
     close(gemv(qa, q, d, x, 32, 0, norm), *plain(q, d, x, 0, norm))
+
+
+@pytest.mark.parametrize("epi,norm", [(0, False), (0, True), (1, True), (2, True)])
+@pytest.mark.parametrize("out,k,group", [(40, 1920, 32), (4096 + 16, 2048, 64), (8208, 512, 128), (16, 128 * 65, 32), (12304, 256, 32)])
+def test_single_row(qa, out, k, group, epi, norm):
+    """One token: column blocks that do not come out even over the waves, more than 64 of them, several tiles per workgroup."""
+    rng = np.random.default_rng(k + epi)
+    out = -(-out // 16) * 16 if epi == 2 else out
+    q, d = weights(rng, out * (2 if epi == 2 else 1), k, group)
+    x = (rng.standard_normal((1, k)) * 3).astype(np.float32)
+    w = (1 + 0.1 * rng.standard_normal(k)).astype(np.float32) if norm else None
+    y0 = rng.standard_normal((1, out)).astype(np.float32) if epi == 1 else None
+    close(gemv(qa, q, d, x, group, epi, w, y0), *plain(q, d, x, epi, w, y0), rel=8e-6 if epi == 2 else 2e-6)
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("kind", ["up", "down", "mixed", "last", "tiny", "huge", "zero"])
+def test_single_row_of_unlike_columns(qa, kind, norm):
+    rng = np.random.default_rng(11)
+    k = 128 * 83
+    q, d = weights(rng, 48, k, 64)
+    x = rng.standard_normal((1, k)).astype(np.float32)
+    up = np.exp2(np.arange(k) // 256 - 20).astype(np.float32)
+    if kind == "up":
+        x *= up
+    elif kind == "down":
+        x *= up[::-1]
+    elif kind == "mixed":
+        x *= rng.permutation(up)
+    elif kind == "last":
+        x[:, :-1] = 0.0
+    elif kind == "tiny":
+        x *= np.float32(1e-30)
+    elif kind == "huge":
+        x *= np.float32(1e30 if not norm else 1e18)
+    else:
+        x[:] = 0.0
+    w = np.ones(k, np.float32) if norm else None
+    got = gemv(qa, q, d, x, 64, 0, w)
+    want, size = plain(q, d, x, 0, w)
+    if kind == "zero":
+        assert (got == 0).all()
+    else:
+        assert np.isfinite(got).all()
+        assert np.linalg.norm(got - want) <= 3e-6 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("at", [0, 1029, 2303, 8400])
+def test_single_row_not_finite(qa, value, at):
+    rng = np.random.default_rng(at)
+    k = 128 * 66
+    q, d = weights(rng, 32, k, 64)
+    q[:16, at], q[16:31, at], q[31, at] = 12, 3, 8
+    x = rng.standard_normal((1, k)).astype(np.float32)
+    x[0, at] = value
+    got = gemv(qa, q, d, x, 64)[0]
+    if np.isnan(value):
+        assert np.isnan(got).all()
+    else:
+        assert (got[:16] == value).all() and (got[16:31] == -value).all() and np.isnan(got[31])
