@@ -33,12 +33,12 @@ constexpr int kTileRows = 16, kTileCols = 128;
 constexpr int kQ4MaxRows = 32;
 constexpr int kQ4Waves = 8;                        // per workgroup
 constexpr int kQ4Threads = kQ4Waves * kWave;
-constexpr int kXBytes = 64 * 1024;                 // of x in LDS at a time: two workgroups per CU
+constexpr int kXMost = 128 * 1024;                 // of x in LDS
 constexpr size_t kQ4Lds = 158 * 1024;              // of the CU's 160 KB, the rest is the kernel's own
-constexpr int kUnitTiles = 2;                     // tiles of a wave's unit where x is whole in LDS
-constexpr int kAhead = 2;                         // blocks whose weights are in flight while one is multiplied (1: 42 instead of 41 us)
+constexpr int kUnitTiles = 2;                      // tiles of a wave's unit where x is whole in LDS
+constexpr int kAhead = 2;                          // blocks whose weights are in flight while one is multiplied (1: 42 instead of 41 us)
 constexpr int kMaxExp = 127;                       // a power of two that is a float: x below 2^-112 keeps fewer bits
-constexpr int kQ4Exp = 15;                        // a row's largest finite |x| goes to [2^14, 2^15)
+constexpr int kQ4Exp = 15;                         // a row's largest finite |x| goes to [2^14, 2^15)
 
 struct Q4Params {
     const uint8_t * W;
@@ -753,7 +753,7 @@ int check_q4(int32_t out_dim, int32_t in_dim, int32_t group, const char * who) {
 }
 
 int launch_q4_kernel(void (*kernel)(Q4Params), const Q4Params & p, dim3 blocks, size_t lds, hipStream_t stream) {
-    if (lds > kXBytes / 2) {
+    if (lds > 32 * 1024) {
         QA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
     }
     hipLaunchKernelGGL(kernel, blocks, dim3(kQ4Threads), lds, stream, p);
@@ -807,7 +807,7 @@ int launch_q4_own(const Q4Params & p, hipStream_t stream) {
 
 // Whether x fits in LDS and a wave's share of a row in its registers.
 bool whole_x(int rows, int in_dim) {
-    return in_dim <= 2048 * row_parts(rows) && static_cast<int64_t>(rows) * in_dim * 4 <= 2 * kXBytes;
+    return in_dim <= 2048 * row_parts(rows) && static_cast<int64_t>(rows) * in_dim * 4 <= kXMost;
 }
 
 template <bool SWIGLU, int GS>
