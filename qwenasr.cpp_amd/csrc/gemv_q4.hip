@@ -81,17 +81,13 @@ struct Unpack {
     }
 };
 
-// 4 neighbouring values of an x row, times the row's factor, as the two f16 parts.
+// 4 neighbouring values of an x row, times the row's power of two (no product is rounded here), as the two f16 parts.
 // inf: the row holds an infinity, whose second part is 0 instead of inf - inf.
-// The product is rounded to f32 once, in a register that both parts come from: contracted into one of the conversions it would
-// round differently there, and the parts would not add up where it lies half way between two f16.
-__device__ inline void split_x(f4 v, float factor, bool inf, _Float16 * to) {
-#pragma clang fp contract(off)
+__device__ inline void split_x(f4 v, float unit, bool inf, _Float16 * to) {
     h4 hi, lo;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        float s = v[e] * factor;
-        asm volatile("" : "+v"(s));
+        const float s = v[e] * unit;
         hi[e] = static_cast<_Float16>(s);
         lo[e] = static_cast<_Float16>(s - static_cast<float>(hi[e]));
         if (inf && fabsf(s) == INFINITY) lo[e] = static_cast<_Float16>(0.0f);
@@ -152,9 +148,8 @@ template <int NB, int NI, bool SWIGLU, int GS>
 __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     _Float16 * sx = reinterpret_cast<_Float16 *>(lds);            // [in_dim / 32][row][part][32]
-    __shared__ float s_factor[kQ4MaxRows];                        // RMSNorm factor of each row, times its power of two
-    __shared__ int s_exp[kQ4MaxRows];                             // that power
-    __shared__ bool s_inf[kQ4MaxRows];
+    __shared__ float s_factor[kQ4MaxRows];                        // RMSNorm factor of each row
+    __shared__ int s_exp[kQ4MaxRows];                             // and the power of two of its x
     __shared__ double s_sum[kQ4Waves];                            // of a row's parts
     __shared__ float s_max[kQ4Waves];                             // a sign: an infinity among them
     const int lane = threadIdx.x & (kWave - 1);
@@ -250,20 +245,17 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
         }
     };
     auto finish_row = [&](int r) {
-        const float f = p.norm_w ? 1.0f / sqrtf(static_cast<float>(ss / p.in_dim) + p.eps) : 1.0f;
-        mx *= f;
-        // 2^127 at most, so that it is a float: x below 2^-112 keeps fewer bits of its own headroom, none of its value
-        const int ex = mx > 0.0f && mx < INFINITY ? min(kQ4Exp - __builtin_amdgcn_frexp_expf(mx), 127) : 0;
-        const float factor = f * ldexpf(1.0f, ex);
+        // RMSNorm's factor is one of the result: the factor of a small row times its power of two is no float
+        const int ex = mx > 0.0f ? min(kQ4Exp - __builtin_amdgcn_frexp_expf(mx), kMaxExp) : 0;
+        const float unit = ldexpf(1.0f, ex);
         if (lane == 0 && part == 0) {
-            s_factor[r] = factor;
+            s_factor[r] = p.norm_w ? 1.0f / sqrtf(static_cast<float>(ss / p.in_dim) + p.eps) : 1.0f;
             s_exp[r] = ex;
-            s_inf[r] = inf;
         }
 #pragma unroll
         for (int u = 0; u < kPer; ++u) {
             const int k = part * kWave + lane + u * step;
-            if (k < n4) split_x(v[u], factor, inf, sx + ((k >> 3) * cols + 2 * r) * 32 + (k & 7) * 4);
+            if (k < n4) split_x(v[u], unit, inf, sx + ((k >> 3) * cols + 2 * r) * 32 + (k & 7) * 4);
         }
     };
     if (parts > 1) {                                              // one row per wave at most, parts of it in several
@@ -353,8 +345,8 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
                     const int o = (SWIGLU ? unit : unit * kUnitTiles + t) * kTileRows + c16;
                     if (o >= p.out_dim) continue;                 // rows and tiles behind the last
                     float * y = p.y + static_cast<int64_t>(r) * p.out_dim + o;
-                    float out = ldexpf(v[t], -s_exp[r]);
-                    if constexpr (SWIGLU) out = out / (1.0f + expf(-out)) * ldexpf(v[1], -s_exp[r]);
+                    float out = ldexpf(v[t] * s_factor[r], -s_exp[r]);
+                    if constexpr (SWIGLU) out = out / (1.0f + expf(-out)) * ldexpf(v[1] * s_factor[r], -s_exp[r]);
                     *y = p.epilogue == kEpiAccumOp ? *y + out : out;
                 }
             }
