@@ -360,8 +360,8 @@ int qa_pack_q4(const float * src, int32_t out_dim, int32_t in_dim, int32_t group
                void * stream);
 /* qa_gemv_fused on 4-bit weights and 1 to 32 rows: y[r] = W x[r] (epilogue 0), y[r] += W x[r] (1), or y[r] = silu(g) * u
  * with W = the packed rows [gate; up], 2 out_dim of them, out_dim % 16 == 0 (2); norm_w != NULL first replaces x[r] by
- * RMSNorm(x[r]) * norm_w (eps).  Products and sums have f32 accuracy.  x: [rows][in_dim], y: [rows][out_dim], which must
- * not overlap.  W_q4, x and norm_w aligned to 16 bytes, scales to 8.                               */
+ * RMSNorm(x[r]) * norm_w (eps).  Products and sums have f32 accuracy; x * norm_w of finite x must be finite in f32 (the norm's
+ * factor comes behind the product).  x: [rows][in_dim], y: [rows][out_dim], which must not overlap.  W_q4, x and norm_w aligned to 16 bytes, scales to 8.                               */
 int qa_gemv_q4(const uint8_t * W_q4, const uint16_t * scales, int32_t group, int32_t out_dim, int32_t in_dim,
                const float * x, int32_t rows, float * y, int32_t epilogue, const float * norm_w, float eps, void * stream);
 /* RMSNorm of each row (text-decoder.cpp:92-98): y = x * (1/sqrtf(mean(x^2) + eps)) * w.          */

@@ -56,6 +56,15 @@ struct Q4Params {
 // Waves that share a row of x when its factor is computed.
 __host__ __device__ inline int row_parts(int rows) { return rows <= 1 ? 8 : rows <= 2 ? 4 : rows <= 4 ? 2 : 1; }
 
+// RMSNorm's factor from a row's sum of squares.  A mean past f32's range (x of 2e19 and more) goes there by 2^-140, where eps
+// is nothing beside it, and its root's half comes back.
+__device__ inline float norm_factor(double sum, int dim, float eps) {
+    const double mean = sum / dim;
+    const bool past = mean > 3e38;
+    const float f = 1.0f / sqrtf(past ? static_cast<float>(mean * 0x1p-140) : static_cast<float>(mean) + eps);
+    return past ? f * 0x1p-70f : f;
+}
+
 // 8 nibbles of a word as q - 8 in column order (column e lies in bits 4 (e / 2) + 16 (e % 2)).
 struct Unpack {
     uint32_t low, high, magic;
@@ -249,7 +258,7 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
         const int ex = mx > 0.0f ? min(kQ4Exp - __builtin_amdgcn_frexp_expf(mx), kMaxExp) : 0;
         const float unit = ldexpf(1.0f, ex);
         if (lane == 0 && part == 0) {
-            s_factor[r] = p.norm_w ? 1.0f / sqrtf(static_cast<float>(ss / p.in_dim) + p.eps) : 1.0f;
+            s_factor[r] = p.norm_w ? norm_factor(ss, p.in_dim, p.eps) : 1.0f;
             s_exp[r] = ex;
         }
 #pragma unroll
@@ -551,7 +560,7 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_rows_kernel(Q4Params p)
             sum += s_sum[k][r];
             least = min(least, s_exp[k][r]);
         }
-        const float f = p.norm_w ? 1.0f / sqrtf(static_cast<float>(sum / p.in_dim) + p.eps) : 1.0f;
+        const float f = p.norm_w ? norm_factor(sum, p.in_dim, p.eps) : 1.0f;
         float * y = p.y + static_cast<int64_t>(row0 + r) * p.out_dim + o;
         float out = ldexpf(v[0] * f, -least);
         if constexpr (SWIGLU) out = out / (1.0f + expf(-out)) * ldexpf(v[1] * f, -least);
@@ -690,7 +699,7 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_token_kernel(Q4Params p
         }
         const int o = (unit * NU + n) * kTileRows + c16;
         if (g4 > 0 || o >= p.out_dim) continue;
-        const float f = p.norm_w ? 1.0f / sqrtf(static_cast<float>(sum / p.in_dim) + p.eps) : 1.0f;
+        const float f = p.norm_w ? norm_factor(sum, p.in_dim, p.eps) : 1.0f;
         float out = ldexpf(v[0] * f, -least);
         if constexpr (SWIGLU) out = out / (1.0f + expf(-out)) * ldexpf(v[1] * f, -least);
         p.y[o] = p.epilogue == kEpiAccumOp ? p.y[o] + out : out;

@@ -50,3 +50,19 @@ def test_norm_of_small_x(qa, out, rows, scale):
     for r in range(rows):
         bar = small_bar(values(q, d), 1000.0) if 0 < np.abs(x[r]).max() < 1e-30 else 0.0
         assert np.linalg.norm(got[r] - want[r]) <= 2e-6 * np.linalg.norm(want[r]) + bar, r
+
+
+@pytest.mark.parametrize("scale", [1e20, 1e30, 3e37])
+@pytest.mark.parametrize("out,rows", [(OUT, 1), (OUT, 2), (OUT, 8), (OUT, 16), (80, 1), (80, 8), (80, 20)])
+def test_norm_of_x_whose_squares_pass_f32(qa, out, rows, scale):
+    """The mean of squares is no f32 from 1.8e19 on; the normalised row is as small as any."""
+    k, group = 1024, 64
+    q, d = matrix(out, k, group)
+    rng = np.random.default_rng(rows)
+    x = np.clip(rng.standard_normal((rows, k)), -5, 5).astype(np.float32) * np.float32(scale)
+    if rows > 2:
+        x[1] = rng.standard_normal(k)
+    w = (1 + 0.1 * rng.standard_normal(k)).astype(np.float32)
+    got = gemv(qa, q, d, x, group, 0, w)
+    want, size = plain(q, d, x, 0, w)
+    close(got, want, size)
