@@ -258,10 +258,9 @@ int qa_paged_attn(const float * q, const void * pages, const qa_kv_layout * layo
  * the order in which the GPU works: pages are given lowest number first, to the rows in list order.
  *
  * qa_pages_extend   gives the sequences of rows[i] (NULL: row i) what they need to write n_new[i] tokens at n_past[i]:
- *                   free pages for the entries of those positions that have none, and, where the first position written
- *                   lies in a page that other entries hold too, a free page with that page's content (all layers) in its
- *                   place; the last holder keeps the page itself.  Pages behind that one are taken as they are.  All or
- *                   nothing: *missing = the pages that were lacking, and 0 means done.  Positions behind the table row
+ *                   free pages for the entries of those positions that have none, and, for those in a page that other
+ *                   entries hold too, a free page with that page's content (all layers) in its place; of the listed rows
+ *                   that write one page the last keeps it, unless others hold it.  All or nothing: *missing = the pages that were lacking, and 0 means done.  Positions behind the table row
  *                   are not provided for.  A row listed again is left out.
  * qa_pages_fork     dst[i]'s row becomes src[i]'s entries of the first len[i] positions, which both hold from then on;
  *                   the pages that dst[i] held are given back.  Nothing is copied: qa_pages_extend copies what is about

@@ -22,8 +22,12 @@ constexpr int kScan = 8;             // counts per thread and pass over them
 constexpr int kPieceBytes = 16384;   // of a page, per workgroup
 constexpr int kCopyThreads = 256;
 
-// int32 workspace: [0] the pairs of a compaction, then the lists
+// int32 workspace: [0] the pairs to copy, then the lists
 constexpr int kWsHead = 16;
+
+// Pairs of an extend: one per list entry, and behind them, where dst says so, one per page given.
+constexpr int kBehind = -2;
+__host__ __device__ inline int64_t extend_pairs(int n_pages) { return static_cast<int64_t>(kMaxList) + n_pages; }
 
 __device__ inline bool is_page(int page, int n_pages) { return page >= 0 && page < n_pages; }
 __host__ __device__ inline int pages_of_positions(int n, int shift) {
@@ -66,6 +70,9 @@ struct ExtendParams {
 // Thread i < n plans list entry i.  The kernel's time is its dependent loads, so each is made for all entries at once: up to
 // kSpan table entries per list entry (a decode step's one or two) by the entry's thread, longer spans by a wave each; the
 // counts of the first pages are read before anything is known.
+// A page that others hold is as a rule the first one written: a beam goes on behind what it shares.  Who copies it is found in
+// LDS.  Only where a sequence has gone back, and is about to write pages behind its first that others hold, all entries
+// are counted per page in the workspace (`spread`).
 constexpr int kSpan = 4;
 
 __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams p) {
@@ -73,10 +80,13 @@ __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams
     __shared__ int s_j0[kMaxList], s_j1[kMaxList];
     __shared__ int s_need[kMaxList];
     __shared__ long long s_base[kMaxList], s_part[kPlanThreads / kWave];
+    __shared__ int s_behind;
     const int i = threadIdx.x, lane = i & (kWave - 1), wave = i >> 6;
     int32_t * src = p.ws + kWsHead;
-    int32_t * dst = src + kMaxList;
-    int32_t * list = dst + kMaxList;          // the free pages that are given, lowest first
+    int32_t * dst = src + extend_pairs(p.n_pages);
+    int32_t * list = dst + extend_pairs(p.n_pages);   // the free pages that are given, lowest first
+    int32_t * spare = list + p.n_pages;       // spread: listed entries that hold a page, less all that do
+    int32_t * last = spare + p.n_pages;       // and the last list entry among them
     // free pages among kScan counts, as a mask
     auto free_mask = [&](int64_t at) {
         unsigned mask = 0;
@@ -98,6 +108,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams
             j0 = min(past >> p.shift, j1);
         }
     }
+    if (i == 0) s_behind = 0;
     const bool wide = __syncthreads_or(j1 - j0 > kSpan);
     s_row[i] = row;
     int32_t * table = p.tables + static_cast<int64_t>(max(row, 0)) * p.stride;
@@ -118,13 +129,18 @@ __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams
         return hits;
     };
     if (count_ahead(s_row, row) > 0) row = -1, j0 = j1 = 0;   // listed before
-    int holders = 0;
-    if (row >= 0 && j0 < j1 && is_page(entry[0], p.n_pages)) {
-        holders = p.refs[entry[0]];
-        if (holders > 1) claim = entry[0];
-    }
+    int held[kSpan];
+#pragma unroll
+    for (int k = 0; k < kSpan; ++k) held[k] = j0 + k < j1 && is_page(entry[k], p.n_pages) ? p.refs[entry[k]] : 0;
+    const int holders = held[0];
+    if (holders > 1) claim = entry[0];
+    bool behind = false;
+#pragma unroll
+    for (int k = 1; k < kSpan; ++k) behind = behind || held[k] > 1;
     s_claim[i] = claim;
+    if (__any(behind) && lane == 0) s_behind = 1;
     __syncthreads();
+    bool spread = s_behind != 0;
     if (claim >= 0) {
         if (holders - count_ahead(s_claim, claim) <= 1) claim = -1;   // those ahead take a copy, the last holder keeps the page
     }
@@ -139,18 +155,56 @@ __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams
     s_j0[i] = j0;
     s_j1[i] = j1;
     s_need[i] = need;
-    if (wide) {
-        __syncthreads();
+    // every entry that list entry s writes, a wave per list entry and 64 entries at a time
+    auto walk = [&](auto && each, auto && done) {
         for (int s = wave; s < p.n; s += kPlanThreads / kWave) {
             const int32_t * of = p.tables + static_cast<int64_t>(max(s_row[s], 0)) * p.stride;
-            int count = 0;
             for (int b = s_j0[s]; b < s_j1[s]; b += kWave) {
-                const int j = b + lane;
-                count += __popcll(__ballot(j < s_j1[s] && !is_page(of[min(j, s_j1[s] - 1)], p.n_pages)));
+                const int j = b + lane, page = of[min(j, s_j1[s] - 1)];
+                each(s, j, j < s_j1[s], page);
             }
-            if (lane == 0) s_need[s] += count;
+            done(s);
         }
         __syncthreads();
+    };
+    const auto nothing = [](int) {};
+    // of the listed entries that hold a page the last one keeps it, unless others hold it; read past the caches, behind atomics
+    auto copied = [&](int s, int page) {
+        const int n = __hip_atomic_load(&spare[page], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return n < 0 || (n == 0 && __hip_atomic_load(&last[page], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != s);
+    };
+    int count = 0;
+    auto add_need = [&](int s) {
+        if (lane == 0) s_need[s] += count;
+        count = 0;
+    };
+    if (wide || spread) __syncthreads();
+    if (wide) {
+        walk([&](int s, int j, bool in, int page) {
+            const bool there = is_page(page, p.n_pages);
+            count += __popcll(__ballot(in && !there));
+            behind = behind || (in && j > s_j0[s] && there && p.refs[page] > 1);
+        }, add_need);
+        spread = __syncthreads_or(behind);
+    }
+    if (spread) {
+        walk([&](int, int, bool in, int page) {
+            if (!in || !is_page(page, p.n_pages)) return;
+            spare[page] = -p.refs[page];
+            last[page] = -1;
+        }, nothing);
+        walk([&](int s, int, bool in, int page) {
+            if (!in || !is_page(page, p.n_pages)) return;
+            atomicAdd(&spare[page], 1);
+            atomicMax(&last[page], s);
+        }, nothing);
+        claim = -1;
+        s_claim[i] = -1;
+        s_need[i] = 0;
+        __syncthreads();
+        walk([&](int s, int, bool in, int page) {
+            count += __popcll(__ballot(in && (!is_page(page, p.n_pages) || copied(s, page))));
+        }, add_need);
     }
     long long total = 0;
     const long long base = block_scan<long long>(i < p.n ? s_need[i] : 0, s_part, &total);
@@ -166,8 +220,9 @@ __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams
         found += here;
     }
     if (i == 0) *p.missing = total <= found ? 0 : static_cast<int32_t>(min(total - found, static_cast<long long>(INT32_MAX)));
-    if (i < p.n && (total > found || claim < 0)) dst[i] = -1;   // nothing to copy for this entry
+    if (i < p.n && (total > found || claim < 0)) dst[i] = spread && total <= found ? kBehind : -1;   // nothing to copy for this entry
     if (total > found) return;                            // nothing is changed
+    if (spread && i == 0) p.ws[0] = static_cast<int32_t>(p.n + total);
     __syncthreads();
     if (i < p.n && need > 0 && claim >= 0) {
         const int page = list[base];
@@ -177,7 +232,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams
         p.refs[page] = 1;
         atomicSub(&p.refs[claim], 1);
     }
-    if (!wide) {
+    if (!wide && !spread) {
         long long at = base + (claim >= 0 ? 1 : 0);
 #pragma unroll
         for (int k = 0; k < kSpan; ++k) {
@@ -194,13 +249,21 @@ __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams
         long long at = s_base[s] + (s_claim[s] >= 0 ? 1 : 0);
         // the first entry of a claim holds a page and is passed over here, whether its new number is visible yet or not
         for (int b = s_j0[s]; b < s_j1[s]; b += kWave) {
-            const int j = b + lane;
-            const bool want = j < s_j1[s] && !is_page(of[min(j, s_j1[s] - 1)], p.n_pages);
+            const int j = b + lane, old = of[min(j, s_j1[s] - 1)];
+            const bool in = j < s_j1[s], none = !is_page(old, p.n_pages);
+            const bool copy = spread && in && !none && copied(s, old);
+            const bool want = (in && none) || copy;
             const uint64_t all = __ballot(want);
             if (want) {
-                const int page = list[at + __popcll(all & ((1ull << lane) - 1))];
+                const long long r = at + __popcll(all & ((1ull << lane) - 1));
+                const int page = list[r];
                 of[j] = page;
                 p.refs[page] = 1;
+                if (spread) {
+                    src[p.n + r] = old;
+                    dst[p.n + r] = copy ? page : -1;
+                }
+                if (copy) atomicSub(&p.refs[old], 1);
             }
             at += __popcll(all);
         }
@@ -251,7 +314,7 @@ struct CopyParams {
     char * pages;
     const int32_t * src;
     const int32_t * dst;
-    const int32_t * count;   // pairs, or null: n
+    const int32_t * count;   // pairs that the device has counted, or null
     int64_t page_bytes;      // one (layer, K or V) block of a page
     int32_t n_pages, n, check;
 };
@@ -261,10 +324,11 @@ struct CopyParams {
 // page find it in the caches: 32 of them 31 us with the plan, 38 past the caches.
 template <bool ONCE>
 __global__ __launch_bounds__(kCopyThreads) void pages_copy_kernel(CopyParams p) {
-    const int n = p.count ? min(*p.count, p.n) : p.n;
+    int n = ONCE ? min(*p.count, p.n) : p.n;
     for (int i = blockIdx.z; i < n; i += gridDim.z) {
         if (p.check && !pair_stands(p.src, p.dst, i, n)) continue;   // uniform for the workgroup
         const int a = p.src[i], b = p.dst[i];
+        if (!ONCE && p.count && b == kBehind) n = *p.count;   // read only then: an extend's usual copies wait for nothing else
         if (!is_page(a, p.n_pages) || !is_page(b, p.n_pages) || a == b) continue;
         const int64_t block = static_cast<int64_t>(blockIdx.y) * p.n_pages;
         const int64_t at = static_cast<int64_t>(blockIdx.x) * kPieceBytes + threadIdx.x * 16;
@@ -370,7 +434,7 @@ int64_t block_bytes(const qa_kv_layout & l) {
 }
 
 int launch_copies(void * pages, const qa_kv_layout & l, const int32_t * src, const int32_t * dst, const int32_t * count, int32_t n,
-                  int32_t most, bool check, hipStream_t stream) {
+                  int32_t most, bool once, bool check, hipStream_t stream) {
     CopyParams p{};
     p.pages = static_cast<char *>(pages);
     p.src = src;
@@ -382,7 +446,7 @@ int launch_copies(void * pages, const qa_kv_layout & l, const int32_t * src, con
     p.check = check ? 1 : 0;
     const dim3 grid(static_cast<unsigned>((p.page_bytes + kPieceBytes - 1) / kPieceBytes), static_cast<unsigned>(2 * l.n_layers),
                     static_cast<unsigned>(std::max(1, std::min(n, most))));
-    const auto kernel = count ? &pages_copy_kernel<true> : &pages_copy_kernel<false>;   // a compaction's pairs are counted on the device
+    const auto kernel = once ? &pages_copy_kernel<true> : &pages_copy_kernel<false>;
     hipLaunchKernelGGL(kernel, grid, dim3(kCopyThreads), 0, stream, p);
     QA_LAUNCH_CHECK("pages_copy_kernel");
     return QA_OK;
@@ -418,7 +482,7 @@ int check_pool(const void * pages, const qa_kv_layout * l, const char * who) {
 extern "C" size_t qa_pages_workspace_bytes(const qa_kv_layout * layout) {
     using namespace qa;
     if (check_pages(layout, "qa_pages_workspace_bytes") != QA_OK) return 0;
-    return (kWsHead + 2 * kMaxList + 3 * static_cast<size_t>(layout->n_streams)) * sizeof(int32_t);
+    return (kWsHead + 2 * static_cast<size_t>(extend_pairs(layout->n_streams)) + 3 * static_cast<size_t>(layout->n_streams)) * sizeof(int32_t);
 }
 
 extern "C" int qa_pages_extend(void * pages, const qa_kv_layout * layout, int32_t * refs, int32_t * tables, int32_t n_rows,
@@ -449,7 +513,8 @@ extern "C" int qa_pages_extend(void * pages, const qa_kv_layout * layout, int32_
     hipLaunchKernelGGL(pages_extend_kernel, dim3(1), dim3(kPlanThreads), 0, as_stream(stream), p);
     QA_LAUNCH_CHECK("pages_extend_kernel");
     if (n == 0) return QA_OK;
-    return launch_copies(pages, *layout, p.ws + kWsHead, p.ws + kWsHead + kMaxList, nullptr, n, n, false, as_stream(stream));
+    const int64_t pairs = extend_pairs(p.n_pages);
+    return launch_copies(pages, *layout, p.ws + kWsHead, p.ws + kWsHead + pairs, p.ws, n, n, false, false, as_stream(stream));
 }
 
 extern "C" int qa_pages_fork(int32_t * refs, int32_t n_pages, int32_t * tables, int32_t n_rows, int32_t table_stride,
@@ -488,7 +553,7 @@ extern "C" int qa_pages_copy(void * pages, const qa_kv_layout * layout, const in
     if (n == 0) return QA_OK;
     if (!src || !dst) return fail(QA_ERR_INVALID, "qa_pages_copy: null pointer");
     if (const int rc = check_stream(stream, who); rc != QA_OK) return rc;
-    return launch_copies(pages, *layout, src, dst, nullptr, n, n, true, as_stream(stream));
+    return launch_copies(pages, *layout, src, dst, nullptr, n, n, false, true, as_stream(stream));
 }
 
 extern "C" int qa_pages_compact(void * pages, const qa_kv_layout * layout, const int32_t * refs, const int32_t * tables, int32_t n_rows,
@@ -509,7 +574,7 @@ extern "C" int qa_pages_compact(void * pages, const qa_kv_layout * layout, const
     QA_LAUNCH_CHECK("pages_compact_plan_kernel");
     const int32_t * holes = ws + kWsHead + n_pages;
     if (n_pages > 1) {
-        const int rc = launch_copies(pages, *layout, holes + n_pages, holes, ws, n_pages / 2, 256, false, as_stream(stream));
+        const int rc = launch_copies(pages, *layout, holes + n_pages, holes, ws, n_pages / 2, 256, true, false, as_stream(stream));
         if (rc != QA_OK) return rc;
     }
     const int64_t entries = static_cast<int64_t>(n_rows) * table_stride;
