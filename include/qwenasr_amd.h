@@ -51,7 +51,7 @@ int qa_copy_to_host(void * host_dst, const void * dev_src, size_t bytes);
 int qa_device_synchronize(void);
 
 /* Device memory, copies and timing on device 0, so hosts (tests, benchmarks, FFI callers) need no
- * second HIP runtime of their own.  stream NULL is the default stream. */
+ * second HIP runtime of their own.  stream NULL is the default stream (as is hipStreamLegacy), here and everywhere. */
 int qa_device_malloc(void ** out, size_t bytes);
 int qa_device_free(void * dev_ptr);
 int qa_copy_to_device(void * dev_dst, const void * host_src, size_t bytes);

@@ -36,7 +36,9 @@ inline int hip_fail(hipError_t e, const char * what) {
         if (qa_e_ != hipSuccess) return ::qa::hip_fail(qa_e_, what);   \
     } while (0)
 
-inline hipStream_t as_stream(void * s) { return reinterpret_cast<hipStream_t>(s); }
+// hipStreamLegacy is another name of the default stream, but the runtime's calls take it for an object's address (a call with it
+// ended the process).
+inline hipStream_t as_stream(void * s) { return s == hipStreamLegacy ? nullptr : reinterpret_cast<hipStream_t>(s); }
 
 constexpr int kHeadDim = 128;
 constexpr int kWave = 64;

@@ -76,7 +76,7 @@ inline int check_batch(const qa_kv_layout * l, int32_t layer, const qa_paged_bat
 
 // Launches go to the current device: a stream of another one is refused before anything is enqueued.
 inline int check_stream(void * stream, const char * who) {
-    if (!stream) return QA_OK;
+    if (!as_stream(stream)) return QA_OK;
     int current = 0;
     hipDevice_t owner = 0;
     if (hipGetDevice(&current) != hipSuccess || hipStreamGetDevice(as_stream(stream), &owner) != hipSuccess) {
