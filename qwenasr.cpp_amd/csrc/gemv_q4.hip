@@ -36,7 +36,7 @@ constexpr int kQ4Threads = kQ4Waves * kWave;
 constexpr int kXMost = 128 * 1024;                 // of x in LDS
 constexpr size_t kQ4Lds = 158 * 1024;              // of the CU's 160 KB, the rest is the kernel's own
 constexpr int kUnitTiles = 2;                      // tiles of a wave's unit where x is whole in LDS
-constexpr int kAhead = 2;                          // blocks whose weights are in flight while one is multiplied (1: 42 instead of 41 us)
+constexpr int kAhead = 2;                          // blocks whose weights are in flight while one is multiplied (1: 43.5 instead of 41.7 us, 16 rows 61.5 / 53.2)
 constexpr int kMaxExp = 127;                       // a power of two that is a float: x below 2^-112 keeps fewer bits
 constexpr int kQ4Exp = 15;                         // a row's largest finite |x| goes to [2^14, 2^15)
 
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(kQ4Threads, 2) void gemv_q4_kernel(Q4Params p) {
             const int64_t at = static_cast<int64_t>(tile) * n_kb + kb;
             const char * wb = reinterpret_cast<const char *>(p.W) + at * (kWave * 16);
             const char * db = reinterpret_cast<const char *>(p.scales) + at * (kGroups * kTileRows * 2);
-            // a matrix of more than 1024 tiles past the caches, which hold it no better (151936 x 2048: 34.5 instead of 35.5 us, 8 rows 44 / 45)
+            // a matrix of more than 1024 tiles past the caches, which hold it no better (151936 x 2048: 8 rows 41.7 instead of 42.3 us, one row alike)
             w[slot][t] = __builtin_nontemporal_load(reinterpret_cast<const u4 *>(wb + w_lane));
             d[slot][t] = *reinterpret_cast<const _Float16 *>(db + d_lane);
         }
@@ -765,8 +765,8 @@ int launch_q4_kernel(void (*kernel)(Q4Params), const Q4Params & p, dim3 blocks, 
 // How the waves divide the work where x is whole in LDS.  Units alone rarely fill the GPU evenly (9496 tiles over 4096 waves are
 // two rounds and a bit), so a unit's columns are shared by up to 8 waves, the more of them the fewer rows x has to be read
 // for: a tile's partial sums then meet in LDS.  No more workgroups run than are resident.
-// Measured with 1 / 2 / 4 / 8 waves per unit, 151936 x 2048: one row 54 / 40 / 34 / 35 us, 8 rows 53 / 45 / 41 / 41, 16 rows
-// 55 / 54 / 59 / 73.
+// Measured with 1 / 2 / 4 / 8 waves per unit, 151936 x 2048: one row 56 / 43 / 37.6 / 38.2 us, 8 rows 57 / 46 / 42.0 / 43.5, 16 rows
+// 56 / 54 / 63 / 77 (one card; the same call differs by 6% between cards, 8 rows 39 to 42).
 template <int NB, int NI, bool SWIGLU, int GS>
 int launch_q4(Q4Params p, hipStream_t stream) {
     p.n_units = SWIGLU ? p.n_tiles : (p.n_tiles + kUnitTiles - 1) / kUnitTiles;
@@ -806,7 +806,9 @@ int launch_q4_own(const Q4Params & p, hipStream_t stream) {
     return launch_q4_kernel(&gemv_q4_rows_kernel<4, SWIGLU, GS>, p, blocks, 0, stream);
 }
 
-// Whether x fits in LDS and a wave's share of a row in its registers.
+// Whether x fits in LDS and a wave's share of a row in its registers.  Behind that limit a vocabulary's x is split again for every
+// four of its tiles: 151936 x 2048 / 2176 columns, 4 rows 36 / 46 us, 8 rows 40 / 81, 16 rows 52 / 149, 32 rows 103 / 284; 4096 columns,
+// 4 rows 66, 8 rows 117.
 bool whole_x(int rows, int in_dim) {
     return in_dim <= 2048 * row_parts(rows) && static_cast<int64_t>(rows) * in_dim * 4 <= kXMost;
 }

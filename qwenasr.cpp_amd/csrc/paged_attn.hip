@@ -435,7 +435,9 @@ constexpr int rows_cols(bool f16, bool few) { return f16 && few ? 8 : 16; }
 constexpr size_t rows_lds(bool f16, bool few) { return kWaves * rows_cols(f16, few) * (kRowsStride + 2) * 4 + 2 * rows_cols(f16, few) * 4; }
 
 // A sequence that is one tile on f16 pages reads its K and V once, whole lines at a time: past the caches (ONCE).  32 sequences of
-// 3914 positions 85 instead of 94 us, of 157 to 3914 55.7 instead of 57.3.  A row of f32 pages is taken by halves of its lines, and
+// 3914 positions 84 instead of 94 us, of 157 to 3914 55.7 instead of 57.3.  That is for sequences with pages of their own; what
+// forked ones share is read once by each of them, and finds less of it in the caches: 32 beams behind 3913 shared positions 46.8
+// us, cached 42.6, behind 1000 19.2 / 18.5, eight behind 3913 22.3 / 21.1.  Nothing tells the two apart before the tables are read.  A row of f32 pages is taken by halves of its lines, and
 // longer chunks read it again: 129 instead of 111 us, and 50 instead of 40 at eight of 64 tokens.
 template <bool ONCE>
 __device__ inline u4 load_row(const void * at) {

@@ -72,7 +72,8 @@ struct ExtendParams {
 // counts of the first pages are read before anything is known.
 // A page that others hold is as a rule the first one written: a beam goes on behind what it shares.  Who copies it is found in
 // LDS.  Only where a sequence has gone back, and is about to write pages behind its first that others hold, all entries
-// are counted per page in the workspace (`spread`).
+// are counted per page in the workspace (`spread`).  Traced, 32 rows behind 3913 positions: 6.4 us where nothing is shared, 9.2 with one
+// shared page each, 17.2 and 18.0 where each has gone back over 4 and 10 shared pages.
 constexpr int kSpan = 4;
 
 __global__ __launch_bounds__(kPlanThreads) void pages_extend_kernel(ExtendParams p) {
