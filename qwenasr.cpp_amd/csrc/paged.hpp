@@ -57,7 +57,7 @@ inline int check_table(int32_t n_rows, int32_t stride, int32_t positions, const 
     return QA_OK;
 }
 
-inline int check_batch(const qa_kv_layout * l, int32_t layer, const qa_paged_batch * b, int32_t n_heads, const char * who) {
+inline int check_batch_sizes(const qa_kv_layout * l, int32_t layer, const qa_paged_batch * b, int32_t n_heads, const char * who) {
     if (check_pages(l, who) != QA_OK) return QA_ERR_INVALID;
     if (!b) return fail(QA_ERR_INVALID, std::string(who) + ": null batch");
     if (layer < 0 || layer >= l->n_layers) return fail(QA_ERR_INVALID, std::string(who) + ": layer out of range");
@@ -68,6 +68,11 @@ inline int check_batch(const qa_kv_layout * l, int32_t layer, const qa_paged_bat
     if (b->n_rows < 0 || b->n_rows >= kMaxCapacity || b->max_tokens < 0 || b->max_len < 0) {
         return fail(QA_ERR_INVALID, std::string(who) + ": row, token or position count out of range");
     }
+    return QA_OK;
+}
+
+inline int check_batch(const qa_kv_layout * l, int32_t layer, const qa_paged_batch * b, int32_t n_heads, const char * who) {
+    if (check_batch_sizes(l, layer, b, n_heads, who) != QA_OK) return QA_ERR_INVALID;
     if (b->n_rows > 0 && (!b->tables || !b->n_past || !b->row_start)) {
         return fail(QA_ERR_INVALID, std::string(who) + ": null pointer");
     }

@@ -984,7 +984,7 @@ int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
 
 extern "C" size_t qa_paged_attn_workspace_bytes(const qa_kv_layout * layout, const qa_paged_batch * batch, int32_t n_heads) {
     using namespace qa;
-    if (check_batch(layout, 0, batch, n_heads, "qa_paged_attn_workspace_bytes") != QA_OK || batch->n_rows == 0) return 0;
+    if (check_batch_sizes(layout, 0, batch, n_heads, "qa_paged_attn_workspace_bytes") != QA_OK || batch->n_rows == 0) return 0;
     const AttnPlan pl = attn_plan(*layout, *batch, n_heads, SIZE_MAX);
     if (pl.parts() <= 1) return 0;
     return static_cast<size_t>(batch->n_rows) * n_heads * pl.parts() * (kHeadDim + 2) * sizeof(float);
