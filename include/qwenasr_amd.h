@@ -218,8 +218,8 @@ int qa_qk_prep(float * qkv, int32_t n_tokens, int32_t n_heads, int32_t n_kv_head
 /* A ragged batch of sequences and their new tokens.  Rows row_start[s] .. row_start[s + 1] - 1 of the row buffers are
  * sequence s's new tokens (none is allowed), the first of them at position n_past[s] >= 0; row_start does not fall.  Rows
  * of no sequence are left as they were.  The three counts below are the host's bounds of what device memory says:
- * max_tokens new tokens of any one sequence (0: n_rows), max_len positions of any sequence with its new tokens
- * (0: what the table holds); max_len sets only how the work is split.                              */
+ * max_tokens new tokens of any one sequence (0: n_rows; the rows of a longer one may be left as they are), max_len
+ * positions of any sequence with its new tokens (0: what the table holds); max_len sets only how the work is split. */
 typedef struct qa_paged_batch {
     const int32_t * tables;      /* device [n_seqs][table_stride] */
     const int32_t * n_past;      /* device [n_seqs] */
