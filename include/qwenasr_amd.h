@@ -74,7 +74,10 @@ int qa_stream_synchronize(void * stream);
  * so for one (layer, kv, stream) the block is exactly the reference's per-layer tensor
  * ne = [head_dim, max_seq_len, n_kv_heads] (text-decoder.cpp:1451-1462): head-major, then
  * position, then dim, i.e. slot (h, p, i) at (h * max_seq_len + p) * head_dim + i.            */
-typedef enum { QA_CACHE_F32 = 0, QA_CACHE_F16 = 1 } qa_cache_type;
+typedef enum { QA_CACHE_F32 = 0, QA_CACHE_F16 = 1, QA_CACHE_Q8 = 2 } qa_cache_type;
+/* QA_CACHE_Q8: 8 bits with a scale per row, for caches in pages (below) alone: head_dim 128, pages of 16, 32, 64, 128 or 256
+ * positions.  Each (layer, kv, page) block holds its rows' int8 values in the order above, then their f32 scales
+ * [head][pos], 132 bytes per row: value = int8 * scale.  The entry points of the flat cache refuse it.  */
 
 typedef struct qa_kv_layout {
     int32_t n_layers;
@@ -87,9 +90,9 @@ typedef struct qa_kv_layout {
 
 int qa_kv_layout_check(const qa_kv_layout * layout);
 size_t qa_kv_elem_bytes(int32_t cache_type);
-/* Total bytes of the K+V allocation; 0 for an invalid layout. */
+/* Total bytes of the K+V allocation, the scales of QA_CACHE_Q8 among them; 0 for an invalid layout. */
 size_t qa_kv_cache_bytes(const qa_kv_layout * layout);
-/* Element index of one slot (see the formula above); -1 when out of range. */
+/* Element index of one slot (see the formula above; QA_CACHE_Q8: the byte of its value); -1 when out of range. */
 int64_t qa_kv_slot_index(const qa_kv_layout * layout, int32_t layer, int32_t kv, int32_t stream,
                          int32_t head, int32_t pos, int32_t dim);
 /* hipMalloc + zero fill (the reference clears its KV buffer, text-decoder.cpp:1472). */
@@ -233,15 +236,24 @@ typedef struct qa_paged_batch {
 
 /* qa_kv_append over pages, the same bits: q_out[r] <- RoPE(RMSNorm(q)), K and V rows into the page of the row's
  * position (dropped where there is none).  qkv: [n_rows][q_dim + 2 kv_dim], q_out: [n_rows][q_dim].  A page that several
- * tables hold is written as it is: qa_pages_extend makes it private first.                         */
+ * tables hold is written as it is: qa_pages_extend makes it private first.
+ * QA_CACHE_Q8: a row's scale is max |x| / 127 (f32, rounded to nearest) and its values are the integers nearest to x / scale,
+ * ties to even, within -127 .. 127; zeros where the scale is 0.  A row that holds an infinity or NaN gets the scale NaN.  */
 int qa_paged_append(const float * qkv, const float * q_norm_w, const float * k_norm_w, float * q_out, void * pages,
                     const qa_kv_layout * layout, int32_t layer, const qa_paged_batch * batch, int32_t n_heads,
                     float rope_theta, float eps, void * stream);
 
+/* The K and V rows of the batch's tokens read back from their pages, what qa_paged_append wrote for them (n_past 0 and as
+ * many rows as a sequence has positions: the whole sequence, for a cache of another kind or for storage outside the GPU).
+ * k_out, v_out: [n_rows][kv_dim] of out_type (QA_CACHE_F32 or QA_CACHE_F16, rounded to nearest); either may be NULL.  Rows
+ * on no page are zeros, rows of no sequence are left as they were.  pages, k_out and v_out aligned to 16 bytes.  */
+int qa_paged_read(const void * pages, const qa_kv_layout * layout, int32_t layer, const qa_paged_batch * batch, void * k_out,
+                  void * v_out, int32_t out_type, void * stream);
+
 /* Causal attention of every sequence's new tokens over its pages: the token at position p attends the positions
  * 0 .. p that lie on a page (a chunk of a prompt, or one token per sequence: a decode step).  A token that sees no
  * position gets zeros.  q: [n_rows][q_dim] f32 (post norm + RoPE), out: [n_rows][q_dim].  Products and sums have f32
- * accuracy for either cache type (q and the probabilities are not rounded to f16 as qa_decode_attn does).  scale > 0.
+ * accuracy for every cache type (q and the probabilities are not rounded to f16 as qa_decode_attn does).  scale > 0.
  * What masked positions hold never matters, NaN included.
  * workspace: results of key ranges that are joined at the end.  Any size works, none included; with less than
  * qa_paged_attn_workspace_bytes (of the same batch; its pointers are not read) the keys are cut into fewer ranges, which
@@ -251,6 +263,40 @@ size_t qa_paged_attn_workspace_bytes(const qa_kv_layout * layout, const qa_paged
 int qa_paged_attn(const float * q, const void * pages, const qa_kv_layout * layout, int32_t layer,
                   const qa_paged_batch * batch, int32_t n_heads, float scale, float * out, void * workspace,
                   size_t workspace_bytes, void * stream);
+
+/* Drafted tokens that are checked in one step: a batch whose rows are, per sequence, the nodes of a tree.  Node 0 is the
+ * last token that is certain, parents[r] is the number of row r's parent among its sequence's nodes, which must be a lower
+ * one than its own; a row whose parents[r] is not (-1, say) is a root.  Node i's K and V rows are written at position
+ * n_past + i, as qa_pages_extend provided for, while its rotary angle is that of n_past + its depth.
+ *
+ * qa_tree_prepare   mask[r][mask_words]: bit i % 32 of word i / 32 where node i is row r's ancestor or r itself, nodes behind
+ *                   32 mask_words left out; depth[r]: the number of its ancestors.  Once per step, for all layers.
+ * qa_paged_tree_append  qa_paged_append with the angles of n_past + depth[r] (anything that the caller wants, in fact).
+ * qa_paged_tree_attn    qa_paged_attn in which a row sees the n_past positions of its sequence and, of the new tokens, those
+ *                   whose bit is set in its mask (any mask will do; bits behind the sequence's rows mean nothing).  A row
+ *                   that sees no position gets zeros.
+ * qa_tree_accept    walks each tree from node 0: of the children of the node it is at, the first one whose ids[row] (the token
+ *                   that was fed) is picks[row of the node] (what the model picked behind it, as by qa_argmax_rows), until
+ *                   there is none.  path: the nodes passed, n_kept[s] of them, in the sequence's rows, and -1 in the rows
+ *                   behind them; next[s]: the pick of the last one.  A sequence without rows keeps 0, and next[s] = -1.
+ * qa_paged_keep     moves the K and V rows of node path[k] to position n_past + k, k < n_kept[s], in every layer: the
+ *                   sequence is then n_past + n_kept[s] positions long, and what lies behind may be written again.
+ *                   path has to rise strictly; from the first entry of a sequence that does not, or is no node, nothing is
+ *                   moved.
+ * batch->n_rows up to 2^24 here; parents, ids, picks, depth and path: device int32[n_rows]; n_kept, next: int32[n_seqs].
+ * Rows of no sequence are left as they were. */
+int qa_tree_prepare(const qa_paged_batch * batch, const int32_t * parents, uint32_t * mask, int32_t mask_words, int32_t * depth,
+                    void * stream);
+int qa_paged_tree_append(const float * qkv, const float * q_norm_w, const float * k_norm_w, float * q_out, void * pages,
+                         const qa_kv_layout * layout, int32_t layer, const qa_paged_batch * batch, const int32_t * depth,
+                         int32_t n_heads, float rope_theta, float eps, void * stream);
+int qa_paged_tree_attn(const float * q, const void * pages, const qa_kv_layout * layout, int32_t layer,
+                       const qa_paged_batch * batch, const uint32_t * mask, int32_t mask_words, int32_t n_heads, float scale,
+                       float * out, void * workspace, size_t workspace_bytes, void * stream);
+int qa_tree_accept(const qa_paged_batch * batch, const int32_t * parents, const int32_t * ids, const int32_t * picks,
+                   int32_t * path, int32_t * n_kept, int32_t * next, void * stream);
+int qa_paged_keep(void * pages, const qa_kv_layout * layout, const qa_paged_batch * batch, const int32_t * path,
+                  const int32_t * n_kept, void * stream);
 
 /* Bookkeeping of pages on the device.  refs[p]: the number of table entries that hold page p; a page with none
  * (refs[p] <= 0) is free.  tables: [n_rows][table_stride], one row per sequence the host keeps a place for; rows, src and
@@ -376,6 +422,29 @@ int qa_add_inplace(float * y, const float * x, size_t n, void * stream);
 size_t qa_argmax_workspace_bytes(int32_t rows);
 int qa_argmax_rows(const float * logits, int32_t rows, int32_t vocab, int32_t * ids, void * workspace,
                    size_t workspace_bytes, void * stream);
+/* Beam search, one step for n_groups utterances of `width` beams each (rows group * width + beam of logits [..][vocab]).  The
+ * candidates of a group are, for each of its beams b with done[b] == 0, every id v with the score
+ * scores[b] + logits[b][v] - log(sum over u of exp(logits[b][u])), and the beam itself, unchanged, where done[b] != 0 (done NULL:
+ * none).  The `width` best become the new beams, best first, ties to the lower beam and then the lower id:
+ * parents (the row that it continues), tokens (its id, -1 for a beam that was done), scores_out, and done_out: 1 where the
+ * parent was done or the id is one of stop_ids (device int32[n_stop], 0 to 64).  Sums, logarithms and comparisons are in 64 bits, scores
+ * rounded once.  A NaN is no candidate and weighs nothing, nor does -inf; a score of -inf or NaN leaves a beam without candidates (the
+ * first step, whose beams are the same: 0 for one of them and -inf for the others); a row with +inf has none.  Where a
+ * group has fewer than width candidates, the remaining new beams are done: parent the own row, token -1, score -inf.
+ * 1 to 64 beams, vocab >= width.  No output may overlap an input.  workspace: qa_beam_select_workspace_bytes, aligned to 16 bytes;
+ * nothing in it outlives the call; calls that share one must be stream-ordered.                     */
+size_t qa_beam_select_workspace_bytes(int32_t n_groups, int32_t width, int32_t vocab);
+int qa_beam_select(const float * logits, int32_t n_groups, int32_t width, int32_t vocab, const float * scores,
+                   const int32_t * done, const int32_t * stop_ids, int32_t n_stop, int32_t * parents, int32_t * tokens,
+                   float * scores_out, int32_t * done_out, void * workspace, size_t workspace_bytes, void * stream);
+/* The states of n beams put in the order of their new parents, in place: rows[i] (NULL: i) is list entry i's row of the tables
+ * and of ids, and becomes what the row of entry parents[i] was: the pages of its first lens[i] positions, none behind them, with refs kept
+ * as in qa_pages_fork, and its ids.  Then ids[rows[i]][ids_len[i]] = tokens[i], where that is a column and the token is not
+ * negative.  refs and tables NULL: only the ids; ids NULL: only the pages.  n <= 1024.  An entry whose row is outside [0, n_rows) or
+ * listed before, or whose parent is outside [0, n) or such an entry, keeps its row and its ids. */
+int qa_beam_reorder(int32_t * refs, int32_t n_pages, int32_t * tables, int32_t n_rows, int32_t table_stride,
+                    int32_t page_size, const int32_t * rows, const int32_t * parents, const int32_t * lens, int32_t n,
+                    int32_t * ids, int32_t ids_stride, const int32_t * tokens, const int32_t * ids_len, void * stream);
 /* out[r] = table[ids[r]] (rows of width dim); ids out of [0, n_rows) give a zero row.            */
 int qa_embed_rows(const float * table, int32_t n_rows, int32_t dim, const int32_t * ids, int32_t rows,
                   float * out, void * stream);

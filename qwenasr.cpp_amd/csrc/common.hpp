@@ -50,6 +50,25 @@ __host__ __device__ inline int64_t cache_row_offset(int layer, int kv, int strea
                 max_seq + pos) * kHeadDim;
 }
 
+// QA_CACHE_Q8: the f32 scales of a block's rows lie behind its values.
+constexpr int kQ8RowBytes = kHeadDim + 4;
+inline bool is_q8_layout(const qa_kv_layout & l) {
+    return l.head_dim == kHeadDim && l.max_seq >= 16 && l.max_seq <= 256 && (l.max_seq & (l.max_seq - 1)) == 0;
+}
+
+// Bytes of one (layer, K or V, stream or page) block.
+inline int64_t block_bytes(const qa_kv_layout & l) {
+    const int64_t rows = static_cast<int64_t>(l.n_kv_heads) * l.max_seq;
+    return rows * (l.cache_type == QA_CACHE_Q8 ? kQ8RowBytes : l.head_dim * static_cast<int64_t>(qa_kv_elem_bytes(l.cache_type)));
+}
+
+// For the entry points of the flat cache, which has no rows of 8 bits.
+inline int check_flat_layout(const qa_kv_layout * l) {
+    if (qa_kv_layout_check(l) != QA_OK) return QA_ERR_INVALID;
+    if (l->cache_type == QA_CACHE_Q8) return fail(QA_ERR_INVALID, "a cache of 8 bits serves the entry points of a cache in pages alone");
+    return QA_OK;
+}
+
 // Inverse RoPE frequencies, computed on the host with the reference's expression
 // exp(-ln(theta) * 2i / d) in double (text-decoder.cpp:611-613) and passed by value.
 struct RopeTable {

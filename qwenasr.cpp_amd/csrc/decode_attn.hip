@@ -263,7 +263,7 @@ extern "C" int qa_decode_attn(const float * q, const void * cache, const qa_kv_l
                               const int32_t * lens, int32_t n_streams, int32_t max_len, int32_t n_heads,
                               float scale, float * out, void * workspace, size_t workspace_bytes, void * stream) {
     using namespace qa;
-    if (qa_kv_layout_check(layout) != QA_OK) return QA_ERR_INVALID;
+    if (check_flat_layout(layout) != QA_OK) return QA_ERR_INVALID;
     if (!q || !cache || !lens || !out) return fail(QA_ERR_INVALID, "qa_decode_attn: null pointer");
     return decode_attn_launch(q, n_heads * kHeadDim, cache, *layout, layer, lens, 0, n_streams, max_len,
                               n_heads, scale, out, workspace, workspace_bytes, as_stream(stream));
@@ -274,7 +274,7 @@ extern "C" int qa_decode_step_attn(const float * qkv, const float * q_norm_w, co
                                    int32_t n_streams, int32_t max_len, int32_t n_heads, float rope_theta, float eps,
                                    float scale, float * out, void * workspace, size_t workspace_bytes, void * stream) {
     using namespace qa;
-    if (qa_kv_layout_check(layout) != QA_OK) return QA_ERR_INVALID;
+    if (check_flat_layout(layout) != QA_OK) return QA_ERR_INVALID;
     if (!qkv || !q_norm_w || !k_norm_w || !cache || !n_past || !out) {
         return fail(QA_ERR_INVALID, "qa_decode_step_attn: null pointer");
     }
@@ -292,7 +292,7 @@ extern "C" int qa_decode_step_attn_noalloc(const float * qkv, const float * q_no
                                            const int32_t * n_past, int32_t n_streams, int32_t max_len, int32_t n_heads,
                                            float rope_theta, float eps, float scale, float * out, void * stream) {
     using namespace qa;
-    if (qa_kv_layout_check(layout) != QA_OK) return QA_ERR_INVALID;
+    if (check_flat_layout(layout) != QA_OK) return QA_ERR_INVALID;
     if (!qkv || !q_norm_w || !k_norm_w || !cache || !n_past || !out) {
         return fail(QA_ERR_INVALID, "qa_decode_step_attn_noalloc: null pointer");
     }

@@ -183,7 +183,7 @@ extern "C" int qa_kv_append(const float * qkv, const float * q_norm_w, const flo
                             const int32_t * n_past, int32_t n_streams, int32_t n_tokens, int32_t n_heads,
                             float rope_theta, float eps, void * stream) {
     using namespace qa;
-    if (qa_kv_layout_check(layout) != QA_OK) return QA_ERR_INVALID;
+    if (check_flat_layout(layout) != QA_OK) return QA_ERR_INVALID;
     if (!qkv || !q_norm_w || !k_norm_w || !q_out || !cache || !n_past) {
         return fail(QA_ERR_INVALID, "qa_kv_append: null pointer");
     }

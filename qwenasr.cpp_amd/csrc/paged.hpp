@@ -79,6 +79,15 @@ inline int check_batch(const qa_kv_layout * l, int32_t layer, const qa_paged_bat
     return QA_OK;
 }
 
+// Trees of drafted tokens: mask_words words per row, and rows that 32 bits count in any of their arrays.
+constexpr int kMaxMaskWords = 32, kMaxTreeRows = 1 << 24;
+inline int check_tree(const qa_paged_batch * b, int32_t mask_words, const char * who) {
+    if (!b) return fail(QA_ERR_INVALID, std::string(who) + ": null batch");
+    if (b->n_seqs <= 0 || b->n_rows < 0 || b->n_rows > kMaxTreeRows) return fail(QA_ERR_INVALID, std::string(who) + ": row count out of range");
+    if (mask_words < 1 || mask_words > kMaxMaskWords) return fail(QA_ERR_INVALID, std::string(who) + ": 1 to 32 words of mask");
+    return QA_OK;
+}
+
 // Launches go to the current device: a stream of another one is refused before anything is enqueued.
 inline int check_stream(void * stream, const char * who) {
     if (!as_stream(stream)) return QA_OK;

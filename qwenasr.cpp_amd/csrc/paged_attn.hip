@@ -38,6 +38,8 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazyLog2 = 8.0f;    // the reference maximum follows when it is behind by more than 2^8
@@ -47,7 +49,11 @@ constexpr int kMaxSplits = 64;       // key ranges whose results the joining ker
 constexpr int kWaves = 4, kThreads = kWaves * kWave;
 // Sequences of few columns: a workgroup holds all of them.  On f16 pages 8 columns lie in both parts in one product.
 constexpr int few_cols(bool f16) { return f16 ? 8 : 16; }
-constexpr int step_keys(bool f16) { return f16 ? 32 : 16; }   // 8 KB of K and 8 KB of V
+constexpr int step_keys(bool f16) { return f16 ? 32 : 16; }   // 8 KB of K and 8 KB of V, half of it on pages of 8 bits
+template <typename CT>
+constexpr bool is_q8 = std::is_same<CT, int8_t>::value;
+template <typename CT>
+constexpr bool f16_products = is_q8<CT> || std::is_same<CT, _Float16>::value;
 
 struct AttnParams {
     const float * q;
@@ -62,6 +68,8 @@ struct AttnParams {
     int32_t splits_many, splits_few, steps_many, steps_few;   // key ranges of each kind, and their steps
     int32_t n_parts;      // ranges that the workspace holds of a (row, head): the more of the two
     float scale;
+    const uint32_t * mask;   // trees: [rows][mask_words], bit i: the row sees its sequence's new token i
+    int32_t mask_words;
 };
 
 __device__ inline uint32_t lo_pair(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
@@ -86,7 +94,7 @@ struct Tile {
 // Block -> (KV head, split, tile); false: nothing to do.  Neighbouring blocks, which go to different XCDs, take different heads.
 // Every lane counts one sequence's tiles, a prefix sum over the wave finds the sequence that holds the tile; what the tile
 // needs is read along.  FEW: the sequences of 1 .. few_max columns, otherwise the longer ones.
-template <int R, int KS, bool FEW>
+template <int R, int KS, bool FEW, bool TREE>
 __device__ inline bool find_tile(const AttnParams & p, int block, int lane, Tile & t, int & head) {
     const int n_tiles = FEW ? p.tiles_few : p.tiles_many, split_steps = FEW ? p.steps_few : p.steps_many;
     head = block % p.n_kv;
@@ -121,7 +129,7 @@ __device__ inline bool find_tile(const AttnParams & p, int block, int lane, Tile
             t.col0 = (count - 1 - (tile - before)) * R;               // the last tile has the most keys: first
             t.n_cols = t.rows * p.group;
             t.cap = p.seqs.table_stride << p.page_shift;
-            t.kend = max(0, min(t.past + (min(t.col0 + R, t.n_cols) - 1) / p.group, t.cap - 1) + 1);
+            t.kend = max(0, min(t.past + (TREE ? t.rows - 1 : (min(t.col0 + R, t.n_cols) - 1) / p.group), t.cap - 1) + 1);
             t.n_steps = (t.kend + KS - 1) / KS;
             t.step_lo = t.split * split_steps;
             t.step_hi = t.split == t.n_splits - 1 ? t.n_steps : min(t.n_steps, t.step_lo + split_steps);
@@ -138,54 +146,60 @@ struct Column {
     const float * q;
 };
 
+template <bool TREE>
 __device__ inline Column column_of(const AttnParams & p, const Tile & t, int head, int col) {
     const bool ok = col < t.n_cols;
     const int token = (ok ? col : t.n_cols - 1) / p.group;
     const int row = (t.row0 + token) * p.n_heads + head * p.group + (ok ? col - token * p.group : 0);
-    return Column{ok ? row : -1, ok ? min(t.past + token, t.cap - 1) : -1, p.q + static_cast<int64_t>(row) * kHeadDim};
+    return Column{ok ? row : -1, ok ? min(t.past + (TREE ? t.rows - 1 : token), t.cap - 1) : -1, p.q + static_cast<int64_t>(row) * kHeadDim};
 }
-
-// The K and V rows of one KV head: page + page_elems per page, V v_elems behind K.
-template <typename CT>
-struct HeadRows {
-    const CT * k;
-    int64_t page_elems, v_elems;
-    __device__ inline HeadRows(const AttnParams & p, int head) {
-        const int64_t rows = static_cast<int64_t>(1) << p.page_shift;
-        page_elems = p.n_kv * rows * kHeadDim;
-        v_elems = p.n_pages * page_elems;
-        k = static_cast<const CT *>(p.pages) + 2 * p.layer * v_elems + head * rows * kHeadDim;
-    }
-    __device__ inline const CT * page(int page) const { return k + page * page_elems; }
-};
 
 // A table entry as the page of the 16 keys from j on, -1 for none.
 __device__ inline int entry_page(const AttnParams & p, const Tile & t, int entry, int j) {
     return j < t.kend && entry >= 0 && entry < p.n_pages ? entry : -1;
 }
 
-// Whether any position up to lim lies on a page.
-__device__ inline bool sees_any(const AttnParams & p, const int32_t * table, int lim) {
-    for (int j = 0; j <= lim; j += 1 << p.page_shift) {
+// 32 bits of a row's mask from new token `first` on; cached positions (numbers below 0) are seen, those behind the mask are not.
+__device__ inline uint32_t mask_window(const AttnParams & p, const uint32_t * words, int first) {
+    const int w = first >> 5;
+    const uint32_t lo = w < 0 ? ~0u : w < p.mask_words ? words[w] : 0u;
+    const uint32_t hi = w + 1 < 0 ? ~0u : w + 1 < p.mask_words ? words[w + 1] : 0u;
+    return __builtin_amdgcn_alignbit(hi, lo, first & 31);
+}
+
+__device__ inline const uint32_t * mask_row(const AttnParams & p, int row) {
+    return p.mask + static_cast<int64_t>(row / p.n_heads) * p.mask_words;
+}
+
+// Whether any position that the row (token and head) sees lies on a page.
+template <bool TREE>
+__device__ inline bool sees_any(const AttnParams & p, const int32_t * table, int lim, int past, int row) {
+    for (int j = 0; j <= (TREE ? min(lim, past - 1) : lim); j += 1 << p.page_shift) {
         if (page_of(table, p.seqs.table_stride, p.page_shift, p.n_pages, j) >= 0) return true;
+    }
+    if constexpr (TREE) {
+        for (int j = max(past, 0); j <= lim; ++j) {
+            if ((mask_window(p, mask_row(p, row), j - past) & 1u) && page_of(table, p.seqs.table_stride, p.page_shift, p.n_pages, j) >= 0) return true;
+        }
     }
     return false;
 }
 
 // 1 / sum, 0 for a row that sees no key; a row whose visible scores are all -inf has sum 0 and is NaN by the formula.
-__device__ inline float inverse_sum(const AttnParams & p, const int32_t * table, int lim, float l) {
-    if (l == 0.0f) return sees_any(p, table, lim) ? NAN : 0.0f;
+template <bool TREE>
+__device__ inline float inverse_sum(const AttnParams & p, const int32_t * table, int lim, int past, int row, float l) {
+    if (l == 0.0f) return sees_any<TREE>(p, table, lim, past, row) ? NAN : 0.0f;
     return 1.0f / l;
 }
 
 // One column over the visible keys of steps step0, step0 + step_inc, .. < step1, in f32, key by key: lane holds dims
 // 2 lane and 2 lane + 1.  m in log2 units.
-template <typename CT, int KS>
-__device__ inline void column_by_keys(const AttnParams & p, const int32_t * table, int head, const float * q, int lim, int step0,
+template <typename CT, int KS, bool TREE>
+__device__ inline void column_by_keys(const AttnParams & p, const int32_t * table, int head, int row, int lim, int past, int step0,
                                       int step1, int step_inc, int lane, float & m, float & l, f2 & o) {
-    const f2 qv = *reinterpret_cast<const f2 *>(q + 2 * lane);
+    const f2 qv = *reinterpret_cast<const f2 *>(p.q + static_cast<int64_t>(row) * kHeadDim + 2 * lane);
     const float c = p.scale * kLog2e;
-    const HeadRows<CT> rows(p, head);
+    const HeadRows<CT> rows(p.pages, p.layer, p.n_kv, p.n_pages, p.page_shift, head);
     m = -INFINITY;
     l = 0.0f;
     o = f2{0.0f, 0.0f};
@@ -193,28 +207,37 @@ __device__ inline void column_by_keys(const AttnParams & p, const int32_t * tabl
         for (int j = st * KS; j < st * KS + KS && j <= lim; ++j) {
             const int page = page_of(table, p.seqs.table_stride, p.page_shift, p.n_pages, j);
             if (page < 0) continue;
-            const int64_t at = static_cast<int64_t>(j & ((1 << p.page_shift) - 1)) * kHeadDim + 2 * lane;
-            const CT * k = rows.page(page) + at;
+            if constexpr (TREE) {
+                if (!(mask_window(p, mask_row(p, row), j - past) & 1u)) continue;
+            }
+            const int slot = j & ((1 << p.page_shift) - 1);
+            const CT * k = rows.page(page) + slot * kHeadDim + 2 * lane;
             const CT * v = k + rows.v_elems;
-            const float s = wave_sum_all(fmaf(qv[0], static_cast<float>(k[0]), qv[1] * static_cast<float>(k[1]))) * c;
+            float ks = 1.0f, vs = 1.0f;
+            if constexpr (is_q8<CT>) {
+                ks = rows.scale(page)[slot];
+                vs = rows.scale(page)[rows.v_elems / 4 + slot];
+            }
+            const float s = wave_sum_all(fmaf(qv[0], static_cast<float>(k[0]) * ks, qv[1] * (static_cast<float>(k[1]) * ks))) * c;
             const float mn = fmaxf(m, s);
             const float ref = mn == -INFINITY ? 0.0f : mn;
             const float f = __builtin_amdgcn_exp2f(m - ref), e = __builtin_amdgcn_exp2f(s - ref);
             l = l * f + e;
-            o[0] = o[0] * f + e * static_cast<float>(v[0]);
-            o[1] = o[1] * f + e * static_cast<float>(v[1]);
+            o[0] = o[0] * f + e * (static_cast<float>(v[0]) * vs);
+            o[1] = o[1] * f + e * (static_cast<float>(v[1]) * vs);
             m = mn;
         }
     }
 }
 
-// A column's q in MFMA order: f16 pages dims 32 ks + 8 (l / 16) .. at [2 ks], f32 pages dims 16 i + 4 (l / 16) .. at [i].
-// Columns that do not exist are zeros.
-template <bool F16>
+// A column's q in MFMA order: f16 pages dims 32 ks + 8 (l / 16) .. at [2 ks], pages of 8 bits dims 64 (ks / 2) + 16 (l / 16) +
+// 8 (ks % 2) .. there, f32 pages dims 16 i + 4 (l / 16) .. at [i].  Columns that do not exist are zeros.
+template <typename CT>
 __device__ inline void load_q(const Column & col, int g4, f4 (&x)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        x[i] = *reinterpret_cast<const f4 *>(col.q + (F16 ? (i >> 1) * 32 + g4 * 8 + (i & 1) * 4 : i * 16 + g4 * 4));
+        x[i] = *reinterpret_cast<const f4 *>(col.q + (is_q8<CT> ? (i >> 2) * 64 + g4 * 16 + (i & 3) * 4
+                                                      : f16_products<CT> ? (i >> 1) * 32 + g4 * 8 + (i & 1) * 4 : i * 16 + g4 * 4));
         if (col.row < 0) x[i] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 }
@@ -265,16 +288,21 @@ __device__ inline void scores_step(const u4 (&a)[8], const h8 (&qh)[NB][4], cons
     }
 }
 
-// -inf where a key lies behind the column's last position or on no page (bit kb of holes: the 16-key block kb).
-template <int NB, int KB>
-__device__ inline void mask_step(f4 (&S)[NB][KB], const int (&lim)[NB], int key0, int g4, int holes) {
+// -inf where a key lies behind the column's last position, on no page (bit kb of holes: the 16-key block kb) or outside its mask.
+template <int NB, int KB, bool TREE>
+__device__ inline void mask_step(const AttnParams & p, f4 (&S)[NB][KB], const int (&lim)[NB], const int (&orow)[NB], int past, int key0,
+                                 int g4, int holes) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
+        uint32_t seen = ~0u;
+        if constexpr (TREE) seen = mask_window(p, mask_row(p, max(orow[nb], 0)), key0 - past);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (key0 + kb * 16 + g4 * 4 + i > lim[nb] || ((holes >> kb) & 1)) S[nb][kb][i] = -INFINITY;
+                bool out = key0 + kb * 16 + g4 * 4 + i > lim[nb] || ((holes >> kb) & 1);
+                if constexpr (TREE) out = out || !((seen >> (kb * 16 + g4 * 4 + i)) & 1u);
+                if (out) S[nb][kb][i] = -INFINITY;
             }
         }
     }
@@ -288,6 +316,83 @@ __device__ inline u4 transposed(const u4 (&v)[8], int db) {
         a[w] = db & 1 ? hi_pair(v[2 * w][db >> 1], v[2 * w + 1][db >> 1]) : lo_pair(v[2 * w][db >> 1], v[2 * w + 1][db >> 1]);
     }
     return a;
+}
+
+// 8 bits as f16.  Bytes are taken with their sign bit turned over (u = x + 128) next to 0x64: 1024 + u in f16, less 1152.
+constexpr uint32_t kSignBits = 0x80808080u;
+__device__ inline uint32_t f16_pair(uint32_t bytes, uint32_t select) {
+    const h2 v = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, bytes, select));
+    return __builtin_bit_cast(uint32_t, v - h2{1152, 1152});
+}
+
+// K operands 4 kb .. 4 kb + 3 of a step from the lane's 2 x 16 bytes of 16-key block kb.
+__device__ inline void k_operands(const u4 (&raw)[4], u4 (&a)[8]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t u = raw[r][w] ^ kSignBits;
+            a[2 * r + (w >> 1)][2 * (w & 1)] = f16_pair(u, 0x04010400u);
+            a[2 * r + (w >> 1)][2 * (w & 1) + 1] = f16_pair(u, 0x04030402u);
+        }
+    }
+}
+
+// V^T operands of a step's rows of 8 bits, 8 dims per lane and key: two keys' bytes side by side first.
+__device__ inline void v_operands(const u2 (&raw)[8], u4 (&a)[8]) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t x = raw[2 * w][h] ^ kSignBits, y = raw[2 * w + 1][h] ^ kSignBits;
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+                const uint32_t pairs = __builtin_amdgcn_perm(y, x, d ? 0x07030602u : 0x05010400u);
+                a[4 * h + 2 * d][w] = f16_pair(pairs, 0x04010400u);
+                a[4 * h + 2 * d + 1][w] = f16_pair(pairs, 0x04030402u);
+            }
+        }
+    }
+}
+
+// The keys' V scales go into the probabilities, which are split into f16 parts behind that: against the largest scale that the
+// wave has met, a power of two (top) that the accumulators follow.  pr <- pr * scale / 2^top.
+constexpr int kNoTop = -1000;
+template <int NB>
+__device__ inline void weigh_step(const f4 (&vs)[2], int & top, float (&pr)[NB][2][4], f4 (&O)[NB][8]) {
+    float most = 0.0f;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = fmaxf(most, vs[kb][i]);     // a NaN is passed over
+    }
+    most = column_max(most);
+    const int ex = most > 0.0f ? __builtin_amdgcn_frexp_expf(most) : kNoTop;
+    if (__any(ex > top)) {                                             // all lanes have the same
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) O[nb][db][i] = ldexpf(O[nb][db][i], top - ex);
+            }
+        }
+        top = ex;
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float w = ldexpf(vs[kb][i], -top);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                pr[nb][kb][i] *= w;
+                // the product as it is rounded here: one that a conversion to f16 takes in unrounded (v_fma_mix) is now and then
+                // another f16 than the one whose rest is the second part
+                asm("" : "+v"(pr[nb][kb][i]));
+            }
+        }
+    }
 }
 
 // Element offset of operand f of a step inside its 16-key block, and that block.  K: key l % 16, dims as q's.  V on f16 pages:
@@ -379,9 +484,10 @@ __device__ inline void split_p(const float (&pr)[2][4], h8 & hi, h8 & lo) {
 }
 
 // 4 values of a column from dim on: the output, or the part of this split (lead: this lane also stores the part's weights).
+template <bool TREE>
 __device__ inline void store_column(const AttnParams & p, const Tile & t, int row, int lim, int dim, f4 v, float mc, float l, bool lead) {
     if (t.n_splits == 1) {
-        *reinterpret_cast<f4 *>(p.out + static_cast<int64_t>(row) * kHeadDim + dim) = v * inverse_sum(p, t.table, lim, l);
+        *reinterpret_cast<f4 *>(p.out + static_cast<int64_t>(row) * kHeadDim + dim) = v * inverse_sum<TREE>(p, t.table, lim, t.past, row, l);
     } else {
         const int64_t at = static_cast<int64_t>(row) * p.n_parts + t.split;
         *reinterpret_cast<f4 *>(p.part_o + at * kHeadDim + dim) = v;
@@ -414,16 +520,16 @@ __device__ inline void close_columns(const int (&orow)[NB], const float (&c)[NB]
 }
 
 // The flagged columns of a block, key by key; their values are stored at once.
-template <typename CT, int KS>
+template <typename CT, int KS, bool TREE>
 __device__ inline void redo_columns(const AttnParams & p, const Tile & t, int head, int lane, int lim, int orow, uint32_t redo) {
     for (uint32_t left = redo; left != 0; left &= left - 1) {
         const int col = __ffs(left) - 1;
         const int row = __builtin_amdgcn_readlane(orow, col), lm = __builtin_amdgcn_readlane(lim, col);
         float cm, cl;
         f2 co;
-        column_by_keys<CT, KS>(p, t.table, head, p.q + static_cast<int64_t>(row) * kHeadDim, lm, t.step_lo, t.step_hi, 1, lane, cm, cl, co);
+        column_by_keys<CT, KS, TREE>(p, t.table, head, row, lm, t.past, t.step_lo, t.step_hi, 1, lane, cm, cl, co);
         const f2 nx = f2{__shfl_down(co[0], 1, kWave), __shfl_down(co[1], 1, kWave)};
-        if ((lane & 1) == 0) store_column(p, t, row, lm, 2 * lane, f4{co[0], co[1], nx[0], nx[1]}, cm, cl, lane == 0);
+        if ((lane & 1) == 0) store_column<TREE>(p, t, row, lm, 2 * lane, f4{co[0], co[1], nx[0], nx[1]}, cm, cl, lane == 0);
     }
 }
 
@@ -439,50 +545,69 @@ constexpr size_t rows_lds(bool f16, bool few) { return kWaves * rows_cols(f16, f
 // forked ones share is read once by each of them, and finds less of it in the caches: 32 beams behind 3913 shared positions 46.8
 // us, cached 42.6, behind 1000 19.2 / 18.5, eight behind 3913 22.3 / 21.1.  Nothing tells the two apart before the tables are read.  A row of f32 pages is taken by halves of its lines, and
 // longer chunks read it again: 129 instead of 111 us, and 50 instead of 40 at eight of 64 tokens.
-template <bool ONCE>
-__device__ inline u4 load_row(const void * at) {
-    if constexpr (ONCE) return __builtin_nontemporal_load(static_cast<const u4 *>(at));
-    else return *static_cast<const u4 *>(at);
+template <bool ONCE, typename VT>
+__device__ inline VT load_row(const void * at) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(static_cast<const VT *>(at));
+    else return *static_cast<const VT *>(at);
 }
 
-template <typename CT, bool FEW>
+template <typename CT, bool FEW, bool TREE>
 __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
-    constexpr bool F16 = std::is_same<CT, _Float16>::value, PACK = FEW && F16;
+    constexpr bool F16 = f16_products<CT>, Q8 = is_q8<CT>, PACK = FEW && F16;
     constexpr int KS = step_keys(F16), KB = KS / 16, R = rows_cols(F16, FEW), NB = 1;
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g4 = lane >> 4;
     Tile t;
     int head;
-    if (!find_tile<R, KS, FEW>(p, block, lane, t, head)) return;          // uniform for the workgroup
-    const Column col = column_of(p, t, head, t.col0 + (PACK ? c16 & 7 : c16));
+    if (!find_tile<R, KS, FEW, TREE>(p, block, lane, t, head)) return;    // uniform for the workgroup
+    const Column col = column_of<TREE>(p, t, head, t.col0 + (PACK ? c16 & 7 : c16));
     f4 x[NB][8];
-    load_q<F16>(col, g4, x[0]);
+    load_q<CT>(col, g4, x[0]);
 
-    const HeadRows<CT> rows(p, head);
+    const HeadRows<CT> rows(p.pages, p.layer, p.n_kv, p.n_pages, p.page_shift, head);
     const int in_page = (1 << p.page_shift) - 1, last_entry = p.seqs.table_stride - 1;
     auto entries_of = [&](int st, int (&out)[KB]) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) out[kb] = t.table[min((st * KS + kb * 16) >> p.page_shift, last_entry)];
     };
-    u4 rk[8], rv[8];
+    // a lane's rows of a step; 8 bits: 2 x 16 bytes of K per 16-key block, 8 of V per key, and the scales of its 4 keys per block
+    u4 rk[Q8 ? 4 : 8], rv[Q8 ? 1 : 8];
+    u2 rv8[8];
+    f4 ks[KB], vs[KB];
     int pg[KB], pg_next[KB], entry[KB];
     const CT * at[KB];
+    const float * scales[KB];
     // a block on no page reads page 0, which there always is, and is masked
     auto place = [&](int st) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             pg_next[kb] = entry_page(p, t, entry[kb], st * KS + kb * 16);
             at[kb] = rows.page(max(pg_next[kb], 0)) + ((st * KS + kb * 16) & in_page) * kHeadDim;
+            if constexpr (Q8) scales[kb] = rows.scale(max(pg_next[kb], 0)) + ((st * KS + kb * 16) & in_page) + g4 * 4;
         }
     };
     auto load_k = [&]() {
+        if constexpr (Q8) {
 #pragma unroll
-        for (int f = 0; f < 8; ++f) rk[f] = load_row<PACK>(at[F16 ? f >> 2 : 0] + k_offset<F16>(f, c16, g4));
+            for (int f = 0; f < 4; ++f) rk[f] = load_row<PACK, u4>(at[f >> 1] + c16 * kHeadDim + (f & 1) * 64 + g4 * 16);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) ks[kb] = *reinterpret_cast<const f4 *>(scales[kb]);
+        } else {
+#pragma unroll
+            for (int f = 0; f < 8; ++f) rk[f] = load_row<PACK, u4>(at[F16 ? f >> 2 : 0] + k_offset<F16>(f, c16, g4));
+        }
     };
     auto load_v = [&]() {
+        if constexpr (Q8) {
 #pragma unroll
-        for (int f = 0; f < 8; ++f) rv[f] = load_row<PACK>(at[F16 ? f >> 2 : 0] + rows.v_elems + v_offset<F16>(f, c16, g4));
+            for (int f = 0; f < 8; ++f) rv8[f] = load_row<PACK, u2>(at[f >> 2] + rows.v_elems + v_offset<true>(f, c16, g4));
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) vs[kb] = *reinterpret_cast<const f4 *>(scales[kb] + rows.v_elems / 4);
+        } else {
+#pragma unroll
+            for (int f = 0; f < 8; ++f) rv[f] = load_row<PACK, u4>(at[F16 ? f >> 2 : 0] + rows.v_elems + v_offset<F16>(f, c16, g4));
+        }
     };
     int st = t.step_lo + wave;
     if (st < t.step_hi) {
@@ -505,7 +630,9 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
         c[0] = p.scale * kLog2e;
     }
     const int lim[NB] = {col.lim}, orow[NB] = {col.row};
-    const int full = max(0, min(t.past + t.col0 / p.group, t.cap - 1) + 1) / KS;   // steps that every column sees whole
+    // steps that every column sees whole
+    const int full = TREE ? max(0, min(t.past, t.cap)) / KS : max(0, min(t.past + t.col0 / p.group, t.cap - 1) + 1) / KS;
+    int top = kNoTop;
     float m[NB] = {-INFINITY}, l[NB] = {0.0f};
     f4 O[NB][8];
 #pragma unroll
@@ -519,8 +646,16 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
             holes |= pg[kb] < 0 ? 1 << kb : 0;
         }
         const bool more = st + kWaves < t.step_hi;
-        f4 S[NB][KB];
-        scores_step<F16, PACK, NB>(rk, qh, ql, x, S);
+        f4 S[NB][KB], key_scale[KB];
+        if constexpr (Q8) {
+            u4 a[8];
+            k_operands(rk, a);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) key_scale[kb] = ks[kb];
+            scores_step<F16, PACK, NB>(a, qh, ql, x, S);
+        } else {
+            scores_step<F16, PACK, NB>(rk, qh, ql, x, S);
+        }
         if (more) {
             place(st + kWaves);
             load_k();
@@ -532,7 +667,11 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
                 for (int i = 0; i < 4; ++i) S[0][kb][i] += row_ror8(S[0][kb][i]);
             }
         }
-        if (st >= full || holes != 0) mask_step<NB, KB>(S, lim, st * KS, g4, holes);
+        if constexpr (Q8) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) S[0][kb] *= key_scale[kb];
+        }
+        if (st >= full || holes != 0) mask_step<NB, KB, TREE>(p, S, lim, orow, t.past, st * KS, g4, holes);
         float pr[NB][KB][4];
         softmax_step<NB, KB>(S, c, m, l, O, pr);
 
@@ -540,16 +679,27 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
         if (st * KS + KS > t.kend || holes != 0) {
 #pragma unroll
             for (int f = 0; f < 8; ++f) {
-                if (st * KS + v_key<F16>(f, g4) >= t.kend || pg[F16 ? f >> 2 : 0] < 0) rv[f] = u4{0, 0, 0, 0};
+                if (st * KS + v_key<F16>(f, g4) >= t.kend || pg[F16 ? f >> 2 : 0] < 0) {
+                    if constexpr (Q8) vs[f >> 2][f & 3] = 0.0f;
+                    else rv[f] = u4{0, 0, 0, 0};
+                }
             }
         }
         if constexpr (F16) {
+            u4 vt[8];
+            if constexpr (Q8) {
+                weigh_step<NB>(vs, top, pr, O);
+                v_operands(rv8, vt);
+            } else {
+#pragma unroll
+                for (int db = 0; db < 8; ++db) vt[db] = transposed(rv, db);
+            }
             h8 ph, pl;
             split_p(pr[0], ph, pl);
             if constexpr (PACK) ph = c16 < 8 ? ph : pl;
 #pragma unroll
             for (int db = 0; db < 8; ++db) {
-                const h8 a = __builtin_bit_cast(h8, transposed(rv, db));
+                const h8 a = __builtin_bit_cast(h8, vt[db]);
                 O[0][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, O[0][db], 0, 0, 0);
                 if constexpr (!PACK) O[0][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, O[0][db], 0, 0, 0);
             }
@@ -571,6 +721,13 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
 
     float mc[NB];
     uint32_t redo[NB];
+    if constexpr (Q8) {
+#pragma unroll
+        for (int db = 0; db < 8; ++db) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) O[0][db][i] = ldexpf(O[0][db][i], top);
+        }
+    }
     close_columns<NB, PACK>(orow, c, m, l, O, mc, redo);
     // merge over the waves
     float * so = reinterpret_cast<float *>(lds);
@@ -602,7 +759,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
         const int row = __builtin_amdgcn_readlane(col.row, cc), lm = __builtin_amdgcn_readlane(col.lim, cc);
         float cm, cl;
         f2 co;
-        column_by_keys<CT, KS>(p, t.table, head, p.q + static_cast<int64_t>(row) * kHeadDim, lm, t.step_lo + wave, t.step_hi, kWaves, lane, cm, cl, co);
+        column_by_keys<CT, KS, TREE>(p, t.table, head, row, lm, t.past, t.step_lo + wave, t.step_hi, kWaves, lane, cm, cl, co);
         // after this wave's own stores above: one wave's LDS accesses stay in order
         __builtin_amdgcn_wave_barrier();
         *reinterpret_cast<f2 *>(so + (base + cc) * kRowsStride + 2 * lane) = co;
@@ -629,7 +786,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
             ls += sl[w * R + cc] * f;
             o += *reinterpret_cast<const f4 *>(so + (w * R + cc) * kRowsStride + dim) * f;
         }
-        store_column(p, t, row, slim[cc], dim, o, M, ls, dim == 0);
+        store_column<TREE>(p, t, row, slim[cc], dim, o, M, ls, dim == 0);
     }
 }
 
@@ -649,42 +806,45 @@ constexpr size_t kTileLds = 2 * kTileSteps * kStepBytes;
 constexpr int kOutStride = kHeadDim + 4, kOutFloats = 16 * kOutStride;   // a wave's 16 columns on their way out
 static_assert(kWaves * kOutFloats * sizeof(float) <= kTileLds, "the outputs go through the operands' LDS");
 
+template <typename CT, bool TREE>
 __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
-    typedef _Float16 CT;
-    constexpr bool F16 = true;
+    constexpr bool F16 = true, Q8 = is_q8<CT>;
     constexpr int KS = step_keys(F16), KB = KS / 16, NB = 2;
+    __shared__ __attribute__((aligned(16))) float s_scale[Q8 ? 2 : 1][Q8 ? kTileSteps : 1][2][KS];   // of K and V
     __shared__ int s_holes[2][kTileSteps];                            // bit kb: 16-key block kb of the step lies on no page
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g4 = lane >> 4;
     Tile t;
     int head;
-    if (!find_tile<kTileCols, KS, false>(p, block, lane, t, head)) return;   // uniform for the workgroup
+    if (!find_tile<kTileCols, KS, false, TREE>(p, block, lane, t, head)) return;   // uniform for the workgroup
 
     // columns: their q is on its way while the first tile is fetched
     int lim[NB], orow[NB];
     f4 x[NB][8];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-        const Column col = column_of(p, t, head, t.col0 + wave * 16 * NB + nb * 16 + c16);
+        const Column col = column_of<TREE>(p, t, head, t.col0 + wave * 16 * NB + nb * 16 + c16);
         lim[nb] = col.lim;
         orow[nb] = col.row;
-        load_q<F16>(col, g4, x[nb]);
+        load_q<CT>(col, g4, x[nb]);
     }
     // keys that the wave's last and first token see (its columns are in order of token)
     const int first_col = t.col0 + wave * 16 * NB;
     int wave_steps = 0, full = 0;                                     // steps behind the first hold nothing that the wave sees
     if (first_col < t.n_cols) {
-        wave_steps = min(t.step_hi, (min(t.past + (min(first_col + 16 * NB, t.n_cols) - 1) / p.group, t.cap - 1) + KS) / KS);
-        full = max(0, min(t.past + first_col / p.group, t.cap - 1) + 1) / KS;
+        wave_steps = TREE ? t.step_hi : min(t.step_hi, (min(t.past + (min(first_col + 16 * NB, t.n_cols) - 1) / p.group, t.cap - 1) + KS) / KS);
+        full = TREE ? max(0, min(t.past, t.cap)) / KS : max(0, min(t.past + first_col / p.group, t.cap - 1) + 1) / KS;
     }
 
     // this wave's share of a tile: K or V of step `mine`
     const bool fetch_v = wave < kTileSteps;
     const int mine = wave & (kTileSteps - 1);
-    const HeadRows<CT> rows(p, head);
+    const HeadRows<CT> rows(p.pages, p.layer, p.n_kv, p.n_pages, p.page_shift, head);
     const int in_page = (1 << p.page_shift) - 1, last_entry = p.seqs.table_stride - 1;
     u4 r[8];
+    u2 r8[8];
+    float r_scale = 0.0f;                                             // lane < KS: its key's
     int pg[KB], entry[KB], st_held = 0;
     auto entries_of = [&](int st) {
 #pragma unroll
@@ -698,14 +858,41 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
             pg[kb] = entry_page(p, t, entry[kb], st * KS + kb * 16);
             at[kb] = rows.page(max(pg[kb], 0)) + ((st * KS + kb * 16) & in_page) * kHeadDim + (fetch_v ? rows.v_elems : 0);
         }
+        if constexpr (Q8) {
+            const int kb = (lane >> 4) & 1;
+            const float * scales = rows.scale(max(pg[kb], 0)) + ((st * KS + kb * 16) & in_page) + (fetch_v ? rows.v_elems / 4 : 0);
+            r_scale = scales[c16];
+            if (fetch_v) {
 #pragma unroll
-        for (int f = 0; f < 8; ++f) {
-            r[f] = *reinterpret_cast<const u4 *>(at[f >> 2] + (fetch_v ? v_offset<F16>(f, c16, g4) : k_offset<F16>(f, c16, g4)));
+                for (int f = 0; f < 8; ++f) r8[f] = *reinterpret_cast<const u2 *>(at[f >> 2] + v_offset<F16>(f, c16, g4));
+            } else {
+#pragma unroll
+                for (int f = 0; f < 4; ++f) r[f] = *reinterpret_cast<const u4 *>(at[f >> 1] + c16 * kHeadDim + (f & 1) * 64 + g4 * 16);
+            }
+        } else {
+#pragma unroll
+            for (int f = 0; f < 8; ++f) {
+                r[f] = *reinterpret_cast<const u4 *>(at[f >> 2] + (fetch_v ? v_offset<F16>(f, c16, g4) : k_offset<F16>(f, c16, g4)));
+            }
         }
     };
     auto put = [&](int buf) {
         char * to = lds + (buf * kTileSteps + mine) * kStepBytes + lane * 16;
-        if (fetch_v) {
+        if constexpr (Q8) {
+            u4 a[8];
+            if (fetch_v) {
+                v_operands(r8, a);
+                // rows that no column sees, and of no page: not even 0 times what memory holds
+                if (st_held * KS + lane >= t.kend || pg[(lane >> 4) & 1] < 0) r_scale = 0.0f;
+            } else {
+                const u4 raw[4] = {r[0], r[1], r[2], r[3]};
+                k_operands(raw, a);
+                if (lane == 0) s_holes[buf][mine] = (pg[0] < 0 ? 1 : 0) | (pg[1] < 0 ? 2 : 0);
+            }
+            if (lane < KS) s_scale[buf][mine][fetch_v ? 1 : 0][lane] = r_scale;
+#pragma unroll
+            for (int f = 0; f < 8; ++f) *reinterpret_cast<u4 *>(to + (fetch_v ? 8 + f : f) * kWave * 16) = a[f];
+        } else if (fetch_v) {
             bool hole = st_held * KS + KS > t.kend;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) hole = hole || pg[kb] < 0;
@@ -736,6 +923,7 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
     for (int nb = 0; nb < NB; ++nb) {
         split_q(x[nb], p.scale, c[nb], qh[nb], ql[nb]);
     }
+    int top = kNoTop;
     float m[NB], l[NB];
     f4 O[NB][8];
 #pragma unroll
@@ -767,9 +955,23 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
 #pragma unroll
             for (int f = 0; f < 8; ++f) v[f] = *reinterpret_cast<const u4 *>(op + (8 + f) * kWave * 16);
             const int holes = __builtin_amdgcn_readfirstlane(s_holes[tile & 1][s]);
-            if (st >= full || holes != 0) mask_step<NB, KB>(S, lim, st * KS, g4, holes);
+            if constexpr (Q8) {
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+                    const f4 ks = *reinterpret_cast<const f4 *>(&s_scale[tile & 1][s][0][kb * 16 + g4 * 4]);
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) S[nb][kb] *= ks;
+                }
+            }
+            if (st >= full || holes != 0) mask_step<NB, KB, TREE>(p, S, lim, orow, t.past, st * KS, g4, holes);
             float pr[NB][KB][4];
             softmax_step<NB, KB>(S, c, m, l, O, pr);
+            if constexpr (Q8) {
+                f4 vs[KB];
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) vs[kb] = *reinterpret_cast<const f4 *>(&s_scale[tile & 1][s][1][kb * 16 + g4 * 4]);
+                weigh_step<NB>(vs, top, pr, O);
+            }
             h8 ph[NB], pl[NB];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) split_p(pr[nb], ph[nb], pl[nb]);
@@ -795,6 +997,16 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
     }
     float mc[NB];
     uint32_t redo[NB];
+    if constexpr (Q8) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) O[nb][db][i] = ldexpf(O[nb][db][i], top);
+            }
+        }
+    }
     close_columns<NB, false>(orow, c, m, l, O, mc, redo);
     // through the wave's own part of LDS, so that a store instruction writes two whole rows; a lane's values would lie 16 bytes
     // in each of 64 lines
@@ -816,38 +1028,39 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
             const int row = __shfl(orow[nb], col, kWave), lm = __shfl(lim[nb], col, kWave);
             const float cm = __shfl(mc[nb], col, kWave), cl = __shfl(l[nb], col, kWave);
             const f4 v = *reinterpret_cast<const f4 *>(so + col * kOutStride + dim);
-            if (row >= 0 && !((redo[nb] >> col) & 1)) store_column(p, t, row, lm, dim, v, cm, cl, dim == 0);
+            if (row >= 0 && !((redo[nb] >> col) & 1)) store_column<TREE>(p, t, row, lm, dim, v, cm, cl, dim == 0);
         }
-        redo_columns<CT, KS>(p, t, head, lane, lim[nb], orow[nb], redo[nb]);
+        redo_columns<CT, KS, TREE>(p, t, head, lane, lim[nb], orow[nb], redo[nb]);
     }
 }
 
 // The launches.  One kind of tile, or longer chunks first and the sequences of few columns behind them.
-template <typename CT, bool FEW>
+template <typename CT, bool FEW, bool TREE>
 __global__ __launch_bounds__(kThreads, 3) void paged_rows_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_rows[];
-    attn_rows<CT, FEW>(p, blockIdx.x, lds_rows);
+    attn_rows<CT, FEW, TREE>(p, blockIdx.x, lds_rows);
 }
 
-template <typename CT>
+template <typename CT, bool TREE>
 __global__ __launch_bounds__(kThreads, 3) void paged_rows_both_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_rows[];
     const int many = p.tiles_many * p.n_kv * p.splits_many, block = blockIdx.x;
-    if (block < many) attn_rows<CT, false>(p, block, lds_rows);
-    else attn_rows<CT, true>(p, block - many, lds_rows);
+    if (block < many) attn_rows<CT, false, TREE>(p, block, lds_rows);
+    else attn_rows<CT, true, TREE>(p, block - many, lds_rows);
 }
 
-template <bool BOTH>
+template <typename CT, bool BOTH, bool TREE>
 __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_tile[];
     const int many = p.tiles_many * p.n_kv * p.splits_many, block = blockIdx.x;
-    if (!BOTH || block < many) attn_tile(p, block, lds_tile);
-    else attn_rows<_Float16, true>(p, block - many, lds_tile);
+    if (!BOTH || block < many) attn_tile<CT, TREE>(p, block, lds_tile);
+    else attn_rows<CT, true, TREE>(p, block - many, lds_tile);
 }
 
 // Joins the splits of each (row, head): one wave each, lane = split for the weights, then lane = 2 dims.  Its time is
 // dependent loads, so the sequences, the weights and the first results are read together; a split that the row does not
 // reach holds whatever the workspace held, and is selected away.
+template <bool TREE>
 __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int ks) {
     constexpr int kFirst = 8;
     const int lane = threadIdx.x & (kWave - 1);
@@ -865,7 +1078,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int ks) {
     const int n_splits = few ? p.splits_few : p.splits_many, split_steps = few ? p.steps_few : p.steps_many;
     if (n_splits == 1) return;                                        // stored by its tile
     const int cap = p.seqs.table_stride << p.page_shift;
-    const int lim = min(at.pos, cap - 1);
+    const int lim = min(TREE ? at.past + at.rows - 1 : at.pos, cap - 1);
     // splits that hold a key which this row sees (the first is always computed)
     const int active = lim < 0 ? 1 : min(n_splits, lim / ks / split_steps + 1);
     if (lane >= active) ml = f2{-INFINITY, 0.0f};
@@ -886,7 +1099,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int ks) {
             if (s0 + s < active) o += part[s] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), s0 + s));
         }
     }
-    const float inv = inverse_sum(p, p.seqs.tables + static_cast<int64_t>(at.seq) * p.seqs.table_stride, lim, L);
+    const float inv = inverse_sum<TREE>(p, p.seqs.tables + static_cast<int64_t>(at.seq) * p.seqs.table_stride, lim, at.past, static_cast<int>(item), L);
     *reinterpret_cast<f2 *>(p.out + item * kHeadDim + 2 * lane) = o * inv;
 }
 
@@ -910,7 +1123,7 @@ void cut_keys(int steps, int64_t blocks, int64_t target, int64_t least, int64_t 
 }
 
 AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_heads, size_t workspace_bytes) {
-    const bool f16 = l.cache_type == QA_CACHE_F16;
+    const bool f16 = l.cache_type != QA_CACHE_F32;                    // products
     const int ks = step_keys(f16);
     const int group = n_heads / l.n_kv_heads;
     const int seqs = std::min(b.n_seqs, b.n_rows);
@@ -953,60 +1166,58 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     return pl;
 }
 
-template <typename CT>
+template <typename CT, bool TREE>
 int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
-    constexpr bool F16 = std::is_same<CT, _Float16>::value;
+    constexpr bool F16 = f16_products<CT>;
     const dim3 grid(static_cast<unsigned>(p.n_kv) * (pl.tiles_many * pl.splits_many + pl.tiles_few * pl.splits_few));
     constexpr size_t lds_few = rows_lds(F16, true), lds_many = rows_lds(F16, false);
     static_assert(lds_few <= kTileLds && lds_few <= lds_many, "a launch of both kinds has the longer ones' LDS");
     if (F16 && pl.tile) {
-        const auto kernel = pl.few_max ? &paged_tile_kernel<true> : &paged_tile_kernel<false>;
+        typedef typename std::conditional<F16, CT, _Float16>::type TT;   // f32 pages have no such kernel
+        const auto kernel = pl.few_max ? &paged_tile_kernel<TT, true, TREE> : &paged_tile_kernel<TT, false, TREE>;
         QA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kTileLds)));
         hipLaunchKernelGGL(kernel, grid, dim3(kThreads), kTileLds, stream, p);
     } else if (!pl.tiles_many) {
-        hipLaunchKernelGGL((paged_rows_kernel<CT, true>), grid, dim3(kThreads), lds_few, stream, p);
+        hipLaunchKernelGGL((paged_rows_kernel<CT, true, TREE>), grid, dim3(kThreads), lds_few, stream, p);
     } else if (pl.few_max) {
-        hipLaunchKernelGGL((paged_rows_both_kernel<CT>), grid, dim3(kThreads), lds_many, stream, p);
+        hipLaunchKernelGGL((paged_rows_both_kernel<CT, TREE>), grid, dim3(kThreads), lds_many, stream, p);
     } else {
-        hipLaunchKernelGGL((paged_rows_kernel<CT, false>), grid, dim3(kThreads), lds_many, stream, p);
+        hipLaunchKernelGGL((paged_rows_kernel<CT, false, TREE>), grid, dim3(kThreads), lds_many, stream, p);
     }
     QA_LAUNCH_CHECK("paged attention kernel");
     if (pl.parts() > 1) {
         const int64_t items = static_cast<int64_t>(p.seqs.n_rows) * p.n_heads;
-        hipLaunchKernelGGL(paged_join_kernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, p, step_keys(F16));
+        hipLaunchKernelGGL(paged_join_kernel<TREE>, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, p, step_keys(F16));
         QA_LAUNCH_CHECK("paged_join_kernel");
     }
     return QA_OK;
 }
 
-}  // namespace
-}  // namespace qa
-
-extern "C" size_t qa_paged_attn_workspace_bytes(const qa_kv_layout * layout, const qa_paged_batch * batch, int32_t n_heads) {
-    using namespace qa;
-    if (check_batch_sizes(layout, 0, batch, n_heads, "qa_paged_attn_workspace_bytes") != QA_OK || batch->n_rows == 0) return 0;
-    const AttnPlan pl = attn_plan(*layout, *batch, n_heads, SIZE_MAX);
-    if (pl.parts() <= 1) return 0;
-    return static_cast<size_t>(batch->n_rows) * n_heads * pl.parts() * (kHeadDim + 2) * sizeof(float);
+template <bool TREE>
+int launch_typed(const AttnPlan & pl, const AttnParams & p, int32_t cache_type, hipStream_t stream) {
+    if (cache_type == QA_CACHE_Q8) return launch_attn<int8_t, TREE>(pl, p, stream);
+    if (cache_type == QA_CACHE_F16) return launch_attn<_Float16, TREE>(pl, p, stream);
+    return launch_attn<float, TREE>(pl, p, stream);
 }
 
-extern "C" int qa_paged_attn(const float * q, const void * pages, const qa_kv_layout * layout, int32_t layer,
-                             const qa_paged_batch * batch, int32_t n_heads, float scale, float * out, void * workspace,
-                             size_t workspace_bytes, void * stream) {
-    using namespace qa;
-    if (check_batch(layout, layer, batch, n_heads, "qa_paged_attn") != QA_OK) return QA_ERR_INVALID;
-    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(QA_ERR_INVALID, "qa_paged_attn: scale must be positive and finite");
+// mask null: causal.
+int attention(const float * q, const void * pages, const qa_kv_layout * layout, int32_t layer, const qa_paged_batch * batch,
+              const uint32_t * mask, int32_t mask_words, int32_t n_heads, float scale, float * out, void * workspace,
+              size_t workspace_bytes, void * stream, const char * name) {
+    const std::string who = name;
+    if (check_batch(layout, layer, batch, n_heads, name) != QA_OK) return QA_ERR_INVALID;
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(QA_ERR_INVALID, who + ": scale must be positive and finite");
     if (batch->n_rows == 0) return QA_OK;
-    if (!q || !pages || !out || (!workspace && workspace_bytes > 0)) return fail(QA_ERR_INVALID, "qa_paged_attn: null pointer");
+    if (!q || !pages || !out || (!workspace && workspace_bytes > 0)) return fail(QA_ERR_INVALID, who + ": null pointer");
     if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(pages) | reinterpret_cast<uintptr_t>(out) |
           reinterpret_cast<uintptr_t>(workspace)) & 15) != 0) {
-        return fail(QA_ERR_INVALID, "qa_paged_attn: pointers must be aligned to 16 bytes");
+        return fail(QA_ERR_INVALID, who + ": pointers must be aligned to 16 bytes");
     }
-    if (static_cast<int64_t>(batch->n_rows) * n_heads > INT32_MAX / 2) return fail(QA_ERR_INVALID, "qa_paged_attn: too many rows");
-    if (const int rc = check_stream(stream, "qa_paged_attn"); rc != QA_OK) return rc;
+    if (static_cast<int64_t>(batch->n_rows) * n_heads > INT32_MAX / 2) return fail(QA_ERR_INVALID, who + ": too many rows");
+    if (const int rc = check_stream(stream, name); rc != QA_OK) return rc;
     const AttnPlan pl = attn_plan(*layout, *batch, n_heads, workspace_bytes);
     if ((static_cast<int64_t>(pl.tiles_many) * pl.splits_many + static_cast<int64_t>(pl.tiles_few) * pl.splits_few) * layout->n_kv_heads > INT32_MAX / kThreads) {
-        return fail(QA_ERR_INVALID, "qa_paged_attn: too many rows");
+        return fail(QA_ERR_INVALID, who + ": too many rows");
     }
     AttnParams p{};
     p.q = q;
@@ -1030,5 +1241,35 @@ extern "C" int qa_paged_attn(const float * q, const void * pages, const qa_kv_la
     p.steps_few = pl.steps_few;
     p.n_parts = pl.parts();
     p.scale = scale;
-    return layout->cache_type == QA_CACHE_F16 ? launch_attn<_Float16>(pl, p, as_stream(stream)) : launch_attn<float>(pl, p, as_stream(stream));
+    p.mask = mask;
+    p.mask_words = mask_words;
+    return mask ? launch_typed<true>(pl, p, layout->cache_type, as_stream(stream))
+                : launch_typed<false>(pl, p, layout->cache_type, as_stream(stream));
+}
+
+}  // namespace
+}  // namespace qa
+
+extern "C" size_t qa_paged_attn_workspace_bytes(const qa_kv_layout * layout, const qa_paged_batch * batch, int32_t n_heads) {
+    using namespace qa;
+    if (check_batch_sizes(layout, 0, batch, n_heads, "qa_paged_attn_workspace_bytes") != QA_OK || batch->n_rows == 0) return 0;
+    const AttnPlan pl = attn_plan(*layout, *batch, n_heads, SIZE_MAX);
+    if (pl.parts() <= 1) return 0;
+    return static_cast<size_t>(batch->n_rows) * n_heads * pl.parts() * (kHeadDim + 2) * sizeof(float);
+}
+
+extern "C" int qa_paged_attn(const float * q, const void * pages, const qa_kv_layout * layout, int32_t layer,
+                             const qa_paged_batch * batch, int32_t n_heads, float scale, float * out, void * workspace,
+                             size_t workspace_bytes, void * stream) {
+    return qa::attention(q, pages, layout, layer, batch, nullptr, 0, n_heads, scale, out, workspace, workspace_bytes, stream, "qa_paged_attn");
+}
+
+extern "C" int qa_paged_tree_attn(const float * q, const void * pages, const qa_kv_layout * layout, int32_t layer,
+                                  const qa_paged_batch * batch, const uint32_t * mask, int32_t mask_words, int32_t n_heads, float scale,
+                                  float * out, void * workspace, size_t workspace_bytes, void * stream) {
+    using namespace qa;
+    const char * who = "qa_paged_tree_attn";
+    if (check_batch(layout, layer, batch, n_heads, who) != QA_OK || check_tree(batch, mask_words, who) != QA_OK) return QA_ERR_INVALID;
+    if (batch->n_rows > 0 && !mask) return fail(QA_ERR_INVALID, "qa_paged_tree_attn: null pointer");
+    return attention(q, pages, layout, layer, batch, mask, mask_words, n_heads, scale, out, workspace, workspace_bytes, stream, who);
 }

@@ -20,6 +20,7 @@ struct RowPlace {
     int seq;    // -1: the row belongs to no sequence
     int pos;
     int rows;   // the sequence's
+    int past;
 };
 
 // The sequence whose rows hold `row`: row_start does not fall, so it is the number of sequences that end at or before
@@ -33,10 +34,27 @@ __device__ inline RowPlace row_place(const PagedSeqs & b, int row, int lane) {
         if (l == kWave) continue;
         const int first = __builtin_amdgcn_readlane(start, l);
         if (s0 + l >= b.n_seqs || first < 0 || first > row) break;
-        return RowPlace{s0 + l, bounded_past(__builtin_amdgcn_readlane(past, l)) + row - first,
-                        rows_between(first, __builtin_amdgcn_readlane(end, l), b.n_rows)};
+        const int behind = bounded_past(__builtin_amdgcn_readlane(past, l));
+        return RowPlace{s0 + l, behind + row - first, rows_between(first, __builtin_amdgcn_readlane(end, l), b.n_rows), behind};
     }
-    return RowPlace{-1, 0, 0};
+    return RowPlace{-1, 0, 0, 0};
 }
+
+// The rows of one KV head in a paged cache: values of page p from page(p) on, V v_elems behind K, both in elements of CT.  8 bits:
+// a page's block ends in its rows' scales, scale(p) is the head's first.
+template <typename CT>
+struct HeadRows {
+    const CT * k;
+    int64_t page_elems, v_elems, scales;
+    __device__ inline HeadRows(const void * pages, int layer, int n_kv, int n_pages, int page_shift, int head) {
+        const int64_t rows = static_cast<int64_t>(1) << page_shift;
+        page_elems = n_kv * rows * (sizeof(CT) == 1 ? kQ8RowBytes : kHeadDim);
+        v_elems = n_pages * page_elems;
+        k = static_cast<const CT *>(pages) + 2 * layer * v_elems + head * rows * kHeadDim;
+        scales = n_kv * rows * kHeadDim - head * rows * (kHeadDim - 4);   // from the head's values to its scales, in bytes
+    }
+    __device__ inline const CT * page(int page) const { return k + page * page_elems; }
+    __device__ inline const float * scale(int page) const { return reinterpret_cast<const float *>(k + page * page_elems + scales); }
+};
 
 }  // namespace qa

@@ -430,10 +430,6 @@ __global__ __launch_bounds__(256) void pages_renumber_kernel(const int32_t * ref
     }
 }
 
-int64_t block_bytes(const qa_kv_layout & l) {
-    return static_cast<int64_t>(l.n_kv_heads) * l.max_seq * l.head_dim * static_cast<int64_t>(qa_kv_elem_bytes(l.cache_type));
-}
-
 int launch_copies(void * pages, const qa_kv_layout & l, const int32_t * src, const int32_t * dst, const int32_t * count, int32_t n,
                   int32_t most, bool once, bool check, hipStream_t stream) {
     CopyParams p{};

@@ -532,7 +532,7 @@ extern "C" int qa_prefill_attn(const float * q, const void * cache, const qa_kv_
                                int32_t stream_idx, int32_t n_past, int32_t n_tokens, int32_t n_heads, float scale,
                                float * out, void * workspace, size_t workspace_bytes, void * stream) {
     using namespace qa;
-    if (qa_kv_layout_check(layout) != QA_OK) return QA_ERR_INVALID;
+    if (check_flat_layout(layout) != QA_OK) return QA_ERR_INVALID;
     if (!q || !cache || !out) return fail(QA_ERR_INVALID, "qa_prefill_attn: null pointer");
     return prefill_attn_launch(q, n_heads * kHeadDim, cache, *layout, layer, stream_idx, n_past, n_tokens, n_heads,
                                scale, out, nullptr, nullptr, workspace, workspace_bytes, as_stream(stream));

@@ -139,23 +139,25 @@ extern "C" int qa_stream_synchronize(void * stream) {
 extern "C" int qa_kv_layout_check(const qa_kv_layout * l) {
     if (!l) return fail(QA_ERR_INVALID, "null KV layout");
     if (l->n_layers <= 0 || l->n_streams <= 0 || l->n_kv_heads <= 0 || l->head_dim <= 0 || l->max_seq <= 0 ||
-        (l->cache_type != QA_CACHE_F32 && l->cache_type != QA_CACHE_F16)) {
+        (l->cache_type != QA_CACHE_F32 && l->cache_type != QA_CACHE_F16 && l->cache_type != QA_CACHE_Q8)) {
         return fail(QA_ERR_INVALID, "invalid text decoder KV-cache configuration");
+    }
+    if (l->cache_type == QA_CACHE_Q8 && !is_q8_layout(*l)) {
+        return fail(QA_ERR_INVALID, "a cache of 8 bits has head_dim 128 and pages of 16, 32, 64, 128 or 256 positions");
     }
     return QA_OK;
 }
 
 extern "C" size_t qa_kv_elem_bytes(int32_t cache_type) {
-    return cache_type == QA_CACHE_F16 ? 2 : 4;
+    return cache_type == QA_CACHE_Q8 ? 1 : cache_type == QA_CACHE_F16 ? 2 : 4;
 }
 
 extern "C" size_t qa_kv_cache_bytes(const qa_kv_layout * l) {
     if (!l || l->n_layers <= 0 || l->n_streams <= 0 || l->n_kv_heads <= 0 || l->head_dim <= 0 || l->max_seq <= 0 ||
-        (l->cache_type != QA_CACHE_F32 && l->cache_type != QA_CACHE_F16)) {
+        (l->cache_type != QA_CACHE_F32 && l->cache_type != QA_CACHE_F16 && !(l->cache_type == QA_CACHE_Q8 && is_q8_layout(*l)))) {
         return 0;
     }
-    return static_cast<size_t>(l->n_layers) * 2 * l->n_streams * l->n_kv_heads * l->max_seq * l->head_dim *
-           qa_kv_elem_bytes(l->cache_type);
+    return static_cast<size_t>(l->n_layers) * 2 * l->n_streams * static_cast<size_t>(block_bytes(*l));
 }
 
 extern "C" int64_t qa_kv_slot_index(const qa_kv_layout * l, int32_t layer, int32_t kv, int32_t stream, int32_t head,
@@ -165,8 +167,9 @@ extern "C" int64_t qa_kv_slot_index(const qa_kv_layout * l, int32_t layer, int32
         head >= l->n_kv_heads || pos < 0 || pos >= l->max_seq || dim < 0 || dim >= l->head_dim) {
         return -1;
     }
-    return ((((static_cast<int64_t>(layer) * 2 + kv) * l->n_streams + stream) * l->n_kv_heads + head) * l->max_seq +
-            pos) * l->head_dim + dim;
+    const int64_t block = (static_cast<int64_t>(layer) * 2 + kv) * l->n_streams + stream;
+    return block * (block_bytes(*l) / static_cast<int64_t>(qa_kv_elem_bytes(l->cache_type))) +
+           (static_cast<int64_t>(head) * l->max_seq + pos) * l->head_dim + dim;
 }
 
 extern "C" int qa_kv_cache_alloc(const qa_kv_layout * l, void ** dev_cache) {

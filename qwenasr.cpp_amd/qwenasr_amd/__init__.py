@@ -21,7 +21,7 @@ _PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG_DIR, "libqwenasr_amd.so")
 
 QA_OK, QA_ERR_INVALID, QA_ERR_CAPACITY, QA_ERR_DEVICE, QA_ERR_NO_DEVICE, QA_ERR_ALLOC, QA_ERR_RANGE = range(7)
-QA_CACHE_F32, QA_CACHE_F16 = 0, 1
+QA_CACHE_F32, QA_CACHE_F16, QA_CACHE_Q8 = 0, 1, 2
 QA_NOALLOC_SCRATCH_BYTES = 48 << 20   # include/qwenasr_amd.h
 
 
@@ -113,6 +113,17 @@ SIGNATURES = {
     "qa_paged_append": (C.c_int, vp, vp, vp, vp, vp, C.POINTER(KvLayout), i32, C.POINTER(PagedBatch), i32, f32, f32, vp),
     "qa_paged_attn_workspace_bytes": (sz, C.POINTER(KvLayout), C.POINTER(PagedBatch), i32),
     "qa_paged_attn": (C.c_int, vp, vp, C.POINTER(KvLayout), i32, C.POINTER(PagedBatch), i32, f32, vp, vp, sz, vp),
+    "qa_paged_read": (C.c_int, vp, C.POINTER(KvLayout), i32, C.POINTER(PagedBatch), vp, vp, i32, vp),
+    "qa_tree_prepare": (C.c_int, C.POINTER(PagedBatch), vp, vp, i32, vp, vp),
+    "qa_paged_tree_append": (C.c_int, vp, vp, vp, vp, vp, C.POINTER(KvLayout), i32, C.POINTER(PagedBatch), vp, i32, f32, f32,
+                             vp),
+    "qa_paged_tree_attn": (C.c_int, vp, vp, C.POINTER(KvLayout), i32, C.POINTER(PagedBatch), vp, i32, i32, f32, vp, vp, sz,
+                           vp),
+    "qa_tree_accept": (C.c_int, C.POINTER(PagedBatch), vp, vp, vp, vp, vp, vp, vp),
+    "qa_paged_keep": (C.c_int, vp, C.POINTER(KvLayout), C.POINTER(PagedBatch), vp, vp, vp),
+    "qa_beam_select_workspace_bytes": (sz, i32, i32, i32),
+    "qa_beam_select": (C.c_int, vp, i32, i32, i32, vp, vp, vp, i32, vp, vp, vp, vp, vp, sz, vp),
+    "qa_beam_reorder": (C.c_int, vp, i32, vp, i32, i32, i32, vp, vp, vp, i32, vp, i32, vp, vp, vp),
     "qa_pages_workspace_bytes": (sz, C.POINTER(KvLayout)),
     "qa_pages_extend": (C.c_int, vp, C.POINTER(KvLayout), vp, vp, i32, i32, vp, vp, vp, i32, vp, vp, sz, vp),
     "qa_pages_fork": (C.c_int, vp, i32, vp, i32, i32, i32, vp, vp, vp, i32, vp),
