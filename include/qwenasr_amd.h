@@ -427,8 +427,8 @@ int qa_argmax_rows(const float * logits, int32_t rows, int32_t vocab, int32_t * 
  * scores[b] + logits[b][v] - log(sum over u of exp(logits[b][u])), and the beam itself, unchanged, where done[b] != 0 (done NULL:
  * none).  The `width` best become the new beams, best first, ties to the lower beam and then the lower id:
  * parents (the row that it continues), tokens (its id, -1 for a beam that was done), scores_out, and done_out: 1 where the
- * parent was done or the id is one of stop_ids (device int32[n_stop], 0 to 64).  Sums, logarithms and comparisons are in 64 bits, scores
- * rounded once.  A NaN is no candidate and weighs nothing, nor does -inf; a score of -inf or NaN leaves a beam without candidates (the
+ * parent was done or the id is one of stop_ids (device int32[n_stop], 0 to 64).  Sums and comparisons are in 64 bits (a row's
+ * logarithm of its sum is good to 2^-22), scores rounded once.  A NaN is no candidate and weighs nothing, nor does -inf; a score of -inf or NaN leaves a beam without candidates (the
  * first step, whose beams are the same: 0 for one of them and -inf for the others); a row with +inf has none.  Where a
  * group has fewer than width candidates, the remaining new beams are done: parent the own row, token -1, score -inf.
  * 1 to 64 beams, vocab >= width.  No output may overlap an input.  workspace: qa_beam_select_workspace_bytes, aligned to 16 bytes;

@@ -1,12 +1,12 @@
 // Beam search: the best continuations over a group's beams and the vocabulary, and the beams' states put in their new order.
 //
 // Selection in two launches.  The first streams the logits once (a wave takes a unit of a row, values in registers): the largest
-// value of every 64, and the unit's maximum and sum of exponentials.  The second, a workgroup per group, needs no more than
+// value of every 256, and the unit's maximum and sum of exponentials.  The second, a workgroup per group, needs no more than
 // those: a row's logarithm of its sum turns maxima into scores, and the new beams are among the values of the `width` best
-// 64s, as any value outside has `width` better ones (of 64s that tie, the earlier has the lower ids).  It reads those again,
-// width x 256 bytes.  Both of its choices, of 64s and of values, go the same way: a bound that at least `width` entries
+// 256s, as any value outside has `width` better ones (of 256s that tie, the earlier has the lower ids).  It reads those again,
+// width x 1 KB.  Both of its choices, of 256s and of values, go the same way: a bound that at least `width` entries
 // reach, a list of the entries that reach it, and each entry's rank in the list by counting.
-// Exponentials are f32, sums and logarithms f64, and so are scores, so that candidates of different beams compare as in the formula.
+// Exponentials are f32, sums and scores f64, so that candidates of different beams compare as in the formula.
 #include "common.hpp"
 #include "paged.hpp"
 #include "wave.hpp"
@@ -16,9 +16,10 @@
 namespace qa {
 namespace {
 
+typedef int i4 __attribute__((ext_vector_type(4)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));   // rows of an odd vocabulary start anywhere
 
-constexpr int kSeg = 64;             // values per maximum
+constexpr int kSeg = 256;            // values per maximum: a wave's load
 constexpr int kMaxWidth = 64;
 constexpr int kMaxStops = 64;
 constexpr int kPickThreads = 1024, kPickWaves = kPickThreads / kWave;
@@ -43,17 +44,27 @@ struct BeamParams {
     int32_t n_rows, width, vocab, n_stop, n_units, n_segs;
 };
 
-// LOADS x 256 values per wave.
-template <int LOADS>
+// 2^t to 2^-23 of itself: what t loses as an f32 goes in behind the instruction.  (A difference x - most rounded to f32 would be off by
+// 2^-24 |x - most|, the same way for many equal values.)
+constexpr double kLog2e = 1.4426950408889634;
+__device__ inline float exp2_of(double t) {
+    const float hi = static_cast<float>(t), lo = static_cast<float>(t - static_cast<double>(hi));
+    const float e = __builtin_amdgcn_exp2f(hi);
+    return hi > -INFINITY ? fmaf(e * lo, 0.6931472f, e) : 0.0f;
+}
+
+// 512 values per wave: 64 rows of 151936 in 1, 2, 4 and 8 loads per lane 13, 9.7, 10.8 and 12.3 us (read at 4 TB/s; a wave's
+// instructions take as long as its values, and short waves overlap the two), 4 rows 3.0 in 2 and 4.5 in 8.
+constexpr int kLoads = 2;
 __global__ __launch_bounds__(256) void beam_units_kernel(BeamParams p) {
     const int lane = threadIdx.x & (kWave - 1);
     const int unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = blockIdx.y;
     if (unit >= p.n_units || (p.done && p.done[row] != 0)) return;       // a beam that is done has one candidate
     const float * x = p.logits + static_cast<int64_t>(row) * p.vocab;
-    const int first = unit * LOADS * 256 + lane * 4;
-    f4u v[LOADS];
+    const int first = unit * kLoads * 256 + lane * 4;
+    f4u v[kLoads];
 #pragma unroll
-    for (int u = 0; u < LOADS; ++u) {
+    for (int u = 0; u < kLoads; ++u) {
         const int at = first + u * 256;
         if (at + 4 <= p.vocab) {
             v[u] = *reinterpret_cast<const f4u *>(x + at);
@@ -64,49 +75,43 @@ __global__ __launch_bounds__(256) void beam_units_kernel(BeamParams p) {
     }
     float most = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < LOADS; ++u) {
+    for (int u = 0; u < kLoads; ++u) {
         float seg = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            v[u][e] = v[u][e] == v[u][e] ? v[u][e] : -INFINITY;
+            v[u][e] = fmaxf(v[u][e], -INFINITY);           // NaN: none
             seg = fmaxf(seg, v[u][e]);
         }
-        seg = fmaxf(seg, dpp_f<0xB1>(seg));
-        seg = fmaxf(seg, dpp_f<0x4E>(seg));
-        seg = fmaxf(seg, dpp_f<0x141>(seg));
-        seg = fmaxf(seg, dpp_f<0x140>(seg));
-        const int s = (unit * LOADS + u) * 4 + (lane >> 4);
-        if ((lane & 15) == 0 && s < p.n_segs) p.seg_max[static_cast<int64_t>(row) * p.n_segs + s] = seg;
+        seg = wave_max_all(seg);
+        const int s = unit * kLoads + u;
+        if (lane == 0 && s < p.n_segs) p.seg_max[static_cast<int64_t>(row) * p.n_segs + s] = seg;
         most = fmaxf(most, seg);
     }
-    most = wave_max_all(most);
     double sum = 0.0;
     if (most > -INFINITY) {
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
+        for (int u = 0; u < kLoads; ++u) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += static_cast<double>(expf(v[u][e] - most));
+            for (int e = 0; e < 4; ++e) sum += static_cast<double>(exp2_of((static_cast<double>(v[u][e]) - most) * kLog2e));
         }
     }
     sum = wave_sum_d_all(sum);
     if (lane == 0) p.units[static_cast<int64_t>(row) * p.n_units + unit] = Unit{sum, most, 0.0f};
 }
 
-// A candidate: its score and its number in the order that settles ties.  -inf: none.
+// A candidate: its score, and its beam and place, which settle ties: the lower first.
 struct Entry {
     double score;
-    int64_t at;
+    uint64_t at;
 };
-__device__ inline bool better(double a, int64_t i, double b, int64_t j) { return a > b || (a == b && i < j); }
+__device__ inline uint64_t place_of(int beam, int place) { return (static_cast<uint64_t>(beam) << 32) | static_cast<uint32_t>(place); }
+__device__ inline bool better(const Entry & a, const Entry & b) { return a.score > b.score || (a.score == b.score && a.at < b.at); }
 
-__device__ inline double wave_best(double v, int64_t & at) {
-#pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-        const double o = __shfl_xor(v, d, kWave);
-        const int64_t i = __shfl_xor(at, d, kWave);
-        if (better(o, i, v, at)) v = o, at = i;
-    }
-    return v;
+// log x of a sum, to 2^-24: the mantissa's in f32.  (In f64 throughout the workgroup waited 1 us for it.)
+__device__ inline double log_of(double x) {
+    int e;
+    const double m = frexp(x, &e);
+    return e * 0.6931471805599453 + static_cast<double>(logf(static_cast<float>(m)));
 }
 
 struct PickLds {
@@ -115,170 +120,255 @@ struct PickLds {
     Entry list[kListMax];
     Entry chosen[kMaxWidth];
     Entry wave[kPickWaves];
-    int count, n_chosen;
+    double sum[kMaxWidth];           // of a beam's exponentials, less its largest value
+    float most[kMaxWidth];
+    float row_most[4 * kMaxWidth];   // the largest maximum of every 16 lanes, a wave's (or a beam's) four together
+    double bound;
+    int count;
 };
 
-// The `width` best of n entries, best first, into chosen.  score(i) is the i-th one's, which settles ties as well.
-template <typename F>
-__device__ inline void choose(PickLds & s, int width, int64_t n, F && score) {
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
-    // every wave's k-th best lane, k the same for all: at least k x waves >= width entries reach the least of them
-    double best = -INFINITY;
-    int64_t at = n;
-    for (int64_t i = threadIdx.x; i < n; i += kPickThreads) {
-        const double v = score(i);
-        if (v > best) best = v, at = i;
+// The `width` best of the list, best first, into chosen: an entry's place is the number of better ones, which 8 lanes count.
+__device__ inline void rank_list(PickLds & s, int count, int width) {
+    constexpr int kLanes = 8;
+    for (int first = 0; first < count; first += kPickThreads / kLanes) {
+        const int i = first + static_cast<int>(threadIdx.x) / kLanes;
+        const Entry e = s.list[min(i, count - 1)];
+        int rank = 0;
+        for (int k = threadIdx.x & (kLanes - 1); k < count; k += kLanes) rank += better(s.list[k], e);
+        rank += __builtin_amdgcn_mov_dpp(rank, 0xB1, 0xf, 0xf, false);
+        rank += __builtin_amdgcn_mov_dpp(rank, 0x4E, 0xf, 0xf, false);
+        rank += __builtin_amdgcn_mov_dpp(rank, 0x141, 0xf, 0xf, false);
+        if (i < count && rank < width && (threadIdx.x & (kLanes - 1)) == 0) s.chosen[rank] = e;
     }
-    double bound = best;
-    int64_t bound_at = at;
-    for (int k = (width + kPickWaves - 1) / kPickWaves; k > 0; --k) {
-        double v = best;
-        int64_t i = at;
-        v = wave_best(v, i);
-        bound = v;
-        bound_at = i;
-        if (best == v && at == i) best = -INFINITY, at = n;
-    }
-    if (threadIdx.x == 0) s.count = 0, s.n_chosen = 0;
-    if (lane == 0) s.wave[wave] = Entry{bound, bound_at};
-    __syncthreads();
-    for (int w = 0; w < kPickWaves; ++w) {
-        if (better(bound, bound_at, s.wave[w].score, s.wave[w].at)) bound = s.wave[w].score, bound_at = s.wave[w].at;
-    }
-    for (int64_t i = threadIdx.x; i < n; i += kPickThreads) {
-        const double v = score(i);
-        if (!(v > -INFINITY) || better(bound, bound_at, v, i)) continue;
-        const int to = atomicAdd(&s.count, 1);
-        if (to < kListMax) s.list[to] = Entry{v, i};
-    }
-    __syncthreads();
-    const int count = s.count;
-    if (count <= kListMax) {
-        if (static_cast<int>(threadIdx.x) < count) {
-            const Entry e = s.list[threadIdx.x];
-            int rank = 0;
-            for (int k = 0; k < count; ++k) rank += better(s.list[k].score, s.list[k].at, e.score, e.at);
-            if (rank < width) s.chosen[rank] = e;
-        }
-        if (threadIdx.x == 0) s.n_chosen = min(count, width);
-        __syncthreads();
-        return;
-    }
-    // one by one, each the best of those behind the one before
-    Entry last{INFINITY, -1};
-    for (int r = 0; r < width; ++r) {
-        double v = -INFINITY;
-        int64_t a = n;
-        for (int64_t i = threadIdx.x; i < n; i += kPickThreads) {
-            const double x = score(i);
-            if (x > -INFINITY && better(last.score, last.at, x, i) && better(x, i, v, a)) v = x, a = i;
-        }
-        v = wave_best(v, a);
-        __syncthreads();
-        if (lane == 0) s.wave[wave] = Entry{v, a};
-        __syncthreads();
-        last = s.wave[0];
-        for (int w = 1; w < kPickWaves; ++w) {
-            if (better(s.wave[w].score, s.wave[w].at, last.score, last.at)) last = s.wave[w];
-        }
-        if (threadIdx.x == 0) s.chosen[r] = last;
-    }
-    if (threadIdx.x == 0) s.n_chosen = width;              // more than kListMax entries count
     __syncthreads();
 }
 
+// The same where more entries reach the bound than the list holds (many ties): one after another, each the best of those behind
+// the one before.  entry(i) is the i-th of n.
+template <typename F>
+__device__ inline void one_by_one(PickLds & s, int width, int n, F && entry) {
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+    Entry last{INFINITY, 0};
+    for (int r = 0; r < width; ++r) {
+        Entry best{-INFINITY, ~uint64_t{0}};
+        for (int i = threadIdx.x; i < n; i += kPickThreads) {
+            const Entry e = entry(i);
+            if (e.score > -INFINITY && better(last, e) && better(e, best)) best = e;
+        }
+#pragma unroll
+        for (int d = 1; d < kWave; d <<= 1) {
+            const Entry o{__shfl_xor(best.score, d, kWave), static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(best.at), d, kWave))};
+            if (better(o, best)) best = o;
+        }
+        if (lane == 0) s.wave[wave] = best;
+        __syncthreads();
+        last = s.wave[0];
+        for (int w = 1; w < kPickWaves; ++w) {
+            if (better(s.wave[w], last)) last = s.wave[w];
+        }
+        if (threadIdx.x == 0) s.chosen[r] = last;
+        __syncthreads();
+    }
+}
+
+// Its time is one workgroup's latencies, and fetching its instructions: short loops, and little that is unrolled.  A wave takes the
+// 256s of one beam (or a part of them, for up to 8 beams; or of several beams, one after another, for more than 16), so that it
+// looks at maxima as they are, one comparison each, and only what may count becomes a score in 64 bits.  Up to kKeep maxima per
+// lane are fetched before the row's sums are added and stay in registers for the second look.
+constexpr int kKeep = 10;
+static_assert(kPickThreads == 4 * 4 * kMaxWidth, "four lanes rank each of the rows' maxima");
+
 __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams p) {
     __shared__ PickLds s;
-    __shared__ Entry s_segs[kMaxWidth];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row0 = blockIdx.x * p.width;
-    for (int b = wave; b < p.width; b += kPickWaves) {
-        const int row = row0 + b;
-        const double score = static_cast<double>(p.scores[row]);
-        const bool counts = score > -INFINITY && score < INFINITY, done = p.done && p.done[row] != 0;
-        double off = -INFINITY;
-        if (counts && !done) {
-            const Unit * units = p.units + static_cast<int64_t>(row) * p.n_units;
-            float most = -INFINITY;
-            for (int u = lane; u < p.n_units; u += kWave) most = fmaxf(most, units[u].most);
-            most = wave_max_all(most);
-            double sum = 0.0;
-            for (int u = lane; u < p.n_units; u += kWave) {
-                if (units[u].most > -INFINITY) sum += units[u].sum * exp(static_cast<double>(units[u].most) - most);
-            }
-            sum = wave_sum_d_all(sum);
-            if (most > -INFINITY && most < INFINITY) off = score - (log(sum) + most);
+    const int parts = max(1, kPickWaves / p.width), stride = parts * kWave, per_lane = (p.n_segs + stride - 1) / stride;
+    const int tasks = p.width * parts;
+    const bool keep = tasks <= kPickWaves && per_lane <= kKeep;
+    // kKeep maxima of a task, from its lanes' first one behind `from` on
+    float held[kKeep];
+    auto fetch = [&](int task, int from) {
+        const float * maxima = p.seg_max + static_cast<int64_t>(row0 + task / parts) * p.n_segs;
+#pragma unroll
+        for (int k = 0; k < kKeep; ++k) {
+            const int seg = task % parts * kWave + lane + (from + k) * stride;
+            held[k] = seg < p.n_segs ? maxima[seg] : -INFINITY;
         }
-        if (lane == 0) {
-            s.off[b] = off;
-            s.stay[b] = counts && done ? score : -INFINITY;
-        }
-    }
-    __syncthreads();
-    // entries of a beam: itself, where it is done, and its 64s
-    const int per_beam = p.n_segs + 1;
-    choose(s, p.width, static_cast<int64_t>(p.width) * per_beam, [&](int64_t i) {
-        const int b = static_cast<int>(i / per_beam), seg = static_cast<int>(i - static_cast<int64_t>(b) * per_beam) - 1;
-        if (seg < 0) return s.stay[b];
-        const double off = s.off[b];
-        return off > -INFINITY ? off + static_cast<double>(p.seg_max[static_cast<int64_t>(row0 + b) * p.n_segs + seg]) : -INFINITY;
-    });
-    const int n_segs = s.n_chosen;
-    if (static_cast<int>(threadIdx.x) < n_segs) s_segs[threadIdx.x] = s.chosen[threadIdx.x];
-    __syncthreads();
-    // put in order of beam and place, so that an entry's number settles ties
-    if (static_cast<int>(threadIdx.x) < n_segs) {
-        const Entry e = s_segs[threadIdx.x];
-        int rank = 0;
-        for (int k = 0; k < n_segs; ++k) rank += s_segs[k].at < e.at;
-        s.chosen[rank] = e;
-    }
-    __syncthreads();
-    if (static_cast<int>(threadIdx.x) < n_segs) s_segs[threadIdx.x] = s.chosen[threadIdx.x];
-    __syncthreads();
-    auto place = [&](int64_t i, int & b, int & id) {       // of value i % 64 of the chosen 64
-        const int64_t at = s_segs[i / kSeg].at;
-        b = static_cast<int>(at / per_beam);
-        const int seg = static_cast<int>(at - static_cast<int64_t>(b) * per_beam) - 1;
-        id = seg < 0 ? -1 : seg * kSeg + static_cast<int>(i % kSeg);
-        return seg < 0 ? i % kSeg == 0 : id < p.vocab;
     };
-    choose(s, p.width, static_cast<int64_t>(n_segs) * kSeg, [&](int64_t i) {
-        int b, id;
-        if (!place(i, b, id)) return static_cast<double>(-INFINITY);
-        if (id < 0) return s.stay[b];
-        const float x = p.logits[static_cast<int64_t>(row0 + b) * p.vocab + id];
-        return x == x ? s.off[b] + static_cast<double>(x) : -INFINITY;
-    });
+    if (keep && wave < tasks) fetch(wave, 0);
+    // a lane per beam
+    double score = -INFINITY;
+    bool done = false;
+    if (wave == 0 && lane < p.width) {
+        score = static_cast<double>(p.scores[row0 + lane]);
+        done = p.done && p.done[row0 + lane] != 0;
+    }
+    if (threadIdx.x == 0) s.count = 0;
+    for (int task = wave; task < tasks; task += kPickWaves) {
+        const int b = task / parts;
+        float most = -INFINITY;
+        for (int from = 0; from < per_lane; from += kKeep) {
+            if (!keep) fetch(task, from);
+#pragma unroll
+            for (int k = 0; k < kKeep; ++k) most = fmaxf(most, held[k]);
+        }
+        most = fmaxf(most, dpp_f<0xB1>(most));
+        most = fmaxf(most, dpp_f<0x4E>(most));
+        most = fmaxf(most, dpp_f<0x141>(most));
+        most = fmaxf(most, dpp_f<0x140>(most));
+        if ((lane & 15) == 0) s.row_most[task * 4 + (lane >> 4)] = most;
+        if (task % parts != 0) continue;
+        // the row's sum
+        const Unit * units = p.units + static_cast<int64_t>(row0 + b) * p.n_units;
+        constexpr int kUnits = 5;                          // per lane in registers: 320 of a row
+        Unit u[kUnits];
+        float all = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) u[k] = units[min(lane + k * kWave, p.n_units - 1)];
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) all = fmaxf(all, u[k].most);
+        for (int i = lane + kUnits * kWave; i < p.n_units; i += kWave) all = fmaxf(all, units[i].most);
+        all = wave_max_all(all);
+        double sum = 0.0;
+        auto add = [&](const Unit & x) {
+            if (x.most > -INFINITY) sum += x.sum * static_cast<double>(exp2_of((static_cast<double>(x.most) - all) * kLog2e));
+        };
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+            if (lane + k * kWave < p.n_units) add(u[k]);
+        }
+        for (int i = lane + kUnits * kWave; i < p.n_units; i += kWave) add(units[i]);
+        sum = wave_sum_d_all(sum);
+        if (lane == 0) {
+            s.sum[b] = sum;
+            s.most[b] = all;
+        }
+    }
+    // what a beam's values are raised by: one wave for all beams
+    __syncthreads();
+    if (wave == 0 && lane < p.width) {
+        const bool counts = score > -INFINITY && score < INFINITY;
+        const float most = s.most[lane];
+        s.stay[lane] = counts && done ? score : -INFINITY;
+        s.off[lane] = counts && !done && most > -INFINITY && most < INFINITY ? score - (log_of(s.sum[lane]) + most) : -INFINITY;
+    }
+    __syncthreads();
+    // The bound: of those best of 16 lanes each (a beam that is done is one of them), the width-th.
+    auto row_best = [&](int i) {
+        const int b = (i >> 2) / parts;
+        const double off = s.off[b];
+        return off > -INFINITY ? off + static_cast<double>(s.row_most[i]) : i == b * parts * 4 ? s.stay[b] : -INFINITY;
+    };
+    if (static_cast<int>(threadIdx.x) < tasks * 4) s.list[threadIdx.x].score = row_best(threadIdx.x);
+    __syncthreads();
+    {
+        const int i = threadIdx.x >> 2;
+        const double v = s.list[min(i, tasks * 4 - 1)].score;
+        int rank = 0;
+#pragma unroll 4
+        for (int j = threadIdx.x & 3; j < tasks * 4; j += 4) {
+            const double o = s.list[j].score;
+            rank += o > v || (o == v && j < i);
+        }
+        rank += __builtin_amdgcn_mov_dpp(rank, 0xB1, 0xf, 0xf, false);
+        rank += __builtin_amdgcn_mov_dpp(rank, 0x4E, 0xf, 0xf, false);
+        if (i < tasks * 4 && rank == p.width - 1 && (threadIdx.x & 3) == 0) s.bound = v;
+    }
+    __syncthreads();
+    double bound = s.bound;
+    auto list = [&](const Entry & e) {
+        if (!(e.score > -INFINITY) || e.score < bound) return;
+        const int to = atomicAdd(&s.count, 1);
+        if (to < kListMax) s.list[to] = e;
+    };
+    for (int task = wave; task < tasks; task += kPickWaves) {
+        const int b = task / parts;
+        const double off = s.off[b];
+        if (!(off > -INFINITY)) continue;
+        // below what a maximum needs by more than the difference is rounded
+        const float near = static_cast<float>(bound - off), least = near - fmaxf(fabsf(near), 1e-30f) * 0x1p-22f;
+        for (int from = 0; from < per_lane; from += kKeep) {
+            if (!keep) fetch(task, from);
+            unsigned some = 0;
+#pragma unroll
+            for (int k = 0; k < kKeep; ++k) some |= held[k] >= least ? 1u << k : 0u;
+            for (; some != 0; some &= some - 1) {          // few
+                const int at = __ffs(some) - 1;
+                float v = held[0];
+#pragma unroll
+                for (int k = 1; k < kKeep; ++k) v = k == at ? held[k] : v;
+                list(Entry{off + static_cast<double>(v), place_of(b, task % parts * kWave + lane + (from + at) * stride + 1)});
+            }
+        }
+    }
+    if (static_cast<int>(threadIdx.x) < p.width) list(Entry{s.stay[threadIdx.x], place_of(threadIdx.x, 0)});
+    __syncthreads();
+    int count = s.count;
+    if (count <= kListMax) {
+        rank_list(s, count, p.width);
+    } else {
+        const int n = p.width * p.n_segs;
+        one_by_one(s, p.width, n + p.width, [&](int i) {
+            if (i >= n) return Entry{s.stay[i - n], place_of(i - n, 0)};
+            const int b = i / p.n_segs, seg = i - b * p.n_segs;
+            const double off = s.off[b];
+            return Entry{off > -INFINITY ? off + static_cast<double>(p.seg_max[static_cast<int64_t>(row0) * p.n_segs + i]) : -INFINITY, place_of(b, seg + 1)};
+        });
+    }
+    const int n_segs = min(count, p.width);
+    // The values of the chosen 256s: those that reach the last one's maximum are at least as many.
+    bound = n_segs > 0 ? s.chosen[n_segs - 1].score : 0.0;
+    auto value = [&](const Entry * segs, int i) {
+        const Entry seg = segs[i / kSeg];
+        const int b = static_cast<int>(seg.at >> 32), place = static_cast<int>(static_cast<uint32_t>(seg.at));
+        if (place == 0) return Entry{i % kSeg == 0 ? seg.score : -INFINITY, seg.at};
+        const int id = (place - 1) * kSeg + i % kSeg;
+        const float x = id < p.vocab ? p.logits[static_cast<int64_t>(row0 + b) * p.vocab + id] : -INFINITY;
+        return Entry{x == x ? s.off[b] + static_cast<double>(x) : -INFINITY, place_of(b, id + 1)};
+    };
+    if (threadIdx.x == 0) s.count = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n_segs * kSeg; i += kPickThreads) list(value(s.chosen, i));
+    __syncthreads();
+    count = s.count;
+    Entry mine{-INFINITY, 0};
+    if (count <= kListMax) {
+        rank_list(s, count, p.width);
+        if (static_cast<int>(threadIdx.x) < min(count, p.width)) mine = s.chosen[threadIdx.x];
+    } else {
+        Entry * segs = s.list;                             // chosen takes the values
+        if (static_cast<int>(threadIdx.x) < n_segs) segs[threadIdx.x] = s.chosen[threadIdx.x];
+        __syncthreads();
+        one_by_one(s, p.width, n_segs * kSeg, [&](int i) { return value(segs, i); });
+        if (static_cast<int>(threadIdx.x) < p.width) mine = s.chosen[threadIdx.x];
+    }
     if (static_cast<int>(threadIdx.x) >= p.width) return;
-    const int r = threadIdx.x, out = row0 + r;
-    if (r >= s.n_chosen) {
+    const int out = row0 + threadIdx.x;
+    if (static_cast<int>(threadIdx.x) >= count) {
         p.parents[out] = out;
         p.tokens[out] = -1;
         p.scores_out[out] = -INFINITY;
         p.done_out[out] = 1;
         return;
     }
-    int b, id;
-    place(s.chosen[r].at, b, id);
+    const int id = static_cast<int>(static_cast<uint32_t>(mine.at)) - 1;
     int ended = id < 0;
     for (int k = 0; k < p.n_stop; ++k) ended |= p.stop_ids[k] == id;
-    p.parents[out] = row0 + b;
+    p.parents[out] = row0 + static_cast<int>(mine.at >> 32);
     p.tokens[out] = id;
-    p.scores_out[out] = static_cast<float>(s.chosen[r].score);
+    p.scores_out[out] = static_cast<float>(mine.score);
     p.done_out[out] = ended;
 }
 
-// How the first launch cuts rows: short units where they are what fills the GPU.
 struct BeamPlan {
-    int loads, n_units, n_segs;
+    int n_units, n_segs;
     size_t units_bytes, bytes;
 };
 
 BeamPlan beam_plan(int64_t rows, int32_t vocab) {
     BeamPlan pl{};
-    pl.loads = rows * vocab > (int64_t{1} << 22) ? 8 : 2;
-    pl.n_units = (vocab + pl.loads * 256 - 1) / (pl.loads * 256);
+    pl.n_units = (vocab + kLoads * 256 - 1) / (kLoads * 256);
     pl.n_segs = (vocab + kSeg - 1) / kSeg;
     pl.units_bytes = static_cast<size_t>(rows) * pl.n_units * sizeof(Unit);
     pl.bytes = pl.units_bytes + (static_cast<size_t>(rows) * pl.n_segs * sizeof(float) + 15) / 16 * 16;
@@ -309,7 +399,8 @@ constexpr int kMaxBeams = 1024, kCols = 8, kReorderThreads = 256;
 // A workgroup per 8 columns of the tables or of the ids, with all rows: what the rows hold is read into LDS, and then each entry
 // is written by one thread.  Only counts of entries that change are touched.
 __global__ __launch_bounds__(kReorderThreads) void beam_reorder_kernel(ReorderParams p) {
-    __shared__ int s_row[kMaxBeams], s_old[kMaxBeams * kCols];
+    __shared__ __attribute__((aligned(16))) int s_row[kMaxBeams];
+    __shared__ int s_old[kMaxBeams * kCols];
     const bool pages = static_cast<int>(blockIdx.x) < p.table_blocks;
     int32_t * data = pages ? p.tables : p.ids;
     const int stride = pages ? p.stride : p.ids_stride;
@@ -325,7 +416,15 @@ __global__ __launch_bounds__(kReorderThreads) void beam_reorder_kernel(ReorderPa
         for (int u = 0; u < kMaxBeams / kReorderThreads; ++u) {
             const int i = threadIdx.x + u * kReorderThreads;
             if (i >= p.n) continue;
-            for (int k = 0; k < i; ++k) again[u] = again[u] || s_row[k] == s_row[i];
+            const int row = s_row[i];
+            int hits = 0;
+#pragma unroll 4
+            for (int k = 0; k < i; k += 4) {               // four per LDS read, reads in flight together
+                const i4 v = *reinterpret_cast<const i4 *>(s_row + k);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) hits += k + w < i && v[w] == row;
+            }
+            again[u] = hits > 0;
         }
         __syncthreads();
 #pragma unroll
@@ -404,8 +503,7 @@ extern "C" int qa_beam_select(const float * logits, int32_t n_groups, int32_t wi
     p.n_units = pl.n_units;
     p.n_segs = pl.n_segs;
     const dim3 grid(static_cast<unsigned>((pl.n_units + 3) / 4), static_cast<unsigned>(rows));
-    const auto kernel = pl.loads == 8 ? &beam_units_kernel<8> : &beam_units_kernel<2>;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, as_stream(stream), p);
+    hipLaunchKernelGGL(beam_units_kernel, grid, dim3(256), 0, as_stream(stream), p);
     QA_LAUNCH_CHECK("beam_units_kernel");
     hipLaunchKernelGGL(beam_pick_kernel, dim3(static_cast<unsigned>(n_groups)), dim3(kPickThreads), 0, as_stream(stream), p);
     QA_LAUNCH_CHECK("beam_pick_kernel");
