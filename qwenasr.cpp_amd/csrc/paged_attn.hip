@@ -144,6 +144,7 @@ __device__ inline bool find_tile(const AttnParams & p, int block, int lane, Tile
 struct Column {
     int row, lim;
     const float * q;
+    int mask;       // trees: its row's first word
 };
 
 template <bool TREE>
@@ -151,7 +152,8 @@ __device__ inline Column column_of(const AttnParams & p, const Tile & t, int hea
     const bool ok = col < t.n_cols;
     const int token = (ok ? col : t.n_cols - 1) / p.group;
     const int row = (t.row0 + token) * p.n_heads + head * p.group + (ok ? col - token * p.group : 0);
-    return Column{ok ? row : -1, ok ? min(t.past + (TREE ? t.rows - 1 : token), t.cap - 1) : -1, p.q + static_cast<int64_t>(row) * kHeadDim};
+    return Column{ok ? row : -1, ok ? min(t.past + (TREE ? t.rows - 1 : token), t.cap - 1) : -1, p.q + static_cast<int64_t>(row) * kHeadDim,
+                  TREE ? (t.row0 + token) * p.mask_words : 0};
 }
 
 // A table entry as the page of the 16 keys from j on, -1 for none.
@@ -290,12 +292,12 @@ __device__ inline void scores_step(const u4 (&a)[8], const h8 (&qh)[NB][4], cons
 
 // -inf where a key lies behind the column's last position, on no page (bit kb of holes: the 16-key block kb) or outside its mask.
 template <int NB, int KB, bool TREE>
-__device__ inline void mask_step(const AttnParams & p, f4 (&S)[NB][KB], const int (&lim)[NB], const int (&orow)[NB], int past, int key0,
+__device__ inline void mask_step(const AttnParams & p, f4 (&S)[NB][KB], const int (&lim)[NB], const int (&mask)[NB], int past, int key0,
                                  int g4, int holes) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         uint32_t seen = ~0u;
-        if constexpr (TREE) seen = mask_window(p, mask_row(p, max(orow[nb], 0)), key0 - past);
+        if constexpr (TREE) seen = mask_window(p, p.mask + mask[nb], key0 - past);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -318,11 +320,30 @@ __device__ inline u4 transposed(const u4 (&v)[8], int db) {
     return a;
 }
 
-// 8 bits as f16.  Bytes are taken with their sign bit turned over (u = x + 128) next to 0x64: 1024 + u in f16, less 1152.
-constexpr uint32_t kSignBits = 0x80808080u;
-__device__ inline uint32_t f16_pair(uint32_t bytes, uint32_t select) {
-    const h2 v = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, bytes, select));
-    return __builtin_bit_cast(uint32_t, v - h2{1152, 1152});
+// 8 bits as f16: one instruction per value, which takes its byte and leaves its half of the register.  The last s_nop is the wait
+// that a reader of a half-written register needs.
+__device__ inline void f16_pairs(uint32_t bytes, uint32_t & a, uint32_t & b) {
+    asm("v_cvt_f16_i16_sdwa %0, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
+        "v_cvt_f16_i16_sdwa %1, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+        "v_cvt_f16_i16_sdwa %0, sext(%2) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1\n\t"
+        "v_cvt_f16_i16_sdwa %1, sext(%2) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3\n\t"
+        "s_nop 0" : "=&v"(a), "=&v"(b) : "v"(bytes));
+}
+// (x, y) byte by byte
+__device__ inline void f16_pairs(uint32_t x, uint32_t y, int d, uint32_t & a, uint32_t & b) {
+    if (d == 0) {
+        asm("v_cvt_f16_i16_sdwa %0, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
+            "v_cvt_f16_i16_sdwa %1, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1\n\t"
+            "v_cvt_f16_i16_sdwa %0, sext(%3) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_0\n\t"
+            "v_cvt_f16_i16_sdwa %1, sext(%3) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1\n\t"
+            "s_nop 0" : "=&v"(a), "=&v"(b) : "v"(x), "v"(y));
+    } else {
+        asm("v_cvt_f16_i16_sdwa %0, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+            "v_cvt_f16_i16_sdwa %1, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3\n\t"
+            "v_cvt_f16_i16_sdwa %0, sext(%3) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_2\n\t"
+            "v_cvt_f16_i16_sdwa %1, sext(%3) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3\n\t"
+            "s_nop 0" : "=&v"(a), "=&v"(b) : "v"(x), "v"(y));
+    }
 }
 
 // K operands 4 kb .. 4 kb + 3 of a step from the lane's 2 x 16 bytes of 16-key block kb.
@@ -331,27 +352,22 @@ __device__ inline void k_operands(const u4 (&raw)[4], u4 (&a)[8]) {
     for (int r = 0; r < 4; ++r) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const uint32_t u = raw[r][w] ^ kSignBits;
-            a[2 * r + (w >> 1)][2 * (w & 1)] = f16_pair(u, 0x04010400u);
-            a[2 * r + (w >> 1)][2 * (w & 1) + 1] = f16_pair(u, 0x04030402u);
+            uint32_t lo, hi;
+            f16_pairs(raw[r][w], lo, hi);
+            a[2 * r + (w >> 1)][2 * (w & 1)] = lo;
+            a[2 * r + (w >> 1)][2 * (w & 1) + 1] = hi;
         }
     }
 }
 
-// V^T operands of a step's rows of 8 bits, 8 dims per lane and key: two keys' bytes side by side first.
-__device__ inline void v_operands(const u2 (&raw)[8], u4 (&a)[8]) {
+// V^T operands 4 h + 2 d and 4 h + 2 d + 1 of a step's rows of 8 bits, 8 dims per lane and key.
+__device__ inline void v_operands(const u2 (&raw)[8], int h, int d, u4 & even, u4 & odd) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t x = raw[2 * w][h] ^ kSignBits, y = raw[2 * w + 1][h] ^ kSignBits;
-#pragma unroll
-            for (int d = 0; d < 2; ++d) {
-                const uint32_t pairs = __builtin_amdgcn_perm(y, x, d ? 0x07030602u : 0x05010400u);
-                a[4 * h + 2 * d][w] = f16_pair(pairs, 0x04010400u);
-                a[4 * h + 2 * d + 1][w] = f16_pair(pairs, 0x04030402u);
-            }
-        }
+        uint32_t x, y;
+        f16_pairs(raw[2 * w][h], raw[2 * w + 1][h], d, x, y);
+        even[w] = x;
+        odd[w] = y;
     }
 }
 
@@ -473,13 +489,21 @@ __device__ inline void softmax_step(const f4 (&S)[NB][KB], const float (&c)[NB],
     }
 }
 
-// Probabilities as two f16 parts in the order of the PV product.
+// Probabilities as two f16 parts in the order of the PV product.  The rest v - hi is one instruction that takes hi as f16
+// (v_fma_mix_f32; the factor is hidden, or the compiler makes a conversion and a difference of it).
 __device__ inline void split_p(const float (&pr)[2][4], h8 & hi, h8 & lo) {
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float v = pr[e >> 2][e & 3];
-        hi[e] = static_cast<_Float16>(v);
-        lo[e] = static_cast<_Float16>(v - static_cast<float>(hi[e]));
+    for (int e = 0; e < 8; e += 2) {
+        const f2 v = {pr[e >> 2][e & 3], pr[e >> 2][(e & 3) + 1]};
+        const h2 h = __builtin_convertvector(v, h2);
+        const f2 rest = {fmaf(static_cast<float>(h[0]), minus, v[0]), fmaf(static_cast<float>(h[1]), minus, v[1])};
+        const h2 r = __builtin_convertvector(rest, h2);
+        hi[e] = h[0];
+        hi[e + 1] = h[1];
+        lo[e] = r[0];
+        lo[e + 1] = r[1];
     }
 }
 
@@ -520,16 +544,16 @@ __device__ inline void close_columns(const int (&orow)[NB], const float (&c)[NB]
 }
 
 // The flagged columns of a block, key by key; their values are stored at once.
-template <typename CT, int KS, bool TREE>
+template <typename CT, int KS>
 __device__ inline void redo_columns(const AttnParams & p, const Tile & t, int head, int lane, int lim, int orow, uint32_t redo) {
     for (uint32_t left = redo; left != 0; left &= left - 1) {
         const int col = __ffs(left) - 1;
         const int row = __builtin_amdgcn_readlane(orow, col), lm = __builtin_amdgcn_readlane(lim, col);
         float cm, cl;
         f2 co;
-        column_by_keys<CT, KS, TREE>(p, t.table, head, row, lm, t.past, t.step_lo, t.step_hi, 1, lane, cm, cl, co);
+        column_by_keys<CT, KS, false>(p, t.table, head, row, lm, t.past, t.step_lo, t.step_hi, 1, lane, cm, cl, co);
         const f2 nx = f2{__shfl_down(co[0], 1, kWave), __shfl_down(co[1], 1, kWave)};
-        if ((lane & 1) == 0) store_column<TREE>(p, t, row, lm, 2 * lane, f4{co[0], co[1], nx[0], nx[1]}, cm, cl, lane == 0);
+        if ((lane & 1) == 0) store_column<false>(p, t, row, lm, 2 * lane, f4{co[0], co[1], nx[0], nx[1]}, cm, cl, lane == 0);
     }
 }
 
@@ -549,6 +573,72 @@ template <bool ONCE, typename VT>
 __device__ inline VT load_row(const void * at) {
     if constexpr (ONCE) return __builtin_nontemporal_load(static_cast<const VT *>(at));
     else return *static_cast<const VT *>(at);
+}
+
+// The 4 waves' results of R columns, merged in LDS and stored; what is to be computed again (redo) is, key by key.
+template <typename CT, int R, bool PACK, bool TREE>
+__device__ inline void merge_waves(const AttnParams & p, const Tile & t, int head, char * lds, int wave, int lane, int orow, int lim, float mc,
+                                   float l, const f4 (&O)[8], uint32_t redo) {
+    constexpr int KS = step_keys(f16_products<CT>);
+    const int c16 = lane & 15, g4 = lane >> 4;
+    float * so = reinterpret_cast<float *>(lds);
+    float * sm = so + kWaves * R * kRowsStride;
+    float * sl = sm + kWaves * R;
+    int * srow = reinterpret_cast<int *>(sl + kWaves * R);
+    int * slim = srow + R;
+    const int base = wave * R;
+    if (!PACK || c16 < 8) {
+        float * to = so + (base + c16) * kRowsStride + g4 * 32;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                *reinterpret_cast<f4 *>(to + i * 8 + h * 4) = f4{O[4 * h][i], O[4 * h + 1][i], O[4 * h + 2][i], O[4 * h + 3][i]};
+            }
+        }
+        if (g4 == 0) {
+            sm[base + c16] = mc;
+            sl[base + c16] = l;
+            if (wave == 0) {
+                srow[c16] = orow;
+                slim[c16] = lim;
+            }
+        }
+    }
+    for (uint32_t left = redo; left != 0; left &= left - 1) {
+        const int cc = __ffs(left) - 1;
+        const int row = __builtin_amdgcn_readlane(orow, cc), lm = __builtin_amdgcn_readlane(lim, cc);
+        float cm, cl;
+        f2 co;
+        column_by_keys<CT, KS, TREE>(p, t.table, head, row, lm, t.past, t.step_lo + wave, t.step_hi, kWaves, lane, cm, cl, co);
+        // after this wave's own stores above: one wave's LDS accesses stay in order
+        __builtin_amdgcn_wave_barrier();
+        *reinterpret_cast<f2 *>(so + (base + cc) * kRowsStride + 2 * lane) = co;
+        if (lane == 0) {
+            sm[base + cc] = cm;
+            sl[base + cc] = cl;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int idx = threadIdx.x; idx < R * (kHeadDim / 4); idx += kThreads) {
+        const int cc = idx / (kHeadDim / 4), dim = (idx % (kHeadDim / 4)) * 4;
+        const int row = srow[cc];
+        if (row < 0) continue;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, sm[w * R + cc]);
+        float ls = 0.0f;
+        f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float mw = sm[w * R + cc];
+            const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
+            ls += sl[w * R + cc] * f;
+            o += *reinterpret_cast<const f4 *>(so + (w * R + cc) * kRowsStride + dim) * f;
+        }
+        store_column<TREE>(p, t, row, slim[cc], dim, o, M, ls, dim == 0);
+    }
 }
 
 template <typename CT, bool FEW, bool TREE>
@@ -629,7 +719,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
     } else {
         c[0] = p.scale * kLog2e;
     }
-    const int lim[NB] = {col.lim}, orow[NB] = {col.row};
+    const int lim[NB] = {col.lim}, orow[NB] = {col.row}, mask[NB] = {col.mask};
     // steps that every column sees whole
     const int full = TREE ? max(0, min(t.past, t.cap)) / KS : max(0, min(t.past + t.col0 / p.group, t.cap - 1) + 1) / KS;
     int top = kNoTop;
@@ -671,7 +761,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) S[0][kb] *= key_scale[kb];
         }
-        if (st >= full || holes != 0) mask_step<NB, KB, TREE>(p, S, lim, orow, t.past, st * KS, g4, holes);
+        if (st >= full || holes != 0) mask_step<NB, KB, TREE>(p, S, lim, mask, t.past, st * KS, g4, holes);
         float pr[NB][KB][4];
         softmax_step<NB, KB>(S, c, m, l, O, pr);
 
@@ -686,20 +776,16 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
             }
         }
         if constexpr (F16) {
-            u4 vt[8];
-            if constexpr (Q8) {
-                weigh_step<NB>(vs, top, pr, O);
-                v_operands(rv8, vt);
-            } else {
-#pragma unroll
-                for (int db = 0; db < 8; ++db) vt[db] = transposed(rv, db);
-            }
+            if constexpr (Q8) weigh_step<NB>(vs, top, pr, O);
             h8 ph, pl;
             split_p(pr[0], ph, pl);
             if constexpr (PACK) ph = c16 < 8 ? ph : pl;
+            u4 vt[2];
 #pragma unroll
             for (int db = 0; db < 8; ++db) {
-                const h8 a = __builtin_bit_cast(h8, vt[db]);
+                if constexpr (!Q8) vt[db & 1] = transposed(rv, db);
+                else if (!(db & 1)) v_operands(rv8, db >> 2, (db >> 1) & 1, vt[0], vt[1]);
+                const h8 a = __builtin_bit_cast(h8, vt[db & 1]);
                 O[0][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, O[0][db], 0, 0, 0);
                 if constexpr (!PACK) O[0][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, O[0][db], 0, 0, 0);
             }
@@ -729,64 +815,215 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
         }
     }
     close_columns<NB, PACK>(orow, c, m, l, O, mc, redo);
-    // merge over the waves
-    float * so = reinterpret_cast<float *>(lds);
-    float * sm = so + kWaves * R * kRowsStride;
-    float * sl = sm + kWaves * R;
-    int * srow = reinterpret_cast<int *>(sl + kWaves * R);
-    int * slim = srow + R;
-    const int base = wave * R;
-    if (!PACK || c16 < 8) {
-        float * to = so + (base + c16) * kRowsStride + g4 * 32;
+    merge_waves<CT, R, PACK, TREE>(p, t, head, lds, wave, lane, col.row, col.lim, mc[0], l[0], O[0], redo[0]);
+}
+
+// 16 NB columns whose keys the 4 waves take in turn, as in attn_rows, but with their q in LDS, where the waves read the operands of
+// each step: a wave's registers hold the accumulators, and one read of K and V from memory serves all columns, with no barrier
+// between the steps.
+constexpr int kWideBlocks = 2;
+constexpr size_t wide_q(int nb) { return nb * 8 * kWave * 16; }       // two parts of 4 operands per 16 columns
+constexpr size_t wide_lds(int nb) { return std::max(wide_q(nb) + nb * 16 * 4, rows_lds(true, false)); }
+
+template <typename CT, int NB, bool TREE>
+__device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
+    constexpr bool Q8 = is_q8<CT>;
+    constexpr int KS = step_keys(true), KB = KS / 16;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c16 = lane & 15, g4 = lane >> 4;
+    Tile t;
+    int head;
+    if (!find_tile<16 * NB, KS, false, TREE>(p, block, lane, t, head)) return;   // uniform for the workgroup
+
+    const HeadRows<CT> rows(p.pages, p.layer, p.n_kv, p.n_pages, p.page_shift, head);
+    const int in_page = (1 << p.page_shift) - 1, last_entry = p.seqs.table_stride - 1;
+    auto entries_of = [&](int st, int (&out)[KB]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int kb = 0; kb < KB; ++kb) out[kb] = t.table[min((st * KS + kb * 16) >> p.page_shift, last_entry)];
+    };
+    u4 rk[Q8 ? 4 : 8], rv[Q8 ? 1 : 8];
+    u2 rv8[8];
+    f4 ks[KB], vs[KB];
+    int pg[KB], pg_next[KB], entry[KB];
+    const CT * at[KB];
+    const float * scales[KB];
+    // a block on no page reads page 0, which there always is, and is masked
+    auto place = [&](int st) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                *reinterpret_cast<f4 *>(to + i * 8 + h * 4) = f4{O[0][4 * h][i], O[0][4 * h + 1][i], O[0][4 * h + 2][i], O[0][4 * h + 3][i]};
-            }
+        for (int kb = 0; kb < KB; ++kb) {
+            pg_next[kb] = entry_page(p, t, entry[kb], st * KS + kb * 16);
+            at[kb] = rows.page(max(pg_next[kb], 0)) + ((st * KS + kb * 16) & in_page) * kHeadDim;
+            if constexpr (Q8) scales[kb] = rows.scale(max(pg_next[kb], 0)) + ((st * KS + kb * 16) & in_page) + g4 * 4;
         }
-        if (g4 == 0) {
-            sm[base + c16] = mc[0];
-            sl[base + c16] = l[0];
-            if (wave == 0) {
-                srow[c16] = col.row;
-                slim[c16] = col.lim;
-            }
+    };
+    auto load_k = [&]() {
+        if constexpr (Q8) {
+#pragma unroll
+            for (int f = 0; f < 4; ++f) rk[f] = *reinterpret_cast<const u4 *>(at[f >> 1] + c16 * kHeadDim + (f & 1) * 64 + g4 * 16);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) ks[kb] = *reinterpret_cast<const f4 *>(scales[kb]);
+        } else {
+#pragma unroll
+            for (int f = 0; f < 8; ++f) rk[f] = *reinterpret_cast<const u4 *>(at[f >> 2] + k_offset<true>(f, c16, g4));
         }
+    };
+    auto load_v = [&]() {
+        if constexpr (Q8) {
+#pragma unroll
+            for (int f = 0; f < 8; ++f) rv8[f] = *reinterpret_cast<const u2 *>(at[f >> 2] + rows.v_elems + v_offset<true>(f, c16, g4));
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) vs[kb] = *reinterpret_cast<const f4 *>(scales[kb] + rows.v_elems / 4);
+        } else {
+#pragma unroll
+            for (int f = 0; f < 8; ++f) rv[f] = *reinterpret_cast<const u4 *>(at[f >> 2] + rows.v_elems + v_offset<true>(f, c16, g4));
+        }
+    };
+    int st = t.step_lo + wave;
+    if (st < t.step_hi) {
+        entries_of(st, entry);
+        place(st);
+        load_k();
+        load_v();
+        entries_of(st + kWaves, entry);
     }
-    for (uint32_t left = redo[0]; left != 0; left &= left - 1) {
-        const int cc = __ffs(left) - 1;
-        const int row = __builtin_amdgcn_readlane(col.row, cc), lm = __builtin_amdgcn_readlane(col.lim, cc);
-        float cm, cl;
-        f2 co;
-        column_by_keys<CT, KS, TREE>(p, t.table, head, row, lm, t.past, t.step_lo + wave, t.step_hi, kWaves, lane, cm, cl, co);
-        // after this wave's own stores above: one wave's LDS accesses stay in order
-        __builtin_amdgcn_wave_barrier();
-        *reinterpret_cast<f2 *>(so + (base + cc) * kRowsStride + 2 * lane) = co;
-        if (lane == 0) {
-            sm[base + cc] = cm;
-            sl[base + cc] = cl;
+
+    int lim[NB], orow[NB], mask[NB];
+    float c[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const Column col = column_of<TREE>(p, t, head, t.col0 + nb * 16 + c16);
+        lim[nb] = col.lim;
+        orow[nb] = col.row;
+        mask[nb] = col.mask;
+        if (wave == nb % kWaves) {                                        // a block's q by one wave
+            f4 x[8];
+            h8 qh[4], ql[4];
+            float unit;
+            load_q<CT>(col, g4, x);
+            split_q(x, p.scale, unit, qh, ql);
+            char * to = lds + nb * 8 * kWave * 16 + lane * 16;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                *reinterpret_cast<h8 *>(to + ks * kWave * 16) = qh[ks];
+                *reinterpret_cast<h8 *>(to + (4 + ks) * kWave * 16) = ql[ks];
+            }
+            if (g4 == 0) *reinterpret_cast<float *>(lds + wide_q(NB) + (nb * 16 + c16) * 4) = unit;
         }
     }
     __syncthreads();
 #pragma unroll
-    for (int idx = threadIdx.x; idx < R * (kHeadDim / 4); idx += kThreads) {
-        const int cc = idx / (kHeadDim / 4), dim = (idx % (kHeadDim / 4)) * 4;
-        const int row = srow[cc];
-        if (row < 0) continue;
-        float M = -INFINITY;
+    for (int nb = 0; nb < NB; ++nb) c[nb] = *reinterpret_cast<const float *>(lds + wide_q(NB) + (nb * 16 + c16) * 4);
+    // steps that every column sees whole
+    const int full = TREE ? max(0, min(t.past, t.cap)) / KS : max(0, min(t.past + t.col0 / p.group, t.cap - 1) + 1) / KS;
+    int top = kNoTop;
+    float m[NB], l[NB];
+    f4 O[NB][8];
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, sm[w * R + cc]);
-        float ls = 0.0f;
-        f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int nb = 0; nb < NB; ++nb) {
+        m[nb] = -INFINITY;
+        l[nb] = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float mw = sm[w * R + cc];
-            const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
-            ls += sl[w * R + cc] * f;
-            o += *reinterpret_cast<const f4 *>(so + (w * R + cc) * kRowsStride + dim) * f;
+        for (int db = 0; db < 8; ++db) O[nb][db] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    for (; st < t.step_hi; st += kWaves) {
+        int holes = 0;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            pg[kb] = pg_next[kb];
+            holes |= pg[kb] < 0 ? 1 << kb : 0;
         }
-        store_column<TREE>(p, t, row, slim[cc], dim, o, M, ls, dim == 0);
+        const bool more = st + kWaves < t.step_hi;
+        f4 S[NB][KB], key_scale[KB];
+        {
+            u4 a[8];
+            if constexpr (Q8) {
+                k_operands(rk, a);
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) key_scale[kb] = ks[kb];
+            } else {
+#pragma unroll
+                for (int f = 0; f < 8; ++f) a[f] = rk[f];
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                __builtin_amdgcn_sched_barrier(0);                        // q of one block of columns at a time in registers
+                const char * from = lds + nb * 8 * kWave * 16 + lane * 16;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) S[nb][kb] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int f = 0; f < 8; ++f) {
+                    const h8 q = *reinterpret_cast<const h8 *>(from + f * kWave * 16);
+#pragma unroll
+                    for (int kb = 0; kb < KB; ++kb) {
+                        S[nb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a[kb * 4 + (f & 3)]), q, S[nb][kb], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        if (more) {
+            place(st + kWaves);
+            load_k();
+        }
+        if constexpr (Q8) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) S[nb][kb] *= key_scale[kb];
+            }
+        }
+        if (st >= full || holes != 0) mask_step<NB, KB, TREE>(p, S, lim, mask, t.past, st * KS, g4, holes);
+        float pr[NB][KB][4];
+        softmax_step<NB, KB>(S, c, m, l, O, pr);
+
+        // rows of keys that no column sees, and of no page, are whatever memory holds: not even 0 times that
+        if (st * KS + KS > t.kend || holes != 0) {
+#pragma unroll
+            for (int f = 0; f < 8; ++f) {
+                if (st * KS + v_key<true>(f, g4) >= t.kend || pg[f >> 2] < 0) {
+                    if constexpr (Q8) vs[f >> 2][f & 3] = 0.0f;
+                    else rv[f] = u4{0, 0, 0, 0};
+                }
+            }
+        }
+        if constexpr (Q8) weigh_step<NB>(vs, top, pr, O);
+        h8 ph[NB], pl[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) split_p(pr[nb], ph[nb], pl[nb]);
+        u4 vt[2];
+#pragma unroll
+        for (int db = 0; db < 8; ++db) {
+            if constexpr (!Q8) vt[db & 1] = transposed(rv, db);
+            else if (!(db & 1)) v_operands(rv8, db >> 2, (db >> 1) & 1, vt[0], vt[1]);
+            const h8 a = __builtin_bit_cast(h8, vt[db & 1]);
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) O[nb][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, part ? pl[nb] : ph[nb], O[nb][db], 0, 0, 0);
+            }
+        }
+        if (more) {
+            load_v();
+            entries_of(st + 2 * kWaves, entry);
+        }
+    }
+    float mc[NB];
+    uint32_t redo[NB];
+    if constexpr (Q8) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) O[nb][db][i] = ldexpf(O[nb][db][i], top);
+            }
+        }
+    }
+    close_columns<NB, false>(orow, c, m, l, O, mc, redo);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        __syncthreads();                                                  // q and the block before are no longer read
+        merge_waves<CT, 16, false, TREE>(p, t, head, lds, wave, lane, orow[nb], lim[nb], mc[nb], l[nb], O[nb], redo[nb]);
     }
 }
 
@@ -806,25 +1043,24 @@ constexpr size_t kTileLds = 2 * kTileSteps * kStepBytes;
 constexpr int kOutStride = kHeadDim + 4, kOutFloats = 16 * kOutStride;   // a wave's 16 columns on their way out
 static_assert(kWaves * kOutFloats * sizeof(float) <= kTileLds, "the outputs go through the operands' LDS");
 
-template <typename CT, bool TREE>
 __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
-    constexpr bool F16 = true, Q8 = is_q8<CT>;
+    typedef _Float16 CT;
+    constexpr bool F16 = true;
     constexpr int KS = step_keys(F16), KB = KS / 16, NB = 2;
-    __shared__ __attribute__((aligned(16))) float s_scale[Q8 ? 2 : 1][Q8 ? kTileSteps : 1][2][KS];   // of K and V
     __shared__ int s_holes[2][kTileSteps];                            // bit kb: 16-key block kb of the step lies on no page
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g4 = lane >> 4;
     Tile t;
     int head;
-    if (!find_tile<kTileCols, KS, false, TREE>(p, block, lane, t, head)) return;   // uniform for the workgroup
+    if (!find_tile<kTileCols, KS, false, false>(p, block, lane, t, head)) return;   // uniform for the workgroup
 
     // columns: their q is on its way while the first tile is fetched
     int lim[NB], orow[NB];
     f4 x[NB][8];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-        const Column col = column_of<TREE>(p, t, head, t.col0 + wave * 16 * NB + nb * 16 + c16);
+        const Column col = column_of<false>(p, t, head, t.col0 + wave * 16 * NB + nb * 16 + c16);
         lim[nb] = col.lim;
         orow[nb] = col.row;
         load_q<CT>(col, g4, x[nb]);
@@ -833,8 +1069,8 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
     const int first_col = t.col0 + wave * 16 * NB;
     int wave_steps = 0, full = 0;                                     // steps behind the first hold nothing that the wave sees
     if (first_col < t.n_cols) {
-        wave_steps = TREE ? t.step_hi : min(t.step_hi, (min(t.past + (min(first_col + 16 * NB, t.n_cols) - 1) / p.group, t.cap - 1) + KS) / KS);
-        full = TREE ? max(0, min(t.past, t.cap)) / KS : max(0, min(t.past + first_col / p.group, t.cap - 1) + 1) / KS;
+        wave_steps = min(t.step_hi, (min(t.past + (min(first_col + 16 * NB, t.n_cols) - 1) / p.group, t.cap - 1) + KS) / KS);
+        full = max(0, min(t.past + first_col / p.group, t.cap - 1) + 1) / KS;
     }
 
     // this wave's share of a tile: K or V of step `mine`
@@ -843,8 +1079,6 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
     const HeadRows<CT> rows(p.pages, p.layer, p.n_kv, p.n_pages, p.page_shift, head);
     const int in_page = (1 << p.page_shift) - 1, last_entry = p.seqs.table_stride - 1;
     u4 r[8];
-    u2 r8[8];
-    float r_scale = 0.0f;                                             // lane < KS: its key's
     int pg[KB], entry[KB], st_held = 0;
     auto entries_of = [&](int st) {
 #pragma unroll
@@ -858,41 +1092,14 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
             pg[kb] = entry_page(p, t, entry[kb], st * KS + kb * 16);
             at[kb] = rows.page(max(pg[kb], 0)) + ((st * KS + kb * 16) & in_page) * kHeadDim + (fetch_v ? rows.v_elems : 0);
         }
-        if constexpr (Q8) {
-            const int kb = (lane >> 4) & 1;
-            const float * scales = rows.scale(max(pg[kb], 0)) + ((st * KS + kb * 16) & in_page) + (fetch_v ? rows.v_elems / 4 : 0);
-            r_scale = scales[c16];
-            if (fetch_v) {
 #pragma unroll
-                for (int f = 0; f < 8; ++f) r8[f] = *reinterpret_cast<const u2 *>(at[f >> 2] + v_offset<F16>(f, c16, g4));
-            } else {
-#pragma unroll
-                for (int f = 0; f < 4; ++f) r[f] = *reinterpret_cast<const u4 *>(at[f >> 1] + c16 * kHeadDim + (f & 1) * 64 + g4 * 16);
-            }
-        } else {
-#pragma unroll
-            for (int f = 0; f < 8; ++f) {
-                r[f] = *reinterpret_cast<const u4 *>(at[f >> 2] + (fetch_v ? v_offset<F16>(f, c16, g4) : k_offset<F16>(f, c16, g4)));
-            }
+        for (int f = 0; f < 8; ++f) {
+            r[f] = *reinterpret_cast<const u4 *>(at[f >> 2] + (fetch_v ? v_offset<F16>(f, c16, g4) : k_offset<F16>(f, c16, g4)));
         }
     };
     auto put = [&](int buf) {
         char * to = lds + (buf * kTileSteps + mine) * kStepBytes + lane * 16;
-        if constexpr (Q8) {
-            u4 a[8];
-            if (fetch_v) {
-                v_operands(r8, a);
-                // rows that no column sees, and of no page: not even 0 times what memory holds
-                if (st_held * KS + lane >= t.kend || pg[(lane >> 4) & 1] < 0) r_scale = 0.0f;
-            } else {
-                const u4 raw[4] = {r[0], r[1], r[2], r[3]};
-                k_operands(raw, a);
-                if (lane == 0) s_holes[buf][mine] = (pg[0] < 0 ? 1 : 0) | (pg[1] < 0 ? 2 : 0);
-            }
-            if (lane < KS) s_scale[buf][mine][fetch_v ? 1 : 0][lane] = r_scale;
-#pragma unroll
-            for (int f = 0; f < 8; ++f) *reinterpret_cast<u4 *>(to + (fetch_v ? 8 + f : f) * kWave * 16) = a[f];
-        } else if (fetch_v) {
+        if (fetch_v) {
             bool hole = st_held * KS + KS > t.kend;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) hole = hole || pg[kb] < 0;
@@ -923,7 +1130,6 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
     for (int nb = 0; nb < NB; ++nb) {
         split_q(x[nb], p.scale, c[nb], qh[nb], ql[nb]);
     }
-    int top = kNoTop;
     float m[NB], l[NB];
     f4 O[NB][8];
 #pragma unroll
@@ -955,23 +1161,9 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
 #pragma unroll
             for (int f = 0; f < 8; ++f) v[f] = *reinterpret_cast<const u4 *>(op + (8 + f) * kWave * 16);
             const int holes = __builtin_amdgcn_readfirstlane(s_holes[tile & 1][s]);
-            if constexpr (Q8) {
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    const f4 ks = *reinterpret_cast<const f4 *>(&s_scale[tile & 1][s][0][kb * 16 + g4 * 4]);
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) S[nb][kb] *= ks;
-                }
-            }
-            if (st >= full || holes != 0) mask_step<NB, KB, TREE>(p, S, lim, orow, t.past, st * KS, g4, holes);
+            if (st >= full || holes != 0) mask_step<NB, KB, false>(p, S, lim, lim, t.past, st * KS, g4, holes);
             float pr[NB][KB][4];
             softmax_step<NB, KB>(S, c, m, l, O, pr);
-            if constexpr (Q8) {
-                f4 vs[KB];
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) vs[kb] = *reinterpret_cast<const f4 *>(&s_scale[tile & 1][s][1][kb * 16 + g4 * 4]);
-                weigh_step<NB>(vs, top, pr, O);
-            }
             h8 ph[NB], pl[NB];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) split_p(pr[nb], ph[nb], pl[nb]);
@@ -997,16 +1189,6 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
     }
     float mc[NB];
     uint32_t redo[NB];
-    if constexpr (Q8) {
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-            for (int db = 0; db < 8; ++db) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) O[nb][db][i] = ldexpf(O[nb][db][i], top);
-            }
-        }
-    }
     close_columns<NB, false>(orow, c, m, l, O, mc, redo);
     // through the wave's own part of LDS, so that a store instruction writes two whole rows; a lane's values would lie 16 bytes
     // in each of 64 lines
@@ -1028,9 +1210,9 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
             const int row = __shfl(orow[nb], col, kWave), lm = __shfl(lim[nb], col, kWave);
             const float cm = __shfl(mc[nb], col, kWave), cl = __shfl(l[nb], col, kWave);
             const f4 v = *reinterpret_cast<const f4 *>(so + col * kOutStride + dim);
-            if (row >= 0 && !((redo[nb] >> col) & 1)) store_column<TREE>(p, t, row, lm, dim, v, cm, cl, dim == 0);
+            if (row >= 0 && !((redo[nb] >> col) & 1)) store_column<false>(p, t, row, lm, dim, v, cm, cl, dim == 0);
         }
-        redo_columns<CT, KS, TREE>(p, t, head, lane, lim[nb], orow[nb], redo[nb]);
+        redo_columns<CT, KS>(p, t, head, lane, lim[nb], orow[nb], redo[nb]);
     }
 }
 
@@ -1049,20 +1231,27 @@ __global__ __launch_bounds__(kThreads, 3) void paged_rows_both_kernel(AttnParams
     else attn_rows<CT, true, TREE>(p, block - many, lds_rows);
 }
 
-template <typename CT, bool BOTH, bool TREE>
+template <typename CT, int NB, bool BOTH, bool TREE>
+__global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void paged_wide_kernel(AttnParams p) {
+    extern __shared__ __attribute__((aligned(16))) char lds_wide[];
+    const int many = p.tiles_many * p.n_kv * p.splits_many, block = blockIdx.x;
+    if (!BOTH || block < many) attn_wide<CT, NB, TREE>(p, block, lds_wide);
+    else attn_rows<CT, true, TREE>(p, block - many, lds_wide);
+}
+
+template <bool BOTH>
 __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_tile[];
     const int many = p.tiles_many * p.n_kv * p.splits_many, block = blockIdx.x;
-    if (!BOTH || block < many) attn_tile<CT, TREE>(p, block, lds_tile);
-    else attn_rows<CT, true, TREE>(p, block - many, lds_tile);
+    if (!BOTH || block < many) attn_tile(p, block, lds_tile);
+    else attn_rows<_Float16, true, false>(p, block - many, lds_tile);
 }
 
 // Joins the splits of each (row, head): one wave each, lane = split for the weights, then lane = 2 dims.  Its time is
 // dependent loads, so the sequences, the weights and the first results are read together; a split that the row does not
 // reach holds whatever the workspace held, and is selected away.
-template <bool TREE>
+template <bool TREE, int kFirst>
 __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int ks) {
-    constexpr int kFirst = 8;
     const int lane = threadIdx.x & (kWave - 1);
     const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (item >= static_cast<int64_t>(p.seqs.n_rows) * p.n_heads) return;
@@ -1106,6 +1295,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int ks) {
 // How a call cuts its work: which kinds of tiles there are, their upper bounds, and the key ranges of each kind.
 struct AttnPlan {
     bool tile;               // the longer sequences' tiles are attn_tile's
+    int wide;                // 16-column blocks of those that are attn_wide's, 0: none are
     int tiles_many, tiles_few;
     int few_max;             // 0: sequences of few columns are the longer ones' tiles, too
     int splits_many, splits_few, steps_many, steps_few;
@@ -1122,7 +1312,7 @@ void cut_keys(int steps, int64_t blocks, int64_t target, int64_t least, int64_t 
     splits = std::max(1, (steps + split_steps - 1) / split_steps);
 }
 
-AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_heads, size_t workspace_bytes) {
+AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_heads, size_t workspace_bytes, bool tree) {
     const bool f16 = l.cache_type != QA_CACHE_F32;                    // products
     const int ks = step_keys(f16);
     const int group = n_heads / l.n_kv_heads;
@@ -1139,10 +1329,15 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     // attn_tile (f16 pages) against attn_rows, us.  256 tokens behind 3000 positions 37 / 39, 400 behind 2000 38 / 46, 700 behind
     // 1500 46 / 58, 1024 behind 500 45.5 / 47, behind 2889 80 / 129; but 512 behind 1000 34 / 31, 1024 behind none 38 / 31,
     // eight of 100 tokens behind 2000 (columns left empty) 65 / 53: by the products, where a sequence fills three tiles.
-    pl.tile = f16 && most > 2 * kTileCols && cols * (len - std::min(len, tokens / 2)) > 1600000;
-    const int width = pl.tile ? kTileCols : 16;
+    const bool wide = f16 && (tree || l.cache_type == QA_CACHE_Q8) && most > 16;
+    pl.tile = f16 && !tree && l.cache_type != QA_CACHE_Q8 && most > 2 * kTileCols && cols * (len - std::min(len, tokens / 2)) > 1600000;
+    pl.wide = !wide ? 0 : cols * len >= 1000000 ? kWideBlocks : 1;
+    const int width = pl.tile ? kTileCols : pl.wide ? 16 * pl.wide : 16;
     pl.tiles_many = many ? static_cast<int>(cols / width + seqs) : 0;
-    const bool few = !many || b.n_seqs > 1;                           // one sequence is of one kind
+    // one sequence is of one kind; of several at most so many are of few columns, by the host's counts
+    const int64_t few_tokens = few_cols(f16) / group;
+    const int64_t few_seqs = tokens > few_tokens ? (seqs * tokens - b.n_rows) / (tokens - few_tokens) : seqs;
+    const bool few = !many || (b.n_seqs > 1 && (!wide || 4 * few_seqs >= 3 * seqs));
     pl.few_max = few ? few_cols(f16) : 0;
     pl.tiles_few = few ? seqs : 0;
     // Workgroups to make of the keys, us.  Decode steps, and sequences of one tile: K and V are what they read, and more, shorter
@@ -1157,7 +1352,8 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     const bool one = b.n_seqs == 1;
     // one round of workgroups where their ranges stay short: four sequences of 501 to 3001 in 8 / 12 ranges 13.3 / 16.2 us, f32 pages 18.3 / 23.6
     const int64_t round = std::max<int64_t>(1, 256 / heads), decode = (steps + round - 1) / round <= 24 ? 256 : 1024;
-    if (pl.tile) cut_keys(steps, tiles, one ? 512 : 768, 4, parts, pl.splits_many, pl.steps_many);
+    if (pl.wide) cut_keys(steps, tiles, 512, 16, parts, pl.splits_many, pl.steps_many);
+    else if (pl.tile) cut_keys(steps, tiles, one ? 512 : 768, 4, parts, pl.splits_many, pl.steps_many);
     else if (most <= 16) cut_keys(steps, heads, decode, 8, parts, pl.splits_many, pl.steps_many);
     else cut_keys(steps, tiles, !one ? 640 : steps >= 128 && tiles > 192 ? 1024 : 384, 16, parts, pl.splits_many, pl.steps_many);
     cut_keys(steps, heads, decode, 8, parts, pl.splits_few, pl.steps_few);
@@ -1166,28 +1362,39 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     return pl;
 }
 
+template <bool TREE>
+void launch_join(const AttnParams & p, bool f16, hipStream_t stream) {
+    const int64_t items = static_cast<int64_t>(p.seqs.n_rows) * p.n_heads;
+    const auto kernel = p.n_parts <= 2 ? &paged_join_kernel<TREE, 2> : &paged_join_kernel<TREE, 8>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, p, step_keys(f16));
+}
+
+// The longer sequences' kernel, or both kinds' in one launch.
 template <typename CT, bool TREE>
 int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
     constexpr bool F16 = f16_products<CT>;
     const dim3 grid(static_cast<unsigned>(p.n_kv) * (pl.tiles_many * pl.splits_many + pl.tiles_few * pl.splits_few));
     constexpr size_t lds_few = rows_lds(F16, true), lds_many = rows_lds(F16, false);
-    static_assert(lds_few <= kTileLds && lds_few <= lds_many, "a launch of both kinds has the longer ones' LDS");
-    if (F16 && pl.tile) {
-        typedef typename std::conditional<F16, CT, _Float16>::type TT;   // f32 pages have no such kernel
-        const auto kernel = pl.few_max ? &paged_tile_kernel<TT, true, TREE> : &paged_tile_kernel<TT, false, TREE>;
-        QA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kTileLds)));
-        hipLaunchKernelGGL(kernel, grid, dim3(kThreads), kTileLds, stream, p);
-    } else if (!pl.tiles_many) {
-        hipLaunchKernelGGL((paged_rows_kernel<CT, true, TREE>), grid, dim3(kThreads), lds_few, stream, p);
-    } else if (pl.few_max) {
-        hipLaunchKernelGGL((paged_rows_both_kernel<CT, TREE>), grid, dim3(kThreads), lds_many, stream, p);
-    } else {
-        hipLaunchKernelGGL((paged_rows_kernel<CT, false, TREE>), grid, dim3(kThreads), lds_many, stream, p);
+    static_assert(lds_few <= kTileLds && lds_few <= lds_many && lds_many <= wide_lds(1), "a launch of both kinds has the longer ones' LDS");
+    auto kernel = !pl.tiles_many ? &paged_rows_kernel<CT, true, TREE> : pl.few_max ? &paged_rows_both_kernel<CT, TREE> : &paged_rows_kernel<CT, false, TREE>;
+    size_t lds = !pl.tiles_many ? lds_few : lds_many;
+    if constexpr (std::is_same<CT, _Float16>::value && !TREE) {
+        if (pl.tile) {
+            kernel = pl.few_max ? &paged_tile_kernel<true> : &paged_tile_kernel<false>;
+            lds = kTileLds;
+            QA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kTileLds)));
+        }
+    } else if constexpr (F16) {
+        if (pl.wide) {
+            kernel = pl.wide == 1 ? (pl.few_max ? &paged_wide_kernel<CT, 1, true, TREE> : &paged_wide_kernel<CT, 1, false, TREE>)
+                                  : (pl.few_max ? &paged_wide_kernel<CT, kWideBlocks, true, TREE> : &paged_wide_kernel<CT, kWideBlocks, false, TREE>);
+            lds = wide_lds(pl.wide);
+        }
     }
+    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), lds, stream, p);
     QA_LAUNCH_CHECK("paged attention kernel");
     if (pl.parts() > 1) {
-        const int64_t items = static_cast<int64_t>(p.seqs.n_rows) * p.n_heads;
-        hipLaunchKernelGGL(paged_join_kernel<TREE>, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, p, step_keys(F16));
+        launch_join<TREE>(p, F16, stream);
         QA_LAUNCH_CHECK("paged_join_kernel");
     }
     return QA_OK;
@@ -1215,7 +1422,7 @@ int attention(const float * q, const void * pages, const qa_kv_layout * layout, 
     }
     if (static_cast<int64_t>(batch->n_rows) * n_heads > INT32_MAX / 2) return fail(QA_ERR_INVALID, who + ": too many rows");
     if (const int rc = check_stream(stream, name); rc != QA_OK) return rc;
-    const AttnPlan pl = attn_plan(*layout, *batch, n_heads, workspace_bytes);
+    const AttnPlan pl = attn_plan(*layout, *batch, n_heads, workspace_bytes, mask != nullptr);
     if ((static_cast<int64_t>(pl.tiles_many) * pl.splits_many + static_cast<int64_t>(pl.tiles_few) * pl.splits_few) * layout->n_kv_heads > INT32_MAX / kThreads) {
         return fail(QA_ERR_INVALID, who + ": too many rows");
     }
@@ -1253,9 +1460,10 @@ int attention(const float * q, const void * pages, const qa_kv_layout * layout, 
 extern "C" size_t qa_paged_attn_workspace_bytes(const qa_kv_layout * layout, const qa_paged_batch * batch, int32_t n_heads) {
     using namespace qa;
     if (check_batch_sizes(layout, 0, batch, n_heads, "qa_paged_attn_workspace_bytes") != QA_OK || batch->n_rows == 0) return 0;
-    const AttnPlan pl = attn_plan(*layout, *batch, n_heads, SIZE_MAX);
-    if (pl.parts() <= 1) return 0;
-    return static_cast<size_t>(batch->n_rows) * n_heads * pl.parts() * (kHeadDim + 2) * sizeof(float);
+    // causal or a tree: enough for either
+    const int parts = std::max(attn_plan(*layout, *batch, n_heads, SIZE_MAX, false).parts(), attn_plan(*layout, *batch, n_heads, SIZE_MAX, true).parts());
+    if (parts <= 1) return 0;
+    return static_cast<size_t>(batch->n_rows) * n_heads * parts * (kHeadDim + 2) * sizeof(float);
 }
 
 extern "C" int qa_paged_attn(const float * q, const void * pages, const qa_kv_layout * layout, int32_t layer,
