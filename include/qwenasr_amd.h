@@ -245,7 +245,7 @@ int qa_paged_append(const float * qkv, const float * q_norm_w, const float * k_n
 
 /* The K and V rows of the batch's tokens read back from their pages, what qa_paged_append wrote for them (n_past 0 and as
  * many rows as a sequence has positions: the whole sequence, for a cache of another kind or for storage outside the GPU).
- * k_out, v_out: [n_rows][kv_dim] of out_type (QA_CACHE_F32 or QA_CACHE_F16, rounded to nearest); either may be NULL.  Rows
+ * k_out, v_out: [n_rows][kv_dim] of out_type (QA_CACHE_F32, or QA_CACHE_F16: the f32 values rounded to nearest); either may be NULL.  Rows
  * on no page are zeros, rows of no sequence are left as they were.  pages, k_out and v_out aligned to 16 bytes.  */
 int qa_paged_read(const void * pages, const qa_kv_layout * layout, int32_t layer, const qa_paged_batch * batch, void * k_out,
                   void * v_out, int32_t out_type, void * stream);

@@ -822,19 +822,20 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
 // each step: a wave's registers hold the accumulators, and one read of K and V from memory serves all columns, with no barrier
 // between the steps.
 constexpr int kWideBlocks = 2;
-constexpr size_t wide_q(int nb) { return nb * 8 * kWave * 16; }       // two parts of 4 operands per 16 columns
-constexpr size_t wide_lds(int nb) { return std::max(wide_q(nb) + nb * 16 * 4, rows_lds(true, false)); }
+constexpr int kWideCols = 16 * kWideBlocks;
+constexpr size_t kWideQ = kWideBlocks * 8 * kWave * 16;               // two parts of 4 operands per 16 columns
+constexpr size_t kWideLds = std::max(kWideQ + kWideCols * 4, rows_lds(true, false));
 
-template <typename CT, int NB, bool TREE>
+template <typename CT, bool TREE>
 __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
     constexpr bool Q8 = is_q8<CT>;
-    constexpr int KS = step_keys(true), KB = KS / 16;
+    constexpr int KS = step_keys(true), KB = KS / 16, NB = kWideBlocks;
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c16 = lane & 15, g4 = lane >> 4;
     Tile t;
     int head;
-    if (!find_tile<16 * NB, KS, false, TREE>(p, block, lane, t, head)) return;   // uniform for the workgroup
+    if (!find_tile<kWideCols, KS, false, TREE>(p, block, lane, t, head)) return;   // uniform for the workgroup
 
     const HeadRows<CT> rows(p.pages, p.layer, p.n_kv, p.n_pages, p.page_shift, head);
     const int in_page = (1 << p.page_shift) - 1, last_entry = p.seqs.table_stride - 1;
@@ -908,12 +909,12 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
                 *reinterpret_cast<h8 *>(to + ks * kWave * 16) = qh[ks];
                 *reinterpret_cast<h8 *>(to + (4 + ks) * kWave * 16) = ql[ks];
             }
-            if (g4 == 0) *reinterpret_cast<float *>(lds + wide_q(NB) + (nb * 16 + c16) * 4) = unit;
+            if (g4 == 0) *reinterpret_cast<float *>(lds + kWideQ + (nb * 16 + c16) * 4) = unit;
         }
     }
     __syncthreads();
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) c[nb] = *reinterpret_cast<const float *>(lds + wide_q(NB) + (nb * 16 + c16) * 4);
+    for (int nb = 0; nb < NB; ++nb) c[nb] = *reinterpret_cast<const float *>(lds + kWideQ + (nb * 16 + c16) * 4);
     // steps that every column sees whole
     const int full = TREE ? max(0, min(t.past, t.cap)) / KS : max(0, min(t.past + t.col0 / p.group, t.cap - 1) + 1) / KS;
     int top = kNoTop;
@@ -1231,11 +1232,11 @@ __global__ __launch_bounds__(kThreads, 3) void paged_rows_both_kernel(AttnParams
     else attn_rows<CT, true, TREE>(p, block - many, lds_rows);
 }
 
-template <typename CT, int NB, bool BOTH, bool TREE>
-__global__ __launch_bounds__(kThreads, NB == 1 ? 3 : 2) void paged_wide_kernel(AttnParams p) {
+template <typename CT, bool BOTH, bool TREE>
+__global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_wide[];
     const int many = p.tiles_many * p.n_kv * p.splits_many, block = blockIdx.x;
-    if (!BOTH || block < many) attn_wide<CT, NB, TREE>(p, block, lds_wide);
+    if (!BOTH || block < many) attn_wide<CT, TREE>(p, block, lds_wide);
     else attn_rows<CT, true, TREE>(p, block - many, lds_wide);
 }
 
@@ -1295,7 +1296,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int ks) {
 // How a call cuts its work: which kinds of tiles there are, their upper bounds, and the key ranges of each kind.
 struct AttnPlan {
     bool tile;               // the longer sequences' tiles are attn_tile's
-    int wide;                // 16-column blocks of those that are attn_wide's, 0: none are
+    bool wide;               // or attn_wide's
     int tiles_many, tiles_few;
     int few_max;             // 0: sequences of few columns are the longer ones' tiles, too
     int splits_many, splits_few, steps_many, steps_few;
@@ -1329,15 +1330,18 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     // attn_tile (f16 pages) against attn_rows, us.  256 tokens behind 3000 positions 37 / 39, 400 behind 2000 38 / 46, 700 behind
     // 1500 46 / 58, 1024 behind 500 45.5 / 47, behind 2889 80 / 129; but 512 behind 1000 34 / 31, 1024 behind none 38 / 31,
     // eight of 100 tokens behind 2000 (columns left empty) 65 / 53: by the products, where a sequence fills three tiles.
-    const bool wide = f16 && (tree || l.cache_type == QA_CACHE_Q8) && most > 16;
-    pl.tile = f16 && !tree && l.cache_type != QA_CACHE_Q8 && most > 2 * kTileCols && cols * (len - std::min(len, tokens / 2)) > 1600000;
-    pl.wide = !wide ? 0 : cols * len >= 1000000 ? kWideBlocks : 1;
-    const int width = pl.tile ? kTileCols : pl.wide ? 16 * pl.wide : 16;
+    const bool fresh = tree || l.cache_type == QA_CACHE_Q8;
+    pl.tile = f16 && !fresh && most > 2 * kTileCols && cols * (len - std::min(len, tokens / 2)) > 1600000;
+    // attn_wide against attn_rows (8 bits, or f16 pages and trees), us.  1024 tokens behind 2889 positions 78 / 102, behind none 23.5 / 31, four of
+    // 256 behind 500 to 1500 34 / 40, sixteen trees of 41 behind 156 to 3000 (f16) 49 / 58; but 64 behind 1000 16.0 / 12.6, two of 157
+    // behind 701 and 1037 24.1 / 21.7: by the products.
+    pl.wide = f16 && fresh && most > 16 && cols * len >= 1000000;
+    const int width = pl.tile ? kTileCols : pl.wide ? kWideCols : 16;
     pl.tiles_many = many ? static_cast<int>(cols / width + seqs) : 0;
     // one sequence is of one kind; of several at most so many are of few columns, by the host's counts
     const int64_t few_tokens = few_cols(f16) / group;
     const int64_t few_seqs = tokens > few_tokens ? (seqs * tokens - b.n_rows) / (tokens - few_tokens) : seqs;
-    const bool few = !many || (b.n_seqs > 1 && (!wide || 4 * few_seqs >= 3 * seqs));
+    const bool few = !many || (b.n_seqs > 1 && (!fresh || 4 * few_seqs >= 3 * seqs));
     pl.few_max = few ? few_cols(f16) : 0;
     pl.tiles_few = few ? seqs : 0;
     // Workgroups to make of the keys, us.  Decode steps, and sequences of one tile: K and V are what they read, and more, shorter
@@ -1352,7 +1356,7 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     const bool one = b.n_seqs == 1;
     // one round of workgroups where their ranges stay short: four sequences of 501 to 3001 in 8 / 12 ranges 13.3 / 16.2 us, f32 pages 18.3 / 23.6
     const int64_t round = std::max<int64_t>(1, 256 / heads), decode = (steps + round - 1) / round <= 24 ? 256 : 1024;
-    if (pl.wide) cut_keys(steps, tiles, 512, 16, parts, pl.splits_many, pl.steps_many);
+    if (fresh && most > 16) cut_keys(steps, tiles, one && !pl.wide ? 384 : 512, 16, parts, pl.splits_many, pl.steps_many);
     else if (pl.tile) cut_keys(steps, tiles, one ? 512 : 768, 4, parts, pl.splits_many, pl.steps_many);
     else if (most <= 16) cut_keys(steps, heads, decode, 8, parts, pl.splits_many, pl.steps_many);
     else cut_keys(steps, tiles, !one ? 640 : steps >= 128 && tiles > 192 ? 1024 : 384, 16, parts, pl.splits_many, pl.steps_many);
@@ -1375,7 +1379,7 @@ int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
     constexpr bool F16 = f16_products<CT>;
     const dim3 grid(static_cast<unsigned>(p.n_kv) * (pl.tiles_many * pl.splits_many + pl.tiles_few * pl.splits_few));
     constexpr size_t lds_few = rows_lds(F16, true), lds_many = rows_lds(F16, false);
-    static_assert(lds_few <= kTileLds && lds_few <= lds_many && lds_many <= wide_lds(1), "a launch of both kinds has the longer ones' LDS");
+    static_assert(lds_few <= kTileLds && lds_few <= lds_many && lds_few <= kWideLds, "a launch of both kinds has the longer ones' LDS");
     auto kernel = !pl.tiles_many ? &paged_rows_kernel<CT, true, TREE> : pl.few_max ? &paged_rows_both_kernel<CT, TREE> : &paged_rows_kernel<CT, false, TREE>;
     size_t lds = !pl.tiles_many ? lds_few : lds_many;
     if constexpr (std::is_same<CT, _Float16>::value && !TREE) {
@@ -1386,9 +1390,8 @@ int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
         }
     } else if constexpr (F16) {
         if (pl.wide) {
-            kernel = pl.wide == 1 ? (pl.few_max ? &paged_wide_kernel<CT, 1, true, TREE> : &paged_wide_kernel<CT, 1, false, TREE>)
-                                  : (pl.few_max ? &paged_wide_kernel<CT, kWideBlocks, true, TREE> : &paged_wide_kernel<CT, kWideBlocks, false, TREE>);
-            lds = wide_lds(pl.wide);
+            kernel = pl.few_max ? &paged_wide_kernel<CT, true, TREE> : &paged_wide_kernel<CT, false, TREE>;
+            lds = kWideLds;
         }
     }
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), lds, stream, p);

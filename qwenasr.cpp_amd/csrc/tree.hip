@@ -105,31 +105,37 @@ struct KeepParams {
 constexpr int kKeepHeads = 8, kKeepPer = 4, kKeepThreads = 256;
 
 __global__ __launch_bounds__(kKeepThreads) void paged_keep_kernel(KeepParams p) {
-    __shared__ int s_from[kMaxNodes], s_end;
+    constexpr int kWindow = kMaxNodes / kPageMin + 2;      // table entries of a sequence's nodes
+    __shared__ int s_from[kMaxNodes], s_page[kWindow], s_end;
     const int s = blockIdx.y;
     const int head0 = blockIdx.z * kKeepHeads, heads = min(kKeepHeads, p.n_kv - head0);
+    if (threadIdx.x == 0) s_end = kMaxNodes;
+    __syncthreads();
+    // its time is dependent loads: the sequence's numbers, then its path and its table's entries, then rows
+    const int past = bounded_past(p.seqs.n_past[s]), asked = p.n_kept[s];
     int first;
     const int nodes = nodes_of(p.seqs, s, first);
-    const int past = bounded_past(p.seqs.n_past[s]);
-    const int kept = min(max(p.n_kept[s], 0), nodes);
-    if (threadIdx.x == 0) s_end = kept;
-    for (int k = threadIdx.x; k < kept; k += kKeepThreads) s_from[k] = p.path[first + k];
-    __syncthreads();
+    const int kept = min(max(asked, 0), nodes);
+    const int32_t * table = p.seqs.tables + static_cast<int64_t>(s) * p.seqs.table_stride;
+    const int first_entry = past >> p.page_shift;
     for (int k = threadIdx.x; k < kept; k += kKeepThreads) {
-        const int from = s_from[k], before = k > 0 ? s_from[k - 1] : -1;
+        const int from = p.path[first + k], before = k > 0 ? p.path[first + k - 1] : -1;
+        s_from[k] = from;
         if (from <= before || from >= nodes) atomicMin(&s_end, k);
     }
+    if (static_cast<int>(threadIdx.x) < kWindow) {
+        const int64_t pos = (static_cast<int64_t>(first_entry) + threadIdx.x) << p.page_shift;
+        s_page[threadIdx.x] = pos < kMaxCapacity ? page_of(table, p.seqs.table_stride, p.page_shift, p.n_pages, static_cast<int>(pos)) : -1;
+    }
     __syncthreads();
-    const int n = s_end;
-    const int32_t * table = p.seqs.tables + static_cast<int64_t>(s) * p.seqs.table_stride;
+    const int n = min(s_end, kept);
     char * base = p.pages + static_cast<int64_t>(blockIdx.x) * p.n_pages * p.block_bytes;
     const int units = p.row_bytes / 16, per_row = heads * units, in_page = (1 << p.page_shift) - 1;
     const int chunk = kKeepPer * kKeepThreads / per_row;   // rows at a time
     // Where the k-th row comes from and goes to, in bytes from base, for rows of `bytes` behind `offset` of a block; false: stays
     auto places = [&](int k, int head, int64_t offset, int bytes, int64_t & from, int64_t & to) {
         const int a = past + s_from[k], b = past + k;
-        const int pa = page_of(table, p.seqs.table_stride, p.page_shift, p.n_pages, a);
-        const int pb = page_of(table, p.seqs.table_stride, p.page_shift, p.n_pages, b);
+        const int pa = s_page[(a >> p.page_shift) - first_entry], pb = s_page[(b >> p.page_shift) - first_entry];
         if (a == b || pa < 0 || pb < 0) return false;
         from = pa * p.block_bytes + offset + ((static_cast<int64_t>(head) << p.page_shift) + (a & in_page)) * bytes;
         to = pb * p.block_bytes + offset + ((static_cast<int64_t>(head) << p.page_shift) + (b & in_page)) * bytes;
