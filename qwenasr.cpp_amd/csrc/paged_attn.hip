@@ -562,7 +562,7 @@ __device__ inline void redo_columns(const AttnParams & p, const Tile & t, int he
 // The waves' results are merged in LDS.
 constexpr int kRowsStride = kHeadDim + 4;
 constexpr int rows_cols(bool f16, bool few) { return f16 && few ? 8 : 16; }
-constexpr size_t rows_lds(bool f16, bool few) { return kWaves * rows_cols(f16, few) * (kRowsStride + 2) * 4 + 2 * rows_cols(f16, few) * 4; }
+constexpr size_t rows_lds(bool f16, bool few, int waves = kWaves) { return waves * rows_cols(f16, few) * (kRowsStride + 2) * 4 + 2 * rows_cols(f16, few) * 4; }
 
 // A sequence that is one tile on f16 pages reads its K and V once, whole lines at a time: past the caches (ONCE).  32 sequences of
 // 3914 positions 84 instead of 94 us, of 157 to 3914 55.7 instead of 57.3.  That is for sequences with pages of their own; what
@@ -575,16 +575,16 @@ __device__ inline VT load_row(const void * at) {
     else return *static_cast<const VT *>(at);
 }
 
-// The 4 waves' results of R columns, merged in LDS and stored; what is to be computed again (redo) is, key by key.
-template <typename CT, int R, bool PACK, bool TREE>
+// The W waves' results of R columns, merged in LDS and stored; what is to be computed again (redo) is, key by key.
+template <typename CT, int R, bool PACK, bool TREE, int W>
 __device__ inline void merge_waves(const AttnParams & p, const Tile & t, int head, char * lds, int wave, int lane, int orow, int lim, float mc,
                                    float l, const f4 (&O)[8], uint32_t redo) {
     constexpr int KS = step_keys(f16_products<CT>);
     const int c16 = lane & 15, g4 = lane >> 4;
     float * so = reinterpret_cast<float *>(lds);
-    float * sm = so + kWaves * R * kRowsStride;
-    float * sl = sm + kWaves * R;
-    int * srow = reinterpret_cast<int *>(sl + kWaves * R);
+    float * sm = so + W * R * kRowsStride;
+    float * sl = sm + W * R;
+    int * srow = reinterpret_cast<int *>(sl + W * R);
     int * slim = srow + R;
     const int base = wave * R;
     if (!PACK || c16 < 8) {
@@ -610,7 +610,7 @@ __device__ inline void merge_waves(const AttnParams & p, const Tile & t, int hea
         const int row = __builtin_amdgcn_readlane(orow, cc), lm = __builtin_amdgcn_readlane(lim, cc);
         float cm, cl;
         f2 co;
-        column_by_keys<CT, KS, TREE>(p, t.table, head, row, lm, t.past, t.step_lo + wave, t.step_hi, kWaves, lane, cm, cl, co);
+        column_by_keys<CT, KS, TREE>(p, t.table, head, row, lm, t.past, t.step_lo + wave, t.step_hi, W, lane, cm, cl, co);
         // after this wave's own stores above: one wave's LDS accesses stay in order
         __builtin_amdgcn_wave_barrier();
         *reinterpret_cast<f2 *>(so + (base + cc) * kRowsStride + 2 * lane) = co;
@@ -621,17 +621,17 @@ __device__ inline void merge_waves(const AttnParams & p, const Tile & t, int hea
     }
     __syncthreads();
 #pragma unroll
-    for (int idx = threadIdx.x; idx < R * (kHeadDim / 4); idx += kThreads) {
+    for (int idx = threadIdx.x; idx < R * (kHeadDim / 4); idx += W * kWave) {
         const int cc = idx / (kHeadDim / 4), dim = (idx % (kHeadDim / 4)) * 4;
         const int row = srow[cc];
         if (row < 0) continue;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, sm[w * R + cc]);
+        for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w * R + cc]);
         float ls = 0.0f;
         f4 o = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float mw = sm[w * R + cc];
             const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - M);
             ls += sl[w * R + cc] * f;
@@ -641,7 +641,7 @@ __device__ inline void merge_waves(const AttnParams & p, const Tile & t, int hea
     }
 }
 
-template <typename CT, bool FEW, bool TREE>
+template <typename CT, bool FEW, bool TREE, int W>
 __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
     constexpr bool F16 = f16_products<CT>, Q8 = is_q8<CT>, PACK = FEW && F16;
     constexpr int KS = step_keys(F16), KB = KS / 16, R = rows_cols(F16, FEW), NB = 1;
@@ -705,7 +705,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
         place(st);
         load_k();
         load_v();
-        entries_of(st + kWaves, entry);
+        entries_of(st + W, entry);
     }
 
     float c[NB];
@@ -728,14 +728,14 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
 #pragma unroll
     for (int db = 0; db < 8; ++db) O[0][db] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    for (; st < t.step_hi; st += kWaves) {
+    for (; st < t.step_hi; st += W) {
         int holes = 0;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             pg[kb] = pg_next[kb];
             holes |= pg[kb] < 0 ? 1 << kb : 0;
         }
-        const bool more = st + kWaves < t.step_hi;
+        const bool more = st + W < t.step_hi;
         f4 S[NB][KB], key_scale[KB];
         if constexpr (Q8) {
             u4 a[8];
@@ -747,7 +747,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
             scores_step<F16, PACK, NB>(rk, qh, ql, x, S);
         }
         if (more) {
-            place(st + kWaves);
+            place(st + W);
             load_k();
         }
         if constexpr (PACK) {
@@ -801,7 +801,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
         }
         if (more) {
             load_v();
-            entries_of(st + 2 * kWaves, entry);
+            entries_of(st + 2 * W, entry);
         }
     }
 
@@ -815,7 +815,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
         }
     }
     close_columns<NB, PACK>(orow, c, m, l, O, mc, redo);
-    merge_waves<CT, R, PACK, TREE>(p, t, head, lds, wave, lane, col.row, col.lim, mc[0], l[0], O[0], redo[0]);
+    merge_waves<CT, R, PACK, TREE, W>(p, t, head, lds, wave, lane, col.row, col.lim, mc[0], l[0], O[0], redo[0]);
 }
 
 // 16 NB columns whose keys the 4 waves take in turn, as in attn_rows, but with their q in LDS, where the waves read the operands of
@@ -824,9 +824,9 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
 constexpr int kWideBlocks = 2;
 constexpr int kWideCols = 16 * kWideBlocks;
 constexpr size_t kWideQ = kWideBlocks * 8 * kWave * 16;               // two parts of 4 operands per 16 columns
-constexpr size_t kWideLds = std::max(kWideQ + kWideCols * 4, rows_lds(true, false));
+constexpr size_t wide_lds(int waves) { return std::max(kWideQ + kWideCols * 4, rows_lds(true, false, waves)); }
 
-template <typename CT, bool TREE>
+template <typename CT, bool TREE, int W>
 __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
     constexpr bool Q8 = is_q8<CT>;
     constexpr int KS = step_keys(true), KB = KS / 16, NB = kWideBlocks;
@@ -886,7 +886,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
         place(st);
         load_k();
         load_v();
-        entries_of(st + kWaves, entry);
+        entries_of(st + W, entry);
     }
 
     int lim[NB], orow[NB], mask[NB];
@@ -897,7 +897,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
         lim[nb] = col.lim;
         orow[nb] = col.row;
         mask[nb] = col.mask;
-        if (wave == nb % kWaves) {                                        // a block's q by one wave
+        if (wave == nb % W) {                                        // a block's q by one wave
             f4 x[8];
             h8 qh[4], ql[4];
             float unit;
@@ -927,14 +927,14 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
 #pragma unroll
         for (int db = 0; db < 8; ++db) O[nb][db] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    for (; st < t.step_hi; st += kWaves) {
+    for (; st < t.step_hi; st += W) {
         int holes = 0;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             pg[kb] = pg_next[kb];
             holes |= pg[kb] < 0 ? 1 << kb : 0;
         }
-        const bool more = st + kWaves < t.step_hi;
+        const bool more = st + W < t.step_hi;
         f4 S[NB][KB], key_scale[KB];
         {
             u4 a[8];
@@ -963,7 +963,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
             }
         }
         if (more) {
-            place(st + kWaves);
+            place(st + W);
             load_k();
         }
         if constexpr (Q8) {
@@ -1005,7 +1005,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
         }
         if (more) {
             load_v();
-            entries_of(st + 2 * kWaves, entry);
+            entries_of(st + 2 * W, entry);
         }
     }
     float mc[NB];
@@ -1024,7 +1024,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         __syncthreads();                                                  // q and the block before are no longer read
-        merge_waves<CT, 16, false, TREE>(p, t, head, lds, wave, lane, orow[nb], lim[nb], mc[nb], l[nb], O[nb], redo[nb]);
+        merge_waves<CT, 16, false, TREE, W>(p, t, head, lds, wave, lane, orow[nb], lim[nb], mc[nb], l[nb], O[nb], redo[nb]);
     }
 }
 
@@ -1218,26 +1218,24 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
 }
 
 // The launches.  One kind of tile, or longer chunks first and the sequences of few columns behind them.
-template <typename CT, bool FEW, bool TREE>
-__global__ __launch_bounds__(kThreads, 3) void paged_rows_kernel(AttnParams p) {
+template <typename CT, bool FEW, bool TREE, int W>
+__global__ __launch_bounds__(W * kWave, W == kWaves ? 3 : 2) void paged_rows_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_rows[];
-    attn_rows<CT, FEW, TREE>(p, blockIdx.x, lds_rows);
+    attn_rows<CT, FEW, TREE, W>(p, blockIdx.x, lds_rows);
 }
 
 template <typename CT, bool TREE>
 __global__ __launch_bounds__(kThreads, 3) void paged_rows_both_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_rows[];
     const int many = p.tiles_many * p.n_kv * p.splits_many, block = blockIdx.x;
-    if (block < many) attn_rows<CT, false, TREE>(p, block, lds_rows);
-    else attn_rows<CT, true, TREE>(p, block - many, lds_rows);
+    if (block < many) attn_rows<CT, false, TREE, kWaves>(p, block, lds_rows);
+    else attn_rows<CT, true, TREE, kWaves>(p, block - many, lds_rows);
 }
 
-template <typename CT, bool BOTH, bool TREE>
-__global__ __launch_bounds__(kThreads, 2) void paged_wide_kernel(AttnParams p) {
+template <typename CT, bool TREE, int W>
+__global__ __launch_bounds__(W * kWave, 2) void paged_wide_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_wide[];
-    const int many = p.tiles_many * p.n_kv * p.splits_many, block = blockIdx.x;
-    if (!BOTH || block < many) attn_wide<CT, TREE>(p, block, lds_wide);
-    else attn_rows<CT, true, TREE>(p, block - many, lds_wide);
+    attn_wide<CT, TREE, W>(p, blockIdx.x, lds_wide);
 }
 
 template <bool BOTH>
@@ -1245,7 +1243,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_tile_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_tile[];
     const int many = p.tiles_many * p.n_kv * p.splits_many, block = blockIdx.x;
     if (!BOTH || block < many) attn_tile(p, block, lds_tile);
-    else attn_rows<_Float16, true, false>(p, block - many, lds_tile);
+    else attn_rows<_Float16, true, false, kWaves>(p, block - many, lds_tile);
 }
 
 // Joins the splits of each (row, head): one wave each, lane = split for the weights, then lane = 2 dims.  Its time is
@@ -1297,6 +1295,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int ks) {
 struct AttnPlan {
     bool tile;               // the longer sequences' tiles are attn_tile's
     bool wide;               // or attn_wide's
+    bool eight;              // of 8 waves per workgroup
     int tiles_many, tiles_few;
     int few_max;             // 0: sequences of few columns are the longer ones' tiles, too
     int splits_many, splits_few, steps_many, steps_few;
@@ -1332,16 +1331,25 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     // eight of 100 tokens behind 2000 (columns left empty) 65 / 53: by the products, where a sequence fills three tiles.
     const bool fresh = tree || l.cache_type == QA_CACHE_Q8;
     pl.tile = f16 && !fresh && most > 2 * kTileCols && cols * (len - std::min(len, tokens / 2)) > 1600000;
-    // attn_wide against attn_rows (8 bits, or f16 pages and trees), us.  1024 tokens behind 2889 positions 78 / 102, behind none 23.5 / 31, four of
-    // 256 behind 500 to 1500 34 / 40, sixteen trees of 41 behind 156 to 3000 (f16) 49 / 58; but 64 behind 1000 16.0 / 12.6, two of 157
-    // behind 701 and 1037 24.1 / 21.7: by the products.
-    pl.wide = f16 && fresh && most > 16 && cols * len >= 1000000;
-    const int width = pl.tile ? kTileCols : pl.wide ? kWideCols : 16;
-    pl.tiles_many = many ? static_cast<int>(cols / width + seqs) : 0;
-    // one sequence is of one kind; of several at most so many are of few columns, by the host's counts
+    // one sequence is of one kind; of several at most few_seqs are of few columns, by the host's counts
     const int64_t few_tokens = few_cols(f16) / group;
     const int64_t few_seqs = tokens > few_tokens ? (seqs * tokens - b.n_rows) / (tokens - few_tokens) : seqs;
     const bool few = !many || (b.n_seqs > 1 && (!fresh || 4 * few_seqs >= 3 * seqs));
+    if (fresh && !few && most > 16) {
+        // 8 bits and trees, us.  One workgroup of 8 waves per CU, where tiles and whole ranges of them fill two thirds of the CUs at least: sixteen
+        // trees of up to 41 behind 156 to 3000 in attn_wide of 8 / 4 waves and in attn_rows 43 / 49 / 52, 8 bits 37 / 42 / 40, eight of
+        // 64 behind 400 to 900 19 / - / 22, two of 63 in f32 with attn_rows of 8 / 4 waves 22 / 28; but 300 tokens (152 tiles) behind
+        // 3500 44 / 38.  More tiles, or few: attn_wide for long products (1024 tokens behind 2889 78, attn_rows 102, behind none 23.5 /
+        // 31, four of 256 behind 500 to 1500 34 / 40), attn_rows for short ones (64 behind 1000 16 / 13, in a batch with single tokens 49 / 45).
+        const auto fills = [&](int64_t width) {
+            const int64_t t = (cols + width - 1) / width * l.n_kv_heads;
+            return t <= 256 && t * std::max<int64_t>(1, std::min<int64_t>(256 / t, steps / 16)) >= 166;
+        };
+        pl.eight = f16 ? cols * len >= 400000 && fills(kWideCols) : fills(16);
+        pl.wide = f16 && (pl.eight || cols * len >= 1000000);
+    }
+    const int width = pl.tile ? kTileCols : pl.wide ? kWideCols : 16;
+    pl.tiles_many = many ? static_cast<int>(cols / width + seqs) : 0;
     pl.few_max = few ? few_cols(f16) : 0;
     pl.tiles_few = few ? seqs : 0;
     // Workgroups to make of the keys, us.  Decode steps, and sequences of one tile: K and V are what they read, and more, shorter
@@ -1356,7 +1364,7 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     const bool one = b.n_seqs == 1;
     // one round of workgroups where their ranges stay short: four sequences of 501 to 3001 in 8 / 12 ranges 13.3 / 16.2 us, f32 pages 18.3 / 23.6
     const int64_t round = std::max<int64_t>(1, 256 / heads), decode = (steps + round - 1) / round <= 24 ? 256 : 1024;
-    if (fresh && most > 16) cut_keys(steps, tiles, one && !pl.wide ? 384 : 512, 16, parts, pl.splits_many, pl.steps_many);
+    if (fresh && most > 16) cut_keys(steps, tiles, pl.eight ? 256 : one && !pl.wide ? 384 : 512, 16, parts, pl.splits_many, pl.steps_many);
     else if (pl.tile) cut_keys(steps, tiles, one ? 512 : 768, 4, parts, pl.splits_many, pl.steps_many);
     else if (most <= 16) cut_keys(steps, heads, decode, 8, parts, pl.splits_many, pl.steps_many);
     else cut_keys(steps, tiles, !one ? 640 : steps >= 128 && tiles > 192 ? 1024 : 384, 16, parts, pl.splits_many, pl.steps_many);
@@ -1376,25 +1384,36 @@ void launch_join(const AttnParams & p, bool f16, hipStream_t stream) {
 // The longer sequences' kernel, or both kinds' in one launch.
 template <typename CT, bool TREE>
 int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
-    constexpr bool F16 = f16_products<CT>;
+    constexpr bool F16 = f16_products<CT>, FRESH = TREE || is_q8<CT>;
     const dim3 grid(static_cast<unsigned>(p.n_kv) * (pl.tiles_many * pl.splits_many + pl.tiles_few * pl.splits_few));
     constexpr size_t lds_few = rows_lds(F16, true), lds_many = rows_lds(F16, false);
-    static_assert(lds_few <= kTileLds && lds_few <= lds_many && lds_few <= kWideLds, "a launch of both kinds has the longer ones' LDS");
-    auto kernel = !pl.tiles_many ? &paged_rows_kernel<CT, true, TREE> : pl.few_max ? &paged_rows_both_kernel<CT, TREE> : &paged_rows_kernel<CT, false, TREE>;
+    static_assert(lds_few <= kTileLds && lds_few <= lds_many, "a launch of both kinds has the longer ones' LDS");
+    auto kernel = !pl.tiles_many ? &paged_rows_kernel<CT, true, TREE, kWaves>
+                  : pl.few_max ? &paged_rows_both_kernel<CT, TREE> : &paged_rows_kernel<CT, false, TREE, kWaves>;
     size_t lds = !pl.tiles_many ? lds_few : lds_many;
-    if constexpr (std::is_same<CT, _Float16>::value && !TREE) {
+    int waves = kWaves;
+    if constexpr (F16 && FRESH) {
+        if (pl.wide) {
+            kernel = pl.eight ? &paged_wide_kernel<CT, TREE, 8> : &paged_wide_kernel<CT, TREE, kWaves>;
+            waves = pl.eight ? 8 : kWaves;
+            lds = wide_lds(waves);
+        }
+    } else if constexpr (FRESH) {
+        if (pl.eight) {
+            kernel = &paged_rows_kernel<CT, false, TREE, 8>;
+            waves = 8;
+            lds = rows_lds(F16, false, waves);
+        }
+    } else if constexpr (F16) {
         if (pl.tile) {
             kernel = pl.few_max ? &paged_tile_kernel<true> : &paged_tile_kernel<false>;
             lds = kTileLds;
-            QA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kTileLds)));
-        }
-    } else if constexpr (F16) {
-        if (pl.wide) {
-            kernel = pl.few_max ? &paged_wide_kernel<CT, true, TREE> : &paged_wide_kernel<CT, false, TREE>;
-            lds = kWideLds;
         }
     }
-    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), lds, stream, p);
+    if (lds >= kTileLds) {
+        QA_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+    }
+    hipLaunchKernelGGL(kernel, grid, dim3(static_cast<unsigned>(waves * kWave)), lds, stream, p);
     QA_LAUNCH_CHECK("paged attention kernel");
     if (pl.parts() > 1) {
         launch_join<TREE>(p, F16, stream);
