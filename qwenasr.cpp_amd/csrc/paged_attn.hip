@@ -320,89 +320,124 @@ __device__ inline u4 transposed(const u4 (&v)[8], int db) {
     return a;
 }
 
-// 8 bits as f16: one instruction per value, which takes its byte and leaves its half of the register.  The last s_nop is the wait
-// that a reader of a half-written register needs.
-__device__ inline void f16_pairs(uint32_t bytes, uint32_t & a, uint32_t & b) {
-    asm("v_cvt_f16_i16_sdwa %0, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
-        "v_cvt_f16_i16_sdwa %1, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
-        "v_cvt_f16_i16_sdwa %0, sext(%2) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1\n\t"
-        "v_cvt_f16_i16_sdwa %1, sext(%2) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3\n\t"
-        "s_nop 0" : "=&v"(a), "=&v"(b) : "v"(bytes));
-}
-// (x, y) byte by byte
-__device__ inline void f16_pairs(uint32_t x, uint32_t y, int d, uint32_t & a, uint32_t & b) {
-    if (d == 0) {
-        asm("v_cvt_f16_i16_sdwa %0, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
-            "v_cvt_f16_i16_sdwa %1, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1\n\t"
-            "v_cvt_f16_i16_sdwa %0, sext(%3) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_0\n\t"
-            "v_cvt_f16_i16_sdwa %1, sext(%3) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1\n\t"
-            "s_nop 0" : "=&v"(a), "=&v"(b) : "v"(x), "v"(y));
-    } else {
-        asm("v_cvt_f16_i16_sdwa %0, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
-            "v_cvt_f16_i16_sdwa %1, sext(%2) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3\n\t"
-            "v_cvt_f16_i16_sdwa %0, sext(%3) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_2\n\t"
-            "v_cvt_f16_i16_sdwa %1, sext(%3) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3\n\t"
-            "s_nop 0" : "=&v"(a), "=&v"(b) : "v"(x), "v"(y));
-    }
+// 8 bits as f16: one instruction per value, which takes its byte and leaves the other half of the register.  The s_nop behind 16
+// of them is the wait that a reader of a half-written register needs.
+__device__ inline void f16_words(u4 raw, u4 & lo, u4 & hi) {             // 16 bytes in order
+    uint32_t o[8];
+    asm("v_cvt_f16_i16_sdwa %0, sext(%8) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
+        "v_cvt_f16_i16_sdwa %1, sext(%8) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+        "v_cvt_f16_i16_sdwa %2, sext(%9) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
+        "v_cvt_f16_i16_sdwa %3, sext(%9) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+        "v_cvt_f16_i16_sdwa %4, sext(%10) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
+        "v_cvt_f16_i16_sdwa %5, sext(%10) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+        "v_cvt_f16_i16_sdwa %6, sext(%11) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
+        "v_cvt_f16_i16_sdwa %7, sext(%11) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+        "v_cvt_f16_i16_sdwa %0, sext(%8) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1\n\t"
+        "v_cvt_f16_i16_sdwa %1, sext(%8) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3\n\t"
+        "v_cvt_f16_i16_sdwa %2, sext(%9) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1\n\t"
+        "v_cvt_f16_i16_sdwa %3, sext(%9) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3\n\t"
+        "v_cvt_f16_i16_sdwa %4, sext(%10) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1\n\t"
+        "v_cvt_f16_i16_sdwa %5, sext(%10) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3\n\t"
+        "v_cvt_f16_i16_sdwa %6, sext(%11) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1\n\t"
+        "v_cvt_f16_i16_sdwa %7, sext(%11) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3\n\t"
+        "s_nop 0"
+        : "=&v"(o[0]), "=&v"(o[1]), "=&v"(o[2]), "=&v"(o[3]), "=&v"(o[4]), "=&v"(o[5]), "=&v"(o[6]), "=&v"(o[7])
+        : "v"(raw[0]), "v"(raw[1]), "v"(raw[2]), "v"(raw[3]));
+    lo = u4{o[0], o[1], o[2], o[3]};
+    hi = u4{o[4], o[5], o[6], o[7]};
 }
 
 // K operands 4 kb .. 4 kb + 3 of a step from the lane's 2 x 16 bytes of 16-key block kb.
 __device__ inline void k_operands(const u4 (&raw)[4], u4 (&a)[8]) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            uint32_t lo, hi;
-            f16_pairs(raw[r][w], lo, hi);
-            a[2 * r + (w >> 1)][2 * (w & 1)] = lo;
-            a[2 * r + (w >> 1)][2 * (w & 1) + 1] = hi;
-        }
-    }
+    for (int r = 0; r < 4; ++r) f16_words(raw[r], a[2 * r], a[2 * r + 1]);
 }
 
-// V^T operands 4 h + 2 d and 4 h + 2 d + 1 of a step's rows of 8 bits, 8 dims per lane and key.
-__device__ inline void v_operands(const u2 (&raw)[8], int h, int d, u4 & even, u4 & odd) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        uint32_t x, y;
-        f16_pairs(raw[2 * w][h], raw[2 * w + 1][h], d, x, y);
-        even[w] = x;
-        odd[w] = y;
+// V^T operands 4 h + 2 D and 4 h + 2 D + 1 of a step's rows of 8 bits, 8 dims per lane and key: two keys' values per word.
+template <int D>
+__device__ inline void v_operands(const u2 (&raw)[8], int h, u4 & even, u4 & odd) {
+    uint32_t o[8];
+    if constexpr (D == 0) {
+        asm("v_cvt_f16_i16_sdwa %0, sext(%8) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
+            "v_cvt_f16_i16_sdwa %4, sext(%8) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1\n\t"
+            "v_cvt_f16_i16_sdwa %1, sext(%10) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
+            "v_cvt_f16_i16_sdwa %5, sext(%10) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1\n\t"
+            "v_cvt_f16_i16_sdwa %2, sext(%12) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
+            "v_cvt_f16_i16_sdwa %6, sext(%12) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1\n\t"
+            "v_cvt_f16_i16_sdwa %3, sext(%14) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
+            "v_cvt_f16_i16_sdwa %7, sext(%14) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1\n\t"
+            "v_cvt_f16_i16_sdwa %0, sext(%9) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_0\n\t"
+            "v_cvt_f16_i16_sdwa %4, sext(%9) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1\n\t"
+            "v_cvt_f16_i16_sdwa %1, sext(%11) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_0\n\t"
+            "v_cvt_f16_i16_sdwa %5, sext(%11) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1\n\t"
+            "v_cvt_f16_i16_sdwa %2, sext(%13) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_0\n\t"
+            "v_cvt_f16_i16_sdwa %6, sext(%13) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1\n\t"
+            "v_cvt_f16_i16_sdwa %3, sext(%15) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_0\n\t"
+            "v_cvt_f16_i16_sdwa %7, sext(%15) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1\n\t"
+            "s_nop 0"
+            : "=&v"(o[0]), "=&v"(o[1]), "=&v"(o[2]), "=&v"(o[3]), "=&v"(o[4]), "=&v"(o[5]), "=&v"(o[6]), "=&v"(o[7])
+            : "v"(raw[0][h]), "v"(raw[1][h]), "v"(raw[2][h]), "v"(raw[3][h]), "v"(raw[4][h]), "v"(raw[5][h]), "v"(raw[6][h]), "v"(raw[7][h]));
+    } else {
+        asm("v_cvt_f16_i16_sdwa %0, sext(%8) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+            "v_cvt_f16_i16_sdwa %4, sext(%8) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3\n\t"
+            "v_cvt_f16_i16_sdwa %1, sext(%10) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+            "v_cvt_f16_i16_sdwa %5, sext(%10) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3\n\t"
+            "v_cvt_f16_i16_sdwa %2, sext(%12) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+            "v_cvt_f16_i16_sdwa %6, sext(%12) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3\n\t"
+            "v_cvt_f16_i16_sdwa %3, sext(%14) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
+            "v_cvt_f16_i16_sdwa %7, sext(%14) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3\n\t"
+            "v_cvt_f16_i16_sdwa %0, sext(%9) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_2\n\t"
+            "v_cvt_f16_i16_sdwa %4, sext(%9) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3\n\t"
+            "v_cvt_f16_i16_sdwa %1, sext(%11) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_2\n\t"
+            "v_cvt_f16_i16_sdwa %5, sext(%11) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3\n\t"
+            "v_cvt_f16_i16_sdwa %2, sext(%13) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_2\n\t"
+            "v_cvt_f16_i16_sdwa %6, sext(%13) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3\n\t"
+            "v_cvt_f16_i16_sdwa %3, sext(%15) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_2\n\t"
+            "v_cvt_f16_i16_sdwa %7, sext(%15) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3\n\t"
+            "s_nop 0"
+            : "=&v"(o[0]), "=&v"(o[1]), "=&v"(o[2]), "=&v"(o[3]), "=&v"(o[4]), "=&v"(o[5]), "=&v"(o[6]), "=&v"(o[7])
+            : "v"(raw[0][h]), "v"(raw[1][h]), "v"(raw[2][h]), "v"(raw[3][h]), "v"(raw[4][h]), "v"(raw[5][h]), "v"(raw[6][h]), "v"(raw[7][h]));
     }
+    even = u4{o[0], o[1], o[2], o[3]};
+    odd = u4{o[4], o[5], o[6], o[7]};
 }
 
-// The keys' V scales go into the probabilities, which are split into f16 parts behind that: against the largest scale that the
-// wave has met, a power of two (top) that the accumulators follow.  pr <- pr * scale / 2^top.
-constexpr int kNoTop = -1000;
+// The keys' V scales go into the probabilities, which are split into f16 parts behind that.  So that these stay in f16's range, the
+// column's reference has the largest scale that the wave has met in it, a power of two: p = exp2(s - m - top), and p times
+// the scale is at most what p alone is on pages of f16.  Sum and accumulators follow when top grows.  Scales of less than 2^-80 count
+// as such: p has to be an f32.
+constexpr int kLeastTop = -80;
 template <int NB>
-__device__ inline void weigh_step(const f4 (&vs)[2], int & top, float (&pr)[NB][2][4], f4 (&O)[NB][8]) {
+__device__ inline void follow_scales(const f4 (&vs)[2], int & top, float (&l)[NB], f4 (&O)[NB][8]) {
     float most = 0.0f;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) most = fmaxf(most, vs[kb][i]);     // a NaN is passed over
     }
-    most = column_max(most);
-    const int ex = most > 0.0f ? __builtin_amdgcn_frexp_expf(most) : kNoTop;
-    if (__any(ex > top)) {                                             // all lanes have the same
+    if (!__any(most > ldexpf(1.0f, top))) return;
+    const int ex = max(top, __builtin_amdgcn_frexp_expf(column_max(most)));   // all lanes have the same
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
+    for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-            for (int db = 0; db < 8; ++db) {
+        for (int db = 0; db < 8; ++db) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) O[nb][db][i] = ldexpf(O[nb][db][i], top - ex);
-            }
+            for (int i = 0; i < 4; ++i) O[nb][db][i] = ldexpf(O[nb][db][i], top - ex);
         }
-        top = ex;
+        l[nb] = ldexpf(l[nb], top - ex);
     }
+    top = ex;
+}
+
+template <int NB>
+__device__ inline void weigh_step(const f4 (&vs)[2], float (&pr)[NB][2][4]) {
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float w = ldexpf(vs[kb][i], -top);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                pr[nb][kb][i] *= w;
+                pr[nb][kb][i] *= vs[kb][i];
                 // the product as it is rounded here: one that a conversion to f16 takes in unrounded (v_fma_mix) is now and then
                 // another f16 than the one whose rest is the second part
                 asm("" : "+v"(pr[nb][kb][i]));
@@ -450,7 +485,7 @@ __device__ inline void split_q(const f4 (&x)[8], float scale, float & c, h8 (&qh
 // A masked score is -inf.
 template <int NB, int KB>
 __device__ inline void softmax_step(const f4 (&S)[NB][KB], const float (&c)[NB], float (&m)[NB], float (&l)[NB], f4 (&O)[NB][8],
-                                    float (&pr)[NB][KB][4]) {
+                                    float (&pr)[NB][KB][4], float shift = -kShiftLog2) {
     float mn[NB];
     bool up[NB], any = false;
 #pragma unroll
@@ -477,7 +512,7 @@ __device__ inline void softmax_step(const f4 (&S)[NB][KB], const float (&c)[NB],
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-        const float mc = m[nb] == -INFINITY ? INFINITY : fmaf(m[nb], c[nb], -kShiftLog2);
+        const float mc = m[nb] == -INFINITY ? INFINITY : fmaf(m[nb], c[nb], shift);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -523,11 +558,11 @@ __device__ inline void store_column(const AttnParams & p, const Tile & t, int ro
 // whose values are not all finite.
 template <int NB, bool PACK>
 __device__ inline void close_columns(const int (&orow)[NB], const float (&c)[NB], const float (&m)[NB], float (&l)[NB], f4 (&O)[NB][8],
-                                     float (&mc)[NB], uint32_t (&redo)[NB]) {
+                                     float (&mc)[NB], uint32_t (&redo)[NB], float shift = -kShiftLog2) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         l[nb] = column_sum(l[nb]);
-        mc[nb] = m[nb] == -INFINITY ? -INFINITY : fmaf(m[nb], c[nb], -kShiftLog2);
+        mc[nb] = m[nb] == -INFINITY ? -INFINITY : fmaf(m[nb], c[nb], shift);
         // 0 x is 0 unless x is not finite, and a sum of such products is then NaN
         float zero = 0.0f * l[nb];
 #pragma unroll
@@ -664,25 +699,30 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
     // a lane's rows of a step; 8 bits: 2 x 16 bytes of K per 16-key block, 8 of V per key, and the scales of its 4 keys per block
     u4 rk[Q8 ? 4 : 8], rv[Q8 ? 1 : 8];
     u2 rv8[8];
-    f4 ks[KB], vs[KB];
+    f4 ks[KB], vs_next[KB];
     int pg[KB], pg_next[KB], entry[KB];
     const CT * at[KB];
-    const float * scales[KB];
+    const char * scales[KB];
+    // 8 bits: a lane's place in a 16-key block's K, V and scales, so that addresses are a uniform base and these
+    const uint32_t k_lane = c16 * kHeadDim + g4 * 16, v_lane = g4 * 4 * kHeadDim + c16 * 8, scale_lane = g4 * 16;
     // a block on no page reads page 0, which there always is, and is masked
     auto place = [&](int st) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             pg_next[kb] = entry_page(p, t, entry[kb], st * KS + kb * 16);
             at[kb] = rows.page(max(pg_next[kb], 0)) + ((st * KS + kb * 16) & in_page) * kHeadDim;
-            if constexpr (Q8) scales[kb] = rows.scale(max(pg_next[kb], 0)) + ((st * KS + kb * 16) & in_page) + g4 * 4;
+            if constexpr (Q8) scales[kb] = reinterpret_cast<const char *>(rows.scale(max(pg_next[kb], 0)) + ((st * KS + kb * 16) & in_page));
         }
     };
     auto load_k = [&]() {
         if constexpr (Q8) {
 #pragma unroll
-            for (int f = 0; f < 4; ++f) rk[f] = load_row<PACK, u4>(at[f >> 1] + c16 * kHeadDim + (f & 1) * 64 + g4 * 16);
+            for (int f = 0; f < 4; ++f) rk[f] = load_row<PACK, u4>(at[f >> 1] + k_lane + (f & 1) * 64);
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) ks[kb] = *reinterpret_cast<const f4 *>(scales[kb]);
+            for (int kb = 0; kb < KB; ++kb) {
+                ks[kb] = *reinterpret_cast<const f4 *>(scales[kb] + scale_lane);
+                vs_next[kb] = *reinterpret_cast<const f4 *>(scales[kb] + rows.v_elems + scale_lane);
+            }
         } else {
 #pragma unroll
             for (int f = 0; f < 8; ++f) rk[f] = load_row<PACK, u4>(at[F16 ? f >> 2 : 0] + k_offset<F16>(f, c16, g4));
@@ -691,9 +731,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
     auto load_v = [&]() {
         if constexpr (Q8) {
 #pragma unroll
-            for (int f = 0; f < 8; ++f) rv8[f] = load_row<PACK, u2>(at[f >> 2] + rows.v_elems + v_offset<true>(f, c16, g4));
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) vs[kb] = *reinterpret_cast<const f4 *>(scales[kb] + rows.v_elems / 4);
+            for (int f = 0; f < 8; ++f) rv8[f] = load_row<PACK, u2>(at[f >> 2] + rows.v_elems + v_lane + (f & 3) * kHeadDim);
         } else {
 #pragma unroll
             for (int f = 0; f < 8; ++f) rv[f] = load_row<PACK, u4>(at[F16 ? f >> 2 : 0] + rows.v_elems + v_offset<F16>(f, c16, g4));
@@ -722,7 +760,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
     const int lim[NB] = {col.lim}, orow[NB] = {col.row}, mask[NB] = {col.mask};
     // steps that every column sees whole
     const int full = TREE ? max(0, min(t.past, t.cap)) / KS : max(0, min(t.past + t.col0 / p.group, t.cap - 1) + 1) / KS;
-    int top = kNoTop;
+    int top = kLeastTop;
     float m[NB] = {-INFINITY}, l[NB] = {0.0f};
     f4 O[NB][8];
 #pragma unroll
@@ -736,12 +774,12 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
             holes |= pg[kb] < 0 ? 1 << kb : 0;
         }
         const bool more = st + W < t.step_hi;
-        f4 S[NB][KB], key_scale[KB];
+        f4 S[NB][KB], key_scale[KB], vs[KB];
         if constexpr (Q8) {
             u4 a[8];
             k_operands(rk, a);
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) key_scale[kb] = ks[kb];
+            for (int kb = 0; kb < KB; ++kb) key_scale[kb] = ks[kb], vs[kb] = vs_next[kb];
             scores_step<F16, PACK, NB>(a, qh, ql, x, S);
         } else {
             scores_step<F16, PACK, NB>(rk, qh, ql, x, S);
@@ -762,9 +800,6 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
             for (int kb = 0; kb < KB; ++kb) S[0][kb] *= key_scale[kb];
         }
         if (st >= full || holes != 0) mask_step<NB, KB, TREE>(p, S, lim, mask, t.past, st * KS, g4, holes);
-        float pr[NB][KB][4];
-        softmax_step<NB, KB>(S, c, m, l, O, pr);
-
         // rows of keys that no column sees, and of no page, are whatever memory holds: not even 0 times that
         if (st * KS + KS > t.kend || holes != 0) {
 #pragma unroll
@@ -775,8 +810,15 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
                 }
             }
         }
+        float pr[NB][KB][4];
+        if constexpr (Q8) {
+            follow_scales<NB>(vs, top, l, O);
+            softmax_step<NB, KB>(S, c, m, l, O, pr, static_cast<float>(top) - kShiftLog2);
+            weigh_step<NB>(vs, pr);
+        } else {
+            softmax_step<NB, KB>(S, c, m, l, O, pr);
+        }
         if constexpr (F16) {
-            if constexpr (Q8) weigh_step<NB>(vs, top, pr, O);
             h8 ph, pl;
             split_p(pr[0], ph, pl);
             if constexpr (PACK) ph = c16 < 8 ? ph : pl;
@@ -784,7 +826,8 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
 #pragma unroll
             for (int db = 0; db < 8; ++db) {
                 if constexpr (!Q8) vt[db & 1] = transposed(rv, db);
-                else if (!(db & 1)) v_operands(rv8, db >> 2, (db >> 1) & 1, vt[0], vt[1]);
+                else if (db % 4 == 0) v_operands<0>(rv8, db >> 2, vt[0], vt[1]);
+                else if (db % 4 == 2) v_operands<1>(rv8, db >> 2, vt[0], vt[1]);
                 const h8 a = __builtin_bit_cast(h8, vt[db & 1]);
                 O[0][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, O[0][db], 0, 0, 0);
                 if constexpr (!PACK) O[0][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, O[0][db], 0, 0, 0);
@@ -807,14 +850,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
 
     float mc[NB];
     uint32_t redo[NB];
-    if constexpr (Q8) {
-#pragma unroll
-        for (int db = 0; db < 8; ++db) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) O[0][db][i] = ldexpf(O[0][db][i], top);
-        }
-    }
-    close_columns<NB, PACK>(orow, c, m, l, O, mc, redo);
+    close_columns<NB, PACK>(orow, c, m, l, O, mc, redo, Q8 ? static_cast<float>(top) - kShiftLog2 : -kShiftLog2);
     merge_waves<CT, R, PACK, TREE, W>(p, t, head, lds, wave, lane, col.row, col.lim, mc[0], l[0], O[0], redo[0]);
 }
 
@@ -845,25 +881,30 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
     };
     u4 rk[Q8 ? 4 : 8], rv[Q8 ? 1 : 8];
     u2 rv8[8];
-    f4 ks[KB], vs[KB];
+    f4 ks[KB], vs_next[KB];
     int pg[KB], pg_next[KB], entry[KB];
     const CT * at[KB];
-    const float * scales[KB];
+    const char * scales[KB];
+    // 8 bits: a lane's place in a 16-key block's K, V and scales, so that addresses are a uniform base and these
+    const uint32_t k_lane = c16 * kHeadDim + g4 * 16, v_lane = g4 * 4 * kHeadDim + c16 * 8, scale_lane = g4 * 16;
     // a block on no page reads page 0, which there always is, and is masked
     auto place = [&](int st) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             pg_next[kb] = entry_page(p, t, entry[kb], st * KS + kb * 16);
             at[kb] = rows.page(max(pg_next[kb], 0)) + ((st * KS + kb * 16) & in_page) * kHeadDim;
-            if constexpr (Q8) scales[kb] = rows.scale(max(pg_next[kb], 0)) + ((st * KS + kb * 16) & in_page) + g4 * 4;
+            if constexpr (Q8) scales[kb] = reinterpret_cast<const char *>(rows.scale(max(pg_next[kb], 0)) + ((st * KS + kb * 16) & in_page));
         }
     };
     auto load_k = [&]() {
         if constexpr (Q8) {
 #pragma unroll
-            for (int f = 0; f < 4; ++f) rk[f] = *reinterpret_cast<const u4 *>(at[f >> 1] + c16 * kHeadDim + (f & 1) * 64 + g4 * 16);
+            for (int f = 0; f < 4; ++f) rk[f] = *reinterpret_cast<const u4 *>(at[f >> 1] + k_lane + (f & 1) * 64);
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) ks[kb] = *reinterpret_cast<const f4 *>(scales[kb]);
+            for (int kb = 0; kb < KB; ++kb) {
+                ks[kb] = *reinterpret_cast<const f4 *>(scales[kb] + scale_lane);
+                vs_next[kb] = *reinterpret_cast<const f4 *>(scales[kb] + rows.v_elems + scale_lane);
+            }
         } else {
 #pragma unroll
             for (int f = 0; f < 8; ++f) rk[f] = *reinterpret_cast<const u4 *>(at[f >> 2] + k_offset<true>(f, c16, g4));
@@ -872,9 +913,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
     auto load_v = [&]() {
         if constexpr (Q8) {
 #pragma unroll
-            for (int f = 0; f < 8; ++f) rv8[f] = *reinterpret_cast<const u2 *>(at[f >> 2] + rows.v_elems + v_offset<true>(f, c16, g4));
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) vs[kb] = *reinterpret_cast<const f4 *>(scales[kb] + rows.v_elems / 4);
+            for (int f = 0; f < 8; ++f) rv8[f] = *reinterpret_cast<const u2 *>(at[f >> 2] + rows.v_elems + v_lane + (f & 3) * kHeadDim);
         } else {
 #pragma unroll
             for (int f = 0; f < 8; ++f) rv[f] = *reinterpret_cast<const u4 *>(at[f >> 2] + rows.v_elems + v_offset<true>(f, c16, g4));
@@ -917,7 +956,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
     for (int nb = 0; nb < NB; ++nb) c[nb] = *reinterpret_cast<const float *>(lds + kWideQ + (nb * 16 + c16) * 4);
     // steps that every column sees whole
     const int full = TREE ? max(0, min(t.past, t.cap)) / KS : max(0, min(t.past + t.col0 / p.group, t.cap - 1) + 1) / KS;
-    int top = kNoTop;
+    int top = kLeastTop;
     float m[NB], l[NB];
     f4 O[NB][8];
 #pragma unroll
@@ -935,13 +974,13 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
             holes |= pg[kb] < 0 ? 1 << kb : 0;
         }
         const bool more = st + W < t.step_hi;
-        f4 S[NB][KB], key_scale[KB];
+        f4 S[NB][KB], key_scale[KB], vs[KB];
         {
             u4 a[8];
             if constexpr (Q8) {
                 k_operands(rk, a);
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) key_scale[kb] = ks[kb];
+                for (int kb = 0; kb < KB; ++kb) key_scale[kb] = ks[kb], vs[kb] = vs_next[kb];
             } else {
 #pragma unroll
                 for (int f = 0; f < 8; ++f) a[f] = rk[f];
@@ -974,9 +1013,6 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
             }
         }
         if (st >= full || holes != 0) mask_step<NB, KB, TREE>(p, S, lim, mask, t.past, st * KS, g4, holes);
-        float pr[NB][KB][4];
-        softmax_step<NB, KB>(S, c, m, l, O, pr);
-
         // rows of keys that no column sees, and of no page, are whatever memory holds: not even 0 times that
         if (st * KS + KS > t.kend || holes != 0) {
 #pragma unroll
@@ -987,7 +1023,14 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
                 }
             }
         }
-        if constexpr (Q8) weigh_step<NB>(vs, top, pr, O);
+        float pr[NB][KB][4];
+        if constexpr (Q8) {
+            follow_scales<NB>(vs, top, l, O);
+            softmax_step<NB, KB>(S, c, m, l, O, pr, static_cast<float>(top) - kShiftLog2);
+            weigh_step<NB>(vs, pr);
+        } else {
+            softmax_step<NB, KB>(S, c, m, l, O, pr);
+        }
         h8 ph[NB], pl[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) split_p(pr[nb], ph[nb], pl[nb]);
@@ -995,7 +1038,8 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
 #pragma unroll
         for (int db = 0; db < 8; ++db) {
             if constexpr (!Q8) vt[db & 1] = transposed(rv, db);
-            else if (!(db & 1)) v_operands(rv8, db >> 2, (db >> 1) & 1, vt[0], vt[1]);
+            else if (db % 4 == 0) v_operands<0>(rv8, db >> 2, vt[0], vt[1]);
+            else if (db % 4 == 2) v_operands<1>(rv8, db >> 2, vt[0], vt[1]);
             const h8 a = __builtin_bit_cast(h8, vt[db & 1]);
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
@@ -1010,17 +1054,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
     }
     float mc[NB];
     uint32_t redo[NB];
-    if constexpr (Q8) {
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-            for (int db = 0; db < 8; ++db) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) O[nb][db][i] = ldexpf(O[nb][db][i], top);
-            }
-        }
-    }
-    close_columns<NB, false>(orow, c, m, l, O, mc, redo);
+    close_columns<NB, false>(orow, c, m, l, O, mc, redo, Q8 ? static_cast<float>(top) - kShiftLog2 : -kShiftLog2);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         __syncthreads();                                                  // q and the block before are no longer read
@@ -1218,8 +1252,13 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
 }
 
 // The launches.  One kind of tile, or longer chunks first and the sequences of few columns behind them.
+// Waves per SIMD that the registers are cut for.  16 columns on 8 bits, or with masks, do not fit three of them: two of 157 tokens behind
+// 701 and 1037 positions of 8 bits 24.3 / 20.7 us at three / two.  (With decode steps in the same launch they are three: 30.8 / 33.1.)
+template <typename CT, bool FEW, bool TREE>
+constexpr int rows_occupancy(int waves) { return waves > kWaves || (f16_products<CT> && !FEW && (TREE || is_q8<CT>)) ? 2 : 3; }
+
 template <typename CT, bool FEW, bool TREE, int W>
-__global__ __launch_bounds__(W * kWave, W == kWaves ? 3 : 2) void paged_rows_kernel(AttnParams p) {
+__global__ __launch_bounds__(W * kWave, (rows_occupancy<CT, FEW, TREE>(W))) void paged_rows_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_rows[];
     attn_rows<CT, FEW, TREE, W>(p, blockIdx.x, lds_rows);
 }
@@ -1364,7 +1403,7 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     const bool one = b.n_seqs == 1;
     // one round of workgroups where their ranges stay short: four sequences of 501 to 3001 in 8 / 12 ranges 13.3 / 16.2 us, f32 pages 18.3 / 23.6
     const int64_t round = std::max<int64_t>(1, 256 / heads), decode = (steps + round - 1) / round <= 24 ? 256 : 1024;
-    if (fresh && most > 16) cut_keys(steps, tiles, pl.eight ? 256 : one && !pl.wide ? 384 : 512, 16, parts, pl.splits_many, pl.steps_many);
+    if (fresh && most > 16) cut_keys(steps, tiles, pl.eight ? 256 : one && !pl.wide ? 384 : few ? 640 : 512, 16, parts, pl.splits_many, pl.steps_many);
     else if (pl.tile) cut_keys(steps, tiles, one ? 512 : 768, 4, parts, pl.splits_many, pl.steps_many);
     else if (most <= 16) cut_keys(steps, heads, decode, 8, parts, pl.splits_many, pl.steps_many);
     else cut_keys(steps, tiles, !one ? 640 : steps >= 128 && tiles > 192 ? 1024 : 384, 16, parts, pl.splits_many, pl.steps_many);

@@ -92,7 +92,8 @@ __device__ inline float wave_sum_all(float v) { return bcast63_f(wave_sum_lane63
 __device__ inline float wave_max_all(float v) { return bcast63_f(wave_max_lane63(v)); }
 __device__ inline double wave_sum_d_all(double v) { return bcast63_d(wave_sum_d_lane63(v)); }
 
-__device__ inline float row_ror8(float v) { return dpp_f<0x128>(v); }   // lane c of a row of 16 gets lane c ^ 8's
+// Lane c of a row of 16 gets lane c ^ 8's.  (No lane is without a source; with bound_ctrl set the addition takes the permutation in.)
+__device__ inline float row_ror8(float v) { return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xf, 0xf, true)); }
 
 // Over the lanes c, c + 16, c + 32, c + 48, in each of them: row swaps, no LDS.
 __device__ inline float column_max(float v) {
