@@ -316,8 +316,8 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams p) {
         });
     }
     const int n_segs = min(count, p.width);
-    // The values of the chosen 256s: those that reach the last one's maximum are at least as many.
-    bound = n_segs > 0 ? s.chosen[n_segs - 1].score : 0.0;
+    // The values of the chosen 256s: those that reach the last one's maximum are at least as many, if there are `width` 256s.
+    bound = n_segs == p.width ? s.chosen[n_segs - 1].score : -INFINITY;
     auto value = [&](const Entry * segs, int i) {
         const Entry seg = segs[i / kSeg];
         const int b = static_cast<int>(seg.at >> 32), place = static_cast<int>(static_cast<uint32_t>(seg.at));

@@ -67,6 +67,19 @@ def test_first_step_and_dead_beams(qa):
     check(qa, logits, 4, [0, -np.inf, -np.inf, -np.inf, -np.inf, np.nan, -1.5, -np.inf])
 
 
+@pytest.mark.parametrize("width,vocab", [(4, 40), (8, 8), (8, 300), (64, 64), (64, 700), (33, 9000), (5, 1500)])
+def test_one_beam_of_small_vocabularies(qa, width, vocab):
+    """One beam counts and its row has fewer blocks of values than there are beams: all its values are looked at."""
+    rng = np.random.default_rng(vocab)
+    logits = rng.standard_normal((2 * width, vocab)).astype(np.float32) * 2
+    scores = np.full(2 * width, -np.inf)
+    scores[width // 2], scores[-1] = -0.5, 0
+    check(qa, logits, width, scores)
+    done = np.zeros(2 * width, np.int32)
+    done[0], scores[0] = 1, -1.0
+    check(qa, logits, width, scores, done)
+
+
 def test_fewer_candidates_than_beams(qa):
     """All beams done, no beam that counts, and rows with few values: the rest is done, with -inf."""
     rng = np.random.default_rng(2)
