@@ -440,7 +440,8 @@ int qa_beam_select(const float * logits, int32_t n_groups, int32_t width, int32_
 /* The states of n beams put in the order of their new parents, in place: rows[i] (NULL: i) is list entry i's row of the tables
  * and of ids, and becomes what the row of entry parents[i] was: the pages of its first lens[i] positions, none behind them, with refs kept
  * as in qa_pages_fork, and its ids.  Then ids[rows[i]][ids_len[i]] = tokens[i], where that is a column and the token is not
- * negative.  refs and tables NULL: only the ids; ids NULL: only the pages.  n <= 1024.  An entry whose row is outside [0, n_rows) or
+ * negative.  lens and ids_len are those of the new beams: where beams differ in length, a call with the lengths as ids of one
+ * column puts them in order first.  refs and tables NULL: only the ids; ids NULL: only the pages.  n <= 1024.  An entry whose row is outside [0, n_rows) or
  * listed before, or whose parent is outside [0, n) or such an entry, keeps its row and its ids. */
 int qa_beam_reorder(int32_t * refs, int32_t n_pages, int32_t * tables, int32_t n_rows, int32_t table_stride,
                     int32_t page_size, const int32_t * rows, const int32_t * parents, const int32_t * lens, int32_t n,

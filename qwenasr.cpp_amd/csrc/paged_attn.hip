@@ -766,14 +766,14 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
 #pragma unroll
     for (int db = 0; db < 8; ++db) O[0][db] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    for (; st < t.step_hi; st += W) {
+    // A step; more: the next one's rows are loaded on the way.  Loads under a condition would make every wait one for all loads.
+    auto step = [&](auto more) {
         int holes = 0;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             pg[kb] = pg_next[kb];
             holes |= pg[kb] < 0 ? 1 << kb : 0;
         }
-        const bool more = st + W < t.step_hi;
         f4 S[NB][KB], key_scale[KB], vs[KB];
         if constexpr (Q8) {
             u4 a[8];
@@ -784,7 +784,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
         } else {
             scores_step<F16, PACK, NB>(rk, qh, ql, x, S);
         }
-        if (more) {
+        if constexpr (more.value) {
             place(st + W);
             load_k();
         }
@@ -842,11 +842,13 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
                 }
             }
         }
-        if (more) {
+        if constexpr (more.value) {
             load_v();
             entries_of(st + 2 * W, entry);
         }
-    }
+    };
+    for (; st + W < t.step_hi; st += W) step(std::true_type{});
+    if (st < t.step_hi) step(std::false_type{});
 
     float mc[NB];
     uint32_t redo[NB];
@@ -966,14 +968,14 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
 #pragma unroll
         for (int db = 0; db < 8; ++db) O[nb][db] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    for (; st < t.step_hi; st += W) {
+    // A step; more: the next one's rows are loaded on the way.  Loads under a condition would make every wait one for all loads.
+    auto step = [&](auto more) {
         int holes = 0;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             pg[kb] = pg_next[kb];
             holes |= pg[kb] < 0 ? 1 << kb : 0;
         }
-        const bool more = st + W < t.step_hi;
         f4 S[NB][KB], key_scale[KB], vs[KB];
         {
             u4 a[8];
@@ -1001,7 +1003,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
                 }
             }
         }
-        if (more) {
+        if constexpr (more.value) {
             place(st + W);
             load_k();
         }
@@ -1047,11 +1049,13 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
                 for (int nb = 0; nb < NB; ++nb) O[nb][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, part ? pl[nb] : ph[nb], O[nb][db], 0, 0, 0);
             }
         }
-        if (more) {
+        if constexpr (more.value) {
             load_v();
             entries_of(st + 2 * W, entry);
         }
-    }
+    };
+    for (; st + W < t.step_hi; st += W) step(std::true_type{});
+    if (st < t.step_hi) step(std::false_type{});
     float mc[NB];
     uint32_t redo[NB];
     close_columns<NB, false>(orow, c, m, l, O, mc, redo, Q8 ? static_cast<float>(top) - kShiftLog2 : -kShiftLog2);
