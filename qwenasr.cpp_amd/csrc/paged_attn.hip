@@ -862,7 +862,9 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
 constexpr int kWideBlocks = 2;
 constexpr int kWideCols = 16 * kWideBlocks;
 constexpr size_t kWideQ = kWideBlocks * 8 * kWave * 16;               // two parts of 4 operands per 16 columns
-constexpr size_t wide_lds(int waves) { return std::max(kWideQ + kWideCols * 4, rows_lds(true, false, waves)); }
+constexpr size_t kWideK = kWideQ + 1024;                              // behind q and its units: a step of K per wave
+template <typename CT>
+constexpr size_t wide_lds(int waves) { return std::max(kWideK + waves * 32 * kHeadDim * sizeof(CT), rows_lds(true, false, waves)); }
 
 template <typename CT, bool TREE, int W>
 __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
@@ -877,18 +879,34 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
 
     const HeadRows<CT> rows(p.pages, p.layer, p.n_kv, p.n_pages, p.page_shift, head);
     const int in_page = (1 << p.page_shift) - 1, last_entry = p.seqs.table_stride - 1;
+    // by scalar loads, which the loads into LDS would rule out for memory that might be written
+    const auto * table = reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(reinterpret_cast<uintptr_t>(t.table));
     auto entries_of = [&](int st, int (&out)[KB]) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) out[kb] = t.table[min((st * KS + kb * 16) >> p.page_shift, last_entry)];
+        for (int kb = 0; kb < KB; ++kb) out[kb] = table[min((st * KS + kb * 16) >> p.page_shift, last_entry)];
     };
-    u4 rk[Q8 ? 4 : 8], rv[Q8 ? 1 : 8];
+    u4 rv[Q8 ? 1 : 8];
     u2 rv8[8];
     f4 ks[KB], vs_next[KB];
     int pg[KB], pg_next[KB], entry[KB];
     const CT * at[KB];
     const char * scales[KB];
-    // 8 bits: a lane's place in a 16-key block's K, V and scales, so that addresses are a uniform base and these
-    const uint32_t k_lane = c16 * kHeadDim + g4 * 16, v_lane = g4 * 4 * kHeadDim + c16 * 8, scale_lane = g4 * 16;
+    // K in LDS: a load instruction brings whole rows, a kilobyte in the order of its lanes, 16 bytes each; which of its row's 16 bytes
+    // a lane takes depends on the row, so that the 16 rows of an operand are read from different banks.
+    constexpr int kRow = kHeadDim * sizeof(CT), kInRow = kRow / 16, kAtOnce = kWave / kInRow, kPerBlock = 16 / kAtOnce;
+    char * lds_k = lds + kWideK + wave * (KS * kRow);
+    auto turn = [](int key) { return Q8 ? (key >> 1) & 7 : key & 15; };
+    uint32_t k_lane[kPerBlock];
+#pragma unroll
+    for (int f = 0; f < kPerBlock; ++f) {
+        const int key = f * kAtOnce + lane / kInRow;
+        k_lane[f] = key * kRow + ((lane % kInRow) ^ turn(key)) * 16;
+    }
+    auto k_chunk = [&](int kb, int chunk) {
+        return *reinterpret_cast<const u4 *>(lds_k + kb * 16 * kRow + c16 * kRow + (chunk ^ turn(c16)) * 16);
+    };
+    // 8 bits: a lane's place in a 16-key block's V and scales, so that addresses are a uniform base and these
+    const uint32_t v_lane = g4 * 4 * kHeadDim + c16 * 8, scale_lane = g4 * 16;
     // a block on no page reads page 0, which there always is, and is masked
     auto place = [&](int st) {
 #pragma unroll
@@ -899,17 +917,17 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
         }
     };
     auto load_k = [&]() {
-        if constexpr (Q8) {
 #pragma unroll
-            for (int f = 0; f < 4; ++f) rk[f] = *reinterpret_cast<const u4 *>(at[f >> 1] + k_lane + (f & 1) * 64);
+        for (int f = 0; f < KB * kPerBlock; ++f) {
+            const auto block = __builtin_amdgcn_make_buffer_rsrc(const_cast<CT *>(at[f / kPerBlock]), 0, 16 * kRow, 0x00027000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(block, (__attribute__((address_space(3))) void *)(lds_k + f * 1024), 16, k_lane[f % kPerBlock], 0, 0, 0);
+        }
+        if constexpr (Q8) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 ks[kb] = *reinterpret_cast<const f4 *>(scales[kb] + scale_lane);
                 vs_next[kb] = *reinterpret_cast<const f4 *>(scales[kb] + rows.v_elems + scale_lane);
             }
-        } else {
-#pragma unroll
-            for (int f = 0; f < 8; ++f) rk[f] = *reinterpret_cast<const u4 *>(at[f >> 2] + k_offset<true>(f, c16, g4));
         }
     };
     auto load_v = [&]() {
@@ -926,6 +944,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
         entries_of(st, entry);
         place(st);
         load_k();
+        __builtin_amdgcn_sched_barrier(0);
         load_v();
         entries_of(st + W, entry);
     }
@@ -979,13 +998,17 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
         f4 S[NB][KB], key_scale[KB], vs[KB];
         {
             u4 a[8];
+            asm volatile("s_waitcnt vmcnt(8)" ::: "memory");              // V's 8 loads are behind those of K
             if constexpr (Q8) {
+                u4 rk[4];
+#pragma unroll
+                for (int f = 0; f < 4; ++f) rk[f] = k_chunk(f >> 1, (f & 1) * 4 + g4);
                 k_operands(rk, a);
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) key_scale[kb] = ks[kb], vs[kb] = vs_next[kb];
             } else {
 #pragma unroll
-                for (int f = 0; f < 8; ++f) a[f] = rk[f];
+                for (int f = 0; f < 8; ++f) a[f] = k_chunk(f >> 2, (f & 3) * 4 + g4);
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
@@ -1005,6 +1028,8 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
         }
         if constexpr (more.value) {
             place(st + W);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(0xc07f);                          // lgkmcnt(0): K has been read
             load_k();
         }
         if constexpr (Q8) {
@@ -1439,7 +1464,7 @@ int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
         if (pl.wide) {
             kernel = pl.eight ? &paged_wide_kernel<CT, TREE, 8> : &paged_wide_kernel<CT, TREE, kWaves>;
             waves = pl.eight ? 8 : kWaves;
-            lds = wide_lds(waves);
+            lds = wide_lds<CT>(waves);
         }
     } else if constexpr (FRESH) {
         if (pl.eight) {
