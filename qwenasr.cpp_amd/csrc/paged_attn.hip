@@ -1403,17 +1403,23 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     const int64_t few_tokens = few_cols(f16) / group;
     const int64_t few_seqs = tokens > few_tokens ? (seqs * tokens - b.n_rows) / (tokens - few_tokens) : seqs;
     const bool few = !many || (b.n_seqs > 1 && (!fresh || 4 * few_seqs >= 3 * seqs));
+    int64_t eight_tiles = 0;
     if (fresh && !few && most > 16) {
-        // 8 bits and trees, us.  One workgroup of 8 waves per CU, where tiles and whole ranges of them fill two thirds of the CUs at least: sixteen
-        // trees of up to 41 behind 156 to 3000 in attn_wide of 8 / 4 waves and in attn_rows 43 / 49 / 52, 8 bits 37 / 42 / 40, eight of
-        // 64 behind 400 to 900 19 / - / 22, two of 63 in f32 with attn_rows of 8 / 4 waves 22 / 28; but 300 tokens (152 tiles) behind
-        // 3500 44 / 38.  More tiles, or few: attn_wide for long products (1024 tokens behind 2889 78, attn_rows 102, behind none 23.5 /
-        // 31, four of 256 behind 500 to 1500 34 / 40), attn_rows for short ones (64 behind 1000 16 / 13, in a batch with single tokens 49 / 45).
-        const auto fills = [&](int64_t width) {
-            const int64_t t = (cols + width - 1) / width * l.n_kv_heads;
-            return t <= 256 && t * std::max<int64_t>(1, std::min<int64_t>(256 / t, steps / 16)) >= 166;
-        };
-        pl.eight = f16 ? cols * len >= 400000 && fills(kWideCols) : fills(16);
+        // 8 bits and trees, us.  One workgroup of 8 waves per CU, where the tiles and their ranges fill two thirds of the CUs, or half of them for
+        // not long, and each has enough to do for what it takes to begin and to merge (`worth`): sixteen trees of up to 41 behind
+        // 156 to 3000 in attn_wide of 8 / 4 waves and in attn_rows 37 / 43 / 52, two of 32 behind 2000 15.6 / 16.3 / 18.9, but one of 48 there
+        // 15.2 / 15.6 / 13.9; two of 63 in f32 with attn_rows of 8 / 4 waves 21 / 28.  On 8 bits attn_rows is nearer: 64 tokens behind 3000
+        // 16.3 / 17.3 / 17.6, two trees of 32 behind 2000 16.5 / 17.8 / 17.0, sixteen of 1 to 12 behind 300 to 2000 (tiles mostly empty) 21.2 / 21.8 /
+        // 19.0; 300 tokens (152 tiles) behind 3500 38.5 / 35.6.  More tiles, or few: attn_wide for long products (1024 tokens
+        // behind 2889 73, attn_rows 102, behind none 21 / 31, four of 256 behind 500 to 1500 31 / 40), attn_rows for short ones (64 behind
+        // 1000 16 / 13, in a batch with single tokens 49 / 45).
+        // a sequence's last tile is half full
+        const int64_t columns = f16 ? kWideCols : 16, t = std::max<int64_t>((cols + columns - 1) / columns + (seqs - 1) / 2, seqs) * l.n_kv_heads;
+        const int64_t ranges = std::min<int64_t>(256 / std::min<int64_t>(t, 256), (steps + 15) / 16);
+        const bool fills = t <= 256 && t * ranges >= (steps <= 40 * ranges ? 120 : 166);
+        const bool worth = !f16 || (l.cache_type == QA_CACHE_Q8 ? cols * len >= 300000 && cols >= 24 * seqs : cols * len >= 220000);
+        pl.eight = fills && worth;
+        eight_tiles = t;
         pl.wide = f16 && (pl.eight || cols * len >= 1000000);
     }
     const int width = pl.tile ? kTileCols : pl.wide ? kWideCols : 16;
@@ -1428,7 +1434,8 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     // three, 140 in one.  Sequences differ in length, and the ranges are cut for the longest: 16 of 70 behind 300 to 2000 at
     // 384 / 640 workgroups 38 / 33 (f32: 76 / 59).  attn_tile has 512 at a time: one sequence of 400 behind 3500 at 512 / 768
     // 47 / 56, but two of 600 and ten of one token behind 24 to 3500 98 / 73, four of 256 behind 500 to 1500 53 / 57.
-    const int64_t tiles = std::max<int64_t>(1, (cols + width - 1) / width) * l.n_kv_heads, heads = static_cast<int64_t>(seqs) * l.n_kv_heads;
+    const int64_t heads = static_cast<int64_t>(seqs) * l.n_kv_heads;
+    const int64_t tiles = pl.eight ? eight_tiles : std::max<int64_t>(1, (cols + width - 1) / width) * l.n_kv_heads;
     const bool one = b.n_seqs == 1;
     // one round of workgroups where their ranges stay short: four sequences of 501 to 3001 in 8 / 12 ranges 13.3 / 16.2 us, f32 pages 18.3 / 23.6
     const int64_t round = std::max<int64_t>(1, 256 / heads), decode = (steps + round - 1) / round <= 24 ? 256 : 1024;
