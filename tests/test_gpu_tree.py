@@ -124,6 +124,36 @@ def test_what_siblings_hold_does_not_matter(qa, cache, past, news):
     close(got[~sees], want[~sees], 6.0)
 
 
+FILLING = [([1600, 900, 1300, 40, 700], [41, 36, 31, 26, 21]), ([2000, 1700], [32, 27]), ([700] * 11 + [300], [24, 3] * 5 + [0, 30]),
+           ([500, 30, 900, 100, 250, 31, 0, 64, 200], [40, 4, 3, 1, 4, 2, 4, 1, 3])]
+
+
+@pytest.mark.parametrize("cache", cand.CACHES)
+@pytest.mark.parametrize("past,news", FILLING)
+@pytest.mark.parametrize("page,holes", [(16, ()), (64, [(0, 0, -1), (1, 2, 1 << 30), (0, 7, -1)])])
+def test_trees_that_fill_the_chip(qa, cache, past, news, page, holes):
+    got, want, pool, _ = case(qa, 14, cache, past, news, page, holes=[h for h in holes if h[1] * page < past[h[0]] + news[h[0]]])
+    close(got, want, np.abs(pool.values).max())
+
+
+@pytest.mark.parametrize("cache", cand.CACHES)
+@pytest.mark.parametrize("past,news", FILLING)
+def test_any_mask_where_trees_fill_the_chip(qa, cache, past, news):
+    """Random masks, the cached positions not finite in a page that no table holds."""
+    rng = np.random.default_rng(15)
+    mask = rng.integers(0, 2 ** 32, (sum(news), 2), dtype=np.uint64).astype(np.uint32)
+    mask[::5] = 0
+
+    def change(pool, tables):
+        free = np.setdiff1d(np.arange(pool.raw.shape[2] if cache != "q8" else pool.scales.shape[2]), tables)
+        if cache == "q8":
+            pool.scales[:, :, free] = np.nan
+        else:
+            pool.raw[:, :, free] = np.nan
+    got, want, pool, _ = case(qa, 16, cache, past, news, 16, mask=mask, change=change)
+    close(got, want, 6.0)
+
+
 def test_rows_of_no_sequence_and_no_bounds(qa):
     got, want, pool, b = case(qa, 12, "f16", [40, 0, 300], [9, 20, 1], 16, n_rows=33, fill=2.5, max_tokens=0, max_len=0)
     close(got[:30], want[:30], np.abs(pool.values).max())
