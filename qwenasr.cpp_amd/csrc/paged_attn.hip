@@ -610,6 +610,55 @@ __device__ inline VT load_row(const void * at) {
     else return *static_cast<const VT *>(at);
 }
 
+// A step of K in LDS, a wave's own.  A load instruction brings whole rows straight into LDS, a kilobyte in the order of its lanes, 16 bytes each; which
+// of its row's 16 bytes a lane takes depends on the row, so that the 16 rows of an operand are read from different banks.  (A lane that
+// loads its own operand takes 16 bytes of a row per instruction, and the 16 lanes beside it 16 other rows: four times the cache accesses.)
+template <typename CT, bool ONCE = false>
+struct KStep {
+    static constexpr int kRow = kHeadDim * sizeof(CT), kInRow = kRow / 16, kAtOnce = kWave / kInRow, kPerBlock = 16 / kAtOnce;
+    static constexpr int kBlocks = step_keys(f16_products<CT>) / 16, kBytes = kBlocks * 16 * kRow;
+    char * lds;
+    uint32_t lane_at[kPerBlock];
+    static __device__ inline int turn(int key) { return is_q8<CT> ? (key >> 1) & 7 : key & 15; }
+    __device__ inline KStep(char * to, int lane) : lds(to) {
+#pragma unroll
+        for (int f = 0; f < kPerBlock; ++f) {
+            const int key = f * kAtOnce + lane / kInRow;
+            lane_at[f] = key * kRow + ((lane % kInRow) ^ turn(key)) * 16;
+        }
+    }
+    // at: the step's 16-key blocks.  Buffer loads, as the compiler counts them like any other (after global loads into LDS it waits for all).
+    __device__ inline void load([[maybe_unused]] const CT * const * at) const {
+#ifdef __HIP_DEVICE_COMPILE__                              // the host has no type for the buffer
+#pragma unroll
+        for (int f = 0; f < kBlocks * kPerBlock; ++f) {
+            const auto block = __builtin_amdgcn_make_buffer_rsrc(const_cast<CT *>(at[f / kPerBlock]), 0, 16 * kRow, 0x00027000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(block, (__attribute__((address_space(3))) void *)(lds + f * 1024), 16, lane_at[f % kPerBlock], 0, 0,
+                                                     ONCE ? 2 : 0);
+        }
+#endif
+    }
+    // Before a step's chunks are read: of the loads behind those of K there are V's 8.
+    static __device__ inline void arrived() { asm volatile("s_waitcnt vmcnt(8)" ::: "memory"); }
+    // Before the next step is loaded: this one has been read.
+    static __device__ inline void read() {
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0xc07f);                // lgkmcnt(0)
+    }
+    __device__ inline u4 chunk(int kb, int c16, int chunk) const {
+        return *reinterpret_cast<const u4 *>(lds + kb * 16 * kRow + c16 * kRow + (chunk ^ turn(c16)) * 16);
+    }
+};
+
+// LDS of attn_rows: its waves' K, then their results.
+template <typename CT>
+constexpr size_t rows_bytes(bool few, int waves = kWaves) { return std::max<size_t>(rows_lds(f16_products<CT>, few, waves), waves * KStep<CT>::kBytes); }
+
+// The table of a tile, for scalar loads, which the loads into LDS would rule out for memory that might be written.
+__device__ inline const __attribute__((address_space(4))) int32_t * scalar_table(const Tile & t) {
+    return reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(reinterpret_cast<uintptr_t>(t.table));
+}
+
 // The W waves' results of R columns, merged in LDS and stored; what is to be computed again (redo) is, key by key.
 template <typename CT, int R, bool PACK, bool TREE, int W>
 __device__ inline void merge_waves(const AttnParams & p, const Tile & t, int head, char * lds, int wave, int lane, int orow, int lim, float mc,
@@ -692,19 +741,21 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
 
     const HeadRows<CT> rows(p.pages, p.layer, p.n_kv, p.n_pages, p.page_shift, head);
     const int in_page = (1 << p.page_shift) - 1, last_entry = p.seqs.table_stride - 1;
+    const auto * table = scalar_table(t);
     auto entries_of = [&](int st, int (&out)[KB]) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) out[kb] = t.table[min((st * KS + kb * 16) >> p.page_shift, last_entry)];
+        for (int kb = 0; kb < KB; ++kb) out[kb] = table[min((st * KS + kb * 16) >> p.page_shift, last_entry)];
     };
-    // a lane's rows of a step; 8 bits: 2 x 16 bytes of K per 16-key block, 8 of V per key, and the scales of its 4 keys per block
-    u4 rk[Q8 ? 4 : 8], rv[Q8 ? 1 : 8];
+    // a lane's rows of a step of V; 8 bits: 8 bytes per key, and the scales of its 4 keys per 16-key block, K's and V's
+    const KStep<CT, PACK && !Q8> k_step(lds + wave * KStep<CT>::kBytes, lane);
+    u4 rv[Q8 ? 1 : 8];
     u2 rv8[8];
     f4 ks[KB], vs_next[KB];
     int pg[KB], pg_next[KB], entry[KB];
     const CT * at[KB];
     const char * scales[KB];
-    // 8 bits: a lane's place in a 16-key block's K, V and scales, so that addresses are a uniform base and these
-    const uint32_t k_lane = c16 * kHeadDim + g4 * 16, v_lane = g4 * 4 * kHeadDim + c16 * 8, scale_lane = g4 * 16;
+    // 8 bits: a lane's place in a 16-key block's V and scales, so that addresses are a uniform base and these
+    const uint32_t v_lane = g4 * 4 * kHeadDim + c16 * 8, scale_lane = g4 * 16;
     // a block on no page reads page 0, which there always is, and is masked
     auto place = [&](int st) {
 #pragma unroll
@@ -715,17 +766,13 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
         }
     };
     auto load_k = [&]() {
+        k_step.load(at);
         if constexpr (Q8) {
-#pragma unroll
-            for (int f = 0; f < 4; ++f) rk[f] = load_row<PACK, u4>(at[f >> 1] + k_lane + (f & 1) * 64);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 ks[kb] = *reinterpret_cast<const f4 *>(scales[kb] + scale_lane);
                 vs_next[kb] = *reinterpret_cast<const f4 *>(scales[kb] + rows.v_elems + scale_lane);
             }
-        } else {
-#pragma unroll
-            for (int f = 0; f < 8; ++f) rk[f] = load_row<PACK, u4>(at[F16 ? f >> 2 : 0] + k_offset<F16>(f, c16, g4));
         }
     };
     auto load_v = [&]() {
@@ -742,6 +789,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
         entries_of(st, entry);
         place(st);
         load_k();
+        __builtin_amdgcn_sched_barrier(0);
         load_v();
         entries_of(st + W, entry);
     }
@@ -775,17 +823,23 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
             holes |= pg[kb] < 0 ? 1 << kb : 0;
         }
         f4 S[NB][KB], key_scale[KB], vs[KB];
+        u4 a[8];
+        k_step.arrived();
         if constexpr (Q8) {
-            u4 a[8];
-            k_operands(rk, a);
+            u4 raw[4];
+#pragma unroll
+            for (int f = 0; f < 4; ++f) raw[f] = k_step.chunk(f >> 1, c16, (f & 1) * 4 + g4);
+            k_operands(raw, a);
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) key_scale[kb] = ks[kb], vs[kb] = vs_next[kb];
-            scores_step<F16, PACK, NB>(a, qh, ql, x, S);
         } else {
-            scores_step<F16, PACK, NB>(rk, qh, ql, x, S);
+#pragma unroll
+            for (int f = 0; f < 8; ++f) a[f] = F16 ? k_step.chunk(f >> 2, c16, (f & 3) * 4 + g4) : k_step.chunk(0, c16, f * 4 + g4);
         }
+        scores_step<F16, PACK, NB>(a, qh, ql, x, S);
         if constexpr (more.value) {
             place(st + W);
+            k_step.read();
             load_k();
         }
         if constexpr (PACK) {
@@ -853,6 +907,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
     float mc[NB];
     uint32_t redo[NB];
     close_columns<NB, PACK>(orow, c, m, l, O, mc, redo, Q8 ? static_cast<float>(top) - kShiftLog2 : -kShiftLog2);
+    __syncthreads();                                                      // every wave has read its K
     merge_waves<CT, R, PACK, TREE, W>(p, t, head, lds, wave, lane, col.row, col.lim, mc[0], l[0], O[0], redo[0]);
 }
 
@@ -864,7 +919,7 @@ constexpr int kWideCols = 16 * kWideBlocks;
 constexpr size_t kWideQ = kWideBlocks * 8 * kWave * 16;               // two parts of 4 operands per 16 columns
 constexpr size_t kWideK = kWideQ + 1024;                              // behind q and its units: a step of K per wave
 template <typename CT>
-constexpr size_t wide_lds(int waves) { return std::max(kWideK + waves * 32 * kHeadDim * sizeof(CT), rows_lds(true, false, waves)); }
+constexpr size_t wide_lds(int waves) { return std::max<size_t>(kWideK + waves * KStep<CT>::kBytes, rows_lds(true, false, waves)); }
 
 template <typename CT, bool TREE, int W>
 __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
@@ -879,8 +934,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
 
     const HeadRows<CT> rows(p.pages, p.layer, p.n_kv, p.n_pages, p.page_shift, head);
     const int in_page = (1 << p.page_shift) - 1, last_entry = p.seqs.table_stride - 1;
-    // by scalar loads, which the loads into LDS would rule out for memory that might be written
-    const auto * table = reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(reinterpret_cast<uintptr_t>(t.table));
+    const auto * table = scalar_table(t);
     auto entries_of = [&](int st, int (&out)[KB]) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) out[kb] = table[min((st * KS + kb * 16) >> p.page_shift, last_entry)];
@@ -891,20 +945,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
     int pg[KB], pg_next[KB], entry[KB];
     const CT * at[KB];
     const char * scales[KB];
-    // K in LDS: a load instruction brings whole rows, a kilobyte in the order of its lanes, 16 bytes each; which of its row's 16 bytes
-    // a lane takes depends on the row, so that the 16 rows of an operand are read from different banks.
-    constexpr int kRow = kHeadDim * sizeof(CT), kInRow = kRow / 16, kAtOnce = kWave / kInRow, kPerBlock = 16 / kAtOnce;
-    char * lds_k = lds + kWideK + wave * (KS * kRow);
-    auto turn = [](int key) { return Q8 ? (key >> 1) & 7 : key & 15; };
-    uint32_t k_lane[kPerBlock];
-#pragma unroll
-    for (int f = 0; f < kPerBlock; ++f) {
-        const int key = f * kAtOnce + lane / kInRow;
-        k_lane[f] = key * kRow + ((lane % kInRow) ^ turn(key)) * 16;
-    }
-    auto k_chunk = [&](int kb, int chunk) {
-        return *reinterpret_cast<const u4 *>(lds_k + kb * 16 * kRow + c16 * kRow + (chunk ^ turn(c16)) * 16);
-    };
+    const KStep<CT> k_step(lds + kWideK + wave * KStep<CT>::kBytes, lane);
     // 8 bits: a lane's place in a 16-key block's V and scales, so that addresses are a uniform base and these
     const uint32_t v_lane = g4 * 4 * kHeadDim + c16 * 8, scale_lane = g4 * 16;
     // a block on no page reads page 0, which there always is, and is masked
@@ -917,11 +958,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
         }
     };
     auto load_k = [&]() {
-#pragma unroll
-        for (int f = 0; f < KB * kPerBlock; ++f) {
-            const auto block = __builtin_amdgcn_make_buffer_rsrc(const_cast<CT *>(at[f / kPerBlock]), 0, 16 * kRow, 0x00027000);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(block, (__attribute__((address_space(3))) void *)(lds_k + f * 1024), 16, k_lane[f % kPerBlock], 0, 0, 0);
-        }
+        k_step.load(at);
         if constexpr (Q8) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
@@ -998,17 +1035,17 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
         f4 S[NB][KB], key_scale[KB], vs[KB];
         {
             u4 a[8];
-            asm volatile("s_waitcnt vmcnt(8)" ::: "memory");              // V's 8 loads are behind those of K
+            k_step.arrived();
             if constexpr (Q8) {
                 u4 rk[4];
 #pragma unroll
-                for (int f = 0; f < 4; ++f) rk[f] = k_chunk(f >> 1, (f & 1) * 4 + g4);
+                for (int f = 0; f < 4; ++f) rk[f] = k_step.chunk(f >> 1, c16, (f & 1) * 4 + g4);
                 k_operands(rk, a);
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) key_scale[kb] = ks[kb], vs[kb] = vs_next[kb];
             } else {
 #pragma unroll
-                for (int f = 0; f < 8; ++f) a[f] = k_chunk(f >> 2, (f & 3) * 4 + g4);
+                for (int f = 0; f < 8; ++f) a[f] = k_step.chunk(f >> 2, c16, (f & 3) * 4 + g4);
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
@@ -1028,8 +1065,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
         }
         if constexpr (more.value) {
             place(st + W);
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_waitcnt(0xc07f);                          // lgkmcnt(0): K has been read
+            k_step.read();
             load_k();
         }
         if constexpr (Q8) {
@@ -1461,7 +1497,7 @@ template <typename CT, bool TREE>
 int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
     constexpr bool F16 = f16_products<CT>, FRESH = TREE || is_q8<CT>;
     const dim3 grid(static_cast<unsigned>(p.n_kv) * (pl.tiles_many * pl.splits_many + pl.tiles_few * pl.splits_few));
-    constexpr size_t lds_few = rows_lds(F16, true), lds_many = rows_lds(F16, false);
+    constexpr size_t lds_few = rows_bytes<CT>(true), lds_many = rows_bytes<CT>(false);
     static_assert(lds_few <= kTileLds && lds_few <= lds_many, "a launch of both kinds has the longer ones' LDS");
     auto kernel = !pl.tiles_many ? &paged_rows_kernel<CT, true, TREE, kWaves>
                   : pl.few_max ? &paged_rows_both_kernel<CT, TREE> : &paged_rows_kernel<CT, false, TREE, kWaves>;
@@ -1477,7 +1513,7 @@ int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
         if (pl.eight) {
             kernel = &paged_rows_kernel<CT, false, TREE, 8>;
             waves = 8;
-            lds = rows_lds(F16, false, waves);
+            lds = rows_bytes<CT>(false, waves);
         }
     } else if constexpr (F16) {
         if (pl.tile) {
