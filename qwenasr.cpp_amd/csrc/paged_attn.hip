@@ -446,10 +446,9 @@ __device__ inline void weigh_step(const f4 (&vs)[2], float (&pr)[NB][2][4]) {
     }
 }
 
-// Element offset of operand f of a step inside its 16-key block, and that block.  K: key l % 16, dims as q's.  V on f16 pages:
+// Element offset of operand f of a step inside its 16-key block, and that block.  K on f16 pages: key l % 16, dims as q's.  V there:
 // key 16 (f / 4) + 4 (l / 16) + f % 4, dims 8 (l % 16) ..; on f32 pages key 4 (l / 16) + f / 2, dims 8 (l % 16) + 4 (f % 2) ...
-template <bool F16>
-__device__ inline int k_offset(int f, int c16, int g4) { return c16 * kHeadDim + (F16 ? (f & 3) * 32 + g4 * 8 : f * 16 + g4 * 4); }
+__device__ inline int k_offset(int f, int c16, int g4) { return c16 * kHeadDim + (f & 3) * 32 + g4 * 8; }
 template <bool F16>
 __device__ inline int v_offset(int f, int c16, int g4) {
     return F16 ? (g4 * 4 + (f & 3)) * kHeadDim + c16 * 8 : (g4 * 4 + (f >> 1)) * kHeadDim + c16 * 8 + (f & 1) * 4;
@@ -1194,7 +1193,7 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
         }
 #pragma unroll
         for (int f = 0; f < 8; ++f) {
-            r[f] = *reinterpret_cast<const u4 *>(at[f >> 2] + (fetch_v ? v_offset<F16>(f, c16, g4) : k_offset<F16>(f, c16, g4)));
+            r[f] = *reinterpret_cast<const u4 *>(at[f >> 2] + (fetch_v ? v_offset<F16>(f, c16, g4) : k_offset(f, c16, g4)));
         }
     };
     auto put = [&](int buf) {
@@ -1441,22 +1440,22 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     const bool few = !many || (b.n_seqs > 1 && (!fresh || 4 * few_seqs >= 3 * seqs));
     int64_t eight_tiles = 0;
     if (fresh && !few && most > 16) {
-        // 8 bits and trees, us.  One workgroup of 8 waves per CU, where the tiles and their ranges fill two thirds of the CUs, or half of them for
-        // not long, and each has enough to do for what it takes to begin and to merge (`worth`): sixteen trees of up to 41 behind
-        // 156 to 3000 in attn_wide of 8 / 4 waves and in attn_rows 37 / 43 / 52, two of 32 behind 2000 15.6 / 16.3 / 18.9, but one of 48 there
-        // 15.2 / 15.6 / 13.9; two of 63 in f32 with attn_rows of 8 / 4 waves 21 / 28.  On 8 bits attn_rows is nearer: 64 tokens behind 3000
-        // 16.3 / 17.3 / 17.6, two trees of 32 behind 2000 16.5 / 17.8 / 17.0, sixteen of 1 to 12 behind 300 to 2000 (tiles mostly empty) 21.2 / 21.8 /
-        // 19.0; 300 tokens (152 tiles) behind 3500 38.5 / 35.6.  More tiles, or few: attn_wide for long products (1024 tokens
-        // behind 2889 73, attn_rows 102, behind none 21 / 31, four of 256 behind 500 to 1500 31 / 40), attn_rows for short ones (64 behind
-        // 1000 16 / 13, in a batch with single tokens 49 / 45).
+        // 8 bits and trees, us.  One workgroup of 8 waves per CU, where the tiles and their ranges fill two thirds of the CUs, or half of
+        // them for not long, and each has enough to do for what it takes to begin and to merge (`worth`): sixteen trees of up to 41
+        // behind 156 to 3000 in attn_wide of 8 / 4 waves and in attn_rows 37 / 44 / 45, five behind 1600 18.5 / 20.9 / 20.6, but one
+        // of 64 behind 3000 15.9 / 16.6 / 15.1, six of up to 20 behind 500 to 1500 16.3 / 16.8 / 15.3; two of 63 in f32 with attn_rows
+        // of 8 / 4 waves 20 / 24.  8 bits: 64 tokens behind 3000 16.3 / 17.3 / 17.0, two trees of 32 behind 2000 16.5 / 17.5 / 16.5, sixteen of
+        // 1 to 12 behind 300 to 2000 (tiles mostly empty) 20.9 / 21.7 / 19.5, 300 tokens (152 tiles) behind 3500 38.5 / 35.6 / 48.
+        // More tiles, or few: attn_wide for long products (1024 tokens behind 2889 73, attn_rows 85, behind none 21 / 24, 24 trees of 64
+        // behind 1000 to 3000 69 / 78), attn_rows for short ones (32 trees of up to 41 behind 156 to 1000 on 8 bits 27 / 25).
         // a sequence's last tile is half full
         const int64_t columns = f16 ? kWideCols : 16, t = std::max<int64_t>((cols + columns - 1) / columns + (seqs - 1) / 2, seqs) * l.n_kv_heads;
         const int64_t ranges = std::min<int64_t>(256 / std::min<int64_t>(t, 256), (steps + 15) / 16);
         const bool fills = t <= 256 && t * ranges >= (steps <= 40 * ranges ? 120 : 166);
-        const bool worth = !f16 || (l.cache_type == QA_CACHE_Q8 ? cols * len >= 300000 && cols >= 24 * seqs : cols * len >= 220000);
+        const bool worth = !f16 || (l.cache_type == QA_CACHE_Q8 ? cols * len >= 300000 && cols >= 24 * seqs : cols * len >= 400000);
         pl.eight = fills && worth;
         eight_tiles = t;
-        pl.wide = f16 && (pl.eight || cols * len >= 1000000);
+        pl.wide = f16 && (pl.eight || cols * len >= 2000000);
     }
     const int width = pl.tile ? kTileCols : pl.wide ? kWideCols : 16;
     pl.tiles_many = many ? static_cast<int>(cols / width + seqs) : 0;
