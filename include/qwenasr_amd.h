@@ -245,8 +245,8 @@ int qa_paged_append(const float * qkv, const float * q_norm_w, const float * k_n
 
 /* The K and V rows of the batch's tokens read back from their pages, what qa_paged_append wrote for them (n_past 0 and as
  * many rows as a sequence has positions: the whole sequence, for a cache of another kind or for storage outside the GPU).
- * k_out, v_out: [n_rows][kv_dim] of out_type (QA_CACHE_F32, or QA_CACHE_F16: the f32 values rounded to nearest); either may be NULL.  Rows
- * on no page are zeros, rows of no sequence are left as they were.  pages, k_out and v_out aligned to 16 bytes.  */
+ * k_out, v_out: [n_rows][kv_dim] of out_type (QA_CACHE_F32, or QA_CACHE_F16: the f32 values rounded to nearest); either
+ * may be NULL.  Rows on no page are zeros, rows of no sequence are left as they were.  pages, k_out and v_out aligned to 16 bytes.  */
 int qa_paged_read(const void * pages, const qa_kv_layout * layout, int32_t layer, const qa_paged_batch * batch, void * k_out,
                   void * v_out, int32_t out_type, void * stream);
 
@@ -272,9 +272,9 @@ int qa_paged_attn(const float * q, const void * pages, const qa_kv_layout * layo
  * qa_tree_prepare   mask[r][mask_words]: bit i % 32 of word i / 32 where node i is row r's ancestor or r itself, nodes behind
  *                   32 mask_words left out; depth[r]: the number of its ancestors.  Once per step, for all layers.
  * qa_paged_tree_append  qa_paged_append with the angles of n_past + depth[r] (anything that the caller wants, in fact).
- * qa_paged_tree_attn    qa_paged_attn in which a row sees the n_past positions of its sequence and, of the new tokens, those
- *                   whose bit is set in its mask (any mask will do; bits behind the sequence's rows mean nothing).  A row
- *                   that sees no position gets zeros.
+ * qa_paged_tree_attn    qa_paged_attn, with a workspace as there, in which a row sees the n_past positions of its sequence
+ *                   and, of the new tokens, those whose bit is set in its mask (any mask will do; bits behind the
+ *                   sequence's rows mean nothing).  A row that sees no position gets zeros.
  * qa_tree_accept    walks each tree from node 0: of the children of the node it is at, the first one whose ids[row] (the token
  *                   that was fed) is picks[row of the node] (what the model picked behind it, as by qa_argmax_rows), until
  *                   there is none.  path: the nodes passed, n_kept[s] of them, in the sequence's rows, and -1 in the rows
@@ -283,8 +283,9 @@ int qa_paged_attn(const float * q, const void * pages, const qa_kv_layout * layo
  *                   sequence is then n_past + n_kept[s] positions long, and what lies behind may be written again.
  *                   path has to rise strictly; from the first entry of a sequence that does not, or is no node, nothing is
  *                   moved.
- * batch->n_rows up to 2^24 here; parents, ids, picks, depth and path: device int32[n_rows]; n_kept, next: int32[n_seqs].
- * Rows of no sequence are left as they were. */
+ * A tree has at most 1024 nodes (mask_words 1 to 32): a sequence's rows behind them are no nodes, and qa_tree_prepare and
+ * qa_tree_accept leave them as they were, like rows of no sequence.  batch->n_rows up to 2^24 here; parents, ids, picks, depth
+ * and path: device int32[n_rows]; n_kept, next: int32[n_seqs].  */
 int qa_tree_prepare(const qa_paged_batch * batch, const int32_t * parents, uint32_t * mask, int32_t mask_words, int32_t * depth,
                     void * stream);
 int qa_paged_tree_append(const float * qkv, const float * q_norm_w, const float * k_norm_w, float * q_out, void * pages,
@@ -428,8 +429,9 @@ int qa_argmax_rows(const float * logits, int32_t rows, int32_t vocab, int32_t * 
  * none).  The `width` best become the new beams, best first, ties to the lower beam and then the lower id:
  * parents (the row that it continues), tokens (its id, -1 for a beam that was done), scores_out, and done_out: 1 where the
  * parent was done or the id is one of stop_ids (device int32[n_stop], 0 to 64).  Sums and comparisons are in 64 bits (a row's
- * logarithm of its sum is good to 2^-22), scores rounded once.  A NaN is no candidate and weighs nothing, nor does -inf; a score of -inf or NaN leaves a beam without candidates (the
- * first step, whose beams are the same: 0 for one of them and -inf for the others); a row with +inf has none.  Where a
+ * logarithm of its sum is good to 2^-22), scores rounded once.  A NaN is no candidate and weighs nothing, nor does -inf; a
+ * score that is not finite leaves a beam without candidates (the first step, whose beams are the same: 0 for one of them and
+ * -inf for the others); a row with +inf has none.  Where a
  * group has fewer than width candidates, the remaining new beams are done: parent the own row, token -1, score -inf.
  * 1 to 64 beams, vocab >= width.  No output may overlap an input.  workspace: qa_beam_select_workspace_bytes, aligned to 16 bytes;
  * nothing in it outlives the call; calls that share one must be stream-ordered.                     */
@@ -438,11 +440,11 @@ int qa_beam_select(const float * logits, int32_t n_groups, int32_t width, int32_
                    const int32_t * done, const int32_t * stop_ids, int32_t n_stop, int32_t * parents, int32_t * tokens,
                    float * scores_out, int32_t * done_out, void * workspace, size_t workspace_bytes, void * stream);
 /* The states of n beams put in the order of their new parents, in place: rows[i] (NULL: i) is list entry i's row of the tables
- * and of ids, and becomes what the row of entry parents[i] was: the pages of its first lens[i] positions, none behind them, with refs kept
- * as in qa_pages_fork, and its ids.  Then ids[rows[i]][ids_len[i]] = tokens[i], where that is a column and the token is not
+ * and of ids, and becomes what the row of entry parents[i] was: the pages of its first lens[i] positions, none behind them,
+ * with refs kept as in qa_pages_fork, and its ids.  Then ids[rows[i]][ids_len[i]] = tokens[i], where that is a column and the token is not
  * negative.  lens and ids_len are those of the new beams: where beams differ in length, a call with the lengths as ids of one
- * column puts them in order first.  refs and tables NULL: only the ids; ids NULL: only the pages.  n <= 1024.  An entry whose row is outside [0, n_rows) or
- * listed before, or whose parent is outside [0, n) or such an entry, keeps its row and its ids. */
+ * column puts them in order first.  refs and tables NULL: only the ids; ids NULL: only the pages.  n <= 1024.  An entry whose
+ * row is outside [0, n_rows) or listed before, or whose parent is outside [0, n) or such an entry, keeps its row and its ids. */
 int qa_beam_reorder(int32_t * refs, int32_t n_pages, int32_t * tables, int32_t n_rows, int32_t table_stride,
                     int32_t page_size, const int32_t * rows, const int32_t * parents, const int32_t * lens, int32_t n,
                     int32_t * ids, int32_t ids_stride, const int32_t * tokens, const int32_t * ids_len, void * stream);

@@ -1,19 +1,25 @@
-// Causal attention of each sequence's new tokens over a K/V cache in pages.
+// Attention of each sequence's new tokens over a K/V cache in pages: causal, or by a tree's masks.
 //
 //   o_t = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q_t . k_j - m_t),   j <= n_past + t on a page that exists
+//                                                       (trees: j < n_past, and the new tokens of row t's mask)
 //
 // in one pass over the keys with a running maximum m and sum (the accumulators are rescaled when m grows).  The query
 // heads of a KV head and the tokens of a sequence are columns of the same products: column c of a tile is token c / group
-// and head c % group, so one token of 2 heads and a chunk of a thousand run the same code, in two shapes: a workgroup
-// takes 16 columns (8 in the packed form) and its 4 waves share the keys (attn_rows), or 128, a quarter per wave, and the
-// waves share K and V (attn_tile, long chunks on f16 pages).  A batch with short and long sequences is one launch.
+// and head c % group, so one token of 2 heads and a chunk of a thousand run the same code, in three shapes: a workgroup
+// takes 16 columns (8 in the packed form) or 32 and its 4 or 8 waves share the keys (attn_rows; attn_wide: trees and 8 bits), or
+// 128, a quarter per wave, and the waves share K and V (attn_tile, long causal chunks on f16 pages).  A batch with short and
+// long sequences is one launch.
 //
 // f16 pages on v_mfma_f32_16x16x32_f16: q and p are f32, split into two f16 parts each (a power of two per column brings
 // the largest |q| to 2^14..2^15, p is scaled by 2^6, so the second part keeps its bits); K and V are exact f16.  What the
 // parts leave out is 2^-22 of a value, the result is as near to 64 bits as f32 products are.  Up to 8 columns carry both
 // parts in one 16-column product (PACK), for decode steps.  f32 pages on v_mfma_f32_16x16x4_f32, whose products are f32.
+// Pages of 8 bits: the integers are exact f16, one conversion each; scores are multiplied by their key's scale, which is the
+// product with the dequantised K, and V's scales go into the probabilities before these are split.  What bounds them is the
+// instructions of the conversions (128 of the 320 of a step of 32 keys by 32 columns, which has 64 products) besides memory.
 //
-// Operands without LDS.  S^T = K Q^T takes K rows as they lie: lane l holds key l % 16.  Its result leaves 4 keys of a
+// Operands.  S^T = K Q^T takes K rows as they lie: lane l holds key l % 16.  attn_rows and attn_wide bring K's rows into LDS as they
+// lie and read operands there (KStep); V goes straight from memory into registers.  The result of S^T leaves 4 keys of a
 // column in each lane, which is the B operand of O^T = V^T P^T as it stands.  For V^T a lane loads the rows of those same
 // keys, dims 8 (l % 16) .. + 7: whole rows per load instruction, and all values that it needs are its own, so the
 // transposition is a register permutation (f16) or nothing at all (f32: one key per lane and product).  The output dims
@@ -591,27 +597,31 @@ __device__ inline void redo_columns(const AttnParams & p, const Tile & t, int he
     }
 }
 
-// Up to 16 columns (FEW on f16 pages: 8, in both parts), whose keys the 4 waves take in turn, step by step, straight from
-// memory into the operands: a decode step is the stream of K and V, and nothing stands between the loads and the products.
-// The waves' results are merged in LDS.
+// Up to 16 columns (FEW on f16 pages: 8, in both parts), whose keys the waves take in turn, step by step, each its own K and V, with no
+// barrier between the steps: a decode step is the stream of K and V, and the next step's loads are under way behind the
+// products.  The waves' results are merged in LDS.  32 decode steps behind 156 to 3914 positions on 8 bits (137 MB) 30.4 us, 4.5 TB/s of the
+// 5.1 that a copy reaches.
 constexpr int kRowsStride = kHeadDim + 4;
 constexpr int rows_cols(bool f16, bool few) { return f16 && few ? 8 : 16; }
 constexpr size_t rows_lds(bool f16, bool few, int waves = kWaves) { return waves * rows_cols(f16, few) * (kRowsStride + 2) * 4 + 2 * rows_cols(f16, few) * 4; }
 
 // A sequence that is one tile on f16 pages reads its K and V once, whole lines at a time: past the caches (ONCE).  32 sequences of
-// 3914 positions 84 instead of 94 us, of 157 to 3914 55.7 instead of 57.3.  That is for sequences with pages of their own; what
+// 3914 positions 84 instead of 94 us, of 157 to 3914 54.3 instead of 57.5 (8 bits: V alone 30.4 us, both 31.4, neither 35.3).  That is
+// for sequences with pages of their own; what
 // forked ones share is read once by each of them, and finds less of it in the caches: 32 beams behind 3913 shared positions 46.8
-// us, cached 42.6, behind 1000 19.2 / 18.5, eight behind 3913 22.3 / 21.1.  Nothing tells the two apart before the tables are read.  A row of f32 pages is taken by halves of its lines, and
-// longer chunks read it again: 129 instead of 111 us, and 50 instead of 40 at eight of 64 tokens.
+// us, cached 42.6, behind 1000 19.2 / 18.5, eight behind 3913 22.3 / 21.1.  Nothing tells the two apart before the tables are read.  A row
+// of f32 pages is taken by halves of its lines, and longer chunks read it again: 129 instead of 111 us, and 50 instead of 40 at eight of 64 tokens.
 template <bool ONCE, typename VT>
 __device__ inline VT load_row(const void * at) {
     if constexpr (ONCE) return __builtin_nontemporal_load(static_cast<const VT *>(at));
     else return *static_cast<const VT *>(at);
 }
 
-// A step of K in LDS, a wave's own.  A load instruction brings whole rows straight into LDS, a kilobyte in the order of its lanes, 16 bytes each; which
-// of its row's 16 bytes a lane takes depends on the row, so that the 16 rows of an operand are read from different banks.  (A lane that
-// loads its own operand takes 16 bytes of a row per instruction, and the 16 lanes beside it 16 other rows: four times the cache accesses.)
+// A step of K in LDS, a wave's own.  A load instruction brings whole rows straight into LDS, a kilobyte in the order of its lanes, 16
+// bytes each; which of its row's 16 bytes a lane takes depends on the row, so that the 16 rows of an operand are read from different
+// banks.  (A lane that loads its own operand takes 16 bytes of a row per instruction, and the 15 beside it as many other rows: four
+// times the cache accesses, and registers for all of it.  Sixteen trees of up to 41 nodes 43 us so, 37 through LDS, decode steps on
+// 8 bits 35.7 / 30.4, one tree of 64 10.7 / 9.0.)
 template <typename CT, bool ONCE = false>
 struct KStep {
     static constexpr int kRow = kHeadDim * sizeof(CT), kInRow = kRow / 16, kAtOnce = kWave / kInRow, kPerBlock = 16 / kAtOnce;
@@ -910,9 +920,11 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
     merge_waves<CT, R, PACK, TREE, W>(p, t, head, lds, wave, lane, col.row, col.lim, mc[0], l[0], O[0], redo[0]);
 }
 
-// 16 NB columns whose keys the 4 waves take in turn, as in attn_rows, but with their q in LDS, where the waves read the operands of
-// each step: a wave's registers hold the accumulators, and one read of K and V from memory serves all columns, with no barrier
-// between the steps.
+// 32 columns whose keys the waves take in turn, as in attn_rows, but with their q in LDS, where the waves read the operands of
+// each step: a wave's registers hold the accumulators, and one read of K and V, and on 8 bits one conversion, serves all columns.  1024
+// tokens behind 2889 positions on 8 bits (57 GF with both parts) 73 us, 780 TF/s where a large f16 product reaches 1147: two waves per
+// SIMD, whose 320 other instructions per 64 products do not all find the matrix unit busy.  Three waves (168 registers, q and K read
+// in smaller pieces) 77; more columns do not fit the registers.
 constexpr int kWideBlocks = 2;
 constexpr int kWideCols = 16 * kWideBlocks;
 constexpr size_t kWideQ = kWideBlocks * 8 * kWave * 16;               // two parts of 4 operands per 16 columns
