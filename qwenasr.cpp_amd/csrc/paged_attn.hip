@@ -606,7 +606,7 @@ constexpr int rows_cols(bool f16, bool few) { return f16 && few ? 8 : 16; }
 constexpr size_t rows_lds(bool f16, bool few, int waves = kWaves) { return waves * rows_cols(f16, few) * (kRowsStride + 2) * 4 + 2 * rows_cols(f16, few) * 4; }
 
 // A sequence that is one tile on f16 pages reads its K and V once, whole lines at a time: past the caches (ONCE).  32 sequences of
-// 3914 positions 84 instead of 94 us, of 157 to 3914 54.3 instead of 57.5 (8 bits: V alone 30.4 us, both 31.4, neither 35.3).  That is
+// 3914 positions 84 instead of 94 us, of 157 to 3914 55.7 instead of 57.3 (8 bits: V alone 30.4 us, both 31.4, neither 35.3).  That is
 // for sequences with pages of their own; what
 // forked ones share is read once by each of them, and finds less of it in the caches: 32 beams behind 3913 shared positions 46.8
 // us, cached 42.6, behind 1000 19.2 / 18.5, eight behind 3913 22.3 / 21.1.  Nothing tells the two apart before the tables are read.  A row
@@ -1503,6 +1503,11 @@ void launch_join(const AttnParams & p, bool f16, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, p, step_keys(f16));
 }
 
+// Decode steps of uneven lengths run best with three workgroups per CU and the others behind them: 32 on f16 pages behind 156 to 3914
+// positions 48.3 us, with four, which the registers allow, 54.5, with two 52.6 (8 bits 30.4 and, with two, 35.3).  Of the same length
+// they lose less: 32 behind 1000 30.4 / 29.2, eight behind 3913 32.4 / 31.7.  LDS keeps the fourth out.
+constexpr size_t kThreePerCu = 41 * 1024;
+
 // The longer sequences' kernel, or both kinds' in one launch.
 template <typename CT, bool TREE>
 int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
@@ -1512,7 +1517,7 @@ int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
     static_assert(lds_few <= kTileLds && lds_few <= lds_many, "a launch of both kinds has the longer ones' LDS");
     auto kernel = !pl.tiles_many ? &paged_rows_kernel<CT, true, TREE, kWaves>
                   : pl.few_max ? &paged_rows_both_kernel<CT, TREE> : &paged_rows_kernel<CT, false, TREE, kWaves>;
-    size_t lds = !pl.tiles_many ? lds_few : lds_many;
+    size_t lds = !pl.tiles_many ? std::max(lds_few, kThreePerCu) : lds_many;
     int waves = kWaves;
     if constexpr (F16 && FRESH) {
         if (pl.wide) {
