@@ -1328,13 +1328,9 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
 }
 
 // The launches.  One kind of tile, or longer chunks first and the sequences of few columns behind them.
-// Waves per SIMD that the registers are cut for.  16 columns on 8 bits, or with masks, do not fit three of them: two of 157 tokens behind
-// 701 and 1037 positions of 8 bits 24.3 / 20.7 us at three / two.  (With decode steps in the same launch they are three: 30.8 / 33.1.)
-template <typename CT, bool FEW, bool TREE>
-constexpr int rows_occupancy(int waves) { return waves > kWaves || (f16_products<CT> && !FEW && (TREE || is_q8<CT>)) ? 2 : 3; }
-
+// Registers are cut for three waves per SIMD, or one workgroup of 8 waves per CU.
 template <typename CT, bool FEW, bool TREE, int W>
-__global__ __launch_bounds__(W * kWave, (rows_occupancy<CT, FEW, TREE>(W))) void paged_rows_kernel(AttnParams p) {
+__global__ __launch_bounds__(W * kWave, W > kWaves ? 2 : 3) void paged_rows_kernel(AttnParams p) {
     extern __shared__ __attribute__((aligned(16))) char lds_rows[];
     attn_rows<CT, FEW, TREE, W>(p, blockIdx.x, lds_rows);
 }
