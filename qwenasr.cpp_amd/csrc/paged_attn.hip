@@ -1143,9 +1143,9 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
 // keys is two steps; a step lies in LDS as the MFMA operands themselves, 8 of K and 8 of V^T, 64 lanes x 16 bytes each:
 // every read and write is one unbroken kilobyte and no wave rearranges anything.  Waves 0 and 1 fetch and transpose V of
 // the two steps, waves 2 and 3 fetch K.  Two tiles in LDS, the next one's rows in registers: one barrier per tile, and two
-// workgroups per CU, each multiplying while the other waits at its barrier.  (On f32 pages, before attn_rows took K through LDS, whose products take four times
-// as long, the same scheme took 101 us against 112 of attn_rows at 300 tokens behind 3500 positions, 281 / 302 at 1024 behind
-// 2889, but 88 / 58 at 1024 behind none and 136 / 111 at four of 256 behind 500 to 1500: attn_rows takes them all.)
+// workgroups per CU, each multiplying while the other waits at its barrier.  (On f32 pages, whose products take four times
+// as long, the same scheme took 101 us against 112 of attn_rows at 300 tokens behind 3500 positions, 281 / 302 at 1024 behind 2889, but
+// 88 / 58 at 1024 behind none and 136 / 111 at four of 256 behind 500 to 1500, and attn_rows has become faster since: it takes them all.)
 constexpr int kTileSteps = 2;
 static_assert(kWaves == 2 * kTileSteps, "a wave fetches K or V of one step");
 constexpr int kTileCols = kWaves * 32;
@@ -1470,7 +1470,7 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     pl.tiles_many = many ? static_cast<int>(cols / width + seqs) : 0;
     pl.few_max = few ? few_cols(f16) : 0;
     pl.tiles_few = few ? seqs : 0;
-    // Workgroups to make of the keys, us (taken before K went through LDS, 5 to 15% ago).  Decode steps, and sequences of one tile: K and V are what they read, and more, shorter
+    // Workgroups to make of the keys, us (before K went through LDS, which made all of them 5 to 15% shorter).  Decode steps, and sequences of one tile: K and V are what they read, and more, shorter
     // ranges keep more of them in flight.  Longer ones read K and V once per tile, from L2, and every range writes and reads
     // its columns' partial results: 256 tokens behind 1000 positions (256 tiles) in 1 / 2 / 3 ranges 17.5 / 23 / 24, 64 behind
     // 3000 (64 tiles) in 4 / 6 / 8 38 / 30 / 34 (f32 pages).  With few CUs left over by the tiles of a long context their
