@@ -287,8 +287,10 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamParams p) {
         const int b = task / parts;
         const double off = s.off[b];
         if (!(off > -INFINITY)) continue;
-        // below what a maximum needs by more than the difference is rounded
-        const float near = static_cast<float>(bound - off), least = near - fmaxf(fabsf(near), 1e-30f) * 0x1p-22f;
+        // What a maximum needs, less what is rounded on the way: a score and the difference to 2^-53 of what they come from, which may
+        // be far larger than the difference, and the f32 to 2^-24 of itself.  list() compares the scores.
+        const double near = bound - off;
+        const float least = static_cast<float>(near - (fabs(near) * 0x1p-22 + (fabs(bound) + fabs(off)) * 0x1p-51));
         for (int from = 0; from < per_lane; from += kKeep) {
             if (!keep) fetch(task, from);
             unsigned some = 0;
