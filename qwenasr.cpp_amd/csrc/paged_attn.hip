@@ -15,8 +15,8 @@
 // parts leave out is 2^-22 of a value, the result is as near to 64 bits as f32 products are.  Up to 8 columns carry both
 // parts in one 16-column product (PACK), for decode steps.  f32 pages on v_mfma_f32_16x16x4_f32, whose products are f32.
 // Pages of 8 bits: the integers are exact f16, one conversion each; scores are multiplied by their key's scale, which is the
-// product with the dequantised K, and V's scales go into the probabilities before these are split.  What bounds them is the
-// instructions of the conversions (128 of the 320 of a step of 32 keys by 32 columns, which has 64 products) besides memory.
+// product with the dequantised K, and V's scales go into the probabilities before these are split (weighted_step).  What bounds them is the
+// instructions of the conversions (128 of the 330 of a step of 32 keys by 32 columns, which has 64 products) besides memory.
 //
 // Operands.  S^T = K Q^T takes K rows as they lie: lane l holds key l % 16.  attn_rows and attn_wide bring K's rows into LDS as they
 // lie and read operands there (KStep); V goes straight from memory into registers.  The result of S^T leaves 4 keys of a
@@ -408,50 +408,6 @@ __device__ inline void v_operands(const u2 (&raw)[8], int h, u4 & even, u4 & odd
     odd = u4{o[4], o[5], o[6], o[7]};
 }
 
-// The keys' V scales go into the probabilities, which are split into f16 parts behind that.  So that these stay in f16's range, the
-// column's reference has the largest scale that the wave has met in it, a power of two: p = exp2(s - m - top), and p times
-// the scale is at most what p alone is on pages of f16.  Sum and accumulators follow when top grows.  Scales of less than 2^-80 count
-// as such: p has to be an f32.
-constexpr int kLeastTop = -80;
-template <int NB>
-__device__ inline void follow_scales(const f4 (&vs)[2], int & top, float (&l)[NB], f4 (&O)[NB][8]) {
-    float most = 0.0f;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) most = fmaxf(most, vs[kb][i]);     // a NaN is passed over
-    }
-    if (!__any(most > ldexpf(1.0f, top))) return;
-    const int ex = max(top, __builtin_amdgcn_frexp_expf(column_max(most)));   // all lanes have the same
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int db = 0; db < 8; ++db) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) O[nb][db][i] = ldexpf(O[nb][db][i], top - ex);
-        }
-        l[nb] = ldexpf(l[nb], top - ex);
-    }
-    top = ex;
-}
-
-template <int NB>
-__device__ inline void weigh_step(const f4 (&vs)[2], float (&pr)[NB][2][4]) {
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                pr[nb][kb][i] *= vs[kb][i];
-                // the product as it is rounded here: one that a conversion to f16 takes in unrounded (v_fma_mix) is now and then
-                // another f16 than the one whose rest is the second part
-                asm("" : "+v"(pr[nb][kb][i]));
-            }
-        }
-    }
-}
-
 // Element offset of operand f of a step inside its 16-key block, and that block.  K on f16 pages: key l % 16, dims as q's.  V there:
 // key 16 (f / 4) + 4 (l / 16) + f % 4, dims 8 (l % 16) ..; on f32 pages key 4 (l / 16) + f / 2, dims 8 (l % 16) + 4 (f % 2) ...
 __device__ inline int k_offset(int f, int c16, int g4) { return c16 * kHeadDim + (f & 3) * 32 + g4 * 8; }
@@ -490,7 +446,7 @@ __device__ inline void split_q(const f4 (&x)[8], float scale, float & c, h8 (&qh
 // A masked score is -inf.
 template <int NB, int KB>
 __device__ inline void softmax_step(const f4 (&S)[NB][KB], const float (&c)[NB], float (&m)[NB], float (&l)[NB], f4 (&O)[NB][8],
-                                    float (&pr)[NB][KB][4], float shift = -kShiftLog2) {
+                                    float (&pr)[NB][KB][4]) {
     float mn[NB];
     bool up[NB], any = false;
 #pragma unroll
@@ -517,13 +473,125 @@ __device__ inline void softmax_step(const f4 (&S)[NB][KB], const float (&c)[NB],
     }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-        const float mc = m[nb] == -INFINITY ? INFINITY : fmaf(m[nb], c[nb], shift);
+        const float mc = m[nb] == -INFINITY ? INFINITY : fmaf(m[nb], c[nb], -kShiftLog2);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 pr[nb][kb][i] = __builtin_amdgcn_exp2f(fmaf(S[nb][kb][i], c[nb], -mc));
                 l[nb] += pr[nb][kb][i];
+            }
+        }
+    }
+}
+
+// The same on pages of 8 bits, where the keys' V scales go into the probabilities, which are split into f16 parts behind that.  So that
+// these keep their bits whatever the scales are, the column's reference (log2 units) follows the largest product that the
+// column has: w = exp2(s - m) scale <= 2^14, and a key that it does not see, or hardly, moves nothing, however large its row.
+// Probabilities alone are in m, too, f32 as their sum is, and up to 2^95: scales below 2^kLeastScale, and 0, count as that.  What a column
+// sees of rows so small (but not 0) it computes again key by key (small).
+// Scales of one size, the common case, are bounded per lane by the largest of its 8: at most 6 bits more than needed.  (1024 tokens behind
+// 2889 positions 72.6 us; 78 where all steps have scales up to 2^10 apart, 32 streams 32.0 / 32.9.)  m is whole, so that sum and
+// accumulators follow it without rounding, over any distance.
+constexpr float kLeastScale = -80.0f;
+constexpr float kNearScales = 0x1p-6f, kSmallScale = 0x1p-78f;
+__device__ inline float log2_near(float x) {                          // up to 0.09 below; 128 and more of what is not finite
+    return fmaf(static_cast<float>(__float_as_uint(x)), 0x1p-23f, -127.0f);
+}
+
+// The scales of rows that no column sees (keys from `keys` on, blocks of holes): any finite one will do, as their probability is 0; one of the
+// lane's others keeps the step to scales of one size (one token behind 156 positions 6.50 us, with zeros 6.70; attn_wide, whose
+// registers it costs, has zeros: sixteen trees of up to 41 nodes 34.7, so 35.7).
+__device__ inline void neutral_scales(f4 (&vs)[2], int keys, int holes, int g4) {
+    float other = 0.0f;
+#pragma unroll
+    for (int f = 0; f < 8; ++f) {
+        const bool none = v_key<true>(f, g4) >= keys || ((holes >> (f >> 2)) & 1);
+        other = fmaxf(other, none ? 0.0f : vs[f >> 2][f & 3]);
+    }
+    if (!(other > 0.0f && other < INFINITY)) other = 1.0f;
+#pragma unroll
+    for (int f = 0; f < 8; ++f) {
+        if (v_key<true>(f, g4) >= keys || ((holes >> (f >> 2)) & 1)) vs[f >> 2][f & 3] = other;
+    }
+}
+
+template <int NB>
+__device__ inline void weighted_step(const f4 (&S)[NB][2], const f4 (&vs)[2], const float (&c)[NB], float (&m)[NB], float (&l)[NB],
+                                     f4 (&O)[NB][8], float (&pr)[NB][2][4], bool & small) {
+    float most = 0.0f, least = INFINITY, t[NB];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            most = fmaxf(most, vs[kb][i]);
+            least = fminf(least, vs[kb][i]);
+        }
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) t[nb] = -INFINITY;
+    if (!__any(!(least >= fmaxf(most * kNearScales, kSmallScale)))) {
+        const float size = log2_near(most);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) t[nb] = fmaxf(t[nb], S[nb][kb][i]);
+            }
+            t[nb] = fmaf(t[nb], c[nb], size);
+        }
+    } else {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = fabsf(vs[kb][i]), size = fmaxf(log2_near(x), kLeastScale);
+                bool seen = false;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    t[nb] = fmaxf(t[nb], fmaf(S[nb][kb][i], c[nb], size));
+                    seen = seen || S[nb][kb][i] > -INFINITY;
+                }
+                small = small || (seen && x > 0.0f && x < kSmallScale);
+            }
+        }
+    }
+    float mn[NB];
+    bool up[NB], any = false;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        mn[nb] = fmaxf(m[nb], column_max(t[nb]));
+        up[nb] = mn[nb] - m[nb] > kLazyLog2;             // -inf to finite: yes; -inf to -inf: NaN, no
+        any = any || up[nb];
+    }
+    if (__any(any)) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const float to = rintf(mn[nb]);
+            const int by = up[nb] ? static_cast<int>(fmaxf(m[nb] - to, -1000.0f)) : 0;
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) O[nb][db][i] = ldexpf(O[nb][db][i], by);
+            }
+            l[nb] = ldexpf(l[nb], by);
+            if (up[nb]) m[nb] = to;
+        }
+    }
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const float mc = m[nb] == -INFINITY ? INFINITY : m[nb] - kShiftLog2;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(S[nb][kb][i], c[nb], -mc));
+                l[nb] += e;
+                pr[nb][kb][i] = e * vs[kb][i];
+                // the product as it is rounded here: one that a conversion to f16 takes in unrounded (v_fma_mix) is now and then
+                // another f16 than the one whose rest is the second part
+                asm("" : "+v"(pr[nb][kb][i]));
             }
         }
     }
@@ -560,14 +628,21 @@ __device__ inline void store_column(const AttnParams & p, const Tile & t, int ro
 }
 
 // The end of a wave's steps: the column's sum over its 4 lanes, its reference in log2 units, and the columns of each block
-// whose values are not all finite.
-template <int NB, bool PACK>
+// whose values are not all finite, or flagged (again).  WEIGHTED: m is weighted_step's, and the sums, which may be of any size, are brought to 1/2 .. 1,
+// so that the reference says what they weigh beside other waves' and ranges'.
+template <int NB, bool PACK, bool WEIGHTED>
 __device__ inline void close_columns(const int (&orow)[NB], const float (&c)[NB], const float (&m)[NB], float (&l)[NB], f4 (&O)[NB][8],
-                                     float (&mc)[NB], uint32_t (&redo)[NB], float shift = -kShiftLog2) {
+                                     float (&mc)[NB], uint32_t (&redo)[NB], bool again) {
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         l[nb] = column_sum(l[nb]);
-        mc[nb] = m[nb] == -INFINITY ? -INFINITY : fmaf(m[nb], c[nb], shift);
+        mc[nb] = m[nb] == -INFINITY ? -INFINITY : WEIGHTED ? m[nb] - kShiftLog2 : fmaf(m[nb], c[nb], -kShiftLog2);
+        int ex = 0;
+        if constexpr (WEIGHTED) {
+            ex = __builtin_amdgcn_frexp_expf(l[nb]);                  // 0 of 0 and of what is not finite
+            l[nb] = ldexpf(l[nb], -ex);
+            mc[nb] += static_cast<float>(ex);
+        }
         // 0 x is 0 unless x is not finite, and a sum of such products is then NaN
         float zero = 0.0f * l[nb];
 #pragma unroll
@@ -575,10 +650,11 @@ __device__ inline void close_columns(const int (&orow)[NB], const float (&c)[NB]
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if constexpr (PACK) O[nb][db][i] += row_ror8(O[nb][db][i]);
+                if constexpr (WEIGHTED) O[nb][db][i] = ldexpf(O[nb][db][i], -ex);
                 zero = fmaf(0.0f, O[nb][db][i], zero);
             }
         }
-        const uint64_t bad = __ballot((!(zero == 0.0f) || m[nb] == INFINITY) && orow[nb] >= 0);
+        const uint64_t bad = __ballot((!(zero == 0.0f) || m[nb] == INFINITY || again) && orow[nb] >= 0);
         redo[nb] = static_cast<uint32_t>(bad | (bad >> 16) | (bad >> 32) | (bad >> 48)) & (PACK ? 0xffu : 0xffffu);
     }
 }
@@ -817,7 +893,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
     const int lim[NB] = {col.lim}, orow[NB] = {col.row}, mask[NB] = {col.mask};
     // steps that every column sees whole
     const int full = TREE ? max(0, min(t.past, t.cap)) / KS : max(0, min(t.past + t.col0 / p.group, t.cap - 1) + 1) / KS;
-    int top = kLeastTop;
+    [[maybe_unused]] bool small = false;
     float m[NB] = {-INFINITY}, l[NB] = {0.0f};
     f4 O[NB][8];
 #pragma unroll
@@ -865,19 +941,18 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
         if (st >= full || holes != 0) mask_step<NB, KB, TREE>(p, S, lim, mask, t.past, st * KS, g4, holes);
         // rows of keys that no column sees, and of no page, are whatever memory holds: not even 0 times that
         if (st * KS + KS > t.kend || holes != 0) {
+            if constexpr (Q8) {
+                neutral_scales(vs, t.kend - st * KS, holes, g4);
+            } else {
 #pragma unroll
-            for (int f = 0; f < 8; ++f) {
-                if (st * KS + v_key<F16>(f, g4) >= t.kend || pg[F16 ? f >> 2 : 0] < 0) {
-                    if constexpr (Q8) vs[f >> 2][f & 3] = 0.0f;
-                    else rv[f] = u4{0, 0, 0, 0};
+                for (int f = 0; f < 8; ++f) {
+                    if (st * KS + v_key<F16>(f, g4) >= t.kend || pg[F16 ? f >> 2 : 0] < 0) rv[f] = u4{0, 0, 0, 0};
                 }
             }
         }
         float pr[NB][KB][4];
         if constexpr (Q8) {
-            follow_scales<NB>(vs, top, l, O);
-            softmax_step<NB, KB>(S, c, m, l, O, pr, static_cast<float>(top) - kShiftLog2);
-            weigh_step<NB>(vs, pr);
+            weighted_step<NB>(S, vs, c, m, l, O, pr, small);
         } else {
             softmax_step<NB, KB>(S, c, m, l, O, pr);
         }
@@ -915,7 +990,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
 
     float mc[NB];
     uint32_t redo[NB];
-    close_columns<NB, PACK>(orow, c, m, l, O, mc, redo, Q8 ? static_cast<float>(top) - kShiftLog2 : -kShiftLog2);
+    close_columns<NB, PACK, Q8>(orow, c, m, l, O, mc, redo, small);
     __syncthreads();                                                      // every wave has read its K
     merge_waves<CT, R, PACK, TREE, W>(p, t, head, lds, wave, lane, col.row, col.lim, mc[0], l[0], O[0], redo[0]);
 }
@@ -923,7 +998,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
 // 32 columns whose keys the waves take in turn, as in attn_rows, but with their q in LDS, where the waves read the operands of
 // each step: a wave's registers hold the accumulators, and one read of K and V, and on 8 bits one conversion, serves all columns.  1024
 // tokens behind 2889 positions on 8 bits (57 GF with both parts) 73 us, 780 TF/s where a large f16 product reaches 1147: two waves per
-// SIMD, whose 320 other instructions per 64 products do not all find the matrix unit busy.  Three waves (168 registers, q and K read
+// SIMD, whose 330 other instructions per 64 products do not all find the matrix unit busy.  Three waves (168 registers, q and K read
 // in smaller pieces) 77; more columns do not fit the registers.
 constexpr int kWideBlocks = 2;
 constexpr int kWideCols = 16 * kWideBlocks;
@@ -1025,7 +1100,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
     for (int nb = 0; nb < NB; ++nb) c[nb] = *reinterpret_cast<const float *>(lds + kWideQ + (nb * 16 + c16) * 4);
     // steps that every column sees whole
     const int full = TREE ? max(0, min(t.past, t.cap)) / KS : max(0, min(t.past + t.col0 / p.group, t.cap - 1) + 1) / KS;
-    int top = kLeastTop;
+    [[maybe_unused]] bool small = false;
     float m[NB], l[NB];
     f4 O[NB][8];
 #pragma unroll
@@ -1099,9 +1174,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
         }
         float pr[NB][KB][4];
         if constexpr (Q8) {
-            follow_scales<NB>(vs, top, l, O);
-            softmax_step<NB, KB>(S, c, m, l, O, pr, static_cast<float>(top) - kShiftLog2);
-            weigh_step<NB>(vs, pr);
+            weighted_step<NB>(S, vs, c, m, l, O, pr, small);
         } else {
             softmax_step<NB, KB>(S, c, m, l, O, pr);
         }
@@ -1130,7 +1203,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
     if (st < t.step_hi) step(std::false_type{});
     float mc[NB];
     uint32_t redo[NB];
-    close_columns<NB, false>(orow, c, m, l, O, mc, redo, Q8 ? static_cast<float>(top) - kShiftLog2 : -kShiftLog2);
+    close_columns<NB, false, Q8>(orow, c, m, l, O, mc, redo, small);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         __syncthreads();                                                  // q and the block before are no longer read
@@ -1300,7 +1373,7 @@ __device__ inline void attn_tile(const AttnParams & p, int block, char * lds) {
     }
     float mc[NB];
     uint32_t redo[NB];
-    close_columns<NB, false>(orow, c, m, l, O, mc, redo);
+    close_columns<NB, false, false>(orow, c, m, l, O, mc, redo, false);
     // through the wave's own part of LDS, so that a store instruction writes two whole rows; a lane's values would lie 16 bytes
     // in each of 64 lines
     float * so = reinterpret_cast<float *>(lds) + wave * kOutFloats;
