@@ -723,6 +723,11 @@ struct KStep {
         }
 #endif
     }
+    // Behind K's loads: none of V's, which arrived() counts, is moved ahead of them.
+    static __device__ inline void issued() {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0x81);              // what is no access of memory, or one of LDS, may pass
+    }
     // Before a step's chunks are read: of the loads behind those of K there are V's 8.
     static __device__ inline void arrived() { asm volatile("s_waitcnt vmcnt(8)" ::: "memory"); }
     // Before the next step is loaded: this one has been read.
@@ -859,6 +864,7 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
                 vs_next[kb] = *reinterpret_cast<const f4 *>(scales[kb] + rows.v_elems + scale_lane);
             }
         }
+        KStep<CT>::issued();
     };
     auto load_v = [&]() {
         if constexpr (Q8) {
@@ -874,7 +880,6 @@ __device__ inline void attn_rows(const AttnParams & p, int block, char * lds) {
         entries_of(st, entry);
         place(st);
         load_k();
-        __builtin_amdgcn_sched_barrier(0);
         load_v();
         entries_of(st + W, entry);
     }
@@ -1052,6 +1057,7 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
                 vs_next[kb] = *reinterpret_cast<const f4 *>(scales[kb] + rows.v_elems + scale_lane);
             }
         }
+        KStep<CT>::issued();
     };
     auto load_v = [&]() {
         if constexpr (Q8) {
@@ -1067,7 +1073,6 @@ __device__ inline void attn_wide(const AttnParams & p, int block, char * lds) {
         entries_of(st, entry);
         place(st);
         load_k();
-        __builtin_amdgcn_sched_barrier(0);
         load_v();
         entries_of(st + W, entry);
     }
