@@ -237,8 +237,9 @@ typedef struct qa_paged_batch {
 /* qa_kv_append over pages, the same bits: q_out[r] <- RoPE(RMSNorm(q)), K and V rows into the page of the row's
  * position (dropped where there is none).  qkv: [n_rows][q_dim + 2 kv_dim], q_out: [n_rows][q_dim].  A page that several
  * tables hold is written as it is: qa_pages_extend makes it private first.
- * QA_CACHE_Q8: a row's scale is max |x| / 127 (f32, rounded to nearest) and its values are the integers nearest to x / scale,
- * ties to even, within -127 .. 127; zeros where the scale is 0.  A row that holds an infinity or NaN gets the scale NaN.  */
+ * QA_CACHE_Q8: a row's scale is max |x| / 127 (f32, rounded to nearest) and its values are the integers nearest to the f32 quotients
+ * x / scale, ties to even, within -127 .. 127; zeros where the scale is 0.  A row that holds an infinity or NaN gets the scale
+ * NaN.  pages aligned to 16 bytes.  */
 int qa_paged_append(const float * qkv, const float * q_norm_w, const float * k_norm_w, float * q_out, void * pages,
                     const qa_kv_layout * layout, int32_t layer, const qa_paged_batch * batch, int32_t n_heads,
                     float rope_theta, float eps, void * stream);

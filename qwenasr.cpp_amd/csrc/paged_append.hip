@@ -256,6 +256,10 @@ int append(const float * qkv, const float * q_norm_w, const float * k_norm_w, fl
     if (!(rope_theta > 0.0f)) return fail(QA_ERR_INVALID, who + ": rope_theta must be positive");
     if (batch->n_rows == 0) return QA_OK;
     if (!qkv || !q_norm_w || !k_norm_w || !q_out || !pages) return fail(QA_ERR_INVALID, who + ": null pointer");
+    // 8 bits are stored in words, and their scales as f32
+    if (layout->cache_type == QA_CACHE_Q8 && (reinterpret_cast<uintptr_t>(pages) & 15) != 0) {
+        return fail(QA_ERR_INVALID, who + ": pages must be aligned to 16 bytes");
+    }
     if (const int rc = check_stream(stream, name); rc != QA_OK) return rc;
     PagedAppendParams p{};
     p.qkv = qkv;
