@@ -1578,9 +1578,11 @@ void launch_join(const AttnParams & p, bool f16, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0, stream, p, step_keys(f16));
 }
 
-// Decode steps of uneven lengths run best with three workgroups per CU and the others behind them: 32 on f16 pages behind 156 to 3914
-// positions 48.3 us, with four, which the registers allow, 54.5, with two 52.6 (8 bits 30.4 and, with two, 35.3).  Of the same length
-// they lose less: 32 behind 1000 30.4 / 29.2, eight behind 3913 32.4 / 31.7.  LDS keeps the fourth out.
+// Decode steps on f16 pages run with three workgroups per CU and the others behind them, where registers would allow four: sequences of
+// uneven lengths gain more than those of one length lose.  Behind 156 to 3900 positions, three / four: eight 19.9 / 21.7 us, sixteen
+// 28.1 / 31.3, 32 48.5 / 54.8, 64 94.4 / 93.3; 32 behind 1000 to 3000 49.7 / 50.1; of the same length 32 behind 1000 27.8 / 26.6, 64 46.0 / 45.8,
+// 16 and 32 behind 3900 the same.  (Two per CU: 52.6 for the 32.)  LDS keeps the fourth out.  The other few-column kernels' registers
+// are for three as it is.
 constexpr size_t kThreePerCu = 41 * 1024;
 
 // The longer sequences' kernel, or both kinds' in one launch.
@@ -1592,7 +1594,7 @@ int launch_attn(const AttnPlan & pl, AttnParams p, hipStream_t stream) {
     static_assert(lds_few <= kTileLds && lds_few <= lds_many, "a launch of both kinds has the longer ones' LDS");
     auto kernel = !pl.tiles_many ? &paged_rows_kernel<CT, true, TREE, kWaves>
                   : pl.few_max ? &paged_rows_both_kernel<CT, TREE> : &paged_rows_kernel<CT, false, TREE, kWaves>;
-    size_t lds = !pl.tiles_many ? std::max(lds_few, kThreePerCu) : lds_many;
+    size_t lds = pl.tiles_many ? lds_many : F16 && !FRESH ? std::max(lds_few, kThreePerCu) : lds_few;
     int waves = kWaves;
     if constexpr (F16 && FRESH) {
         if (pl.wide) {
