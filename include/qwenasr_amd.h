@@ -254,8 +254,9 @@ int qa_paged_read(const void * pages, const qa_kv_layout * layout, int32_t layer
 /* Causal attention of every sequence's new tokens over its pages: the token at position p attends the positions
  * 0 .. p that lie on a page (a chunk of a prompt, or one token per sequence: a decode step).  A token that sees no
  * position gets zeros.  q: [n_rows][q_dim] f32 (post norm + RoPE), out: [n_rows][q_dim].  Products and sums have f32
- * accuracy for every cache type (q and the probabilities are not rounded to f16 as qa_decode_attn does).  scale > 0.
- * What masked positions hold never matters, NaN included.
+ * accuracy for every cache type (q and the probabilities are not rounded to f16 as qa_decode_attn does); on f16 pages and
+ * pages of 8 bits an error counts against the sum of each seen row's probability times its largest |v|.  scale > 0.
+ * What masked positions hold never matters, NaN and rows of any size included.
  * workspace: results of key ranges that are joined at the end.  Any size works, none included; with less than
  * qa_paged_attn_workspace_bytes (of the same batch; its pointers are not read) the keys are cut into fewer ranges, which
  * is slower and sums in another order.  Nothing in it outlives the call; calls that share one must be stream-ordered.

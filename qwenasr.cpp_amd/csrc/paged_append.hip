@@ -32,7 +32,7 @@ struct PagedAppendParams {
 // A row of 128 values in 8 bits, lane holding a and b: the integers nearest to x / scale, scale = max |x| / 127.  A prompt's append
 // is bound by its instructions, so the quotients are products with a reciprocal and a correction, which rounds them as a
 // division does, integers come from the low bits of 1.5 2^23 + x, and four lanes put a word together.  Scales that are no ordinary
-// numbers take the divisions.  3913 rows of 16 query and 8 KV heads 26.3 us, 104 MB at 4.0 TB/s (f16 23.7, 112 MB at 4.7; a copy
+// numbers take the divisions.  3913 rows of 16 query and 8 KV heads 26.3 us, 104 MB at 4.0 TB/s (f16 22.4, 112 MB at 5.0; a copy
 // reaches 5.1); 32 rows 4.6.
 struct Q8Row {
     uint32_t a, b;      // the byte at its place in the word of four lanes
@@ -80,9 +80,9 @@ __device__ inline uint32_t quad_word(uint32_t w) {
     return w;
 }
 
-// STREAM: results past the caches (a prompt of kStreamRows tokens or more): 3913 tokens 23.1 instead of 28.4 us, 1024 tokens 9.3
-// instead of 10.4, and the attention that reads them next takes as long.  Fewer results stay in L2 for it (156 tokens with their
-// attention 13.3 us, 13.5 past the caches).
+// STREAM: results past the caches (a prompt of kStreamRows tokens or more).  Six layers' inputs in turn, f16: 1024 tokens 8.9 instead of
+// 9.6 us, 2000 13.5 / 15.4, 3913 26.4 / 28.0 (f32 pages 9.1 / 10.2, 13.7 / 17.8, 27.9 / 30.5), and the attention that reads them next takes as
+// long.  Fewer results stay in L2 for it (156 tokens with their attention 13.3 us, 13.5 past the caches).
 constexpr int kStreamRows = 1024;
 // Waves per row: a wave walks its head slots one after another, which few rows wait for (32 rows of f16 in 4 / 8 / 16 waves 5.2 / 4.6 /
 // 4.6 us); of many rows each wave's angles and place are more to do.

@@ -675,7 +675,7 @@ __device__ inline void redo_columns(const AttnParams & p, const Tile & t, int he
 
 // Up to 16 columns (FEW on f16 pages: 8, in both parts), whose keys the waves take in turn, step by step, each its own K and V, with no
 // barrier between the steps: a decode step is the stream of K and V, and the next step's loads are under way behind the
-// products.  The waves' results are merged in LDS.  32 decode steps behind 156 to 3914 positions on 8 bits (137 MB) 30.4 us, 4.5 TB/s of the
+// products.  The waves' results are merged in LDS.  32 decode steps behind 156 to 3914 positions on 8 bits (137 MB) 30.8 us, 4.5 TB/s of the
 // 5.1 that a copy reaches.
 constexpr int kRowsStride = kHeadDim + 4;
 constexpr int rows_cols(bool f16, bool few) { return f16 && few ? 8 : 16; }
@@ -1493,7 +1493,7 @@ struct AttnPlan {
 
 // Key ranges of `steps` steps for workgroups of which one range has `blocks`: enough to make `target` of them, of `least` steps or
 // so, and more than one only where there are twice as many: two of 5 or 7 steps lose more to the join than they gain (one
-// token behind 400 positions 9.7 us, in one range 8.4; 128 tokens behind 500, `least` 16, 15.3 and 11.6).
+// token behind 400 positions 9.7 us, in one range 8.4, both before K went through LDS; 128 tokens behind 500, `least` 16, 12.7 and 8.9).
 void cut_keys(int steps, int64_t blocks, int64_t target, int64_t least, int64_t most, int & splits, int & split_steps) {
     const int64_t by_length = steps < 2 * least ? 1 : (steps + least - 1) / least;
     const int64_t n = std::max<int64_t>(1, std::min<int64_t>({target / std::max<int64_t>(blocks, 1), by_length, most}));
@@ -1527,8 +1527,8 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     const bool few = !many || (b.n_seqs > 1 && (!fresh || 4 * few_seqs >= 3 * seqs));
     int64_t eight_tiles = 0;
     if (fresh && !few && most > 16) {
-        // 8 bits and trees, us.  One workgroup of 8 waves per CU, where the tiles and their ranges fill two thirds of the CUs, or half of
-        // them for not long, and each has enough to do for what it takes to begin and to merge (`worth`): sixteen trees of up to 41
+        // 8 bits and trees on 8 KV heads, us.  One workgroup of 8 waves per CU, where the tiles and their ranges fill 166 of the 256 CUs, or 120 of
+        // them for 40 steps at most, and each has enough to do for what it takes to begin and to merge (`worth`): sixteen trees of up to 41
         // behind 156 to 3000 in attn_wide of 8 / 4 waves and in attn_rows 37 / 44 / 45, five behind 1600 18.5 / 20.9 / 20.6, but one
         // of 64 behind 3000 15.9 / 16.6 / 15.1, six of up to 20 behind 500 to 1500 16.3 / 16.8 / 15.3; two of 63 in f32 with attn_rows
         // of 8 / 4 waves 20 / 24.  8 bits: 64 tokens behind 3000 16.3 / 17.3 / 17.0, two trees of 32 behind 2000 16.5 / 17.5 / 16.5, sixteen of
@@ -1548,14 +1548,15 @@ AttnPlan attn_plan(const qa_kv_layout & l, const qa_paged_batch & b, int32_t n_h
     pl.tiles_many = many ? static_cast<int>(cols / width + seqs) : 0;
     pl.few_max = few ? few_cols(f16) : 0;
     pl.tiles_few = few ? seqs : 0;
-    // Workgroups to make of the keys, us (before K went through LDS, which made all of them 5 to 15% shorter).  Decode steps, and sequences of one tile: K and V are what they read, and more, shorter
-    // ranges keep more of them in flight.  Longer ones read K and V once per tile, from L2, and every range writes and reads
-    // its columns' partial results: 256 tokens behind 1000 positions (256 tiles) in 1 / 2 / 3 ranges 17.5 / 23 / 24, 64 behind
-    // 3000 (64 tiles) in 4 / 6 / 8 38 / 30 / 34 (f32 pages).  With few CUs left over by the tiles of a long context their
-    // partial results cost less than the wait for the CUs that have one more: 300 behind 3500 (304 tiles), f32 pages, 112 in
-    // three, 140 in one.  Sequences differ in length, and the ranges are cut for the longest: 16 of 70 behind 300 to 2000 at
-    // 384 / 640 workgroups 38 / 33 (f32: 76 / 59).  attn_tile has 512 at a time: one sequence of 400 behind 3500 at 512 / 768
-    // 47 / 56, but two of 600 and ten of one token behind 24 to 3500 98 / 73, four of 256 behind 500 to 1500 53 / 57.
+    // Workgroups to make of the keys, us.  Decode steps, and sequences of one tile: K and V are what they read, and more, shorter
+    // ranges keep more of them in flight.  Longer ones read K and V once per tile, from L2, and every range writes and reads its
+    // columns' partial results: 256 tokens behind 1000 positions (256 tiles) in 1 / 2 / 3 ranges 12.1 / 17.4 / 20.0 (f32 pages 28.7 / 32.6 /
+    // 35.4), 64 behind 3000 (64 tiles) in 4 / 6 / 8 17.5 / 16.2 / 18.2 (34.7 / 27.8 / 30.5).  With few CUs left over by the tiles of a long
+    // context their partial results cost less than the wait for the CUs that have one more: 300 behind 3500 (304 tiles) on f32
+    // pages 124 in one, 98 in two, 92 in three.  Sequences differ in length, and the ranges are cut for the longest: 16 of 70 behind 300
+    // to 2000, 1 / 2 / 3 ranges 64 / 67 / 70 (f32, which takes one, too, 140 / 132 / 134).  attn_tile has 512 workgroups at a time: 400
+    // behind 3500 in 3 / 4 / 9 ranges 64 / 54 / 46, two of 600 and eight of one token behind 24 to 3500 in 3 / 4 / 5 / 6 93 / 78 / 77 / 78, but
+    // four of 256 behind 500 to 1500, which get six, in 3 / 4 / 6 60 / 53 / 59.  128 behind 500 on f32 pages get three, 18.6, one is 16.8.
     const int64_t heads = static_cast<int64_t>(seqs) * l.n_kv_heads;
     const int64_t tiles = pl.eight ? eight_tiles : std::max<int64_t>(1, (cols + width - 1) / width) * l.n_kv_heads;
     const bool one = b.n_seqs == 1;
